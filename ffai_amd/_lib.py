@@ -34,6 +34,9 @@ EXPORTS = [
     "moe_layer_forward", "moe_layer_forward_routed", "moe_layer_forward_residual",
     "moe_layer_path", "moe_layer_forward_noalloc", "moe_layer_noalloc_max_bytes", "moe_add_rmsnorm", "moe_mxfp4_to_affine", "moe_layer_create", "moe_layer_destroy",
     "moe_layer_decode", "moe_layer_decode_many",
+    "moe_balance_loss_workspace_bytes", "moe_balance_loss", "moe_router_backward",
+    "moe_unpermute_backward", "moe_validate_lora", "moe_lora_workspace_bytes", "moe_lora_apply",
+    "moe_lora_backward_workspace_bytes", "moe_lora_backward",
     "moe_st_open", "moe_st_close", "moe_st_count", "moe_st_name", "moe_st_info", "moe_st_read_host",
     "moe_st_upload", "moe_st_is_quantized", "moe_st_stacked_bytes", "moe_st_load_stacked",
     "moe_st_load_stacked_many", "moe_st_mxfp4_bytes", "moe_st_load_mxfp4",
@@ -69,6 +72,12 @@ class LayerDesc(C.Structure):
         ("logit_scale", C.c_float), ("routed_scale", C.c_float), ("expert_scale", C.c_void_p),
         ("router_q", QProj), ("shared_gate_q", QProj),
     ]
+
+
+class Lora(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p),
+                ("dtype", C.c_int32), ("rank", C.c_int32), ("n", C.c_int32), ("k", C.c_int32),
+                ("n_adapters", C.c_int32)]
 
 
 class LayerPaths(C.Structure):
@@ -138,6 +147,20 @@ def load():
     lib.moe_layer_destroy.restype = None
     lib.moe_layer_decode.argtypes = [vp, vp, vp, st]
     lib.moe_layer_decode_many.argtypes = [vp, vp, i32, vp, st]
+    lib.moe_balance_loss_workspace_bytes.argtypes = [i32, i32]
+    lib.moe_balance_loss_workspace_bytes.restype = sz
+    lib.moe_balance_loss.argtypes = [vp, i32, i32, i32, i32, i32, C.c_float, vp, vp, vp, vp, vp,
+                                     vp, sz, st]
+    lib.moe_router_backward.argtypes = [vp, i32, i32, i32, i32, i32, i32, vp, C.c_float, C.c_float,
+                                        vp, vp, vp, vp, C.c_float, C.c_float, vp, vp, st]
+    lib.moe_unpermute_backward.argtypes = [vp, vp, vp, vp, i32, i32, i32, vp, vp, i32, st]
+    lib.moe_validate_lora.argtypes = [C.POINTER(Lora)]
+    lib.moe_lora_workspace_bytes.argtypes = [C.POINTER(Lora), i32]
+    lib.moe_lora_workspace_bytes.restype = sz
+    lib.moe_lora_apply.argtypes = [C.POINTER(Lora), vp, i32, vp, vp, vp, vp, sz, st]
+    lib.moe_lora_backward_workspace_bytes.argtypes = [C.POINTER(Lora), i32]
+    lib.moe_lora_backward_workspace_bytes.restype = sz
+    lib.moe_lora_backward.argtypes = [C.POINTER(Lora), vp, vp, i32, vp, vp, vp, vp, vp, vp, sz, st]
     lib.moe_st_open.argtypes = [C.c_char_p, C.POINTER(vp)]
     lib.moe_st_close.argtypes = [vp]
     lib.moe_st_close.restype = None
@@ -164,7 +187,9 @@ def load():
                  "moe_layer_forward_residual", "moe_layer_path", "moe_layer_forward_noalloc",
                  "moe_add_rmsnorm", "moe_mxfp4_to_affine",
                  "moe_layer_create", "moe_layer_decode",
-                 "moe_layer_decode_many", "moe_st_open", "moe_st_info", "moe_st_read_host",
+                 "moe_layer_decode_many", "moe_balance_loss", "moe_router_backward",
+                 "moe_unpermute_backward", "moe_validate_lora", "moe_lora_apply",
+                 "moe_lora_backward", "moe_st_open", "moe_st_info", "moe_st_read_host",
                  "moe_st_upload", "moe_st_stacked_bytes", "moe_st_load_stacked",
                  "moe_st_load_stacked_many", "moe_st_mxfp4_bytes", "moe_st_load_mxfp4"]:
         getattr(lib, name).restype = C.c_int

@@ -1119,6 +1119,196 @@ extern "C" moe_status moe_unpermute(const void* Y, const uint32_t* inv_perm,
 }
 
 // ---------------------------------------------------------------------------
+// tuning
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// What moe_balance_loss and moe_router_backward ask of a router's rows.
+moe_status validate_router_rows(const char* name, int dtype, int T, int E, int k, int gating,
+                                float logit_scale, float routed_scale) {
+  if (T <= 0) return fail(MOE_ERR_INVALID, "%s: T must be positive", name);
+  if (E <= 0) return fail(MOE_ERR_INVALID, "%s: nExperts must be positive", name);
+  if (k <= 0 || k > E)
+    return fail(MOE_ERR_INVALID, "%s: topK (%d) must be in 1...nExperts (%d)", name, k, E);
+  if (!gating_ok(gating)) return fail(MOE_ERR_INVALID, "%s: bad gating mode", name);
+  if (!scales_ok(logit_scale, routed_scale))
+    return fail(MOE_ERR_INVALID, "%s: logit/routed scales must be finite", name);
+  if (!dt_ok(dtype)) return fail(MOE_ERR_INVALID, "%s: bad dtype", name);
+  if (E > kMaxExperts)
+    return fail(MOE_ERR_UNSUPPORTED, "%s: nExperts=%d above %d", name, E, kMaxExperts);
+  if (k > 64) return fail(MOE_ERR_UNSUPPORTED, "%s: k=%d above 64", name, k);
+  if ((long)T * k > 0x7fffffffL - 4096) return fail(MOE_ERR_INVALID, "%s: T*k too large", name);
+  return MOE_OK;
+}
+
+// Whether [a, a + na) and [b, b + nb) share a byte.
+bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + nb && y < x + na;
+}
+
+LoraDims lora_dims(const moe_lora* l, int T) {
+  return LoraDims{l->dtype, T, l->k, l->n, l->rank, l->n_adapters};
+}
+
+moe_status validate_lora(const moe_lora* l) {
+  if (!l) return fail(MOE_ERR_INVALID, "lora: descriptor is NULL");
+  if (!l->a || !l->b) return fail(MOE_ERR_INVALID, "lora: a and b must be non-NULL");
+  if (!dt_ok(l->dtype)) return fail(MOE_ERR_INVALID, "lora: bad dtype");
+  if (l->rank <= 0 || l->n <= 0 || l->k <= 0 || l->n_adapters <= 0)
+    return fail(MOE_ERR_INVALID, "lora: rank, n, k and n_adapters must be positive");
+  if (l->rank % 8 || l->n % 8 || l->k % 8)
+    return fail(MOE_ERR_UNSUPPORTED, "lora: rank (%d), n (%d) and k (%d) must be multiples of 8",
+                l->rank, l->n, l->k);
+  if (l->rank > 128) return fail(MOE_ERR_UNSUPPORTED, "lora: rank %d above 128", l->rank);
+  if (l->n > 1 << 20 || l->k > 1 << 20)
+    return fail(MOE_ERR_UNSUPPORTED, "lora: n (%d) and k (%d) at most 2^20", l->n, l->k);
+  if (!aligned16(l->a) || !aligned16(l->b))
+    return fail(MOE_ERR_INVALID, "lora: a and b must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(l->scale) & 3)
+    return fail(MOE_ERR_INVALID, "lora: scale must be 4-byte aligned");
+  return MOE_OK;
+}
+
+}  // namespace
+
+extern "C" size_t moe_balance_loss_workspace_bytes(int32_t T, int32_t n_experts) {
+  if (T <= 0 || n_experts <= 0 || n_experts > kMaxExperts) return 0;
+  return balance_ws_bytes(T, n_experts);
+}
+
+extern "C" moe_status moe_balance_loss(const void* logits, int32_t dtype, int32_t T,
+                                       int32_t n_experts, int32_t k, int32_t gating,
+                                       float logit_scale, const uint32_t* topk_idx,
+                                       const uint8_t* mask, uint32_t* counts, float* prob_sum,
+                                       float* losses, void* workspace, size_t workspace_bytes,
+                                       hipStream_t stream) {
+  if (!logits || !topk_idx || !counts || !prob_sum || !losses)
+    return fail(MOE_ERR_INVALID, "balance_loss: NULL pointer");
+  MOE_TRY(validate_router_rows("balance_loss", dtype, T, n_experts, k, gating, logit_scale, 1.f));
+  const size_t need = balance_ws_bytes(T, n_experts);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(MOE_ERR_WORKSPACE, "balance_loss: workspace of %zu bytes needed", need);
+  MOE_HIP(launch_balance_loss(logits, dtype, T, n_experts, k, gating == MOE_SIGMOID_TOPK,
+                              logit_scale == 0.f ? 1.f : logit_scale, topk_idx, mask, counts,
+                              prob_sum, losses, workspace, stream),
+          "balance loss launch");
+  return ok();
+}
+
+extern "C" moe_status moe_router_backward(const void* logits, int32_t dtype, int32_t T,
+                                          int32_t n_experts, int32_t k, int32_t gating,
+                                          int32_t norm_topk_prob, const float* expert_bias,
+                                          float logit_scale, float routed_scale,
+                                          const float* expert_scale, const uint32_t* topk_idx,
+                                          const float* d_weight, const uint32_t* counts,
+                                          float balance_coef, float z_coef, const uint8_t* mask,
+                                          void* d_logits, hipStream_t stream) {
+  if (!logits || !topk_idx || !d_logits) return fail(MOE_ERR_INVALID, "router_backward: NULL pointer");
+  MOE_TRY(validate_router_rows("router_backward", dtype, T, n_experts, k, gating, logit_scale,
+                               routed_scale));
+  if (!std::isfinite(balance_coef) || !std::isfinite(z_coef))
+    return fail(MOE_ERR_INVALID, "router_backward: coefficients must be finite");
+  if (!counts && (balance_coef != 0.f || z_coef != 0.f))
+    return fail(MOE_ERR_INVALID, "router_backward: the losses' gradients need counts");
+  const size_t bytes = (size_t)T * n_experts * dt_size(dtype);
+  if (overlaps(logits, bytes, d_logits, bytes))
+    return fail(MOE_ERR_INVALID, "router_backward: d_logits overlaps logits");
+  const RouteOpts ro = route_opts(gating, norm_topk_prob, expert_bias, logit_scale, routed_scale,
+                                  expert_scale);
+  MOE_HIP(launch_router_backward(logits, dtype, T, n_experts, k, ro, topk_idx, d_weight,
+                                 balance_coef != 0.f || z_coef != 0.f ? counts : nullptr,
+                                 balance_coef, z_coef, mask, d_logits, stream),
+          "router backward launch");
+  return ok();
+}
+
+extern "C" moe_status moe_unpermute_backward(const void* d_out, const void* Y,
+                                             const uint32_t* inv_perm, const float* topk_weight,
+                                             int32_t T, int32_t hidden, int32_t k, void* dY,
+                                             float* d_weight, int32_t dtype, hipStream_t stream) {
+  if (!d_out || !Y || !inv_perm || !topk_weight || !d_weight)
+    return fail(MOE_ERR_INVALID, "unpermute_backward: NULL pointer");
+  if (T <= 0 || hidden <= 0 || k <= 0)
+    return fail(MOE_ERR_INVALID, "unpermute_backward: T, hidden and k must be positive");
+  if ((long)T * k > 0x7fffffffL) return fail(MOE_ERR_INVALID, "unpermute_backward: T*k too large");
+  if (hidden % 8) return fail(MOE_ERR_UNSUPPORTED, "unpermute_backward: hidden must be a multiple of 8");
+  if (!dt_ok(dtype)) return fail(MOE_ERR_INVALID, "unpermute_backward: bad dtype");
+  if (!aligned16(d_out) || !aligned16(Y) || !aligned16(dY))
+    return fail(MOE_ERR_INVALID, "unpermute_backward: rows must be 16-byte aligned");
+  const size_t row = (size_t)hidden * dt_size(dtype), all = row * T * k;
+  if (overlaps(d_out, row * T, dY, all) || (dY != Y && overlaps(Y, all, dY, all)))
+    return fail(MOE_ERR_INVALID, "unpermute_backward: dY overlaps an input");
+  MOE_HIP(launch_unpermute_backward(d_out, Y, inv_perm, topk_weight, T, hidden, k, dY, d_weight,
+                                    dtype, stream),
+          "unpermute backward launch");
+  return ok();
+}
+
+extern "C" moe_status moe_validate_lora(const moe_lora* l) {
+  MOE_TRY(validate_lora(l));
+  return ok();
+}
+
+extern "C" size_t moe_lora_workspace_bytes(const moe_lora* l, int32_t T) {
+  if (T <= 0 || validate_lora(l) != MOE_OK) return 0;
+  return lora_ws_bytes(lora_dims(l, T));
+}
+
+extern "C" moe_status moe_lora_apply(const moe_lora* l, const void* x, int32_t T,
+                                     const int32_t* adapter, const void* y_in, void* y,
+                                     void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  MOE_TRY(validate_lora(l));
+  if (!x || !adapter || !y) return fail(MOE_ERR_INVALID, "lora_apply: NULL pointer");
+  if (T <= 0) return fail(MOE_ERR_INVALID, "lora_apply: T must be positive");
+  if (!aligned16(x) || !aligned16(y_in) || !aligned16(y))
+    return fail(MOE_ERR_INVALID, "lora_apply: rows must be 16-byte aligned");
+  const LoraDims d = lora_dims(l, T);
+  const size_t xb = (size_t)T * l->k * dt_size(l->dtype), yb = (size_t)T * l->n * dt_size(l->dtype);
+  if (overlaps(x, xb, y, yb)) return fail(MOE_ERR_INVALID, "lora_apply: y overlaps x");
+  if (y_in != y && overlaps(y_in, yb, y, yb))
+    return fail(MOE_ERR_INVALID, "lora_apply: y overlaps y_in (equal or apart)");
+  const size_t need = lora_ws_bytes(d);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return fail(MOE_ERR_WORKSPACE, "lora_apply: 16-byte aligned workspace of %zu bytes needed", need);
+  MOE_HIP(launch_lora(d, x, l->a, l->b, l->scale, adapter, y_in, y, workspace, stream),
+          "adapter launch");
+  return ok();
+}
+
+extern "C" size_t moe_lora_backward_workspace_bytes(const moe_lora* l, int32_t T) {
+  if (T <= 0 || validate_lora(l) != MOE_OK || l->n_adapters > 1024) return 0;
+  return lora_backward_ws_bytes(lora_dims(l, T));
+}
+
+extern "C" moe_status moe_lora_backward(const moe_lora* l, const void* x, const void* dy,
+                                        int32_t T, const int32_t* adapter, const void* dx_in,
+                                        void* dx, void* da, void* db, void* workspace,
+                                        size_t workspace_bytes, hipStream_t stream) {
+  MOE_TRY(validate_lora(l));
+  if (!x || !dy || !adapter) return fail(MOE_ERR_INVALID, "lora_backward: NULL pointer");
+  if (!dx && !da && !db) return fail(MOE_ERR_INVALID, "lora_backward: no gradient asked for");
+  if (dx_in && !dx) return fail(MOE_ERR_INVALID, "lora_backward: dx_in without dx");
+  if (T <= 0) return fail(MOE_ERR_INVALID, "lora_backward: T must be positive");
+  if (l->n_adapters > 1024)
+    return fail(MOE_ERR_UNSUPPORTED, "lora_backward: n_adapters above 1024");
+  for (const void* p : {x, dy, dx_in, (const void*)dx, (const void*)da, (const void*)db})
+    if (!aligned16(p)) return fail(MOE_ERR_INVALID, "lora_backward: buffers must be 16-byte aligned");
+  const LoraDims d = lora_dims(l, T);
+  const size_t es = dt_size(l->dtype);
+  const size_t xb = (size_t)T * l->k * es, yb = (size_t)T * l->n * es;
+  if (overlaps(x, xb, dx, xb) || overlaps(dy, yb, dx, xb) || (dx_in != dx && overlaps(dx_in, xb, dx, xb)))
+    return fail(MOE_ERR_INVALID, "lora_backward: dx overlaps an input (dx_in: equal or apart)");
+  const size_t need = lora_backward_ws_bytes(d);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return fail(MOE_ERR_WORKSPACE, "lora_backward: 16-byte aligned workspace of %zu bytes needed", need);
+  const LoraBackward a{x, dy, l->a, l->b, l->scale, adapter, dx_in, dx, da, db, workspace};
+  MOE_HIP(launch_lora_backward(d, a, stream), "adapter backward launch");
+  return ok();
+}
+
+// ---------------------------------------------------------------------------
 // whole layer
 // ---------------------------------------------------------------------------
 

@@ -4,6 +4,8 @@
 //   unpermute      Ops.moeUnpermute (Sources/FFAI/Ops/Ops.swift:5030-5110) with
 //                  the combine weights rounded to the activation dtype first
 //                  (Sources/FFAI/Models/MoELayer.swift:921-935)
+//   unpermute backward   its gradient: expert rows and combine weights (the
+//                  reference only runs forward)
 //   shared add     MoELayer.swift:620-624 (unconditional add) and
 //                  Ops.sigmoidScalarFMA (Ops.swift:6256-6317; Qwen3xText.swift:
 //                  1054-1103): y = round(routed + sigmoid(g) * shared)
@@ -21,38 +23,6 @@
 #include "moe_internal.hpp"
 
 namespace moe {
-
-template <typename T> struct Vec8 {
-  static __device__ __forceinline__ void load(const T* p, float (&v)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      v[2 * j] = to_f<T>(__builtin_bit_cast(T, (uint16_t)(w[j] & 0xFFFFu)));
-      v[2 * j + 1] = to_f<T>(__builtin_bit_cast(T, (uint16_t)(w[j] >> 16)));
-    }
-  }
-  static __device__ __forceinline__ void store(T* p, const float (&v)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const uint16_t lo = __builtin_bit_cast(uint16_t, from_f<T>(v[2 * j]));
-      const uint16_t hi = __builtin_bit_cast(uint16_t, from_f<T>(v[2 * j + 1]));
-      w[j] = (uint32_t)lo | ((uint32_t)hi << 16);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-template <> struct Vec8<float> {
-  static __device__ __forceinline__ void load(const float* p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  }
-  static __device__ __forceinline__ void store(float* p, const float (&v)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  }
-};
 
 // shared_mode: 0 none, 1 unconditional add, 2 sigmoid-gated add.
 template <typename XT>
@@ -117,6 +87,68 @@ __global__ __launch_bounds__(256) void unpermute_kernel(const XT* __restrict__ Y
       for (int j = 0; j < 8; j++) acc[j] = acc[j] + g * sv[j];
     }
     Vec8<XT>::store(out + (size_t)t * H + h, acc);
+  }
+}
+
+// Gradient of the combine out[t] = sum_s round(w[t,s]) Y[p(t,s)]:
+//   dY[p(t,s)] = round(w[t,s]) g[t],   dw[t,s] = <g[t], Y[p(t,s)]>
+// One block per token. The ranks go in batches of kCombineBatch, whose rows
+// are all in flight together; a thread keeps its share of the batch's dot
+// products over its chunks of the row, and the block adds them along a fixed
+// tree. The gradient row is read once per batch (from cache after the first).
+// Y and dY may be one buffer: a thread reads its values before it stores them
+// and every position belongs to one block. A position past M has a zero dw
+// and no row.
+template <typename XT>
+__global__ __launch_bounds__(256) void unpermute_backward_kernel(const XT* __restrict__ g,
+                                                                 const XT* Y,
+                                                                 const uint32_t* __restrict__ inv,
+                                                                 const float* __restrict__ w,
+                                                                 int T, int H, int k, XT* dY,
+                                                                 float* __restrict__ dw) {
+  __shared__ float part[4][kCombineBatch];
+  const int t = blockIdx.x;
+  const uint32_t M = (uint32_t)T * (uint32_t)k;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int s0 = 0; s0 < k; s0 += kCombineBatch) {
+    uint32_t p[kCombineBatch];
+    float ws[kCombineBatch], dot[kCombineBatch];
+#pragma unroll
+    for (int q = 0; q < kCombineBatch; q++) {
+      const int s = min(s0 + q, k - 1);
+      p[q] = s0 + q < k ? inv[(size_t)t * k + s] : 0xFFFFFFFFu;
+      ws[q] = round_to<XT>(w[(size_t)t * k + s]);
+      dot[q] = 0.f;
+    }
+    for (int h = threadIdx.x * 8; h < H; h += 256 * 8) {
+      float gv[8], y[kCombineBatch][8];
+      Vec8<XT>::load(g + (size_t)t * H + h, gv);
+#pragma unroll
+      for (int q = 0; q < kCombineBatch; q++)
+        if (p[q] < M) Vec8<XT>::load(Y + (size_t)p[q] * H + h, y[q]);
+#pragma unroll
+      for (int q = 0; q < kCombineBatch; q++) {
+        if (p[q] < M) {
+          float o[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            dot[q] = __builtin_fmaf(gv[j], y[q][j], dot[q]);
+            o[j] = ws[q] * gv[j];
+          }
+          if (dY) Vec8<XT>::store(dY + (size_t)p[q] * H + h, o);
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kCombineBatch; q++) {
+      const float d = group_sum(dot[q], 6);
+      if (lane == 63) part[wave][q] = d;
+    }
+    __syncthreads();
+    if (threadIdx.x < kCombineBatch && s0 + (int)threadIdx.x < k)
+      dw[(size_t)t * k + s0 + threadIdx.x] = (part[0][threadIdx.x] + part[1][threadIdx.x]) +
+                                             (part[2][threadIdx.x] + part[3][threadIdx.x]);
+    __syncthreads();
   }
 }
 
@@ -260,6 +292,18 @@ hipError_t launch_unpermute(const void* Y, const uint32_t* inv, const float* w, 
   return hipGetLastError();
   MOE_BY_DT(dt, MOE_UP)
 #undef MOE_UP
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_unpermute_backward(const void* g, const void* Y, const uint32_t* inv,
+                                     const float* w, int T, int H, int k, void* dY, float* dw,
+                                     int dt, hipStream_t st) {
+#define MOE_UB(XT)                                                                            \
+  hipLaunchKernelGGL((unpermute_backward_kernel<XT>), dim3(T), dim3(256), 0, st, (const XT*)g, \
+                     (const XT*)Y, inv, w, T, H, k, (XT*)dY, dw);                             \
+  return hipGetLastError();
+  MOE_BY_DT(dt, MOE_UB)
+#undef MOE_UB
   return hipErrorInvalidValue;
 }
 

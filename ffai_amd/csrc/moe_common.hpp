@@ -29,6 +29,39 @@ template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v
 
 template <typename T> __device__ __forceinline__ float round_to(float v) { return to_f<T>(from_f<T>(v)); }
 
+// Eight consecutive values of a row as fp32, 16-byte aligned (float: 32 bytes).
+template <typename T> struct Vec8 {
+  static __device__ __forceinline__ void load(const T* p, float (&v)[8]) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      v[2 * j] = to_f<T>(__builtin_bit_cast(T, (uint16_t)(w[j] & 0xFFFFu)));
+      v[2 * j + 1] = to_f<T>(__builtin_bit_cast(T, (uint16_t)(w[j] >> 16)));
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint16_t lo = __builtin_bit_cast(uint16_t, from_f<T>(v[2 * j]));
+      const uint16_t hi = __builtin_bit_cast(uint16_t, from_f<T>(v[2 * j + 1]));
+      w[j] = (uint32_t)lo | ((uint32_t)hi << 16);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <> struct Vec8<float> {
+  static __device__ __forceinline__ void load(const float* p, float (&v)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+};
+
 // --------------------------------------------------------- wave reductions --
 __device__ __forceinline__ float wave_sum_width(float v, int width) {
   for (int off = width >> 1; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);

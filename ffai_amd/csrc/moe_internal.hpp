@@ -211,6 +211,11 @@ hipError_t launch_unpermute(const void* Y, const uint32_t* inv, const float* w, 
                             int k, void* out, int dt, const void* shared_out,
                             const void* shared_logit, int shared_mode, hipStream_t st,
                             const void* res = nullptr);
+// Gradient of launch_unpermute without the shared expert and the residual:
+// dY rows (nullable; may be Y) and dw.
+hipError_t launch_unpermute_backward(const void* g, const void* Y, const uint32_t* inv,
+                                     const float* w, int T, int H, int k, void* dY, float* dw,
+                                     int dt, hipStream_t st);
 hipError_t launch_add_shared(void* y, const void* shared_out, const void* shared_logit,
                              int shared_mode, int T, int H, int dt, hipStream_t st,
                              const void* res = nullptr);
@@ -288,5 +293,39 @@ hipError_t launch_gemm(int bits, int xdt, int sbdt, bool gateup, const GemmArgs&
 // Elementwise bf16 -> f16 * 2^-kA16Shift (saturating), n a multiple of 8,
 // 16-byte aligned buffers.
 hipError_t launch_to_a16(const void* x, void* y, int64_t n, hipStream_t st);
+
+// --------------------------------------------------------------- tuning --
+// Router losses and the gradient of the router's logits (router_grad.hip);
+// E at most 512.
+size_t balance_ws_bytes(int T, int E);
+hipError_t launch_balance_loss(const void* logits, int dt, int T, int E, int k, bool sigmoid,
+                               float ls, const uint32_t* idx, const uint8_t* mask,
+                               uint32_t* counts, float* prob_sum, float* losses, void* ws,
+                               hipStream_t st);
+hipError_t launch_router_backward(const void* logits, int dt, int T, int E, int k,
+                                  const RouteOpts& ro, const uint32_t* idx, const float* dw,
+                                  const uint32_t* counts, float bal, float z, const uint8_t* mask,
+                                  void* out, hipStream_t st);
+
+// Low-rank adapters (lora.hip): T rows, K inputs, N outputs, rank R, G
+// adapters. K, N and R are multiples of 8, R at most 128.
+struct LoraDims {
+  int dt, T, K, N, R, G;
+};
+struct LoraBackward {
+  const void *x, *dy, *a, *b;
+  const float* scale;
+  const int32_t* adapter;
+  const void* dx_in;
+  void *dx, *da, *db;  // each nullable
+  void* ws;
+};
+int lora_shares(int T, int G, int K, int dt);
+size_t lora_ws_bytes(const LoraDims& d);
+size_t lora_backward_ws_bytes(const LoraDims& d);
+hipError_t launch_lora(const LoraDims& d, const void* x, const void* a, const void* b,
+                       const float* scale, const int32_t* adapter, const void* yin, void* y,
+                       void* ws, hipStream_t st);
+hipError_t launch_lora_backward(const LoraDims& d, const LoraBackward& a, hipStream_t st);
 
 }  // namespace moe

@@ -1,0 +1,662 @@
+// router_grad.hip — the router's losses and the gradient of its logits for
+// gfx950.
+//
+//   balance loss  per-expert counts c_e of the picks, P_e = sum_t p_te over
+//                 the counted rows, balance = E sum_e c_e / (k N) P_e / N and
+//                 z = sum_t lse(s_t)^2 / N, s = logit_scale * logits
+//   backward      d logits of both losses and of the routing weights, every
+//                 element written once
+//
+// No counterpart in the reference, which only runs forward; the rules that
+// are differentiated are MoERouter.route's (MoELayer.swift:140-205) and the
+// NemotronH sigmoid router's (NemotronHText.swift:838-868).
+//
+// Both kernels read a row's logits once: a lane holds 8 neighbouring experts
+// (16 bytes of a 16-bit row), 2^lg = ceil(E / 8) lanes hold a row and a wave
+// 64 / 2^lg rows, so that the row's maximum and sums take lg steps for all of
+// a wave's rows together. Sums stay in fp32 along a fixed tree; only integer
+// atomics are used on shared counts, so results do not depend on the order
+// of blocks or waves.
+#include <algorithm>
+
+#include "moe_common.hpp"
+#include "moe_internal.hpp"
+
+namespace moe {
+
+namespace {
+
+constexpr int kCols = 8;  // experts per lane
+
+// Eight logits of a row as fp32, `pad` past E. vec: E % 8 == 0 and 16-byte
+// aligned rows.
+template <typename XT>
+__device__ __forceinline__ void load_cols(const XT* __restrict__ row, int c0, int E, bool vec,
+                                          float pad, float (&v)[kCols]) {
+  if (vec) {
+#pragma unroll
+    for (int j = 0; j < kCols; j++) v[j] = pad;
+    if (c0 < E) Vec8<XT>::load(row + c0, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kCols; j++) {
+      const float x = to_f<XT>(row[min(c0 + j, E - 1)]);
+      v[j] = c0 + j < E ? x : pad;
+    }
+  }
+}
+
+template <typename XT>
+__device__ __forceinline__ void store_cols(XT* __restrict__ row, int c0, int E, bool vec,
+                                           const float (&v)[kCols]) {
+  if (vec) {
+    if (c0 < E) Vec8<XT>::store(row + c0, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kCols; j++)
+      if (c0 + j < E) row[c0 + j] = from_f<XT>(v[j]);
+  }
+}
+
+// Sum / maximum over each aligned group of 2^LG lanes, in every lane of it.
+template <int LG> __device__ __forceinline__ float row_sum(float v) {
+  if constexpr (LG >= 1) v += dpp_f32<0xB1, 0xF>(0.f, v);
+  if constexpr (LG >= 2) v += dpp_f32<0x4E, 0xF>(0.f, v);
+  if constexpr (LG >= 3) v += dpp_f32<0x141, 0xF>(0.f, v);
+  if constexpr (LG >= 4) v += dpp_f32<0x140, 0xF>(0.f, v);
+  if constexpr (LG >= 5) v += __shfl_xor(v, 16, kWave);
+  if constexpr (LG >= 6) v += __shfl_xor(v, 32, kWave);
+  return v;
+}
+template <int LG> __device__ __forceinline__ float row_max(float v) {
+  if constexpr (LG >= 1) v = fmaxf(v, dpp_f32<0xB1, 0xF>(v, v));
+  if constexpr (LG >= 2) v = fmaxf(v, dpp_f32<0x4E, 0xF>(v, v));
+  if constexpr (LG >= 3) v = fmaxf(v, dpp_f32<0x141, 0xF>(v, v));
+  if constexpr (LG >= 4) v = fmaxf(v, dpp_f32<0x140, 0xF>(v, v));
+  if constexpr (LG >= 5) v = fmaxf(v, __shfl_xor(v, 16, kWave));
+  if constexpr (LG >= 6) v = fmaxf(v, __shfl_xor(v, 32, kWave));
+  return v;
+}
+
+// exp(x) to about 1.5 ulp: 2^t with t = x log2(e) in fp32 and the product's
+// rounding error put back as a first-order factor (e^(d) = 1 + d). The clamp
+// keeps infinities out of the correction (2^+-288 already is inf / 0); NaN
+// passes the comparisons and stays.
+__device__ __forceinline__ float exp_acc(float x) {
+  x = x < -200.f ? -200.f : x;
+  x = x > 200.f ? 200.f : x;
+  constexpr float L = 1.44269502162933349609375f;      // log2(e) rounded to fp32
+  constexpr float Llo = 1.925963033500011e-8f;         // log2(e) - L
+  const float t = x * L;
+  float d = __builtin_fmaf(x, L, -t);
+  d = __builtin_fmaf(x, Llo, d);
+  const float y = __builtin_amdgcn_exp2f(t);
+  const float c = d * 0.693147180559945f;
+  return y > 1e38f ? y : __builtin_fmaf(y, c, y);  // inf * 0 would be NaN
+}
+
+// Row statistics of 2^LG lanes: e_j = exp(s_j - m), 1 / sum e and lse. A row
+// of -inf only has e = 0, inv = 0 and lse = 0 (no probability, no loss);
+// NaN or +inf in a row makes all of it NaN.
+struct RowStat {
+  float m, inv, lse;
+};
+template <int LG>
+__device__ __forceinline__ RowStat row_softmax(const float (&s)[kCols], float (&e)[kCols]) {
+  float m = s[0];
+#pragma unroll
+  for (int j = 1; j < kCols; j++) m = fmaxf(m, s[j]);
+  m = row_max<LG>(m);
+  if (m == -__builtin_huge_valf()) m = 0.f;
+  float z = 0.f;
+#pragma unroll
+  for (int j = 0; j < kCols; j++) {
+    e[j] = exp_acc(s[j] - m);
+    z += e[j];
+  }
+  z = row_sum<LG>(z);
+  RowStat r;
+  r.m = m;
+  r.inv = z == 0.f ? 0.f : 1.0f / z;
+  r.lse = z == 0.f ? 0.f : m + logf(z);
+  return r;
+}
+
+__device__ __forceinline__ float sigmoid_acc(float s) { return 1.0f / (1.0f + exp_acc(-s)); }
+
+}  // namespace
+
+// ---------------------------------------------------------- balance loss --
+constexpr int kBalWaves = 4;
+
+// Sums over one launch's blocks (or one block's rows): the losses of `n`
+// counted rows. col: this thread's P and count summed over e by the caller.
+__device__ __forceinline__ void store_losses(double dot, double zsum, uint32_t n, int E, int k,
+                                             float* losses) {
+  const double dn = n ? (double)n : 1.0;
+  losses[0] = (float)(dot * (double)E / (dn * dn * (double)k));
+  losses[1] = (float)(zsum / dn);
+}
+
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+
+// Partials of block b: P [E] fp32, picks [E] u32, then z and the counted rows.
+struct BalancePart {
+  float* P;
+  uint32_t* cnt;
+  float* z;
+  uint32_t* n;
+};
+__host__ __device__ inline BalancePart balance_part(void* ws, int nb, int E) {
+  BalancePart p;
+  p.P = reinterpret_cast<float*>(ws);
+  p.cnt = reinterpret_cast<uint32_t*>(p.P + (size_t)nb * E);
+  p.z = reinterpret_cast<float*>(p.cnt + (size_t)nb * E);
+  p.n = reinterpret_cast<uint32_t*>(p.z + nb);
+  return p;
+}
+static size_t balance_part_bytes(int nb, int E) { return (size_t)nb * (E + 1) * 8; }
+
+// Block b takes rows [b rpb, (b + 1) rpb). A lane keeps the probability sums
+// of its 8 experts in registers over its rows; the waves' rows and the picks'
+// counts meet in LDS.
+template <typename XT, int LG>
+__global__ __launch_bounds__(256) void balance_rows_kernel(
+    const XT* __restrict__ logits, const uint32_t* __restrict__ idx,
+    const uint8_t* __restrict__ mask, int T, int E, int k, int rpb, float ls, int sigmoid, int vec,
+    void* ws, uint32_t* __restrict__ counts, float* __restrict__ prob_sum,
+    float* __restrict__ losses) {
+  __shared__ float sP[kBalWaves][kTopkMaxE];
+  __shared__ uint32_t sCnt[kTopkMaxE];
+  __shared__ float sZ[kBalWaves];
+  __shared__ uint32_t sN[kBalWaves];
+  __shared__ double sDot[kBalWaves];
+  constexpr int LPR = 1 << LG, RPW = kWave >> LG;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int c0 = (lane & (LPR - 1)) * kCols;
+  for (int e = tid; e < E; e += 256) sCnt[e] = 0u;
+  __syncthreads();
+  const int r0 = blockIdx.x * rpb, r1 = min(T, r0 + rpb);
+  // picks of the block's rows
+  {
+    const size_t i0 = (size_t)r0 * k;
+    const int ne = (r1 - r0) * k;
+    for (int i = tid; i < ne; i += 256) {
+      const uint32_t e = idx[i0 + i];
+      const bool on = mask == nullptr || mask[r0 + i / k] != 0;
+      if (on && e < (uint32_t)E) atomicAdd(&sCnt[e], 1u);
+    }
+  }
+  float P[kCols];
+#pragma unroll
+  for (int j = 0; j < kCols; j++) P[j] = 0.f;
+  float zs = 0.f;
+  uint32_t n = 0;
+  const float NEG = -__builtin_huge_valf();
+  for (int rb = r0 + wave * RPW; rb < r1; rb += kBalWaves * RPW) {
+    const int r = rb + (lane >> LG);
+    const bool in = r < r1;
+    const bool on = in && (mask == nullptr || mask[r] != 0);
+    float s[kCols], e[kCols];
+    load_cols<XT>(logits + (size_t)(in ? r : r1 - 1) * E, c0, E, vec, NEG, s);
+#pragma unroll
+    for (int j = 0; j < kCols; j++) s[j] = c0 + j < E ? s[j] * ls : NEG;
+    const RowStat st = row_softmax<LG>(s, e);
+    float inv = st.inv;
+    if (sigmoid) {
+      float z = 0.f;
+#pragma unroll
+      for (int j = 0; j < kCols; j++) {
+        e[j] = sigmoid_acc(s[j]);
+        z += e[j];
+      }
+      z = row_sum<LG>(z);
+      inv = z == 0.f ? 0.f : 1.0f / z;
+    }
+    if (on) {
+#pragma unroll
+      for (int j = 0; j < kCols; j++) P[j] = __builtin_fmaf(e[j], inv, P[j]);
+      if (c0 == 0) {
+        zs = __builtin_fmaf(st.lse, st.lse, zs);
+        n++;
+      }
+    }
+  }
+  // rows of the wave, then the block's waves
+#pragma unroll
+  for (int off = LPR; off < kWave; off <<= 1) {
+#pragma unroll
+    for (int j = 0; j < kCols; j++) P[j] += __shfl_xor(P[j], off, kWave);
+    zs += __shfl_xor(zs, off, kWave);
+    n += (uint32_t)__shfl_xor((int)n, off, kWave);
+  }
+  if (lane < LPR) {
+#pragma unroll
+    for (int j = 0; j < kCols; j++)
+      if (c0 + j < E) sP[wave][c0 + j] = P[j];
+  }
+  if (lane == 0) {
+    sZ[wave] = zs;
+    sN[wave] = n;
+  }
+  __syncthreads();
+  float z = 0.f;
+  uint32_t nn = 0;
+#pragma unroll
+  for (int w = 0; w < kBalWaves; w++) {
+    z += sZ[w];
+    nn += sN[w];
+  }
+  if (gridDim.x == 1) {
+    // the only block has everything: the losses without a second launch
+    double dot = 0.0;
+    for (int e = tid; e < E; e += 256) {
+      const float p = (sP[0][e] + sP[1][e]) + (sP[2][e] + sP[3][e]);
+      prob_sum[e] = p;
+      counts[e] = sCnt[e];
+      dot += (double)p * (double)sCnt[e];
+    }
+    dot = wave_sum_f64(dot);
+    if (lane == 0) sDot[wave] = dot;
+    __syncthreads();
+    if (tid == 0) {
+      counts[E] = nn;
+      store_losses((sDot[0] + sDot[1]) + (sDot[2] + sDot[3]), (double)z, nn, E, k, losses);
+    }
+    return;
+  }
+  const BalancePart bp = balance_part(ws, gridDim.x, E);
+  for (int e = tid; e < E; e += 256) {
+    bp.P[(size_t)blockIdx.x * E + e] = (sP[0][e] + sP[1][e]) + (sP[2][e] + sP[3][e]);
+    bp.cnt[(size_t)blockIdx.x * E + e] = sCnt[e];
+  }
+  if (tid == 0) {
+    bp.z[blockIdx.x] = z;
+    bp.n[blockIdx.x] = nn;
+  }
+}
+
+// Adds the blocks' partials and forms the losses: one workgroup, 2^lgc >= E
+// lanes across the experts, the rest of the threads across the blocks.
+__global__ __launch_bounds__(1024) void balance_final_kernel(void* ws, int nb, int E, int k, int lgc,
+                                                             uint32_t* __restrict__ counts,
+                                                             float* __restrict__ prob_sum,
+                                                             float* __restrict__ losses) {
+  __shared__ double sP[1024];
+  __shared__ uint32_t sC[1024];
+  __shared__ double sDot[16], sZ[16];
+  __shared__ uint32_t sN[16];
+  const BalancePart bp = balance_part(ws, nb, E);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int e = tid & ((1 << lgc) - 1), sl = tid >> lgc, ns = 1024 >> lgc;
+  double p = 0.0, z = 0.0;
+  uint32_t c = 0, n = 0;
+  if (e < E) {
+#pragma unroll 8
+    for (int b = sl; b < nb; b += ns) {
+      p += (double)bp.P[(size_t)b * E + e];
+      c += bp.cnt[(size_t)b * E + e];
+    }
+  }
+  if (tid < nb) {  // at most 1024 blocks
+    z = (double)bp.z[tid];
+    n = bp.n[tid];
+  }
+  sP[tid] = p;
+  sC[tid] = c;
+  __syncthreads();
+  double dot = 0.0;
+  if (sl == 0 && e < E) {
+    for (int q = 1; q < ns; q++) {
+      p += sP[(q << lgc) + e];
+      c += sC[(q << lgc) + e];
+    }
+    prob_sum[e] = (float)p;
+    counts[e] = c;
+    dot = p * (double)c;
+  }
+  dot = wave_sum_f64(dot);
+  z = wave_sum_f64(z);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) n += (uint32_t)__shfl_xor((int)n, off, kWave);
+  if (lane == 0) {
+    sDot[wave] = dot;
+    sZ[wave] = z;
+    sN[wave] = n;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    double d = 0.0, zz = 0.0;
+    uint32_t nn = 0;
+    for (int w = 0; w < 16; w++) {
+      d += sDot[w];
+      zz += sZ[w];
+      nn += sN[w];
+    }
+    counts[E] = nn;
+    store_losses(d, zz, nn, E, k, losses);
+  }
+}
+
+namespace {
+
+int lanes_lg(int E) {
+  int lg = 0;
+  while ((kCols << lg) < E) lg++;
+  return lg;
+}
+
+// Blocks of a balance pass: one for a few rows (one launch), otherwise up to
+// 256 (one per CU, so that the second launch has few partials to add) of at
+// least a row per wave slot.
+int balance_blocks(int T, int E) {
+  const int rows = kBalWaves * (kWave >> lanes_lg(E));  // a block's rows in flight
+  if (T <= 2 * rows) return 1;
+  return (int)std::min<long>(256, (T + rows - 1) / rows);
+}
+
+}  // namespace
+
+size_t balance_ws_bytes(int T, int E) {
+  const int nb = balance_blocks(T, E);
+  return nb == 1 ? 0 : balance_part_bytes(nb, E);
+}
+
+#define MOE_LG(lg, MACRO) \
+  switch (lg) {           \
+    case 0: MACRO(0)      \
+    case 1: MACRO(1)      \
+    case 2: MACRO(2)      \
+    case 3: MACRO(3)      \
+    case 4: MACRO(4)      \
+    case 5: MACRO(5)      \
+    case 6: MACRO(6)      \
+  }
+
+template <typename XT>
+static hipError_t balance_typed(const void* logits, int T, int E, int k, bool sigmoid, float ls,
+                                const uint32_t* idx, const uint8_t* mask, uint32_t* counts,
+                                float* prob_sum, float* losses, void* ws, hipStream_t st) {
+  int nb = balance_blocks(T, E);
+  const int rpb = (T + nb - 1) / nb;
+  nb = (T + rpb - 1) / rpb;
+  const int vec = E % kCols == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
+#define MOE_BL(LG)                                                                               \
+  hipLaunchKernelGGL((balance_rows_kernel<XT, LG>), dim3(nb), dim3(256), 0, st,                  \
+                     (const XT*)logits, idx, mask, T, E, k, rpb, ls, (int)sigmoid, vec, ws,      \
+                     counts, prob_sum, losses);                                                  \
+  break;
+  MOE_LG(lanes_lg(E), MOE_BL)
+#undef MOE_BL
+  if (nb > 1) {
+    int lgc = 0;
+    while ((1 << lgc) < E) lgc++;
+    hipLaunchKernelGGL(balance_final_kernel, dim3(1), dim3(1024), 0, st, ws, nb, E, k, lgc, counts,
+                       prob_sum, losses);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_balance_loss(const void* logits, int dt, int T, int E, int k, bool sigmoid,
+                               float ls, const uint32_t* idx, const uint8_t* mask,
+                               uint32_t* counts, float* prob_sum, float* losses, void* ws,
+                               hipStream_t st) {
+  if (E > kTopkMaxE) return hipErrorInvalidValue;
+  if (dt == DT_BF16)
+    return balance_typed<bf16_t>(logits, T, E, k, sigmoid, ls, idx, mask, counts, prob_sum, losses, ws, st);
+  if (dt == DT_F16)
+    return balance_typed<f16_t>(logits, T, E, k, sigmoid, ls, idx, mask, counts, prob_sum, losses, ws, st);
+  return balance_typed<float>(logits, T, E, k, sigmoid, ls, idx, mask, counts, prob_sum, losses, ws, st);
+}
+
+// -------------------------------------------------------------- backward --
+// d logits, with s = ls * logits, p / q the row's softmax / normalised
+// sigmoids, f_e = balance_coef E c_e / (k N^2):
+//   balance, softmax    p_j (f_j - sum f p)
+//   balance, sigmoid    q_j (1 - sigmoid(s_j)) (f_j - sum f q)
+//   z                   z_coef 2 / N lse p_j
+//   weights             g_r = d_weight_r routed_scale escale[e_r] of the picks:
+//     softmax over the picks  w_r (g_r - sum g w)
+//     full softmax (+ bias)   d p_r = g_r, or (g_r - sum g v / S) / S of the
+//                             renormalised v_r = p_r + ebias, S = sum v; then
+//                             p_j (dp_j - sum dp p)
+//     sigmoid                 (the same with v = sigmoid, S = sum v + 1e-20)
+//                             times v (1 - v)
+// all times ls. The picks' values are added into a row image in LDS, from
+// which every lane takes its 8 experts (an id that appears twice adds twice).
+// Rows whose mask is 0 get zeros whatever they hold.
+enum { kPickSoftmax = 0, kFullSoftmax = 1, kSigmoid = 2 };
+
+struct RouterGradArgs {
+  const void* logits;
+  const uint32_t* idx;
+  const float* dw;         // nullable [T, k]
+  const uint32_t* counts;  // nullable [E + 1]
+  const uint8_t* mask;     // nullable [T]
+  const float* ebias;      // nullable [E]
+  const float* escale;     // nullable [E]
+  void* out;
+  int T, E, k, mode, sigmoid, norm, vec;
+  float ls, rs, bal, z;
+};
+
+template <typename XT, int LG>
+__global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) {
+  constexpr int LPR = 1 << LG, RPW = kWave >> LG;
+  __shared__ __attribute__((aligned(16))) float img[4][kWave * kCols];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int rl = lane & (LPR - 1), c0 = rl * kCols, E = a.E, k = a.k;
+  float* im = &img[wave][(lane >> LG) * (LPR * kCols)];  // this row's image
+  const float NEG = -__builtin_huge_valf();
+  float f[kCols];
+  float zc = 0.f;
+#pragma unroll
+  for (int j = 0; j < kCols; j++) f[j] = 0.f;
+  if (a.counts) {
+    const uint32_t n = a.counts[E];
+    const float fn = n ? (float)n : 1.0f;
+    const float fs = a.bal * (float)E / ((float)k * fn) / fn;
+    zc = a.z * 2.0f / fn;
+#pragma unroll
+    for (int j = 0; j < kCols; j++)
+      if (c0 + j < E) f[j] = fs * (float)a.counts[c0 + j];
+  }
+  const XT* __restrict__ logits = reinterpret_cast<const XT*>(a.logits);
+  XT* __restrict__ out = reinterpret_cast<XT*>(a.out);
+  for (long rb = ((long)blockIdx.x * 4 + wave) * RPW; rb < a.T; rb += (long)gridDim.x * 4 * RPW) {
+    const long r = rb + (lane >> LG);
+    const bool in = r < a.T;
+    const size_t rr = (size_t)(in ? r : a.T - 1);
+    const bool on = in && (a.mask == nullptr || a.mask[rr] != 0);
+    const XT* __restrict__ row = logits + rr * E;
+    float s[kCols], p[kCols];
+    load_cols<XT>(row, c0, E, a.vec, NEG, s);
+#pragma unroll
+    for (int j = 0; j < kCols; j++) s[j] = c0 + j < E ? s[j] * a.ls : NEG;
+    const RowStat st = row_softmax<LG>(s, p);
+#pragma unroll
+    for (int j = 0; j < kCols; j++) p[j] *= st.inv;
+    // the losses: d_j and the row sum it is centred by
+    float d[kCols];
+    const float zl = zc * st.lse;
+    if (a.sigmoid) {
+      float q[kCols], sg[kCols], S = 0.f;
+#pragma unroll
+      for (int j = 0; j < kCols; j++) {
+        sg[j] = sigmoid_acc(s[j]);
+        S += sg[j];
+      }
+      S = row_sum<LG>(S);
+      const float inv = S == 0.f ? 0.f : 1.0f / S;
+      float c = 0.f;
+#pragma unroll
+      for (int j = 0; j < kCols; j++) {
+        q[j] = sg[j] * inv;
+        c = __builtin_fmaf(q[j], f[j], c);
+      }
+      c = row_sum<LG>(c);
+#pragma unroll
+      for (int j = 0; j < kCols; j++) d[j] = q[j] * (1.0f - sg[j]) * (f[j] - c) + zl * p[j];
+    } else {
+      float c = 0.f;
+#pragma unroll
+      for (int j = 0; j < kCols; j++) c = __builtin_fmaf(p[j], f[j], c);
+      c = row_sum<LG>(c);
+#pragma unroll
+      for (int j = 0; j < kCols; j++) d[j] = p[j] * (f[j] - c + zl);
+    }
+    if (a.dw) {
+      // zero image
+#pragma unroll
+      for (int j = 0; j < kCols; j += 4)
+        *reinterpret_cast<float4*>(im + c0 + j) = make_float4(0.f, 0.f, 0.f, 0.f);
+      wave_sync();
+      // picks rl, rl + LPR, ... of the row (at most 8 a lane: k <= E)
+      float v[kCols], g[kCols];
+      uint32_t pe[kCols];
+      float mx = NEG;
+#pragma unroll
+      for (int i = 0; i < kCols; i++) {
+        v[i] = NEG;
+        g[i] = 0.f;
+        pe[i] = 0xFFFFFFFFu;
+        if (i * LPR < k) {
+          const int q = rl + i * LPR;
+          if (q < k) {
+            const uint32_t e = a.idx[rr * k + q];
+            if (e < (uint32_t)E) {
+              pe[i] = e;
+              v[i] = to_f<XT>(row[e]) * a.ls;
+              g[i] = a.dw[rr * k + q] * a.rs * (a.escale ? a.escale[e] : 1.0f);
+            }
+          }
+          mx = fmaxf(mx, v[i]);
+        }
+      }
+      float S = 0.f, G = 0.f;  // sum of the weights before renormalising, sum g v
+      if (a.mode == kPickSoftmax) {
+        mx = row_max<LG>(mx);
+        if (mx == NEG) mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < kCols; i++)
+          if (i * LPR < k) {
+            v[i] = exp_acc(v[i] - mx);
+            S += v[i];
+            G = __builtin_fmaf(g[i], v[i], G);
+          }
+        S = row_sum<LG>(S);
+        G = row_sum<LG>(G);
+        const float inv = S == 0.f ? 0.f : 1.0f / S;
+        G *= inv;
+#pragma unroll
+        for (int i = 0; i < kCols; i++)
+          if (i * LPR < k) g[i] = v[i] * inv * (g[i] - G);
+      } else {
+        float pv[kCols];  // p of the pick (full softmax) or sigmoid' (sigmoid)
+#pragma unroll
+        for (int i = 0; i < kCols; i++) {
+          pv[i] = 0.f;
+          if (i * LPR < k) {
+            if (a.mode == kSigmoid) {
+              v[i] = sigmoid_acc(v[i]);
+              pv[i] = v[i] * (1.0f - v[i]);
+            } else {
+              v[i] = exp_acc(v[i] - st.m) * st.inv;
+              pv[i] = v[i];
+              if (a.ebias && pe[i] != 0xFFFFFFFFu) v[i] += a.ebias[pe[i]];
+            }
+            S += v[i];
+            G = __builtin_fmaf(g[i], v[i], G);
+          }
+        }
+        S = row_sum<LG>(S);
+        G = row_sum<LG>(G);
+        const bool renorm = a.norm && (a.mode == kSigmoid ? k > 1 : S > 0.f);
+        const float inv = renorm ? 1.0f / (a.mode == kSigmoid ? S + 1e-20f : S) : 1.0f;
+        const float Gn = renorm ? G * inv : 0.f;
+        float c = 0.f;
+#pragma unroll
+        for (int i = 0; i < kCols; i++)
+          if (i * LPR < k) {
+            g[i] = (g[i] - Gn) * inv;
+            if (a.mode == kSigmoid) g[i] *= pv[i];
+            else c = __builtin_fmaf(g[i], pv[i], c);
+          }
+        if (a.mode == kFullSoftmax) {
+          c = row_sum<LG>(c);
+#pragma unroll
+          for (int j = 0; j < kCols; j++) d[j] = __builtin_fmaf(-p[j], c, d[j]);
+#pragma unroll
+          for (int i = 0; i < kCols; i++) g[i] *= pv[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kCols; i++)
+        if (i * LPR < k && pe[i] != 0xFFFFFFFFu) unsafeAtomicAdd(im + pe[i], g[i]);
+      wave_sync();
+#pragma unroll
+      for (int j = 0; j < kCols; j += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(im + c0 + j);
+        d[j] += t.x; d[j + 1] += t.y; d[j + 2] += t.z; d[j + 3] += t.w;
+      }
+      wave_sync();
+    }
+#pragma unroll
+    for (int j = 0; j < kCols; j++) d[j] = on ? d[j] * a.ls : 0.f;
+    if (in) store_cols<XT>(out + rr * E, c0, E, a.vec, d);
+  }
+}
+
+hipError_t launch_router_backward(const void* logits, int dt, int T, int E, int k,
+                                  const RouteOpts& ro, const uint32_t* idx, const float* dw,
+                                  const uint32_t* counts, float bal, float z, const uint8_t* mask,
+                                  void* out, hipStream_t st) {
+  if (E > kTopkMaxE) return hipErrorInvalidValue;
+  RouterGradArgs a{};
+  a.logits = logits;
+  a.idx = idx;
+  a.dw = dw;
+  a.counts = counts;
+  a.mask = mask;
+  a.ebias = ro.ebias;
+  a.escale = ro.escale;
+  a.out = out;
+  a.T = T;
+  a.E = E;
+  a.k = k;
+  a.sigmoid = ro.gating == 2;
+  a.norm = ro.norm;
+  // as wave_topk forms the weights: softmax over the picks for top-k then
+  // softmax and for a renormalised softmax without a bias
+  a.mode = ro.gating == 2 ? kSigmoid
+           : (ro.gating == 1 || (ro.norm && ro.ebias == nullptr)) ? kPickSoftmax : kFullSoftmax;
+  a.vec = E % kCols == 0 &&
+          ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  a.ls = ro.logit_scale;
+  a.rs = ro.routed_scale;
+  a.bal = bal;
+  a.z = z;
+  const int lg = lanes_lg(E);
+  const int rows = 4 * (kWave >> lg);
+  const int grid = (int)std::min<long>(2048, ((long)T + rows - 1) / rows);
+#define MOE_RB2(XT, LG)                                                                     \
+  hipLaunchKernelGGL((router_backward_kernel<XT, LG>), dim3(grid), dim3(256), 0, st, a);    \
+  break;
+#define MOE_RB_B(LG) MOE_RB2(bf16_t, LG)
+#define MOE_RB_H(LG) MOE_RB2(f16_t, LG)
+#define MOE_RB_F(LG) MOE_RB2(float, LG)
+  if (dt == DT_BF16) { MOE_LG(lg, MOE_RB_B) }
+  else if (dt == DT_F16) { MOE_LG(lg, MOE_RB_H) }
+  else { MOE_LG(lg, MOE_RB_F) }
+#undef MOE_RB_B
+#undef MOE_RB_H
+#undef MOE_RB_F
+#undef MOE_RB2
+  return hipGetLastError();
+}
+
+}  // namespace moe

@@ -1,0 +1,247 @@
+"""Tuning a router and low-rank adapters beside frozen experts, and serving
+many adapters at once, over PyTorch device buffers through the C ABI.
+
+    counts and losses   b = balance_loss(router, logits, topk_idx, mask=mask)
+    combine             dY, dw = unpermute_backward(d_out, Y, inv_perm, topk_weight)
+    router              dl = router_backward(router, logits, topk_idx, d_weight=dw,
+                                             counts=b.counts, balance_coef=.01, mask=mask)
+    adapters            y = LoRAAdapters(a, b, scale).apply(x, adapter, y)
+                        dx, da, db = adapters.backward(x, dy, adapter, dx=dx)
+
+Gradients are plain results, not recorded by autograd. Every function takes
+contiguous tensors of one device, checks them before any launch, and runs on
+`stream` (default: that device's current stream), on which its results and its
+workspace are allocated: a result used on another stream has to be waited for
+there, and all calls can be captured into a graph. PyTorch only provides
+memory and streams; every computation is a libmoehip.so kernel.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from ._lib import Lora, check
+from .layer import MoERouter, moe_dtype
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _check(name: str, t: Optional[torch.Tensor], shape, dtypes, device) -> Optional[int]:
+    """The address of a tensor the kernels read or write through a raw pointer
+    (None for None)."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} dtype {t.dtype} is not {' or '.join(str(d) for d in dtypes)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+class _on:
+    """The device and stream a call runs on: `stream`, or the current stream of
+    the tensors' device, which need not be the current device."""
+    __slots__ = ("_ctx", "handle")
+
+    def __init__(self, device: torch.device, stream):
+        if device.type != "cuda":
+            raise ValueError(f"tensors must be on a GPU, not on {device}")
+        self._ctx = None
+        if stream is not None:
+            if stream.device != device:
+                raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
+            self._ctx = torch.cuda.stream(stream)
+        elif device.index != torch.cuda.current_device():
+            self._ctx = torch.cuda.device(device)
+        s = torch.cuda.current_stream(device) if stream is None else stream
+        self.handle = C.c_void_p(s.cuda_stream)
+
+    def __enter__(self):
+        if self._ctx is not None:
+            self._ctx.__enter__()
+        return self.handle
+
+    def __exit__(self, *exc):
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
+
+
+def _rows(name: str, t, dims: int) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        raise ValueError(f"{name} must be a tensor of {dims} dimensions")
+    if t.dtype not in _FLOATS:
+        raise ValueError(f"{name} dtype {t.dtype} is not a float32, float16 or bfloat16")
+    if t.shape[0] <= 0:
+        raise ValueError(f"{name} must have rows")
+    return t
+
+
+_MASK = (torch.bool, torch.uint8)
+
+
+def _bias(router: MoERouter, t, name, device):
+    return _check(f"router.{name}", t, (router.nExperts,), (torch.float32,), device)
+
+
+class BalanceLoss(NamedTuple):
+    """counts [E + 1] int32 (the last: counted rows), prob_sum [E] float32,
+    losses [2] float32 (balance, z), as moe_balance_loss defines them."""
+    counts: torch.Tensor
+    prob_sum: torch.Tensor
+    losses: torch.Tensor
+
+
+def balance_loss(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Tensor,
+                 mask: Optional[torch.Tensor] = None, stream=None) -> BalanceLoss:
+    """Per-expert counts, probability sums and the balance and z losses of
+    logits [T, E] and their picks topk_idx [T, k] int32, over the rows where
+    mask [T] (bool or uint8) is true."""
+    T, E, k = _rows("logits", logits, 2).shape[0], router.nExperts, router.topK
+    dev = logits.device
+    lp = _check("logits", logits, (T, E), _FLOATS, dev)
+    ip = _check("topk_idx", topk_idx, (T, k), (torch.int32,), dev)
+    mp = _check("mask", mask, (T,), _MASK, dev)
+    lib = _lib.load()
+    with _on(dev, stream) as st:
+        counts = torch.empty(E + 1, dtype=torch.int32, device=dev)
+        sums = torch.empty(E + 2, dtype=torch.float32, device=dev)
+        need = lib.moe_balance_loss_workspace_bytes(T, E)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        at = sums.data_ptr()
+        check(lib.moe_balance_loss(lp, moe_dtype(logits.dtype), T, E, k, router.gatingMode,
+                                   router.logitScale, ip, mp, counts.data_ptr(), at, at + 4 * E,
+                                   None if ws is None else ws.data_ptr(), need, st))
+    return BalanceLoss(counts, sums[:E], sums[E:])
+
+
+def router_backward(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Tensor,
+                    d_weight: Optional[torch.Tensor] = None,
+                    counts: Optional[torch.Tensor] = None, balance_coef: float = 0.0,
+                    z_coef: float = 0.0, mask: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """Gradient of logits [T, E] for d_weight [T, k] float32, the gradient of
+    the routing weights, and balance_coef * balance + z_coef * z, whose counts
+    [E + 1] balance_loss returned (or their sum over a job's ranks)."""
+    T, E, k = _rows("logits", logits, 2).shape[0], router.nExperts, router.topK
+    dev = logits.device
+    lp = _check("logits", logits, (T, E), _FLOATS, dev)
+    ip = _check("topk_idx", topk_idx, (T, k), (torch.int32,), dev)
+    dp = _check("d_weight", d_weight, (T, k), (torch.float32,), dev)
+    cp = _check("counts", counts, (E + 1,), (torch.int32,), dev)
+    mp = _check("mask", mask, (T,), _MASK, dev)
+    _check("out", out, (T, E), (logits.dtype,), dev)
+    with _on(dev, stream) as st:
+        if out is None:
+            out = torch.empty_like(logits)
+        check(_lib.load().moe_router_backward(
+            lp, moe_dtype(logits.dtype), T, E, k, router.gatingMode, int(bool(router.normTopKProb)),
+            _bias(router, router.expertBias, "expertBias", dev), router.logitScale,
+            router.routedScale, _bias(router, router.expertScale, "expertScale", dev), ip, dp, cp,
+            balance_coef, z_coef, mp, out.data_ptr(), st))
+    return out
+
+
+def unpermute_backward(d_out: torch.Tensor, Y: torch.Tensor, inv_perm: torch.Tensor,
+                       topk_weight: torch.Tensor, dY: Optional[torch.Tensor] = None, stream=None):
+    """Gradient of the weighted combine of expert rows Y [T * k, hidden] for
+    d_out [T, hidden]: (dY, d_weight [T, k] float32). inv_perm (T * k int32)
+    comes from the dispatch plan; dY may be Y itself."""
+    T, H = _rows("d_out", d_out, 2).shape
+    dev = d_out.device
+    k = _rows("topk_weight", topk_weight, 2).shape[1]
+    gp = _check("d_out", d_out, (T, H), _FLOATS, dev)
+    yp = _check("Y", Y, (T * k, H), (d_out.dtype,), dev)
+    wp = _check("topk_weight", topk_weight, (T, k), (torch.float32,), dev)
+    ip = _check("inv_perm", inv_perm, (T * k,) if inv_perm.dim() == 1 else (T, k), (torch.int32,), dev)
+    _check("dY", dY, (T * k, H), (d_out.dtype,), dev)
+    with _on(dev, stream) as st:
+        if dY is None:
+            dY = torch.empty_like(Y)
+        dw = torch.empty(T, k, dtype=torch.float32, device=dev)
+        check(_lib.load().moe_unpermute_backward(gp, yp, ip, wp, T, H, k, dY.data_ptr(),
+                                                 dw.data_ptr(), moe_dtype(d_out.dtype), st))
+    return dY, dw
+
+
+@dataclass(frozen=True)
+class LoRAAdapters:
+    """A stack of low-rank adapters of one [N, K] projection: a [G, R, K],
+    b [G, N, R], scale [G] float32 (None: 1). Ranks that differ are padded
+    with zeros to a multiple of 8, at most 128. The tensors may be updated in
+    place (a slot overwritten, an optimiser's step)."""
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: Optional[torch.Tensor] = None
+
+    def __post_init__(self):
+        G, R, K = _rows("a", self.a, 3).shape
+        N = _rows("b", self.b, 3).shape[1]
+        dev = self.a.device
+        desc = Lora(_check("a", self.a, (G, R, K), _FLOATS, dev),
+                    _check("b", self.b, (G, N, R), (self.a.dtype,), dev),
+                    _check("scale", self.scale, (G,), (torch.float32,), dev),
+                    moe_dtype(self.a.dtype), R, N, K, G)
+        check(_lib.load().moe_validate_lora(C.byref(desc)))
+        object.__setattr__(self, "_struct", desc)
+
+    def _ids(self, adapter, T):
+        return _check("adapter", adapter, (T,), (torch.int32,), self.a.device)
+
+    def apply(self, x: torch.Tensor, adapter: torch.Tensor, y: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """y + scale * b (a x) for x [T, K], row t with adapter[t] (int32; -1:
+        none). y [T, N] is the shared projection's output (None: zeros); the
+        result goes to out, by default to y itself."""
+        l, dt, dev = self._struct, (self.a.dtype,), self.a.device
+        T = _rows("x", x, 2).shape[0]
+        xp = _check("x", x, (T, l.k), dt, dev)
+        ap = self._ids(adapter, T)
+        yp = _check("y", y, (T, l.n), dt, dev)
+        _check("out", out, (T, l.n), dt, dev)
+        lib = _lib.load()
+        with _on(dev, stream) as st:
+            if out is None:
+                out = torch.empty(T, l.n, dtype=x.dtype, device=dev) if y is None else y
+            need = lib.moe_lora_workspace_bytes(C.byref(l), T)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            check(lib.moe_lora_apply(C.byref(l), xp, T, ap, yp, out.data_ptr(), ws.data_ptr(),
+                                     need, st))
+        return out
+
+    def backward(self, x: torch.Tensor, dy: torch.Tensor, adapter: torch.Tensor,
+                 dx: Optional[torch.Tensor] = None, dx_out: Optional[torch.Tensor] = None,
+                 need_dx: bool = True, stream=None):
+        """(dx, da, db) of apply for dy [T, N], the gradient of its result.
+        dx [T, K] is the gradient from the shared projection that the adapters'
+        is added to (None: zeros); the sum goes to dx_out, by default to dx
+        itself. need_dx=False leaves it out (dx is then None)."""
+        l, dt, dev = self._struct, (self.a.dtype,), self.a.device
+        T = _rows("x", x, 2).shape[0]
+        xp = _check("x", x, (T, l.k), dt, dev)
+        yp = _check("dy", dy, (T, l.n), dt, dev)
+        ap = self._ids(adapter, T)
+        dp = _check("dx", dx, (T, l.k), dt, dev)
+        _check("dx_out", dx_out, (T, l.k), dt, dev)
+        if not need_dx and (dx is not None or dx_out is not None):
+            raise ValueError("dx or dx_out given with need_dx=False")
+        lib = _lib.load()
+        with _on(dev, stream) as st:
+            if need_dx and dx_out is None:
+                dx_out = torch.empty(T, l.k, dtype=x.dtype, device=dev) if dx is None else dx
+            da, db = torch.empty_like(self.a), torch.empty_like(self.b)
+            need = lib.moe_lora_backward_workspace_bytes(C.byref(l), T)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            check(lib.moe_lora_backward(C.byref(l), xp, yp, T, ap, dp,
+                                        None if dx_out is None else dx_out.data_ptr(),
+                                        da.data_ptr(), db.data_ptr(), ws.data_ptr(), need, st))
+        return dx_out, da, db

@@ -288,6 +288,105 @@ moe_status moe_add_rmsnorm(const void* a, const void* b, const void* weight, flo
                            int32_t n_rows, int32_t row_size, int32_t dtype, void* residual_out,
                            void* normed_out, hipStream_t stream);
 
+/* ---- tuning a router and low-rank adapters ------------------------------ */
+
+/* The reference only runs forward; these entry points differentiate its
+ * routing (MoELayer.swift:140-205, NemotronHText.swift:838-868), its combine
+ * (Ops.swift:5030-5110), and add low-rank adapters beside a projection. With
+ * them a router and adapters are tuned while the quantised experts stay as
+ * they are. All results are the same from call to call. */
+
+/* Load of the experts over the rows whose mask byte is not 0 (mask nullable
+ * [T]: all rows), N of them, with s = logit_scale * logits:
+ *   counts[e]      picks of expert e (ids >= n_experts are not counted);
+ *   counts[E]      N
+ *   prob_sum[e]    P_e = sum_t p_te, p the softmax of a row's s, or for
+ *                  MOE_SIGMOID_TOPK its sigmoids divided by their sum
+ *   losses[0]      balance: E * sum_e counts[e] / (k N) * P_e / N (1 when even)
+ *   losses[1]      z: sum_t logsumexp(s_t)^2 / N
+ * Both losses are 0 when N is 0. A row of -inf only counts as a row with no
+ * probability and no z; NaN or +inf in a counted row makes the probabilities
+ * and losses NaN. n_experts at most 512, k at most 64 and n_experts, T * k
+ * below 2^31. The workspace may be NULL where its size is 0. */
+size_t moe_balance_loss_workspace_bytes(int32_t T, int32_t n_experts);
+moe_status moe_balance_loss(const void* logits, int32_t dtype, int32_t T, int32_t n_experts,
+                            int32_t k, int32_t gating, float logit_scale,
+                            const uint32_t* topk_idx, const uint8_t* mask, uint32_t* counts,
+                            float* prob_sum, float* losses, void* workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+
+/* Gradient of the logits with the router options of moe_router_topk_scaled:
+ *   d_logits = d/d logits ( sum_tr d_weight[t,r] weight[t,r]
+ *                           + balance_coef * balance + z_coef * z )
+ * d_weight [T, k] (nullable) is the gradient of the routing weights as
+ * moe_router_topk_scaled returns them. counts [n_experts + 1] as
+ * moe_balance_loss wrote them, or their sum over the ranks of a job (a rank's
+ * rows then share the job's means); they may be NULL when both coefficients
+ * are 0, and are constants, like expert_bias and expert_scale. Every element
+ * of d_logits [T, n_experts] (dtype) is written, rows whose mask byte is 0
+ * with zeros whatever they hold; it may not overlap logits. An id that a row
+ * holds twice adds twice, an id >= n_experts adds nothing. */
+moe_status moe_router_backward(const void* logits, int32_t dtype, int32_t T, int32_t n_experts,
+                               int32_t k, int32_t gating, int32_t norm_topk_prob,
+                               const float* expert_bias, float logit_scale, float routed_scale,
+                               const float* expert_scale, const uint32_t* topk_idx,
+                               const float* d_weight, const uint32_t* counts,
+                               float balance_coef, float z_coef, const uint8_t* mask,
+                               void* d_logits, hipStream_t stream);
+
+/* Gradient of moe_unpermute:
+ *   dY[inv_perm[t*k+s], :] = round(w[t,s]) * d_out[t,:]   (nullable; may be Y)
+ *   d_weight[t,s]          = <d_out[t,:], Y[inv_perm[t*k+s], :]>   (f32)
+ * Rows of dY that no position names stay as they are; a position >= T * k
+ * has a zero d_weight. d_out, Y and dY 16-byte aligned. */
+moe_status moe_unpermute_backward(const void* d_out, const void* Y, const uint32_t* inv_perm,
+                                  const float* topk_weight, int32_t T, int32_t hidden, int32_t k,
+                                  void* dY, float* d_weight, int32_t dtype, hipStream_t stream);
+
+/* A stack of low-rank adapters of one [n, k] projection, all of one rank
+ * (smaller ones padded with zeros): a [n_adapters, rank, k], b [n_adapters,
+ * n, rank], in dtype like the rows they meet, 16-byte aligned; scale
+ * (nullable: 1) [n_adapters] f32. rank 8..128, rank, n and k multiples of 8,
+ * n and k at most 2^20. */
+typedef struct moe_lora {
+    const void* a;
+    const void* b;
+    const float* scale;
+    int32_t dtype;
+    int32_t rank;
+    int32_t n;
+    int32_t k;
+    int32_t n_adapters;
+} moe_lora;
+moe_status moe_validate_lora(const moe_lora* l);
+
+/* The adapters of many requests beside their shared projection (whose output
+ * rows, from moe_router_logits or moe_expert_matmul, are y_in):
+ *   y[t,:] = round(y_in[t,:] + scale[g] * b[g] (a[g] x[t,:])),  g = adapter[t]
+ * with the inner sums in f32. A row whose id is not in [0, n_adapters) (-1)
+ * has no adapter: its y is y_in. y_in [T, n] may be y (then such rows are not
+ * touched) or NULL (zeros). x [T, k] and y in l->dtype, 16-byte aligned,
+ * apart from each other. The workspace is free to be reused by work that the
+ * stream runs later. */
+size_t moe_lora_workspace_bytes(const moe_lora* l, int32_t T);
+moe_status moe_lora_apply(const moe_lora* l, const void* x, int32_t T, const int32_t* adapter,
+                          const void* y_in, void* y, void* workspace, size_t workspace_bytes,
+                          hipStream_t stream);
+
+/* Gradients of moe_lora_apply for the gradient dy [T, n] of its output, each
+ * nullable (one at least is asked for):
+ *   dx[t,:] = round(dx_in[t,:] + a[g]^T u_t),  u_t = scale[g] * b[g]^T dy[t,:]
+ *   da[g]   = round(sum_t u_t x[t,:]^T)                     [G, rank, k]
+ *   db[g]   = round(sum_t dy[t,:] (scale[g] a[g] x[t,:])^T) [G, n, rank]
+ * over the rows t of adapter g, sums in f32; an adapter without rows gets
+ * zeros. dx_in as y_in above (the gradient from the shared projection; may be
+ * dx, or NULL). All in l->dtype, 16-byte aligned; n_adapters at most 1024. */
+size_t moe_lora_backward_workspace_bytes(const moe_lora* l, int32_t T);
+moe_status moe_lora_backward(const moe_lora* l, const void* x, const void* dy, int32_t T,
+                             const int32_t* adapter, const void* dx_in, void* dx, void* da,
+                             void* db, void* workspace, size_t workspace_bytes,
+                             hipStream_t stream);
+
 /* ---- whole layer ------------------------------------------------------- */
 
 /* Workspace for moe_layer_forward at up to max_tokens rows. */
