@@ -28,6 +28,9 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t kOut = 0x7FFFFFF0u;  // past the end of every view: reads 0
+// A lane offset with this in it lies past every view (views hold at most 2^29
+// bytes: 2^20 columns of 128 ranks of 4 bytes), also with another one added.
+constexpr uint32_t kFar = 0x40000000u;
 constexpr int kTile = 16;               // rows per matrix tile
 
 // D += A B^T over 16 x 16 tiles: lane (c, q) = (lane % 16, lane / 16) holds
@@ -130,10 +133,11 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs p) {
 }
 
 // ---------------------------------------------------------------- expand --
-// y[t][n] = round(y_in[t][n] + sum_r scale_g s[t][r] b[g][n][r]), s summed
-// over its shares of K. A wave takes 16 rows x 64 columns: the b rows are the
-// matrix operand whose row m of the j-th product is column 16 (m / 4) + 4 j +
-// m % 4, so that lane (c, q) ends with 16 neighbouring columns (q) of row c.
+// y[t][n] = round(y_in[t][n] + sum_r scale_g s[t][r] b[g][n][r]), with s either
+// computed by the same block (FUSED: eight waves share K for a tile of 16
+// rows, meet in LDS, and then share N, so that a call is one launch) or added
+// up from a shrink launch's shares of K (the columns are then also shared by
+// gridDim.z blocks: few rows with large adapters).
 //
 // For 16-bit adapters s enters the product as two 16-bit parts, hi = round(s)
 // and lo = round(s - hi), laid side by side along the product's 32-value
@@ -141,29 +145,123 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs p) {
 // it: for rank 16 one instruction holds both. f16 rows are first scaled by a
 // power of two to a maximum in [2^14, 2^15), so that neither part over- or
 // underflows, and the sum back afterwards.
-struct ExpandArgs {
-  const float* s;          // [S, T, R]
+struct FusedArgs {
+  const void* x;           // [T, K]
+  const void* a;           // [G, R, K]
   const void* b;           // [G, N, R]
   const float* scale;      // nullable [G]
   const int32_t* adapter;  // [T]
   const void* yin;         // nullable [T, N], may be y
-  void* y;                 // [T, N]
-  int T, N, R, G, S;
+  void* y;                 // nullable [T, N]
+  float* s;                // nullable [T, R], receives scale * s
+  const float* part;       // not FUSED: [S, T, R]
+  int T, K, N, R, G, S;
 };
 
+constexpr int kFusedWaves = 8;
+
+// scale * s of tile row c (c8 chunks of 16 bytes' worth of values in LDS) as
+// the matrix operand of expand (see there), a step at a time; back: what the
+// products have to be multiplied by.
 template <typename XT, int RT>
-__global__ __launch_bounds__(256) void lora_expand_kernel(ExpandArgs p) {
+__device__ __forceinline__ void expand_operand(const float* row, int c8, int q, bool mine,
+                                               u32x4_t (&sv)[RT], float& back) {
   constexpr bool F32 = sizeof(XT) == 4;
   constexpr int V = 16 / sizeof(XT);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
+  auto chunk = [&](int i, float (&v)[V]) {
+    const int ci = 4 * i + q, cc = F32 || ci < c8 ? ci : ci - c8;
+    const bool in = mine && cc < c8;
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(row + min(cc, c8 - 1) * V + j);
+      v[j] = in ? f.x : 0.f; v[j + 1] = in ? f.y : 0.f;
+      v[j + 2] = in ? f.z : 0.f; v[j + 3] = in ? f.w : 0.f;
+    }
+  };
+  back = 1.f;
+  float fw = 1.f;
+  if constexpr (__is_same(XT, f16_t)) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+      float v[V];
+      chunk(i, v);
+#pragma unroll
+      for (int j = 0; j < V; j++) m = fmaxf(m, fabsf(v[j]));
+    }
+    m = fmaxf(m, __shfl_xor(m, 16, kWave));
+    m = fmaxf(m, __shfl_xor(m, 32, kWave));
+    const int eb = (int)((__float_as_uint(m) >> 23) & 255u);
+    const int sh = eb == 255 ? 0 : min(14 - (eb - 127), 100);
+    back = __builtin_ldexpf(1.f, -sh);
+    fw = __builtin_ldexpf(1.f, sh);
+  }
+#pragma unroll
+  for (int i = 0; i < RT; i++) {
+    float v[V];
+    chunk(i, v);
+    if constexpr (F32) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) sv[i][j] = __float_as_uint(v[j]);
+    } else {
+      const bool lo = 4 * i + q >= c8;
+      uint32_t h[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float f = v[j] * fw, hi = round_to<XT>(f);
+        const float rest = __builtin_isfinite(hi) ? f - hi : 0.f;
+        h[j] = (uint32_t)__builtin_bit_cast(uint16_t, from_f<XT>(lo ? rest : hi));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) sv[i][j] = h[2 * j] | (h[2 * j + 1] << 16);
+    }
+    if (RT == 8) __builtin_amdgcn_sched_barrier(0);  // registers: one step's values at a time
+  }
+}
+
+// Orders this wave's LDS accesses of different lanes; loads from global memory
+// stay in flight across it.
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <typename XT, int RT, bool FUSED>
+__global__ __launch_bounds__(64 * kFusedWaves) void lora_expand_kernel(FusedArgs p) {
+  constexpr bool F32 = sizeof(XT) == 4;
+  constexpr uint32_t ES = sizeof(XT);
+  constexpr int V = 16 / sizeof(XT), LD = RT * 16 + 4, W = kFusedWaves;
+  constexpr int UNIT = 8 * V;                             // a unit of K: 128 bytes of a row
+  constexpr int D = RT == 1 ? 4 : RT == 8 ? 1 : 2;        // units in flight
+  constexpr int J = F32 ? (RT == 8 ? 2 : 4) : 4;  // neighbouring columns of a lane
+  constexpr int NC = 16 * J;                              // columns of a group
+  constexpr int C8 = RT * 16 / V;                         // 16-byte chunks of the widest adapter row
+  constexpr int BL = NC * C8 / 64;                        // loads of a column group's b rows
+  constexpr bool EARLY = BL < 8;  // the first group's loads go out before the shrink half
+  constexpr int AREA = (1 + RT) * 128 > NC * (C8 | 1) ? (1 + RT) * 128 : NC * (C8 | 1);  // 16-byte slots
+  static_assert(AREA * 4 >= kTile * LD, "the sums of a wave fit its area");
+  // a wave's area holds in turn its units, its sums and its column groups
+  __shared__ u32x4_t area[W][AREA];
+  __shared__ __attribute__((aligned(16))) float sum[kTile * LD];
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int t0 = blockIdx.x * kTile, rows = min(kTile, p.T - t0);
-  const int ad = tile_adapter(p.adapter, t0, rows, c, p.G);
-  const int N = p.N, R = p.R;
-  const int nb = (blockIdx.z * 4 + wave) * 64;
-  if (nb >= N) return;
-  const XT* yin = (const XT*)p.yin;
-  XT* y = (XT*)p.y;
-  const int c8 = R / V;  // 16-byte chunks of an adapter row
+  const int ad = tile_adapter(p.adapter, t0, rows, tid & 15, p.G);
+  const int K = p.K, N = p.N, R = p.R, c8 = R / V;
+  const rsrc_t xr = make_rsrc((const XT*)p.x + (size_t)t0 * K, (uint32_t)rows * (uint32_t)K * ES);
+  const rsrc_t yr = make_rsrc((const XT*)p.yin + (p.yin ? (size_t)t0 * N : 0),
+                              p.yin ? (uint32_t)rows * (uint32_t)N * ES : 0u);
+  const rsrc_t wr = make_rsrc((XT*)p.y + (p.y ? (size_t)t0 * N : 0), p.y ? (uint32_t)rows * (uint32_t)N * ES : 0u);
+  u32x4_t* const mem = area[wave];
+  // a wave's units of K and groups of columns are neighbours, the waves' shares
+  // apart: rows are often a multiple of the 4 KB that the memory channels
+  // repeat after, so that all rows of a tile ask one channel for the same k
+  const int units = (K + UNIT - 1) / UNIT, uper = (units + W - 1) / W;
+  const int u0 = wave * uper, u1 = min(units, u0 + uper);
+  const int cw = FUSED ? wave : (int)blockIdx.z * W + wave, cws = FUSED ? W : (int)gridDim.z * W;
+  const int groups = (N + NC - 1) / NC, gper = (groups + cws - 1) / cws;
+  const int g0 = cw * gper, g1 = min(groups, g0 + gper);
   uint32_t rem = (1u << rows) - 1u;
   for (int d = 0; rem; d++) {
     const int lead = __builtin_ctz(rem);
@@ -171,202 +269,400 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(ExpandArgs p) {
     const uint32_t same = (uint32_t)__ballot(ad == g) & rem;
     rem &= ~same;
     if (d % (int)gridDim.y != (int)blockIdx.y) continue;
-    if (g < 0 && p.yin == p.y) continue;  // rows without an adapter, in place
-    f32x4_t acc[4] = {};
-    float back = 1.f;
-    if (g >= 0) {
-      const float sc = p.scale ? p.scale[g] : 1.f;
-      // this lane's chunks of s (row c): values 8 cc .. (16-bit), 4 cc ..
+    // (opaque: else what follows from the lane alone, some hundred addresses,
+    // is computed ahead of the loop and spilled)
+    int lane = tid & 63;
+    asm volatile("" : "+v"(lane));
+    const int c = lane & 15, q = lane >> 4;
+    if (g < 0) {  // rows without an adapter: y = y_in
+      if (p.y == nullptr || p.yin == p.y) continue;
+      for (int n = (cw * 8 + (lane & 7)) * V; n < N; n += 8 * cws * V) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int r = 8 * h + (lane >> 3);
+          const uint32_t off = (same >> r) & 1u ? ((uint32_t)r * N + n) * ES : kFar;
+          bstore128(wr, off, bload128(yr, off));
+        }
+      }
+      continue;
+    }
+    const rsrc_t ar = make_rsrc((const XT*)p.a + (size_t)g * R * K, (uint32_t)R * (uint32_t)K * ES);
+    const rsrc_t br = make_rsrc((const XT*)p.b + (size_t)g * N * R, (uint32_t)N * (uint32_t)R * ES);
+    // ---- loads of b and y
+    const uint32_t pieces = (uint32_t)NC * c8;  // a multiple of 64
+    uint32_t yo[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      yo[i] = ((same >> (4 * q + i)) & 1u ? (uint32_t)(4 * q + i) * N * ES : kFar) + (uint32_t)(J * c) * ES;
+    u32x4_t bv[BL];
+    uint32_t yv[4][J * ES / 4], yn[4][J * ES / 4];
+    auto load_y = [&](int grp, uint32_t (&yb)[4][J * ES / 4]) {
+      const uint32_t no = grp < g1 && grp * NC + J * c < N ? (uint32_t)grp * NC * ES : kFar;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if constexpr (J * ES == 16) {
+          const u32x4_t v = bload128(yr, yo[i] + no);
+#pragma unroll
+          for (int j = 0; j < 4; j++) yb[i][j] = v[j];
+        } else {
+          const u32x2_t v = bload64(yr, yo[i] + no);
+          yb[i][0] = v[0];
+          yb[i][1] = v[1];
+        }
+      }
+    };
+    auto load_b = [&](int grp) {
+      const uint32_t go = grp < g1 ? (uint32_t)grp * NC * R * ES + 16u * lane : kFar;
+#pragma unroll
+      for (int i = 0; i < BL; i++) bv[i] = bload128(br, 64u * i < pieces ? go + 1024u * i : kFar);
+    };
+    auto first_cols = [&] {
+      load_b(g0);
+      load_y(g0, yn);
+    };
+    // ---- shrink. Eight lanes load a row's 128 bytes (lane l: piece l % 8 of
+    // row l / 8): the load unit takes 64 neighbouring bytes a clock but only 16
+    // when neighbouring lanes are in different rows, as the matrix operands
+    // have them. So the pieces change lanes through LDS, piece j of row r in slot
+    // 8 r + (j ^ r % 8).
+    f32x4_t acc[RT] = {};
+    if constexpr (FUSED) {
+      const int pr = lane >> 3, pj = lane & 7;
+      uint32_t xo[2], ao[2 * RT];
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        xo[h] = ((same >> (h * 8 + pr)) & 1u ? (uint32_t)(h * 8 + pr) * K * ES : kFar) + 16u * pj;
+#pragma unroll
+      for (int i = 0; i < 2 * RT; i++)
+        ao[i] = (i * 8 + pr < R ? (uint32_t)(i * 8 + pr) * K * ES : kFar) + 16u * pj;
+      u32x4_t xv[D][2], av[D][2 * RT];
+      auto load = [&](int u, u32x4_t (&xb)[2], u32x4_t (&ab)[2 * RT]) {
+        const uint32_t ko = u < u1 && u * UNIT + pj * V < K ? (uint32_t)u * 128u : kFar;
+#pragma unroll
+        for (int h = 0; h < 2; h++) xb[h] = bload128(xr, xo[h] + ko);
+#pragma unroll
+        for (int i = 0; i < 2 * RT; i++) ab[i] = bload128(ar, ao[i] + ko);
+      };
+      u32x4_t* const put = mem + pr * 8 + (pj ^ pr);
+      const u32x4_t* const get = mem + c * 8;
+#pragma unroll
+      for (int b = 0; b < D; b++) load(u0 + b, xv[b], av[b]);
+      if (EARLY && p.y) first_cols();
+      for (int u = u0; u < u1; u += D) {
+#pragma unroll
+        for (int b = 0; b < D; b++) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) put[h * 64] = xv[b][h];
+#pragma unroll
+          for (int i = 0; i < 2 * RT; i++) put[128 + i * 64] = av[b][i];
+          wave_lds_sync();
+          load(u + b + D, xv[b], av[b]);
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const int at = (4 * h + q) ^ (c & 7);
+            const u32x4_t xf = get[at];
+#pragma unroll
+            for (int i = 0; i < RT; i++) acc[i] = mma<XT>(get[128 + i * 128 + at], xf, acc[i]);
+            if (RT == 8) __builtin_amdgcn_sched_barrier(0);
+          }
+          wave_lds_sync();
+        }
+      }
+    }
+    uint32_t slot[BL];
+    {
+      int n = lane / c8, cc = lane % c8;
+      const int dn = 64 / c8, dc = 64 % c8;
+#pragma unroll
+      for (int i = 0; i < BL; i++) {  // piece 64 i + lane: chunk cc of column n
+        slot[i] = (uint32_t)((n % J) * 16 + n / J) * (c8 | 1) + cc;
+        n += dn;
+        cc += dc;
+        if (cc >= c8) {
+          cc -= c8;
+          n++;
+        }
+      }
+    }
+    // ---- the waves' sums meet
+    if (!FUSED && EARLY && p.y) first_cols();
+    float* const red = reinterpret_cast<float*>(mem);
+    if constexpr (FUSED) {
+#pragma unroll
+      for (int i = 0; i < RT; i++) *reinterpret_cast<f32x4_t*>(red + c * LD + i * 16 + 4 * q) = acc[i];
+      lds_barrier();
+    }
+    const float sc = p.scale ? p.scale[g] : 1.f;
+    for (int e = tid; e < RT * 256; e += 64 * W) {
+      const int t = e / (RT * 16), r = e % (RT * 16), at = t * LD + r;
+      float v = 0.f;
+      if constexpr (FUSED) {
+#pragma unroll
+        for (int w = 0; w < W; w += 2)
+          v += reinterpret_cast<float*>(area[w])[at] + reinterpret_cast<float*>(area[w + 1])[at];
+      } else if (r < R && ((same >> t) & 1u)) {
+        const float* ps = p.part + (size_t)(t0 + t) * R + r;
+#pragma unroll 8
+        for (int z = 0; z < p.S; z++) v += ps[(size_t)z * p.T * R];
+      }
+      v *= sc;
+      sum[at] = v;
+      if (p.s && (FUSED || blockIdx.z == 0) && r < R && ((same >> t) & 1u)) p.s[(size_t)(t0 + t) * R + r] = v;
+    }
+    lds_barrier();
+    if (p.y) {
+      // ---- expand: rows of s against the column group's b rows; lane (c, q)
+      // gets columns J c .. of rows 4 q .., so that 16 lanes read and write 128
+      // neighbouring bytes of y
       u32x4_t sv[RT];
-      float v[RT][8];
+      float back, bk[4] = {1.f, 1.f, 1.f, 1.f};
+      expand_operand<XT, RT>(&sum[c * LD], c8, q, (same >> c) & 1u, sv, back);
+      if constexpr (__is_same(XT, f16_t)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) bk[i] = __shfl(back, 4 * q + i, kWave);
+      }
+      if (!EARLY) {
+        __builtin_amdgcn_sched_barrier(0);
+        first_cols();
+      }
+      uint32_t at[RT];
 #pragma unroll
       for (int i = 0; i < RT; i++) {
-        const int ci = 4 * i + q;
-        const int cc = F32 || ci < c8 ? ci : ci - c8;
-        const bool in = cc < c8 && c < rows;
+        const int ci = 4 * i + q, cc = F32 || ci < c8 ? ci : ci - c8;
+        at[i] = (uint32_t)c * (c8 | 1) + min(cc, c8 - 1);
+      }
+      for (int grp = g0; grp < g1; grp++) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[i][j] = 0.f;
-        if (in) {
-          for (int z = 0; z < p.S; z++) {
-            const float* at = p.s + ((size_t)z * p.T + t0 + c) * R + cc * V;
+        for (int i = 0; i < BL; i++)
+          if (64u * i < pieces) mem[slot[i]] = bv[i];
 #pragma unroll
-            for (int j = 0; j < V; j += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(at + j);
-              v[i][j] += f.x; v[i][j + 1] += f.y; v[i][j + 2] += f.z; v[i][j + 3] += f.w;
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int j = 0; j < (int)(J * ES / 4); j++) yv[i][j] = yn[i][j];
+        wave_lds_sync();
+        load_b(grp + 1);
+        load_y(grp + 1, yn);
+        f32x4_t o[J] = {};
+        if (!F32 && RT > 1 && c8 == C8) {
+          // chunks fill whole products: hi and lo meet the same b operand
+#pragma unroll
+          for (int i = 0; i < RT / 2; i++) {
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+              const u32x4_t bf = mem[(uint32_t)j * 16 * (c8 | 1) + at[i]];
+              o[j] = mma<XT>(sv[i], bf, o[j]);
+              o[j] = mma<XT>(sv[i + RT / 2], bf, o[j]);
+            }
+            if (BL >= 16) __builtin_amdgcn_sched_barrier(0);  // registers: no operands further ahead
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < RT; i++) {
+#pragma unroll
+            for (int j = 0; j < J; j++) o[j] = mma<XT>(sv[i], mem[(uint32_t)j * 16 * (c8 | 1) + at[i]], o[j]);
+            if (BL >= 16) __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        wave_lds_sync();
+        const uint32_t no = grp < g1 && (grp) * NC + J * c < N ? (uint32_t)(grp) * NC * ES : kFar;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          uint32_t w[J * ES / 4];
+          if constexpr (F32) {
+#pragma unroll
+            for (int j = 0; j < J; j++) w[j] = __float_as_uint(__uint_as_float(yv[i][j]) + o[j][i]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < J / 2; j++) {
+              const uint32_t y2 = yv[i][j];
+              const float lo = __builtin_fmaf(o[2 * j][i], bk[i], to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(y2 & 0xFFFFu))));
+              const float hi = __builtin_fmaf(o[2 * j + 1][i], bk[i], to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(y2 >> 16))));
+              w[j] = (uint32_t)__builtin_bit_cast(uint16_t, from_f<XT>(lo)) |
+                     ((uint32_t)__builtin_bit_cast(uint16_t, from_f<XT>(hi)) << 16);
             }
           }
-        }
-#pragma unroll
-        for (int j = 0; j < V; j++) v[i][j] *= sc;
-      }
-      // rows of other adapters hold no sums of this one (or none at all):
-      // they take zeros, and are not stored
-      const bool mine = (same >> c) & 1u;
-      if constexpr (__is_same(XT, f16_t)) {
-        float m = 0.f;
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-#pragma unroll
-          for (int j = 0; j < V; j++) m = fmaxf(m, fabsf(v[i][j]));
-        m = fmaxf(m, __shfl_xor(m, 16, kWave));
-        m = fmaxf(m, __shfl_xor(m, 32, kWave));
-        const int eb = (int)((__float_as_uint(m) >> 23) & 255u);
-        const int sh = eb == 255 ? 0 : min(14 - (eb - 127), 100);
-        back = __builtin_ldexpf(1.f, -sh);
-        const float fw = __builtin_ldexpf(1.f, sh);
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-#pragma unroll
-          for (int j = 0; j < V; j++) v[i][j] *= fw;
-      }
-#pragma unroll
-      for (int i = 0; i < RT; i++) {
-        if constexpr (F32) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) sv[i][j] = mine ? __float_as_uint(v[i][j]) : 0u;
-        } else {
-          const bool lo = 4 * i + q >= c8;
-          uint32_t h[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const float hi = round_to<XT>(v[i][j]);
-            const float rest = __builtin_isfinite(hi) ? v[i][j] - hi : 0.f;
-            h[j] = mine ? (uint32_t)__builtin_bit_cast(uint16_t, from_f<XT>(lo ? rest : hi)) : 0u;
-          }
-#pragma unroll
-          for (int j = 0; j < 4; j++) sv[i][j] = h[2 * j] | (h[2 * j + 1] << 16);
-        }
-      }
-      const rsrc_t br = make_rsrc((const XT*)p.b + (size_t)g * N * R, (uint32_t)((size_t)N * R * sizeof(XT)));
-#pragma unroll
-      for (int i = 0; i < RT; i++) {
-        const int ci = 4 * i + q;
-        const int cc = F32 || ci < c8 ? ci : ci - c8;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int n = nb + 16 * (c >> 2) + 4 * j + (c & 3);
-          const u32x4_t bv = bload128(br, cc < c8 && n < N ? (uint32_t)(n * R + cc * V) * (uint32_t)sizeof(XT) : kOut);
-          acc[j] = mma<XT>(bv, sv[i], acc[j]);
+          if constexpr (J * ES == 16) bstore128(wr, yo[i] + no, u32x4_t{w[0], w[1], w[2], w[3]});
+          else __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{w[0], w[1]}, wr, yo[i] + no, 0, 0);
         }
       }
     }
-    if ((same >> c) & 1u) {
-      const size_t row = (size_t)(t0 + c) * N;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int n = nb + 16 * q + 8 * h;
-        if (n < N) {
-          float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (yin) Vec8<XT>::load(yin + row + n, o);
-#pragma unroll
-          for (int j = 0; j < 8; j++)
-            o[j] = g < 0 ? o[j] : __builtin_fmaf(acc[2 * h + (j >> 2)][j & 3], back, o[j]);
-          Vec8<XT>::store(y + row + n, o);
-        }
-      }
-    }
+    lds_barrier();  // before the areas' and the sums' next adapter
   }
 }
 
 // ------------------------------------------------------------- transpose --
-// [G, P, Q] -> [G, Q, P] by tiles of 32 x 32 through LDS: the backward's
-// products run along the other axis of A and B.
+// [G, P, Q] -> [G, Q, P] of one or two stacks by tiles of 32 x 32 through LDS:
+// the backward's products run along the other axis of A and B.
+struct TransposeArgs {
+  const void* in[2];
+  void* out[2];
+  int P[2], Q[2];
+  int tiles0;  // tiles of one matrix of the first stack
+};
+
 template <typename E>
-__global__ __launch_bounds__(256) void lora_transpose_kernel(const E* __restrict__ in,
-                                                             E* __restrict__ out, int P, int Q) {
+__global__ __launch_bounds__(256) void lora_transpose_kernel(TransposeArgs a) {
   __shared__ E tile[32][33];
-  const size_t base = (size_t)blockIdx.z * P * Q;
+  const int w = (int)blockIdx.x >= a.tiles0, at = (int)blockIdx.x - (w ? a.tiles0 : 0);
+  const int P = a.P[w], Q = a.Q[w], qt = (Q + 31) / 32;
+  const size_t base = (size_t)blockIdx.y * P * Q;
+  const E* __restrict__ in = (const E*)a.in[w] + base;
+  E* __restrict__ out = (E*)a.out[w] + base;
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int p0 = blockIdx.y * 32, q0 = blockIdx.x * 32;
+  const int p0 = at / qt * 32, q0 = at % qt * 32;
 #pragma unroll
-  for (int i = y; i < 32; i += 8)
-    if (p0 + i < P && q0 + x < Q) tile[i][x] = in[base + (size_t)(p0 + i) * Q + q0 + x];
+  for (int i = 0; i < 32; i += 8)
+    if (p0 + y + i < P && q0 + x < Q) tile[y + i][x] = in[(size_t)(p0 + y + i) * Q + q0 + x];
   __syncthreads();
 #pragma unroll
-  for (int i = y; i < 32; i += 8)
-    if (q0 + i < Q && p0 + x < P) out[base + (size_t)(q0 + i) * P + p0 + x] = tile[x][i];
+  for (int i = 0; i < 32; i += 8)
+    if (q0 + y + i < Q && p0 + x < P) out[(size_t)(q0 + y + i) * P + p0 + x] = tile[x][y + i];
 }
 
 // ----------------------------------------------------- adapter gradients --
 // dA_g[r][k] = sum_t u[t][r] x[t][k] and dB_g[n][r] = sum_t s[t][r] dy[t][n]
-// over the rows of adapter g, which a dispatch plan lists (perm, offsets).
-// fp32 matrix products of 4 rows a step: a lane reads 8 neighbouring columns
-// of one row, each of which is one product's operand, so the wide rows go
-// from memory to the operand registers as they lie. A block takes 4 x 128
-// columns, up to two rank tiles and a share of the adapter's rows; with more
-// than one share the fp32 partials are added by lora_sum_kernel.
+// over the rows of adapter g, which a dispatch plan lists (perm, offsets);
+// u and s with their scale. fp32 matrix products of 4 rows a step: a lane
+// reads 8 neighbouring columns of one row, each of which is one product's
+// operand, so the wide rows go from memory to the operand registers as they
+// lie. A block takes 128 columns, up to four rank tiles and a share of the
+// adapter's rows, its eight waves parts of that share, which meet in LDS; with
+// more than one share the fp32 partials are added by lora_sum_kernel. Steps of
+// 16 rows are loaded one ahead, the list of rows two ahead.
 struct OuterSide {
   const void* wide;    // [T, cols]: x or dy
-  const float* small;  // [S, T, R]: u or s before scale
+  const float* small;  // [T, R]: u or s
   void* out;           // the gradient, or its fp32 partials [shares, G, ...]
-  int cols, S;
+  int cols;
   int rank_major;      // out [R, cols] (dA) or [cols, R] (dB)
 };
 struct OuterArgs {
   OuterSide side[2];
   const uint32_t* perm;
   const uint32_t* offsets;
-  const float* scale;
   int T, R, G, sides, shares;
 };
+constexpr int kOuterWaves = 8, kOuterCols = 128;
 
 template <typename XT, typename OT, int RB>
-__global__ __launch_bounds__(256) void lora_outer_kernel(OuterArgs p) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
+__global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs p) {
+  constexpr int XW = sizeof(XT) / 2;  // 16-byte loads of 8 columns
+  __shared__ f32x4_t red[kOuterWaves / 2][RB * 8 * 64];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = (int)blockIdx.z / p.sides;
-  const OuterSide& sd = p.side[(int)blockIdx.z % p.sides];
+  const OuterSide sd = p.side[(int)blockIdx.z % p.sides];
   const int share = (int)blockIdx.y % p.shares, r0 = (int)blockIdx.y / p.shares * (RB * 16);
-  const int R = p.R, cols = sd.cols;
-  const int cb = (blockIdx.x * 4 + wave) * 128;
+  const int R = p.R, cols = sd.cols, cb = blockIdx.x * kOuterCols;
   if (cb >= cols) return;
   const int col = cb + 8 * c;
   const uint32_t o0 = p.offsets[g], o1 = p.offsets[g + 1];
-  const uint32_t len = (o1 - o0 + p.shares - 1) / p.shares;
-  const uint32_t b0 = min(o1, o0 + share * len), b1 = min(o1, b0 + len);
-  const float sc = p.scale ? p.scale[g] : 1.f;
+  // this wave's rows: parts of a multiple of 4
+  const uint32_t parts = (uint32_t)p.shares * kOuterWaves;
+  const uint32_t len = ((o1 - o0 + parts - 1) / parts + 3u) & ~3u;
+  const uint32_t b0 = min((uint64_t)o1, o0 + (uint64_t)(share * kOuterWaves + wave) * len), b1 = min(o1, b0 + len);
+  const XT* const wide = (const XT*)sd.wide + col;
+  const float* const small = sd.small + r0 + c;
   f32x4_t acc[RB][8] = {};
-  for (uint32_t at = b0; at < b1; at += 4) {
-    const bool in = at + q < b1;
-    const uint32_t t = in ? p.perm[at + q] : 0u;
-    float w[8], s[RB];
+  u32x4_t wv[4][XW];
+  float sv[4][RB];
+  auto rows_at = [&](uint32_t at) { return p.perm[min(at + c, b1 - 1)]; };  // 16 rows, one per lane of a group
+  auto load = [&](uint32_t at, uint32_t pv) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) w[j] = 0.f;
-    if (in && col < cols) Vec8<XT>::load((const XT*)sd.wide + (size_t)t * cols + col, w);
+    for (int i = 0; i < 4; i++) {
+      const uint32_t t = (uint32_t)__shfl((int)pv, 4 * i + q, kWave);
+      const bool in = at + 4 * i + q < b1;
 #pragma unroll
-    for (int i = 0; i < RB; i++) {
-      const int r = r0 + i * 16 + c;
-      s[i] = 0.f;
-      if (in && r < R) {
-        for (int z = 0; z < sd.S; z++) s[i] += sd.small[((size_t)z * p.T + t) * R + r];
-        s[i] *= sc;
+      for (int h = 0; h < XW; h++) wv[i][h] = u32x4_t{0u, 0u, 0u, 0u};
+      if (in && col < cols) {
+#pragma unroll
+        for (int h = 0; h < XW; h++)
+          wv[i][h] = *reinterpret_cast<const u32x4_t*>(wide + (size_t)t * cols + h * 4);
+      }
+#pragma unroll
+      for (int j = 0; j < RB; j++) {
+        sv[i][j] = 0.f;
+        if (in && r0 + j * 16 + c < R) sv[i][j] = small[(size_t)t * R + j * 16];
       }
     }
+  };
+  if (b0 < b1) {
+    uint32_t pv = rows_at(b0), pn = rows_at(b0 + 16);
+    load(b0, pv);
+    for (uint32_t at = b0; at < b1; at += 16) {
+      u32x4_t w0[4][XW];
+      float s0[4][RB];
 #pragma unroll
-    for (int i = 0; i < RB; i++)
+      for (int i = 0; i < 4; i++) {
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        acc[i][j] = sd.rank_major ? __builtin_amdgcn_mfma_f32_16x16x4f32(s[i], w[j], acc[i][j], 0, 0, 0)
-                                  : __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], s[i], acc[i][j], 0, 0, 0);
+        for (int h = 0; h < XW; h++) w0[i][h] = wv[i][h];
+#pragma unroll
+        for (int j = 0; j < RB; j++) s0[i][j] = sv[i][j];
+      }
+      pv = pn;
+      pn = rows_at(at + 32);
+      load(at + 16, pv);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          if constexpr (XW == 2) w[j] = __uint_as_float(w0[i][j >> 2][j & 3]);
+          else w[j] = to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(w0[i][0][j >> 1] >> (16 * (j & 1)))));
+        }
+#pragma unroll
+        for (int k = 0; k < RB; k++) {
+          if (sd.rank_major) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+              acc[k][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s0[i][k], w[j], acc[k][j], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+              acc[k][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], s0[i][k], acc[k][j], 0, 0, 0);
+          }
+        }
+      }
+    }
   }
+  // the upper half of the waves hands its sums to the lower, down to one
+#pragma unroll
+  for (int half = kOuterWaves / 2; half >= 1; half >>= 1) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int k = 0; k < RB; k++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) red[wave - half][(k * 8 + j) * 64 + lane] = acc[k][j];
+    }
+    lds_barrier();
+    if (wave < half) {
+#pragma unroll
+      for (int k = 0; k < RB; k++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) acc[k][j] += red[wave][(k * 8 + j) * 64 + lane];
+    }
+    lds_barrier();
+  }
+  if (wave != 0) return;
   OT* out = (OT*)sd.out + ((size_t)share * p.G + g) * R * cols;
 #pragma unroll
-  for (int i = 0; i < RB; i++) {
+  for (int k = 0; k < RB; k++) {
 #pragma unroll
     for (int h = 0; h < 4; h++) {
       if (sd.rank_major) {
-        const int r = r0 + i * 16 + 4 * q + h;
+        const int r = r0 + k * 16 + 4 * q + h;
         if (r < R && col < cols) {
           float o[8];
 #pragma unroll
-          for (int j = 0; j < 8; j++) o[j] = acc[i][j][h];
+          for (int j = 0; j < 8; j++) o[j] = acc[k][j][h];
           Vec8<OT>::store(out + (size_t)r * cols + col, o);
         }
       } else {
-        const int r = r0 + i * 16 + c;
+        const int r = r0 + k * 16 + c;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           const int n = cb + 8 * (4 * q + h) + j;
-          if (r < R && n < cols) out[(size_t)n * R + r] = from_f<OT>(acc[i][j][h]);
+          if (r < R && n < cols) out[(size_t)n * R + r] = from_f<OT>(acc[k][j][h]);
         }
       }
     }
@@ -396,10 +692,12 @@ namespace {
 int tiles_of(int T) { return (T + kTile - 1) / kTile; }
 
 // Blocks that share a tile's distinct adapters: as many as a tile can hold
-// while the launch is small, one where the tiles alone fill the chip.
+// while that leaves one block per CU, one where the tiles alone fill the chip (a
+// block that finds no adapter left costs its dispatch: 4 of them per tile took
+// 4096 rows of 8 requests from 20 to 25 us).
 int leaders(int T, int G, bool none) {
   const int most = std::min(std::min(kTile, T), G + (none ? 1 : 0));
-  return std::max(1, std::min(most, 1024 / tiles_of(T)));
+  return std::max(1, std::min(most, 256 / tiles_of(T)));
 }
 
 template <typename XT>
@@ -414,14 +712,23 @@ hipError_t shrink_typed(const ShrinkArgs& a, int S, hipStream_t st) {
   return hipGetLastError();
 }
 
+// S > 0: the sums come from a shrink launch's S shares at a.part.
 template <typename XT>
-hipError_t expand_typed(const ExpandArgs& a, hipStream_t st) {
-  const dim3 grid(tiles_of(a.T), leaders(a.T, a.G, true), (a.N + 255) / 256);
-#define MOE_EX(RT) hipLaunchKernelGGL((lora_expand_kernel<XT, RT>), grid, dim3(256), 0, st, a)
-  if (a.R <= 16) MOE_EX(1);
-  else if (a.R <= 32) MOE_EX(2);
-  else if (a.R <= 64) MOE_EX(4);
-  else MOE_EX(8);
+hipError_t expand_typed(const FusedArgs& a, hipStream_t st) {
+  const int lead = leaders(a.T, a.G, a.y != nullptr && a.yin != a.y);
+#define MOE_EX(RT)                                                                                 \
+  if (a.S == 0) {                                                                                  \
+    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, true>), dim3(tiles_of(a.T), lead),              \
+                       dim3(64 * kFusedWaves), 0, st, a);                                          \
+  } else {                                                                                         \
+    const int shares = a.y ? (a.N + 64 * kFusedWaves - 1) / (64 * kFusedWaves) : 1;                         \
+    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, false>), dim3(tiles_of(a.T), lead, shares),     \
+                       dim3(64 * kFusedWaves), 0, st, a);                                          \
+  }
+  if (a.R <= 16) { MOE_EX(1) }
+  else if (a.R <= 32) { MOE_EX(2) }
+  else if (a.R <= 64) { MOE_EX(4) }
+  else { MOE_EX(8) }
 #undef MOE_EX
   return hipGetLastError();
 }
@@ -435,16 +742,21 @@ size_t partial_rows(int T, int G) {
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Shares of the adapters' rows in the outer products.
+// Rank tiles of a block of the outer products: all of them up to four, so that
+// the wide rows are read once.
+int outer_ranks(int R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
+
+// Shares of an adapter's rows in the outer products: two blocks per CU, no
+// shares below 64 rows.
 int outer_shares(const LoraDims& d) {
-  const int es = d.dt == DT_F32 ? 4 : 2;
-  (void)es;
-  const long blocks = (long)d.G * 2 * ((std::max(d.K, d.N) + 511) / 512) * ((d.R + 31) / 32);
+  const int rt = outer_ranks(d.R) * 16;
+  const long blocks = (long)d.G * ((d.K + kOuterCols - 1) / kOuterCols + (d.N + kOuterCols - 1) / kOuterCols) *
+                      ((d.R + rt - 1) / rt);
   return (int)std::max(1L, std::min({512 / blocks, (long)(d.T + 63) / 64, 16L}));
 }
 
 struct BackwardLayout {
-  size_t s, u, at, bt, counts, offsets, perm, inv, used, scratch, scratch_bytes, part, total;
+  size_t s, u, part_u, at, bt, counts, offsets, perm, inv, used, scratch, scratch_bytes, part, total;
 };
 BackwardLayout backward_layout(const LoraDims& d) {
   BackwardLayout l{};
@@ -455,8 +767,9 @@ BackwardLayout backward_layout(const LoraDims& d) {
     return o;
   };
   const size_t es = d.dt == DT_F32 ? 4 : 2, T = d.T, R = d.R, G = d.G, K = d.K, N = d.N;
-  l.s = take(partial_rows(d.T, d.G) * R * 4);
-  l.u = take(partial_rows(d.T, d.G) * R * 4);
+  l.s = take(T * R * 4);
+  l.u = take(T * R * 4);
+  l.part_u = take(partial_rows(d.T, d.G) * R * 4);
   l.at = take(G * K * R * es);
   l.bt = take(G * N * R * es);
   l.counts = take(G * 4);
@@ -478,31 +791,35 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
   char* ws = reinterpret_cast<char*>(a.ws);
   float* s = reinterpret_cast<float*>(ws + l.s);
   float* u = reinterpret_cast<float*>(ws + l.u);
+  float* part_u = reinterpret_cast<float*>(ws + l.part_u);
   XT* at = reinterpret_cast<XT*>(ws + l.at);
   XT* bt = reinterpret_cast<XT*>(ws + l.bt);
-  const bool grads = a.da || a.db;
   hipError_t e;
 #define MOE_OKAY(expr) \
   if ((e = (expr)) != hipSuccess) return e
-  const int Ss = lora_shares(d.T, d.G, d.K, d.dt), Su = lora_shares(d.T, d.G, d.N, d.dt);
   if (a.dx || a.da) {
-    hipLaunchKernelGGL((lora_transpose_kernel<XT>), dim3((d.R + 31) / 32, (d.N + 31) / 32, d.G),
-                       dim3(256), 0, st, (const XT*)a.b, bt, d.N, d.R);
+    TransposeArgs tr{{a.b, a.a}, {bt, at}, {d.N, d.R}, {d.R, d.K}, 0};
+    tr.tiles0 = ((d.N + 31) / 32) * ((d.R + 31) / 32);
+    const int tiles = tr.tiles0 + (a.dx ? ((d.K + 31) / 32) * ((d.R + 31) / 32) : 0);
+    hipLaunchKernelGGL((lora_transpose_kernel<XT>), dim3(tiles, d.G), dim3(256), 0, st, tr);
     MOE_OKAY(hipGetLastError());
-    const ShrinkArgs sh{a.dy, bt, a.adapter, u, d.T, d.N, d.R, d.G};
-    MOE_OKAY(shrink_typed<XT>(sh, Su, st));
-  }
-  if (a.dx) {
-    hipLaunchKernelGGL((lora_transpose_kernel<XT>), dim3((d.K + 31) / 32, (d.R + 31) / 32, d.G),
-                       dim3(256), 0, st, (const XT*)a.a, at, d.R, d.K);
-    MOE_OKAY(hipGetLastError());
-    const ExpandArgs ex{u, at, a.scale, a.adapter, a.dx_in, a.dx, d.T, d.K, d.R, d.G, Su};
+    // u and dx: the forward's launches with B^T and A^T in the place of A and B
+    // (u is the same with and without dx)
+    const LoraDims back{d.dt, d.T, d.N, d.K, d.R, d.G};
+    const int S = lora_fused(back) ? 0 : lora_shares(d.T, d.G, d.N, d.dt);
+    if (S) {
+      const ShrinkArgs sh{a.dy, bt, a.adapter, part_u, d.T, d.N, d.R, d.G};
+      MOE_OKAY(shrink_typed<XT>(sh, S, st));
+    }
+    const FusedArgs ex{a.dy, bt, at, a.scale, a.adapter, a.dx_in, a.dx, a.da ? u : nullptr, part_u,
+                       d.T, d.N, d.K, d.R, d.G, S};
     MOE_OKAY(expand_typed<XT>(ex, st));
   }
-  if (!grads) return hipSuccess;
+  if (!a.da && !a.db) return hipSuccess;
   if (a.db) {
-    const ShrinkArgs sh{a.x, a.a, a.adapter, s, d.T, d.K, d.R, d.G};
-    MOE_OKAY(shrink_typed<XT>(sh, Ss, st));
+    const FusedArgs ex{a.x, a.a, a.b, a.scale, a.adapter, nullptr, nullptr, s, nullptr,
+                       d.T, d.K, d.N, d.R, d.G, 0};
+    MOE_OKAY(expand_typed<XT>(ex, st));
   }
   uint32_t* offsets = reinterpret_cast<uint32_t*>(ws + l.offsets);
   uint32_t* perm = reinterpret_cast<uint32_t*>(ws + l.perm);
@@ -514,7 +831,6 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
   OuterArgs o{};
   o.perm = perm;
   o.offsets = offsets;
-  o.scale = a.scale;
   o.T = d.T;
   o.R = d.R;
   o.G = d.G;
@@ -524,24 +840,25 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
   float* pb = pa + (size_t)o.shares * na;
   int cols = 0;
   if (a.da) {
-    o.side[o.sides++] = {a.x, u, o.shares > 1 ? (void*)pa : a.da, d.K, Su, 1};
+    o.side[o.sides++] = {a.x, u, o.shares > 1 ? (void*)pa : a.da, d.K, 1};
     cols = std::max(cols, d.K);
   }
   if (a.db) {
-    o.side[o.sides++] = {a.dy, s, o.shares > 1 ? (void*)pb : a.db, d.N, Ss, 0};
+    o.side[o.sides++] = {a.dy, s, o.shares > 1 ? (void*)pb : a.db, d.N, 0};
     cols = std::max(cols, d.N);
   }
-  const int RB = d.R <= 16 ? 1 : 2;
-  const dim3 grid((cols + 511) / 512, o.shares * ((d.R + RB * 16 - 1) / (RB * 16)), d.G * o.sides);
-#define MOE_OU(OT, RB) hipLaunchKernelGGL((lora_outer_kernel<XT, OT, RB>), grid, dim3(256), 0, st, o)
-  if (o.shares > 1) {
-    if (RB == 1) MOE_OU(float, 1);
-    else MOE_OU(float, 2);
-  } else {
-    if (RB == 1) MOE_OU(XT, 1);
-    else MOE_OU(XT, 2);
-  }
+  const int RB = outer_ranks(d.R);
+  const dim3 grid((cols + kOuterCols - 1) / kOuterCols, o.shares * ((d.R + RB * 16 - 1) / (RB * 16)), d.G * o.sides);
+#define MOE_OU2(OT, RB) \
+  hipLaunchKernelGGL((lora_outer_kernel<XT, OT, RB>), grid, dim3(64 * kOuterWaves), 0, st, o)
+#define MOE_OU(RB)                   \
+  if (o.shares > 1) MOE_OU2(float, RB); \
+  else MOE_OU2(XT, RB);
+  if (RB == 1) { MOE_OU(1) }
+  else if (RB == 2) { MOE_OU(2) }
+  else { MOE_OU(4) }
 #undef MOE_OU
+#undef MOE_OU2
   MOE_OKAY(hipGetLastError());
   if (o.shares > 1) {
     auto add = [&](const float* part, void* out, size_t n) {
@@ -567,6 +884,15 @@ int lora_shares(int T, int G, int K, int dt) {
   return std::max(1, std::min({512 / blocks, units / 4, 16}));
 }
 
+// One launch, unless few blocks would each read a large adapter alone: one
+// row of 2048 -> 2048 takes 6.9 us fused and 6.7 + a launch apart at rank 16, 21.8
+// and 15.2 at rank 128 (of 4096 -> 4096: 34 and 17), 64 rows of 64 adapters of 4096
+// -> 4096 at rank 64 25 and 26.
+bool lora_fused(const LoraDims& d) {
+  const size_t bytes = (size_t)d.R * (d.K + d.N) * (d.dt == DT_F32 ? 4 : 2);
+  return bytes < (256u << 10) || tiles_of(d.T) * std::min(std::min(kTile, d.T), d.G) > 32;
+}
+
 size_t lora_ws_bytes(const LoraDims& d) {
   return up256(partial_rows(d.T, d.G) * d.R * 4);
 }
@@ -575,14 +901,17 @@ size_t lora_backward_ws_bytes(const LoraDims& d) { return backward_layout(d).tot
 hipError_t launch_lora(const LoraDims& d, const void* x, const void* a, const void* b,
                        const float* scale, const int32_t* adapter, const void* yin, void* y,
                        void* ws, hipStream_t st) {
-  const int S = lora_shares(d.T, d.G, d.K, d.dt);
+  const int S = lora_fused(d) ? 0 : lora_shares(d.T, d.G, d.K, d.dt);
   float* s = reinterpret_cast<float*>(ws);
   const ShrinkArgs sh{x, a, adapter, s, d.T, d.K, d.R, d.G};
-  const ExpandArgs ex{s, b, scale, adapter, yin, y, d.T, d.N, d.R, d.G, S};
-#define MOE_LO(XT)                                   \
-  {                                                  \
-    const hipError_t e = shrink_typed<XT>(sh, S, st); \
-    return e != hipSuccess ? e : expand_typed<XT>(ex, st); \
+  const FusedArgs ex{x, a, b, scale, adapter, yin, y, nullptr, s, d.T, d.K, d.N, d.R, d.G, S};
+#define MOE_LO(XT)                                          \
+  {                                                         \
+    if (S) {                                                \
+      const hipError_t e = shrink_typed<XT>(sh, S, st);     \
+      if (e != hipSuccess) return e;                        \
+    }                                                       \
+    return expand_typed<XT>(ex, st);                        \
   }
   if (d.dt == DT_BF16) MOE_LO(bf16_t)
   if (d.dt == DT_F16) MOE_LO(f16_t)
