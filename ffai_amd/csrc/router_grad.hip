@@ -58,14 +58,35 @@ __device__ __forceinline__ void store_cols(XT* __restrict__ row, int c0, int E, 
   }
 }
 
+// v and the v of the lane 16 (32) away, in either order: v_permlane16_swap
+// exchanges the odd rows of 16 lanes of one register with the even rows of the
+// other (permlane32: halves of 32), both holding v.
+struct Halves {
+  float a, b;
+};
+__device__ __forceinline__ Halves swap16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+__device__ __forceinline__ Halves swap32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+
 // Sum / maximum over each aligned group of 2^LG lanes, in every lane of it.
 template <int LG> __device__ __forceinline__ float row_sum(float v) {
   if constexpr (LG >= 1) v += dpp_f32<0xB1, 0xF>(0.f, v);
   if constexpr (LG >= 2) v += dpp_f32<0x4E, 0xF>(0.f, v);
   if constexpr (LG >= 3) v += dpp_f32<0x141, 0xF>(0.f, v);
   if constexpr (LG >= 4) v += dpp_f32<0x140, 0xF>(0.f, v);
-  if constexpr (LG >= 5) v += __shfl_xor(v, 16, kWave);
-  if constexpr (LG >= 6) v += __shfl_xor(v, 32, kWave);
+  if constexpr (LG >= 5) {
+    const Halves h = swap16(v);
+    v = h.a + h.b;
+  }
+  if constexpr (LG >= 6) {
+    const Halves h = swap32(v);
+    v = h.a + h.b;
+  }
   return v;
 }
 template <int LG> __device__ __forceinline__ float row_max(float v) {
@@ -73,33 +94,32 @@ template <int LG> __device__ __forceinline__ float row_max(float v) {
   if constexpr (LG >= 2) v = fmaxf(v, dpp_f32<0x4E, 0xF>(v, v));
   if constexpr (LG >= 3) v = fmaxf(v, dpp_f32<0x141, 0xF>(v, v));
   if constexpr (LG >= 4) v = fmaxf(v, dpp_f32<0x140, 0xF>(v, v));
-  if constexpr (LG >= 5) v = fmaxf(v, __shfl_xor(v, 16, kWave));
-  if constexpr (LG >= 6) v = fmaxf(v, __shfl_xor(v, 32, kWave));
+  if constexpr (LG >= 5) {
+    const Halves h = swap16(v);
+    v = fmaxf(h.a, h.b);
+  }
+  if constexpr (LG >= 6) {
+    const Halves h = swap32(v);
+    v = fmaxf(h.a, h.b);
+  }
   return v;
 }
 
-// exp(x) to about 1.5 ulp: 2^t with t = x log2(e) in fp32 and the product's
-// rounding error put back as a first-order factor (e^(d) = 1 + d). The clamp
-// keeps infinities out of the correction (2^+-288 already is inf / 0); NaN
-// passes the comparisons and stays.
-__device__ __forceinline__ float exp_acc(float x) {
-  x = x < -200.f ? -200.f : x;
-  x = x > 200.f ? 200.f : x;
-  constexpr float L = 1.44269502162933349609375f;      // log2(e) rounded to fp32
-  constexpr float Llo = 1.925963033500011e-8f;         // log2(e) - L
-  const float t = x * L;
-  float d = __builtin_fmaf(x, L, -t);
-  d = __builtin_fmaf(x, Llo, d);
-  const float y = __builtin_amdgcn_exp2f(t);
-  const float c = d * 0.693147180559945f;
-  return y > 1e38f ? y : __builtin_fmaf(y, c, y);  // inf * 0 would be NaN
+constexpr float kLog2e = 1.44269504088896341f;
+
+// exp(s - m) as 2^(s log2(e) - m log2(e)) with one rounding of the exponent's
+// sum: the rounding of m log2(e), ml here, is common to a row and cancels in its
+// ratios, and the sum's own, 2^-25 of its size, weighs little where the power
+// is large. -inf gives 0 (m finite), NaN stays.
+__device__ __forceinline__ float exp_off(float s, float ml) {
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(s, kLog2e, -ml));
 }
 
 // Row statistics of 2^LG lanes: e_j = exp(s_j - m), 1 / sum e and lse. A row
 // of -inf only has e = 0, inv = 0 and lse = 0 (no probability, no loss);
 // NaN or +inf in a row makes all of it NaN.
 struct RowStat {
-  float m, inv, lse;
+  float ml, inv, lse;  // ml: m log2(e)
 };
 template <int LG>
 __device__ __forceinline__ RowStat row_softmax(const float (&s)[kCols], float (&e)[kCols]) {
@@ -108,29 +128,37 @@ __device__ __forceinline__ RowStat row_softmax(const float (&s)[kCols], float (&
   for (int j = 1; j < kCols; j++) m = fmaxf(m, s[j]);
   m = row_max<LG>(m);
   if (m == -__builtin_huge_valf()) m = 0.f;
+  RowStat r;
+  r.ml = m * kLog2e;
   float z = 0.f;
 #pragma unroll
   for (int j = 0; j < kCols; j++) {
-    e[j] = exp_acc(s[j] - m);
+    e[j] = exp_off(s[j], r.ml);
     z += e[j];
   }
   z = row_sum<LG>(z);
-  RowStat r;
-  r.m = m;
   r.inv = z == 0.f ? 0.f : 1.0f / z;
   r.lse = z == 0.f ? 0.f : m + logf(z);
   return r;
 }
 
-__device__ __forceinline__ float sigmoid_acc(float s) { return 1.0f / (1.0f + exp_acc(-s)); }
+// 1 / (1 + exp(-s)); the exponent's rounding is put back as a first-order
+// factor (2^d = 1 + d ln 2) where the power is finite, since here it does not
+// cancel.
+__device__ __forceinline__ float sigmoid_acc(float s) {
+  const float t = -s * kLog2e;
+  float e = __builtin_amdgcn_exp2f(t);
+  const float d = __builtin_fmaf(-s, kLog2e, -t);
+  e = __builtin_fabsf(t) < 126.f ? __builtin_fmaf(e, d * 0.69314718f, e) : e;
+  return 1.0f / (1.0f + e);
+}
 
 }  // namespace
 
 // ---------------------------------------------------------- balance loss --
-constexpr int kBalWaves = 4;
+constexpr int kBalWaves = 16;
 
-// Sums over one launch's blocks (or one block's rows): the losses of `n`
-// counted rows. col: this thread's P and count summed over e by the caller.
+// The losses from sum_e c_e P_e, sum lse^2 and the counted rows.
 __device__ __forceinline__ void store_losses(double dot, double zsum, uint32_t n, int E, int k,
                                              float* losses) {
   const double dn = n ? (double)n : 1.0;
@@ -138,55 +166,88 @@ __device__ __forceinline__ void store_losses(double dot, double zsum, uint32_t n
   losses[1] = (float)(zsum / dn);
 }
 
+// Sum over the wave in its last lane, by DPP (group_sum's steps).
+template <int CTRL, int ROW_MASK> __device__ __forceinline__ double dpp_f64(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)dpp_i32<CTRL, ROW_MASK>(0, (int)(uint32_t)b);
+  const uint32_t hi = (uint32_t)dpp_i32<CTRL, ROW_MASK>(0, (int)(uint32_t)(b >> 32));
+  return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+}
 __device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  v += dpp_f64<0xB1, 0xF>(v);
+  v += dpp_f64<0x4E, 0xF>(v);
+  v += dpp_f64<0x141, 0xF>(v);
+  v += dpp_f64<0x140, 0xF>(v);
+  v += dpp_f64<0x142, 0xA>(v);
+  v += dpp_f64<0x143, 0xC>(v);
   return v;
 }
 
-// Partials of block b: P [E] fp32, picks [E] u32, then z and the counted rows.
+// Partials of block b: P [E4] fp32 and picks [E4] u32 (E4 = E rounded up to
+// 4, the rest zeros), then z and the counted rows.
 struct BalancePart {
   float* P;
   uint32_t* cnt;
   float* z;
   uint32_t* n;
 };
-__host__ __device__ inline BalancePart balance_part(void* ws, int nb, int E) {
+__host__ __device__ inline BalancePart balance_part(void* ws, int nb, int E4) {
   BalancePart p;
   p.P = reinterpret_cast<float*>(ws);
-  p.cnt = reinterpret_cast<uint32_t*>(p.P + (size_t)nb * E);
-  p.z = reinterpret_cast<float*>(p.cnt + (size_t)nb * E);
+  p.cnt = reinterpret_cast<uint32_t*>(p.P + (size_t)nb * E4);
+  p.z = reinterpret_cast<float*>(p.cnt + (size_t)nb * E4);
   p.n = reinterpret_cast<uint32_t*>(p.z + nb);
   return p;
 }
-static size_t balance_part_bytes(int nb, int E) { return (size_t)nb * (E + 1) * 8; }
+
+struct BalanceArgs {
+  const void* logits;
+  const uint32_t* idx;
+  const uint8_t* mask;  // nullable
+  void* ws;
+  uint32_t* counts;
+  float* prob_sum;
+  float* losses;
+  int T, E, k, rpb, sigmoid, vec;
+  float ls;
+};
 
 // Block b takes rows [b rpb, (b + 1) rpb). A lane keeps the probability sums
-// of its 8 experts in registers over its rows; the waves' rows and the picks'
-// counts meet in LDS.
-template <typename XT, int LG>
-__global__ __launch_bounds__(256) void balance_rows_kernel(
-    const XT* __restrict__ logits, const uint32_t* __restrict__ idx,
-    const uint8_t* __restrict__ mask, int T, int E, int k, int rpb, float ls, int sigmoid, int vec,
-    void* ws, uint32_t* __restrict__ counts, float* __restrict__ prob_sum,
-    float* __restrict__ losses) {
-  __shared__ float sP[kBalWaves][kTopkMaxE];
-  __shared__ uint32_t sCnt[kTopkMaxE];
+// of its 8 experts in registers over its rows, the next row's logits in flight;
+// the waves' rows and the picks' counts meet in LDS. FULL: rows are 16-byte
+// aligned and of exactly 8 * 2^LG experts.
+template <typename XT, int LG, bool FULL>
+__global__ __launch_bounds__(64 * kBalWaves) void balance_rows_kernel(BalanceArgs a) {
+  __shared__ float sP[kBalWaves][kCols << LG];
+  __shared__ uint32_t sCnt[kCols << LG];
   __shared__ float sZ[kBalWaves];
   __shared__ uint32_t sN[kBalWaves];
   __shared__ double sDot[kBalWaves];
-  constexpr int LPR = 1 << LG, RPW = kWave >> LG;
+  constexpr int LPR = 1 << LG, RPW = kWave >> LG, NT = 64 * kBalWaves;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c0 = (lane & (LPR - 1)) * kCols;
-  for (int e = tid; e < E; e += 256) sCnt[e] = 0u;
+  const int E = FULL ? kCols << LG : a.E, k = a.k;
+  const uint8_t* __restrict__ mask = a.mask;
+  for (int e = tid; e < (kCols << LG); e += NT) sCnt[e] = 0u;
   __syncthreads();
-  const int r0 = blockIdx.x * rpb, r1 = min(T, r0 + rpb);
+  const int r0 = blockIdx.x * a.rpb, r1 = min(a.T, r0 + a.rpb);
+  const float NEG = -__builtin_huge_valf();
+  const XT* __restrict__ logits = reinterpret_cast<const XT*>(a.logits);
+  auto load = [&](int r, float (&s)[kCols], bool& on) {
+    const int rr = min(r, r1 - 1);
+    on = r < r1 && (mask == nullptr || mask[rr] != 0);
+    load_cols<XT>(logits + (size_t)rr * E, c0, E, FULL || a.vec, NEG, s);
+  };
+  float sn[kCols];
+  bool on_next;
+  const int rw = r0 + wave * RPW + (lane >> LG);
+  load(rw, sn, on_next);
   // picks of the block's rows
   {
     const size_t i0 = (size_t)r0 * k;
     const int ne = (r1 - r0) * k;
-    for (int i = tid; i < ne; i += 256) {
-      const uint32_t e = idx[i0 + i];
+    for (int i = tid; i < ne; i += NT) {
+      const uint32_t e = a.idx[i0 + i];
       const bool on = mask == nullptr || mask[r0 + i / k] != 0;
       if (on && e < (uint32_t)E) atomicAdd(&sCnt[e], 1u);
     }
@@ -196,18 +257,15 @@ __global__ __launch_bounds__(256) void balance_rows_kernel(
   for (int j = 0; j < kCols; j++) P[j] = 0.f;
   float zs = 0.f;
   uint32_t n = 0;
-  const float NEG = -__builtin_huge_valf();
-  for (int rb = r0 + wave * RPW; rb < r1; rb += kBalWaves * RPW) {
-    const int r = rb + (lane >> LG);
-    const bool in = r < r1;
-    const bool on = in && (mask == nullptr || mask[r] != 0);
+  for (int rb = rw; __any(rb < r1); rb += kBalWaves * RPW) {
     float s[kCols], e[kCols];
-    load_cols<XT>(logits + (size_t)(in ? r : r1 - 1) * E, c0, E, vec, NEG, s);
+    const bool on = on_next;
 #pragma unroll
-    for (int j = 0; j < kCols; j++) s[j] = c0 + j < E ? s[j] * ls : NEG;
+    for (int j = 0; j < kCols; j++) s[j] = FULL || c0 + j < E ? sn[j] * a.ls : NEG;
+    load(rb + kBalWaves * RPW, sn, on_next);
     const RowStat st = row_softmax<LG>(s, e);
     float inv = st.inv;
-    if (sigmoid) {
+    if (a.sigmoid) {
       float z = 0.f;
 #pragma unroll
       for (int j = 0; j < kCols; j++) {
@@ -220,13 +278,12 @@ __global__ __launch_bounds__(256) void balance_rows_kernel(
     if (on) {
 #pragma unroll
       for (int j = 0; j < kCols; j++) P[j] = __builtin_fmaf(e[j], inv, P[j]);
-      if (c0 == 0) {
-        zs = __builtin_fmaf(st.lse, st.lse, zs);
-        n++;
-      }
+      zs = __builtin_fmaf(st.lse, st.lse, zs);
+      n++;
     }
   }
-  // rows of the wave, then the block's waves
+  // rows of the wave (z and n are the same in all lanes of a row), then the
+  // block's waves
 #pragma unroll
   for (int off = LPR; off < kWave; off <<= 1) {
 #pragma unroll
@@ -236,14 +293,21 @@ __global__ __launch_bounds__(256) void balance_rows_kernel(
   }
   if (lane < LPR) {
 #pragma unroll
-    for (int j = 0; j < kCols; j++)
-      if (c0 + j < E) sP[wave][c0 + j] = P[j];
+    for (int j = 0; j < kCols; j += 4)
+      *reinterpret_cast<float4*>(&sP[wave][c0 + j]) = make_float4(P[j], P[j + 1], P[j + 2], P[j + 3]);
   }
   if (lane == 0) {
     sZ[wave] = zs;
     sN[wave] = n;
   }
   __syncthreads();
+  const int E4 = (E + 3) & ~3;
+  float p = 0.f;  // thread e: expert e's sum over the block
+  if (tid < E4) {
+#pragma unroll
+    for (int w = 0; w < kBalWaves; w += 2) p += sP[w][tid] + sP[w + 1][tid];
+    p = tid < E ? p : 0.f;
+  }
   float z = 0.f;
   uint32_t nn = 0;
 #pragma unroll
@@ -254,25 +318,27 @@ __global__ __launch_bounds__(256) void balance_rows_kernel(
   if (gridDim.x == 1) {
     // the only block has everything: the losses without a second launch
     double dot = 0.0;
-    for (int e = tid; e < E; e += 256) {
-      const float p = (sP[0][e] + sP[1][e]) + (sP[2][e] + sP[3][e]);
-      prob_sum[e] = p;
-      counts[e] = sCnt[e];
-      dot += (double)p * (double)sCnt[e];
+    if (tid < E) {
+      a.prob_sum[tid] = p;
+      a.counts[tid] = sCnt[tid];
+      dot = (double)p * (double)sCnt[tid];
     }
     dot = wave_sum_f64(dot);
-    if (lane == 0) sDot[wave] = dot;
+    if (lane == 63) sDot[wave] = dot;
     __syncthreads();
     if (tid == 0) {
-      counts[E] = nn;
-      store_losses((sDot[0] + sDot[1]) + (sDot[2] + sDot[3]), (double)z, nn, E, k, losses);
+      double all = 0.0;
+      const int waves = (E + 63) / 64;
+      for (int w = 0; w < waves; w++) all += sDot[w];
+      a.counts[E] = nn;
+      store_losses(all, (double)z, nn, E, k, a.losses);
     }
     return;
   }
-  const BalancePart bp = balance_part(ws, gridDim.x, E);
-  for (int e = tid; e < E; e += 256) {
-    bp.P[(size_t)blockIdx.x * E + e] = (sP[0][e] + sP[1][e]) + (sP[2][e] + sP[3][e]);
-    bp.cnt[(size_t)blockIdx.x * E + e] = sCnt[e];
+  const BalancePart bp = balance_part(a.ws, gridDim.x, E4);
+  if (tid < E4) {
+    bp.P[(size_t)blockIdx.x * E4 + tid] = p;
+    bp.cnt[(size_t)blockIdx.x * E4 + tid] = tid < E ? sCnt[tid] : 0u;
   }
   if (tid == 0) {
     bp.z[blockIdx.x] = z;
@@ -280,59 +346,85 @@ __global__ __launch_bounds__(256) void balance_rows_kernel(
   }
 }
 
-// Adds the blocks' partials and forms the losses: one workgroup, 2^lgc >= E
-// lanes across the experts, the rest of the threads across the blocks.
+// Adds the blocks' partials and forms the losses: one workgroup, four experts
+// a thread (16-byte loads), 2^lgc >= E4 / 4 threads across the experts, the
+// others across the blocks.
+constexpr int kBalMaxBlocks = 256;
 __global__ __launch_bounds__(1024) void balance_final_kernel(void* ws, int nb, int E, int k, int lgc,
                                                              uint32_t* __restrict__ counts,
                                                              float* __restrict__ prob_sum,
                                                              float* __restrict__ losses) {
-  __shared__ double sP[1024];
-  __shared__ uint32_t sC[1024];
+  __shared__ float sP[1024][4];
+  __shared__ uint32_t sC[1024][4];
   __shared__ double sDot[16], sZ[16];
   __shared__ uint32_t sN[16];
-  const BalancePart bp = balance_part(ws, nb, E);
+  const int E4 = (E + 3) & ~3;
+  const BalancePart bp = balance_part(ws, nb, E4);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int e = tid & ((1 << lgc) - 1), sl = tid >> lgc, ns = 1024 >> lgc;
-  double p = 0.0, z = 0.0;
-  uint32_t c = 0, n = 0;
-  if (e < E) {
-#pragma unroll 8
-    for (int b = sl; b < nb; b += ns) {
-      p += (double)bp.P[(size_t)b * E + e];
-      c += bp.cnt[(size_t)b * E + e];
-    }
-  }
-  if (tid < nb) {  // at most 1024 blocks
-    z = (double)bp.z[tid];
-    n = bp.n[tid];
-  }
-  sP[tid] = p;
-  sC[tid] = c;
-  __syncthreads();
-  double dot = 0.0;
-  if (sl == 0 && e < E) {
-    for (int q = 1; q < ns; q++) {
-      p += sP[(q << lgc) + e];
-      c += sC[(q << lgc) + e];
-    }
-    prob_sum[e] = (float)p;
-    counts[e] = c;
-    dot = p * (double)c;
-  }
-  dot = wave_sum_f64(dot);
-  z = wave_sum_f64(z);
+  const int e0 = (tid & ((1 << lgc) - 1)) * 4, sl = tid >> lgc, ns = 1024 >> lgc;
+  const float zb = tid < nb ? bp.z[tid] : 0.f;
+  const uint32_t nbk = tid < nb ? bp.n[tid] : 0u;
+  float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
+  uint4 c = make_uint4(0u, 0u, 0u, 0u);
+  if (e0 < E4) {
+    for (int b0 = sl; b0 < nb; b0 += 8 * ns) {  // 16 loads in flight
+      float4 v[8];
+      uint4 w[8];
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) n += (uint32_t)__shfl_xor((int)n, off, kWave);
-  if (lane == 0) {
-    sDot[wave] = dot;
-    sZ[wave] = z;
-    sN[wave] = n;
+      for (int i = 0; i < 8; i++) {
+        const int b = b0 + i * ns;
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        w[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (b < nb) {
+          v[i] = *reinterpret_cast<const float4*>(bp.P + (size_t)b * E4 + e0);
+          w[i] = *reinterpret_cast<const uint4*>(bp.cnt + (size_t)b * E4 + e0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        p.x += v[i].x; p.y += v[i].y; p.z += v[i].z; p.w += v[i].w;
+        c.x += w[i].x; c.y += w[i].y; c.z += w[i].z; c.w += w[i].w;
+      }
+    }
+  }
+  *reinterpret_cast<float4*>(sP[tid]) = p;
+  *reinterpret_cast<uint4*>(sC[tid]) = c;
+  __syncthreads();
+  // thread e: expert e over the slices, 8 to 256 of them
+  double dot = 0.0;
+  if (tid < E) {
+    const float* ps = &sP[tid >> 2][tid & 3];
+    const uint32_t* cs = &sC[tid >> 2][tid & 3];
+    double pe = 0.0;
+    uint32_t ce = 0;
+    for (int q = 0; q < ns; q += 8) {
+      float a[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) a[i] = ps[(size_t)((q + i) << lgc) * 4];
+#pragma unroll
+      for (int i = 0; i < 8; i++) ce += cs[(size_t)((q + i) << lgc) * 4];
+      pe += (double)(((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7])));
+    }
+    prob_sum[tid] = (float)pe;
+    counts[tid] = ce;
+    dot = pe * (double)ce;
+  }
+  const int waves = (max(E, nb) + 63) / 64;  // those that hold an expert or a block
+  if (wave < waves) {
+    dot = wave_sum_f64(dot);
+    const double z = wave_sum_f64((double)zb);
+    const uint32_t n = wave_scan_u32(nbk);
+    if (lane == 63) {
+      sDot[wave] = dot;
+      sZ[wave] = z;
+      sN[wave] = n;
+    }
   }
   __syncthreads();
   if (tid == 0) {
     double d = 0.0, zz = 0.0;
     uint32_t nn = 0;
-    for (int w = 0; w < 16; w++) {
+    for (int w = 0; w < waves; w++) {
       d += sDot[w];
       zz += sZ[w];
       nn += sN[w];
@@ -356,14 +448,14 @@ int lanes_lg(int E) {
 int balance_blocks(int T, int E) {
   const int rows = kBalWaves * (kWave >> lanes_lg(E));  // a block's rows in flight
   if (T <= 2 * rows) return 1;
-  return (int)std::min<long>(256, (T + rows - 1) / rows);
+  return (int)std::min<long>(kBalMaxBlocks, (T + rows - 1) / rows);
 }
 
 }  // namespace
 
 size_t balance_ws_bytes(int T, int E) {
   const int nb = balance_blocks(T, E);
-  return nb == 1 ? 0 : balance_part_bytes(nb, E);
+  return nb == 1 ? 0 : (size_t)nb * (((E + 3) & ~3) + 1) * 8;
 }
 
 #define MOE_LG(lg, MACRO) \
@@ -385,16 +477,18 @@ static hipError_t balance_typed(const void* logits, int T, int E, int k, bool si
   const int rpb = (T + nb - 1) / nb;
   nb = (T + rpb - 1) / rpb;
   const int vec = E % kCols == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
-#define MOE_BL(LG)                                                                               \
-  hipLaunchKernelGGL((balance_rows_kernel<XT, LG>), dim3(nb), dim3(256), 0, st,                  \
-                     (const XT*)logits, idx, mask, T, E, k, rpb, ls, (int)sigmoid, vec, ws,      \
-                     counts, prob_sum, losses);                                                  \
+  const int lg = lanes_lg(E);
+  const bool full = vec && E == kCols << lg;
+  const BalanceArgs a{logits, idx, mask, ws, counts, prob_sum, losses, T, E, k, rpb, (int)sigmoid, vec, ls};
+#define MOE_BL(LG)                                                                                      \
+  if (full) hipLaunchKernelGGL((balance_rows_kernel<XT, LG, true>), dim3(nb), dim3(64 * kBalWaves), 0, st, a); \
+  else hipLaunchKernelGGL((balance_rows_kernel<XT, LG, false>), dim3(nb), dim3(64 * kBalWaves), 0, st, a);     \
   break;
-  MOE_LG(lanes_lg(E), MOE_BL)
+  MOE_LG(lg, MOE_BL)
 #undef MOE_BL
   if (nb > 1) {
     int lgc = 0;
-    while ((1 << lgc) < E) lgc++;
+    while ((4 << lgc) < E) lgc++;
     hipLaunchKernelGGL(balance_final_kernel, dim3(1), dim3(1024), 0, st, ws, nb, E, k, lgc, counts,
                        prob_sum, losses);
   }
@@ -444,12 +538,13 @@ struct RouterGradArgs {
   float ls, rs, bal, z;
 };
 
-template <typename XT, int LG>
+// NP: picks per lane, 1 where k fits a row's lanes, else 8 (k <= E <= 8 lanes).
+template <typename XT, int LG, bool FULL, int NP>
 __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) {
   constexpr int LPR = 1 << LG, RPW = kWave >> LG;
   __shared__ __attribute__((aligned(16))) float img[4][kWave * kCols];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int rl = lane & (LPR - 1), c0 = rl * kCols, E = a.E, k = a.k;
+  const int rl = lane & (LPR - 1), c0 = rl * kCols, E = FULL ? kCols << LG : a.E, k = a.k;
   float* im = &img[wave][(lane >> LG) * (LPR * kCols)];  // this row's image
   const float NEG = -__builtin_huge_valf();
   float f[kCols];
@@ -463,7 +558,7 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
     zc = a.z * 2.0f / fn;
 #pragma unroll
     for (int j = 0; j < kCols; j++)
-      if (c0 + j < E) f[j] = fs * (float)a.counts[c0 + j];
+      if (FULL || c0 + j < E) f[j] = fs * (float)a.counts[c0 + j];
   }
   const XT* __restrict__ logits = reinterpret_cast<const XT*>(a.logits);
   XT* __restrict__ out = reinterpret_cast<XT*>(a.out);
@@ -471,12 +566,39 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
     const long r = rb + (lane >> LG);
     const bool in = r < a.T;
     const size_t rr = (size_t)(in ? r : a.T - 1);
-    const bool on = in && (a.mask == nullptr || a.mask[rr] != 0);
     const XT* __restrict__ row = logits + rr * E;
-    float s[kCols], p[kCols];
-    load_cols<XT>(row, c0, E, a.vec, NEG, s);
+    // everything the row needs is asked for at once: its mask, picks rl, rl +
+    // LPR, ... with their gradients, its logits, then the picks' own logits
+    const uint32_t mk = a.mask ? a.mask[rr] : 1u;
+    float v[NP], g[NP];
+    uint32_t pe[NP];
+    if (a.dw) {
 #pragma unroll
-    for (int j = 0; j < kCols; j++) s[j] = c0 + j < E ? s[j] * a.ls : NEG;
+      for (int i = 0; i < NP; i++) {
+        const int q = rl + i * LPR;
+        const size_t at = rr * k + min(q, k - 1);
+        pe[i] = a.idx[at];
+        g[i] = a.dw[at];
+        if (q >= k) pe[i] = 0xFFFFFFFFu;
+      }
+    }
+    float s[kCols], p[kCols];
+    load_cols<XT>(row, c0, E, FULL || a.vec, NEG, s);
+    if (a.dw) {
+#pragma unroll
+      for (int i = 0; i < NP; i++) {
+        const bool ok = pe[i] < (uint32_t)E;
+        const uint32_t e = ok ? pe[i] : 0u;
+        v[i] = to_f<XT>(row[e]);
+        g[i] *= a.rs * (a.escale ? a.escale[e] : 1.0f);
+        v[i] = ok ? v[i] * a.ls : NEG;
+        g[i] = ok ? g[i] : 0.f;
+        pe[i] = ok ? pe[i] : 0xFFFFFFFFu;
+      }
+    }
+    const bool on = in && mk != 0;
+#pragma unroll
+    for (int j = 0; j < kCols; j++) s[j] = FULL || c0 + j < E ? s[j] * a.ls : NEG;
     const RowStat st = row_softmax<LG>(s, p);
 #pragma unroll
     for (int j = 0; j < kCols; j++) p[j] *= st.inv;
@@ -515,36 +637,17 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
       for (int j = 0; j < kCols; j += 4)
         *reinterpret_cast<float4*>(im + c0 + j) = make_float4(0.f, 0.f, 0.f, 0.f);
       wave_sync();
-      // picks rl, rl + LPR, ... of the row (at most 8 a lane: k <= E)
-      float v[kCols], g[kCols];
-      uint32_t pe[kCols];
       float mx = NEG;
 #pragma unroll
-      for (int i = 0; i < kCols; i++) {
-        v[i] = NEG;
-        g[i] = 0.f;
-        pe[i] = 0xFFFFFFFFu;
-        if (i * LPR < k) {
-          const int q = rl + i * LPR;
-          if (q < k) {
-            const uint32_t e = a.idx[rr * k + q];
-            if (e < (uint32_t)E) {
-              pe[i] = e;
-              v[i] = to_f<XT>(row[e]) * a.ls;
-              g[i] = a.dw[rr * k + q] * a.rs * (a.escale ? a.escale[e] : 1.0f);
-            }
-          }
-          mx = fmaxf(mx, v[i]);
-        }
-      }
+      for (int i = 0; i < NP; i++) mx = fmaxf(mx, v[i]);
       float S = 0.f, G = 0.f;  // sum of the weights before renormalising, sum g v
       if (a.mode == kPickSoftmax) {
         mx = row_max<LG>(mx);
-        if (mx == NEG) mx = 0.f;
+        mx = mx == NEG ? 0.f : mx * kLog2e;
 #pragma unroll
-        for (int i = 0; i < kCols; i++)
-          if (i * LPR < k) {
-            v[i] = exp_acc(v[i] - mx);
+        for (int i = 0; i < NP; i++)
+          if ((NP == 1 || i * LPR < k)) {
+            v[i] = exp_off(v[i], mx);
             S += v[i];
             G = __builtin_fmaf(g[i], v[i], G);
           }
@@ -553,19 +656,19 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
         const float inv = S == 0.f ? 0.f : 1.0f / S;
         G *= inv;
 #pragma unroll
-        for (int i = 0; i < kCols; i++)
-          if (i * LPR < k) g[i] = v[i] * inv * (g[i] - G);
+        for (int i = 0; i < NP; i++)
+          if ((NP == 1 || i * LPR < k)) g[i] = v[i] * inv * (g[i] - G);
       } else {
-        float pv[kCols];  // p of the pick (full softmax) or sigmoid' (sigmoid)
+        float pv[NP];  // p of the pick (full softmax) or sigmoid' (sigmoid)
 #pragma unroll
-        for (int i = 0; i < kCols; i++) {
+        for (int i = 0; i < NP; i++) {
           pv[i] = 0.f;
-          if (i * LPR < k) {
+          if ((NP == 1 || i * LPR < k)) {
             if (a.mode == kSigmoid) {
               v[i] = sigmoid_acc(v[i]);
               pv[i] = v[i] * (1.0f - v[i]);
             } else {
-              v[i] = exp_acc(v[i] - st.m) * st.inv;
+              v[i] = exp_off(v[i], st.ml) * st.inv;
               pv[i] = v[i];
               if (a.ebias && pe[i] != 0xFFFFFFFFu) v[i] += a.ebias[pe[i]];
             }
@@ -580,8 +683,8 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
         const float Gn = renorm ? G * inv : 0.f;
         float c = 0.f;
 #pragma unroll
-        for (int i = 0; i < kCols; i++)
-          if (i * LPR < k) {
+        for (int i = 0; i < NP; i++)
+          if ((NP == 1 || i * LPR < k)) {
             g[i] = (g[i] - Gn) * inv;
             if (a.mode == kSigmoid) g[i] *= pv[i];
             else c = __builtin_fmaf(g[i], pv[i], c);
@@ -591,12 +694,12 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
 #pragma unroll
           for (int j = 0; j < kCols; j++) d[j] = __builtin_fmaf(-p[j], c, d[j]);
 #pragma unroll
-          for (int i = 0; i < kCols; i++) g[i] *= pv[i];
+          for (int i = 0; i < NP; i++) g[i] *= pv[i];
         }
       }
 #pragma unroll
-      for (int i = 0; i < kCols; i++)
-        if (i * LPR < k && pe[i] != 0xFFFFFFFFu) unsafeAtomicAdd(im + pe[i], g[i]);
+      for (int i = 0; i < NP; i++)
+        if ((NP == 1 || i * LPR < k) && pe[i] != 0xFFFFFFFFu) unsafeAtomicAdd(im + pe[i], g[i]);
       wave_sync();
 #pragma unroll
       for (int j = 0; j < kCols; j += 4) {
@@ -607,7 +710,7 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
     }
 #pragma unroll
     for (int j = 0; j < kCols; j++) d[j] = on ? d[j] * a.ls : 0.f;
-    if (in) store_cols<XT>(out + rr * E, c0, E, a.vec, d);
+    if (in) store_cols<XT>(out + rr * E, c0, E, FULL || a.vec, d);
   }
 }
 
@@ -643,8 +746,14 @@ hipError_t launch_router_backward(const void* logits, int dt, int T, int E, int 
   const int lg = lanes_lg(E);
   const int rows = 4 * (kWave >> lg);
   const int grid = (int)std::min<long>(2048, ((long)T + rows - 1) / rows);
-#define MOE_RB2(XT, LG)                                                                     \
-  hipLaunchKernelGGL((router_backward_kernel<XT, LG>), dim3(grid), dim3(256), 0, st, a);    \
+  const bool full = a.vec && E == kCols << lg, one = k <= 1 << lg;
+#define MOE_RB3(XT, LG, FULL, NP) \
+  hipLaunchKernelGGL((router_backward_kernel<XT, LG, FULL, NP>), dim3(grid), dim3(256), 0, st, a)
+#define MOE_RB2(XT, LG)                  \
+  if (full && one) MOE_RB3(XT, LG, true, 1);  \
+  else if (full) MOE_RB3(XT, LG, true, 8);    \
+  else if (one) MOE_RB3(XT, LG, false, 1);    \
+  else MOE_RB3(XT, LG, false, 8);             \
   break;
 #define MOE_RB_B(LG) MOE_RB2(bf16_t, LG)
 #define MOE_RB_H(LG) MOE_RB2(f16_t, LG)
@@ -656,6 +765,7 @@ hipError_t launch_router_backward(const void* logits, int dt, int T, int E, int 
 #undef MOE_RB_H
 #undef MOE_RB_F
 #undef MOE_RB2
+#undef MOE_RB3
   return hipGetLastError();
 }
 
