@@ -1270,7 +1270,7 @@ extern "C" moe_status moe_lora_apply(const moe_lora* l, const void* x, int32_t T
   if (y_in != y && overlaps(y_in, yb, y, yb))
     return fail(MOE_ERR_INVALID, "lora_apply: y overlaps y_in (equal or apart)");
   const size_t need = lora_ws_bytes(d);
-  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(MOE_ERR_WORKSPACE, "lora_apply: 16-byte aligned workspace of %zu bytes needed", need);
   MOE_HIP(launch_lora(d, x, l->a, l->b, l->scale, adapter, y_in, y, workspace, stream),
           "adapter launch");

@@ -733,11 +733,35 @@ hipError_t expand_typed(const FusedArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Rows of a shrink launch's output over all its shares, at most, for up to T
-// rows (lora_shares keeps shares x blocks within 512), so that a workspace
-// sized for many rows also serves a call of few.
-size_t partial_rows(int T, int G) {
-  return std::max((size_t)T, std::min((size_t)T * 16, (size_t)512 * kTile / std::min(kTile, G)));
+// Shares of the inner axis in a shrink launch: enough for two blocks per CU
+// when there are few rows, at least one unit for each of a block's waves.
+int lora_shares(int T, int G, int K, int dt) {
+  const int unit = dt == DT_F32 ? 32 : 64;
+  const int units = (K + unit - 1) / unit;
+  const int blocks = tiles_of(T) * std::min(std::min(kTile, T), G);
+  return std::max(1, std::min({512 / blocks, units / 4, 16}));
+}
+
+size_t adapter_bytes(const LoraDims& d) {
+  return (size_t)d.R * (d.K + d.N) * (d.dt == DT_F32 ? 4 : 2);
+}
+
+// One launch, unless few blocks would each read a large adapter alone: one
+// row of 2048 -> 2048 takes 6.9 us fused and 6.7 + a launch apart at rank 16, 21.8
+// and 15.2 at rank 128 (of 4096 -> 4096: 34 and 17), 64 rows of 64 adapters of 4096
+// -> 4096 at rank 64 25 and 26.
+constexpr size_t kFusedBytes = 256u << 10;
+constexpr int kSplitBlocks = 32;
+bool lora_fused(const LoraDims& d) {
+  return adapter_bytes(d) < kFusedBytes || tiles_of(d.T) * std::min(std::min(kTile, d.T), d.G) > kSplitBlocks;
+}
+
+// Bytes of a shrink launch's output over all its shares, at most, for up to T
+// rows (lora_shares keeps shares at 16 and shares x blocks at 512), so that a
+// workspace sized for many rows also serves a call of few.
+size_t partial_bytes(const LoraDims& d) {
+  if (adapter_bytes(d) < kFusedBytes) return 0;
+  return std::min((size_t)d.T * 16, (size_t)512 * kTile / std::min(kTile, d.G)) * d.R * 4;
 }
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -769,7 +793,7 @@ BackwardLayout backward_layout(const LoraDims& d) {
   const size_t es = d.dt == DT_F32 ? 4 : 2, T = d.T, R = d.R, G = d.G, K = d.K, N = d.N;
   l.s = take(T * R * 4);
   l.u = take(T * R * 4);
-  l.part_u = take(partial_rows(d.T, d.G) * R * 4);
+  l.part_u = take(partial_bytes(d));
   l.at = take(G * K * R * es);
   l.bt = take(G * N * R * es);
   l.counts = take(G * 4);
@@ -875,26 +899,8 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
 
 }  // namespace
 
-// Shares of the inner axis in a shrink launch: enough for two blocks per CU
-// when there are few rows, at least one unit for each of a block's waves.
-int lora_shares(int T, int G, int K, int dt) {
-  const int unit = dt == DT_F32 ? 32 : 64;
-  const int units = (K + unit - 1) / unit;
-  const int blocks = tiles_of(T) * std::min(std::min(kTile, T), G);
-  return std::max(1, std::min({512 / blocks, units / 4, 16}));
-}
-
-// One launch, unless few blocks would each read a large adapter alone: one
-// row of 2048 -> 2048 takes 6.9 us fused and 6.7 + a launch apart at rank 16, 21.8
-// and 15.2 at rank 128 (of 4096 -> 4096: 34 and 17), 64 rows of 64 adapters of 4096
-// -> 4096 at rank 64 25 and 26.
-bool lora_fused(const LoraDims& d) {
-  const size_t bytes = (size_t)d.R * (d.K + d.N) * (d.dt == DT_F32 ? 4 : 2);
-  return bytes < (256u << 10) || tiles_of(d.T) * std::min(std::min(kTile, d.T), d.G) > 32;
-}
-
 size_t lora_ws_bytes(const LoraDims& d) {
-  return up256(partial_rows(d.T, d.G) * d.R * 4);
+  return up256(partial_bytes(d));
 }
 size_t lora_backward_ws_bytes(const LoraDims& d) { return backward_layout(d).total; }
 

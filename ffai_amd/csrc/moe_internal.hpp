@@ -320,8 +320,6 @@ struct LoraBackward {
   void *dx, *da, *db;  // each nullable
   void* ws;
 };
-bool lora_fused(const LoraDims& d);
-int lora_shares(int T, int G, int K, int dt);
 size_t lora_ws_bytes(const LoraDims& d);
 size_t lora_backward_ws_bytes(const LoraDims& d);
 hipError_t launch_lora(const LoraDims& d, const void* x, const void* a, const void* b,

@@ -37,21 +37,21 @@ def _check(name: str, t: Optional[torch.Tensor], shape, dtypes, device) -> Optio
         return None
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape == shape and t.dtype in dtypes and t.device == device and t.is_contiguous():
+        return t.data_ptr()
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} dtype {t.dtype} is not {' or '.join(str(d) for d in dtypes)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{name} must be contiguous")
 
 
 class _on:
     """The device and stream a call runs on: `stream`, or the current stream of
     the tensors' device, which need not be the current device."""
-    __slots__ = ("_ctx", "handle")
+    __slots__ = ("_ctx", "_handle")
 
     def __init__(self, device: torch.device, stream):
         if device.type != "cuda":
@@ -61,19 +61,26 @@ class _on:
             if stream.device != device:
                 raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
             self._ctx = torch.cuda.stream(stream)
-        elif device.index != torch.cuda.current_device():
-            self._ctx = torch.cuda.device(device)
-        s = torch.cuda.current_stream(device) if stream is None else stream
-        self.handle = C.c_void_p(s.cuda_stream)
+            self._handle = stream.cuda_stream
+        else:
+            if device.index != torch.cuda.current_device():
+                self._ctx = torch.cuda.device(device)
+            self._handle = _raw_stream(device.index)
 
-    def __enter__(self):
+    def __enter__(self) -> int:
         if self._ctx is not None:
             self._ctx.__enter__()
-        return self.handle
+        return self._handle
 
     def __exit__(self, *exc):
         if self._ctx is not None:
             self._ctx.__exit__(*exc)
+
+
+# The current stream's handle of a device, without a Stream object where
+# PyTorch offers it (0.1 us instead of 1.8).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _rows(name: str, t, dims: int) -> torch.Tensor:
@@ -89,8 +96,7 @@ def _rows(name: str, t, dims: int) -> torch.Tensor:
 _MASK = (torch.bool, torch.uint8)
 
 
-def _bias(router: MoERouter, t, name, device):
-    return _check(f"router.{name}", t, (router.nExperts,), (torch.float32,), device)
+_I32, _F32 = (torch.int32,), (torch.float32,)
 
 
 class BalanceLoss(NamedTuple):
@@ -109,19 +115,19 @@ def balance_loss(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Tensor
     T, E, k = _rows("logits", logits, 2).shape[0], router.nExperts, router.topK
     dev = logits.device
     lp = _check("logits", logits, (T, E), _FLOATS, dev)
-    ip = _check("topk_idx", topk_idx, (T, k), (torch.int32,), dev)
+    ip = _check("topk_idx", topk_idx, (T, k), _I32, dev)
     mp = _check("mask", mask, (T,), _MASK, dev)
     lib = _lib.load()
     with _on(dev, stream) as st:
         counts = torch.empty(E + 1, dtype=torch.int32, device=dev)
-        sums = torch.empty(E + 2, dtype=torch.float32, device=dev)
+        prob_sum = torch.empty(E, dtype=torch.float32, device=dev)
+        losses = torch.empty(2, dtype=torch.float32, device=dev)
         need = lib.moe_balance_loss_workspace_bytes(T, E)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        at = sums.data_ptr()
         check(lib.moe_balance_loss(lp, moe_dtype(logits.dtype), T, E, k, router.gatingMode,
-                                   router.logitScale, ip, mp, counts.data_ptr(), at, at + 4 * E,
-                                   None if ws is None else ws.data_ptr(), need, st))
-    return BalanceLoss(counts, sums[:E], sums[E:])
+                                   router.logitScale, ip, mp, counts.data_ptr(), prob_sum.data_ptr(),
+                                   losses.data_ptr(), None if ws is None else ws.data_ptr(), need, st))
+    return BalanceLoss(counts, prob_sum, losses)
 
 
 def router_backward(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Tensor,
@@ -135,9 +141,9 @@ def router_backward(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Ten
     T, E, k = _rows("logits", logits, 2).shape[0], router.nExperts, router.topK
     dev = logits.device
     lp = _check("logits", logits, (T, E), _FLOATS, dev)
-    ip = _check("topk_idx", topk_idx, (T, k), (torch.int32,), dev)
-    dp = _check("d_weight", d_weight, (T, k), (torch.float32,), dev)
-    cp = _check("counts", counts, (E + 1,), (torch.int32,), dev)
+    ip = _check("topk_idx", topk_idx, (T, k), _I32, dev)
+    dp = _check("d_weight", d_weight, (T, k), _F32, dev)
+    cp = _check("counts", counts, (E + 1,), _I32, dev)
     mp = _check("mask", mask, (T,), _MASK, dev)
     _check("out", out, (T, E), (logits.dtype,), dev)
     with _on(dev, stream) as st:
@@ -145,8 +151,9 @@ def router_backward(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Ten
             out = torch.empty_like(logits)
         check(_lib.load().moe_router_backward(
             lp, moe_dtype(logits.dtype), T, E, k, router.gatingMode, int(bool(router.normTopKProb)),
-            _bias(router, router.expertBias, "expertBias", dev), router.logitScale,
-            router.routedScale, _bias(router, router.expertScale, "expertScale", dev), ip, dp, cp,
+            _check("router.expertBias", router.expertBias, (E,), _F32, dev), router.logitScale,
+            router.routedScale, _check("router.expertScale", router.expertScale, (E,), _F32, dev),
+            ip, dp, cp,
             balance_coef, z_coef, mp, out.data_ptr(), st))
     return out
 
@@ -161,8 +168,8 @@ def unpermute_backward(d_out: torch.Tensor, Y: torch.Tensor, inv_perm: torch.Ten
     k = _rows("topk_weight", topk_weight, 2).shape[1]
     gp = _check("d_out", d_out, (T, H), _FLOATS, dev)
     yp = _check("Y", Y, (T * k, H), (d_out.dtype,), dev)
-    wp = _check("topk_weight", topk_weight, (T, k), (torch.float32,), dev)
-    ip = _check("inv_perm", inv_perm, (T * k,) if inv_perm.dim() == 1 else (T, k), (torch.int32,), dev)
+    wp = _check("topk_weight", topk_weight, (T, k), _F32, dev)
+    ip = _check("inv_perm", inv_perm, (T * k,) if inv_perm.dim() == 1 else (T, k), _I32, dev)
     _check("dY", dY, (T * k, H), (d_out.dtype,), dev)
     with _on(dev, stream) as st:
         if dY is None:
@@ -189,13 +196,13 @@ class LoRAAdapters:
         dev = self.a.device
         desc = Lora(_check("a", self.a, (G, R, K), _FLOATS, dev),
                     _check("b", self.b, (G, N, R), (self.a.dtype,), dev),
-                    _check("scale", self.scale, (G,), (torch.float32,), dev),
+                    _check("scale", self.scale, (G,), _F32, dev),
                     moe_dtype(self.a.dtype), R, N, K, G)
         check(_lib.load().moe_validate_lora(C.byref(desc)))
         object.__setattr__(self, "_struct", desc)
 
     def _ids(self, adapter, T):
-        return _check("adapter", adapter, (T,), (torch.int32,), self.a.device)
+        return _check("adapter", adapter, (T,), _I32, self.a.device)
 
     def apply(self, x: torch.Tensor, adapter: torch.Tensor, y: Optional[torch.Tensor] = None,
               out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
@@ -213,9 +220,9 @@ class LoRAAdapters:
             if out is None:
                 out = torch.empty(T, l.n, dtype=x.dtype, device=dev) if y is None else y
             need = lib.moe_lora_workspace_bytes(C.byref(l), T)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            check(lib.moe_lora_apply(C.byref(l), xp, T, ap, yp, out.data_ptr(), ws.data_ptr(),
-                                     need, st))
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            check(lib.moe_lora_apply(C.byref(l), xp, T, ap, yp, out.data_ptr(),
+                                     None if ws is None else ws.data_ptr(), need, st))
         return out
 
     def backward(self, x: torch.Tensor, dy: torch.Tensor, adapter: torch.Tensor,

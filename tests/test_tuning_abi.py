@@ -122,7 +122,7 @@ BACK = dict(x=p(0), dy=p(1), T=4, ad=p(2), dxin=p(3), dx=p(4), da=p(5), db=p(6),
     (dict(ws=C.c_void_p(BIG * 5 + 4)), MOE_ERR_WORKSPACE, "aligned"),
 ])
 def test_lora_apply_refuses(kw, status, needle):
-    l = lora()
+    l = lora(n=4096, k=4096, rank=64)  # large enough that a few rows need a workspace
     assert _lib.load().moe_lora_apply(C.byref(l), *{**APPLY, **kw}.values(), None) == status
     assert needle in _lib.last_error()
 
@@ -151,8 +151,11 @@ def test_lora_backward_refuses_many_adapters():
 
 
 def test_workspace_sizes():
-    """Workspaces grow with the rows; a few rows of a balance loss need none."""
-    lib, l = _lib.load(), lora()
+    """Workspaces grow with the rows; a few rows of a balance loss and small
+    adapters need none."""
+    lib, l = _lib.load(), lora(n=4096, k=4096, rank=64)
+    small = lora()
+    assert [lib.moe_lora_workspace_bytes(C.byref(small), T) for T in (1, 100, 10000)] == [0, 0, 0]
     assert lib.moe_balance_loss_workspace_bytes(1, 32) == 0
     assert lib.moe_balance_loss_workspace_bytes(65536, 256) > 0
     assert lib.moe_balance_loss_workspace_bytes(0, 32) == lib.moe_balance_loss_workspace_bytes(8, 513) == 0
@@ -160,7 +163,7 @@ def test_workspace_sizes():
         assert 0 < f(C.byref(l), 1) <= f(C.byref(l), 100) <= f(C.byref(l), 10000)
         assert f(C.byref(l), 0) == 0
         for G in (1, 3, 40):
-            g = lora(n_adapters=G)
+            g = lora(n_adapters=G, n=4096, k=4096, rank=64)
             sizes = [f(C.byref(g), T) for T in list(range(1, 700)) + [1000, 4096, 40000]]
             assert sizes == sorted(sizes)
 
