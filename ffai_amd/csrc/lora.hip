@@ -145,7 +145,7 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs p) {
 // it: for rank 16 one instruction holds both. f16 rows are first scaled by a
 // power of two to a maximum in [2^14, 2^15), so that neither part over- or
 // underflows, and the sum back afterwards.
-struct FusedArgs {
+struct ExpandArgs {
   const void* x;           // [T, K]
   const void* a;           // [G, R, K]
   const void* b;           // [G, N, R]
@@ -156,6 +156,14 @@ struct FusedArgs {
   float* s;                // nullable [T, R], receives scale * s
   const float* part;       // not FUSED: [S, T, R]
   int T, K, N, R, G, S;
+};
+
+// FUSED: blockIdx.y picks one of up to two calls over the same rows, which then
+// run side by side.
+struct ExpandJobs {
+  ExpandArgs job[2];
+  int leaders;  // blocks of a tile
+  int run;      // tiles of an XCD, 0 for few
 };
 
 constexpr int kFusedWaves = 8;
@@ -227,26 +235,47 @@ __device__ __forceinline__ void wave_lds_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Waves per SIMD: two blocks on a CU where LDS has room for them, so that a few
+// blocks more than CUs (requests that end inside a tile) cost no second round.
+constexpr int expand_waves(size_t es, int rt) { return rt <= (es == 4 ? 2 : 4) ? 4 : 2; }
+
 template <typename XT, int RT, bool FUSED>
-__global__ __launch_bounds__(64 * kFusedWaves) void lora_expand_kernel(FusedArgs p) {
+__global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) void lora_expand_kernel(ExpandJobs jobs) {
+  const ExpandArgs& p = jobs.job[FUSED ? blockIdx.y : 0];
+  // Consecutive blocks go to the eight XCDs in turn. Many tiles: each XCD takes a
+  // run of neighbours, whose rows share adapters in its L2, all first leaders
+  // before the second ones. Few: the tiles' first leaders are spread, then the
+  // second ones.
+  const int lead_of = jobs.leaders;
+  int leader, tile;
+  if (jobs.run > 0) {
+    const int i = (int)(blockIdx.x >> 3);
+    leader = i / jobs.run;
+    tile = (int)(blockIdx.x & 7u) * jobs.run + i % jobs.run;
+  } else {
+    const uint32_t tiles = (uint32_t)(p.T + kTile - 1) / kTile;
+    leader = (int)(blockIdx.x / tiles);
+    tile = (int)(blockIdx.x % tiles);
+  }
+  if (tile * (long)kTile >= p.T) return;
   constexpr bool F32 = sizeof(XT) == 4;
   constexpr uint32_t ES = sizeof(XT);
   constexpr int V = 16 / sizeof(XT), LD = RT * 16 + 4, W = kFusedWaves;
   constexpr int UNIT = 8 * V;                             // a unit of K: 128 bytes of a row
-  constexpr int D = RT == 1 ? 4 : RT == 8 ? 1 : 2;        // units in flight
   constexpr int J = F32 ? (RT == 8 ? 2 : 4) : 4;  // neighbouring columns of a lane
   constexpr int NC = 16 * J;                              // columns of a group
   constexpr int C8 = RT * 16 / V;                         // 16-byte chunks of the widest adapter row
   constexpr int BL = NC * C8 / 64;                        // loads of a column group's b rows
-  constexpr bool EARLY = BL < 8;  // the first group's loads go out before the shrink half
+  constexpr bool EARLY = BL < 4;  // the first group's loads go out before the shrink half
   constexpr int AREA = (1 + RT) * 128 > NC * (C8 | 1) ? (1 + RT) * 128 : NC * (C8 | 1);  // 16-byte slots
-  static_assert(AREA * 4 >= kTile * LD, "the sums of a wave fit its area");
-  // a wave's area holds in turn its units, its sums and its column groups
+  static_assert(AREA * 4 >= 2 * kTile * LD, "the sums of a wave and of the block fit an area");
+  // a wave's area holds in turn its units, its sums and its column groups; the
+  // first one's second half the block's sums
   __shared__ u32x4_t area[W][AREA];
-  __shared__ __attribute__((aligned(16))) float sum[kTile * LD];
+  float* const sum = reinterpret_cast<float*>(area[0]) + kTile * LD;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int t0 = blockIdx.x * kTile, rows = min(kTile, p.T - t0);
+  const int t0 = tile * kTile, rows = min(kTile, p.T - t0);
   const int ad = tile_adapter(p.adapter, t0, rows, tid & 15, p.G);
   const int K = p.K, N = p.N, R = p.R, c8 = R / V;
   const rsrc_t xr = make_rsrc((const XT*)p.x + (size_t)t0 * K, (uint32_t)rows * (uint32_t)K * ES);
@@ -268,7 +297,7 @@ __global__ __launch_bounds__(64 * kFusedWaves) void lora_expand_kernel(FusedArgs
     const int g = __builtin_amdgcn_readlane(ad, lead);
     const uint32_t same = (uint32_t)__ballot(ad == g) & rem;
     rem &= ~same;
-    if (d % (int)gridDim.y != (int)blockIdx.y) continue;
+    if (d % lead_of != leader) continue;
     // (opaque: else what follows from the lane alone, some hundred addresses,
     // is computed ahead of the loop and spilled)
     int lane = tid & 63;
@@ -335,38 +364,34 @@ __global__ __launch_bounds__(64 * kFusedWaves) void lora_expand_kernel(FusedArgs
 #pragma unroll
       for (int i = 0; i < 2 * RT; i++)
         ao[i] = (i * 8 + pr < R ? (uint32_t)(i * 8 + pr) * K * ES : kFar) + 16u * pj;
-      u32x4_t xv[D][2], av[D][2 * RT];
-      auto load = [&](int u, u32x4_t (&xb)[2], u32x4_t (&ab)[2 * RT]) {
+      u32x4_t xv[2], av[2 * RT];
+      auto load = [&](int u) {
         const uint32_t ko = u < u1 && u * UNIT + pj * V < K ? (uint32_t)u * 128u : kFar;
 #pragma unroll
-        for (int h = 0; h < 2; h++) xb[h] = bload128(xr, xo[h] + ko);
+        for (int h = 0; h < 2; h++) xv[h] = bload128(xr, xo[h] + ko);
 #pragma unroll
-        for (int i = 0; i < 2 * RT; i++) ab[i] = bload128(ar, ao[i] + ko);
+        for (int i = 0; i < 2 * RT; i++) av[i] = bload128(ar, ao[i] + ko);
       };
       u32x4_t* const put = mem + pr * 8 + (pj ^ pr);
       const u32x4_t* const get = mem + c * 8;
-#pragma unroll
-      for (int b = 0; b < D; b++) load(u0 + b, xv[b], av[b]);
+      load(u0);
       if (EARLY && p.y) first_cols();
-      for (int u = u0; u < u1; u += D) {
+      for (int u = u0; u < u1; u++) {
 #pragma unroll
-        for (int b = 0; b < D; b++) {
+        for (int h = 0; h < 2; h++) put[h * 64] = xv[h];
 #pragma unroll
-          for (int h = 0; h < 2; h++) put[h * 64] = xv[b][h];
+        for (int i = 0; i < 2 * RT; i++) put[128 + i * 64] = av[i];
+        wave_lds_sync();
+        load(u + 1);
 #pragma unroll
-          for (int i = 0; i < 2 * RT; i++) put[128 + i * 64] = av[b][i];
-          wave_lds_sync();
-          load(u + b + D, xv[b], av[b]);
+        for (int h = 0; h < 2; h++) {
+          const int at = (4 * h + q) ^ (c & 7);
+          const u32x4_t xf = get[at];
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const int at = (4 * h + q) ^ (c & 7);
-            const u32x4_t xf = get[at];
-#pragma unroll
-            for (int i = 0; i < RT; i++) acc[i] = mma<XT>(get[128 + i * 128 + at], xf, acc[i]);
-            if (RT == 8) __builtin_amdgcn_sched_barrier(0);
-          }
-          wave_lds_sync();
+          for (int i = 0; i < RT; i++) acc[i] = mma<XT>(get[128 + i * 128 + at], xf, acc[i]);
+          if (RT == 8) __builtin_amdgcn_sched_barrier(0);
         }
+        wave_lds_sync();
       }
     }
     uint32_t slot[BL];
@@ -416,7 +441,8 @@ __global__ __launch_bounds__(64 * kFusedWaves) void lora_expand_kernel(FusedArgs
       // neighbouring bytes of y
       u32x4_t sv[RT];
       float back, bk[4] = {1.f, 1.f, 1.f, 1.f};
-      expand_operand<XT, RT>(&sum[c * LD], c8, q, (same >> c) & 1u, sv, back);
+      expand_operand<XT, RT>(sum + c * LD, c8, q, (same >> c) & 1u, sv, back);
+      lds_barrier();  // the first wave's column groups overwrite the sums
       if constexpr (__is_same(XT, f16_t)) {
 #pragma unroll
         for (int i = 0; i < 4; i++) bk[i] = __shfl(back, 4 * q + i, kWave);
@@ -490,25 +516,91 @@ __global__ __launch_bounds__(64 * kFusedWaves) void lora_expand_kernel(FusedArgs
   }
 }
 
-// ------------------------------------------------------------- transpose --
-// [G, P, Q] -> [G, Q, P] of one or two stacks by tiles of 32 x 32 through LDS:
-// the backward's products run along the other axis of A and B.
-struct TransposeArgs {
+// ------------------------------------------------------------------ prep --
+// What the backward's launches start from, in one: blocks below plan_blocks
+// list the rows of one adapter each (offsets, and perm in ascending order: the
+// layout of moe_dispatch_plan), the others transpose [G, P, Q] -> [G, Q, P] of
+// one or two stacks by tiles of 32 x 32 through LDS, since the backward's
+// products run along the other axis of A and B.
+struct PrepArgs {
+  const int32_t* adapter;
+  uint32_t* offsets;
+  uint32_t* perm;
+  int T, G, plan_blocks;
   const void* in[2];
   void* out[2];
-  int P[2], Q[2];
-  int tiles0;  // tiles of one matrix of the first stack
+  int P[2], Q[2], tiles[2];  // tiles of one matrix of either stack
 };
 
 template <typename E>
-__global__ __launch_bounds__(256) void lora_transpose_kernel(TransposeArgs a) {
+__global__ __launch_bounds__(256) void lora_prep_kernel(PrepArgs a) {
   __shared__ E tile[32][33];
-  const int w = (int)blockIdx.x >= a.tiles0, at = (int)blockIdx.x - (w ? a.tiles0 : 0);
+  __shared__ uint32_t wlt[4], weq[4];
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x < a.plan_blocks) {
+    // a thread counts ids below and equal to g in a run of 16-byte groups of
+    // rows; its rows follow those of the threads before it
+    const int g = blockIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int groups = (a.T + 3) / 4, per = (groups + 255) / 256;
+    const int q0 = min(groups, tid * per), q1 = min(groups, q0 + per);
+    const bool vec = (reinterpret_cast<uintptr_t>(a.adapter) & 15) == 0;
+    auto ids = [&](int q, int32_t (&v)[4]) {
+      if (vec && q * 4 + 4 <= a.T) {
+        const int4 w = *reinterpret_cast<const int4*>(a.adapter + q * 4);
+        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = q * 4 + j < a.T ? a.adapter[q * 4 + j] : -1;
+      }
+    };
+    uint32_t lt = 0, eq = 0;
+    for (int q = q0; q < q1; q++) {
+      int32_t v[4];
+      ids(q, v);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        lt += v[j] >= 0 && v[j] < g;
+        eq += v[j] == g;
+      }
+    }
+    const uint32_t clt = wave_scan_u32(lt), ceq = wave_scan_u32(eq);
+    if (lane == 63) {
+      wlt[wave] = clt;
+      weq[wave] = ceq;
+    }
+    __syncthreads();
+    uint32_t base = 0, before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      base += wlt[w];
+      all += weq[w];
+      before += w < wave ? weq[w] : 0u;
+    }
+    if (tid == 0) {
+      a.offsets[g] = base;
+      if (g == a.G - 1) a.offsets[a.G] = base + all;
+    }
+    if (eq == 0) return;
+    uint32_t at = base + before + ceq - eq;
+    for (int q = q0; q < q1; q++) {
+      int32_t v[4];
+      ids(q, v);
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (v[j] == g) a.perm[at++] = (uint32_t)(q * 4 + j);
+    }
+    return;
+  }
+  int at = (int)blockIdx.x - a.plan_blocks;
+  const int w = at >= a.tiles[0] * a.G;
+  if (w) at -= a.tiles[0] * a.G;
+  const int g = at / a.tiles[w];
+  at %= a.tiles[w];
   const int P = a.P[w], Q = a.Q[w], qt = (Q + 31) / 32;
-  const size_t base = (size_t)blockIdx.y * P * Q;
+  const size_t base = (size_t)g * P * Q;
   const E* __restrict__ in = (const E*)a.in[w] + base;
   E* __restrict__ out = (E*)a.out[w] + base;
-  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int x = tid & 31, y = tid >> 5;
   const int p0 = at / qt * 32, q0 = at % qt * 32;
 #pragma unroll
   for (int i = 0; i < 32; i += 8)
@@ -669,20 +761,29 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
   }
 }
 
-// out[i] = sum over the shares of their fp32 partials, 8 values a thread.
+// out[i] = sum over the shares of their fp32 partials, 8 values a thread, of
+// both gradients one after the other.
+struct SumArgs {
+  const float* part[2];
+  void* out[2];
+  int64_t n[2];
+  int shares;
+};
 template <typename XT>
-__global__ __launch_bounds__(256) void lora_sum_kernel(const float* __restrict__ part,
-                                                       XT* __restrict__ out, int64_t n, int shares) {
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
+__global__ __launch_bounds__(256) void lora_sum_kernel(SumArgs p) {
+  const int64_t all = p.n[0] + p.n[1];
+  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; at < all; at += (int64_t)gridDim.x * 2048) {
+    const int w = at >= p.n[0];
+    const int64_t i = at - (w ? p.n[0] : 0), n = p.n[w];
     float a[8];
-    Vec8<float>::load(part + i, a);
-    for (int z = 1; z < shares; z++) {
+    Vec8<float>::load(p.part[w] + i, a);
+    for (int z = 1; z < p.shares; z++) {
       float b[8];
-      Vec8<float>::load(part + (size_t)z * n + i, b);
+      Vec8<float>::load(p.part[w] + (size_t)z * n + i, b);
 #pragma unroll
       for (int j = 0; j < 8; j++) a[j] += b[j];
     }
-    Vec8<XT>::store(out + i, a);
+    Vec8<XT>::store((XT*)p.out[w] + i, a);
   }
 }
 
@@ -692,12 +793,12 @@ namespace {
 int tiles_of(int T) { return (T + kTile - 1) / kTile; }
 
 // Blocks that share a tile's distinct adapters: as many as a tile can hold
-// while that leaves one block per CU, one where the tiles alone fill the chip (a
-// block that finds no adapter left costs its dispatch: 4 of them per tile took
-// 4096 rows of 8 requests from 20 to 25 us).
+// while that leaves one block per CU, and two where the tiles fill the chip, for
+// the tiles in which one request ends and the next begins (a block that finds
+// no adapter left costs its dispatch, about a microsecond of a CU).
 int leaders(int T, int G, bool none) {
   const int most = std::min(std::min(kTile, T), G + (none ? 1 : 0));
-  return std::max(1, std::min(most, 256 / tiles_of(T)));
+  return std::min(most, std::max(2, 256 / tiles_of(T)));
 }
 
 template <typename XT>
@@ -712,19 +813,27 @@ hipError_t shrink_typed(const ShrinkArgs& a, int S, hipStream_t st) {
   return hipGetLastError();
 }
 
-// S > 0: the sums come from a shrink launch's S shares at a.part.
+constexpr int kRunTiles = 64;
+
+// S > 0: the sums come from a shrink launch's S shares at a.part; otherwise
+// `also` (nullable) runs beside a.
 template <typename XT>
-hipError_t expand_typed(const FusedArgs& a, hipStream_t st) {
-  const int lead = leaders(a.T, a.G, a.y != nullptr && a.yin != a.y);
-#define MOE_EX(RT)                                                                                 \
-  if (a.S == 0) {                                                                                  \
-    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, true>), dim3(tiles_of(a.T), lead),              \
-                       dim3(64 * kFusedWaves), 0, st, a);                                          \
-  } else {                                                                                         \
-    const int shares = a.y ? (a.N + 64 * kFusedWaves - 1) / (64 * kFusedWaves) : 1;                         \
-    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, false>), dim3(tiles_of(a.T), lead, shares),     \
-                       dim3(64 * kFusedWaves), 0, st, a);                                          \
-  }
+hipError_t expand_typed(const ExpandArgs& a, hipStream_t st, const ExpandArgs* also = nullptr) {
+  ExpandJobs j{};
+  j.job[0] = a;
+  if (also) j.job[1] = *also;
+  j.leaders = leaders(a.T, a.G, a.y != nullptr && a.yin != a.y);
+  const int tiles = tiles_of(a.T);
+  j.run = tiles >= kRunTiles ? (tiles + 7) / 8 : 0;
+  const uint32_t blocks = (uint32_t)(j.run ? 8 * j.run : tiles) * (uint32_t)j.leaders;
+  const int shares = a.y ? (a.N + 64 * kFusedWaves - 1) / (64 * kFusedWaves) : 1;
+#define MOE_EX(RT)                                                                                  \
+  if (a.S == 0)                                                                                     \
+    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, true>), dim3(blocks, also ? 2 : 1),              \
+                       dim3(64 * kFusedWaves), 0, st, j);                                           \
+  else                                                                                              \
+    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, false>), dim3(blocks, 1, shares),                \
+                       dim3(64 * kFusedWaves), 0, st, j);
   if (a.R <= 16) { MOE_EX(1) }
   else if (a.R <= 32) { MOE_EX(2) }
   else if (a.R <= 64) { MOE_EX(4) }
@@ -764,19 +873,21 @@ size_t partial_bytes(const LoraDims& d) {
   return std::min((size_t)d.T * 16, (size_t)512 * kTile / std::min(kTile, d.G)) * d.R * 4;
 }
 
+constexpr int kPrepRows = 16384;  // rows the prep launch lists; more take a plan of their own
+
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 // Rank tiles of a block of the outer products: all of them up to four, so that
 // the wide rows are read once.
 int outer_ranks(int R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
 
-// Shares of an adapter's rows in the outer products: two blocks per CU, no
-// shares below 64 rows.
+// Shares of an adapter's rows in the outer products: a block per CU, no shares
+// below 64 rows.
 int outer_shares(const LoraDims& d) {
   const int rt = outer_ranks(d.R) * 16;
   const long blocks = (long)d.G * ((d.K + kOuterCols - 1) / kOuterCols + (d.N + kOuterCols - 1) / kOuterCols) *
                       ((d.R + rt - 1) / rt);
-  return (int)std::max(1L, std::min({512 / blocks, (long)(d.T + 63) / 64, 16L}));
+  return (int)std::max(1L, std::min({256 / blocks, (long)(d.T + 63) / 64, 16L}));
 }
 
 struct BackwardLayout {
@@ -818,40 +929,60 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
   float* part_u = reinterpret_cast<float*>(ws + l.part_u);
   XT* at = reinterpret_cast<XT*>(ws + l.at);
   XT* bt = reinterpret_cast<XT*>(ws + l.bt);
+  uint32_t* offsets = reinterpret_cast<uint32_t*>(ws + l.offsets);
+  uint32_t* perm = reinterpret_cast<uint32_t*>(ws + l.perm);
   hipError_t e;
 #define MOE_OKAY(expr) \
   if ((e = (expr)) != hipSuccess) return e
-  if (a.dx || a.da) {
-    TransposeArgs tr{{a.b, a.a}, {bt, at}, {d.N, d.R}, {d.R, d.K}, 0};
-    tr.tiles0 = ((d.N + 31) / 32) * ((d.R + 31) / 32);
-    const int tiles = tr.tiles0 + (a.dx ? ((d.K + 31) / 32) * ((d.R + 31) / 32) : 0);
-    hipLaunchKernelGGL((lora_transpose_kernel<XT>), dim3(tiles, d.G), dim3(256), 0, st, tr);
+  const bool grads = a.da || a.db, need_u = a.dx || a.da;
+  PrepArgs pr{};
+  pr.adapter = a.adapter;
+  pr.offsets = offsets;
+  pr.perm = perm;
+  pr.T = d.T;
+  pr.G = d.G;
+  pr.plan_blocks = grads && d.T <= kPrepRows ? d.G : 0;
+  auto side = [&](int w, const void* in, void* out, int P, int Q) {
+    pr.in[w] = in;
+    pr.out[w] = out;
+    pr.P[w] = P;
+    pr.Q[w] = Q;
+    pr.tiles[w] = ((P + 31) / 32) * ((Q + 31) / 32);
+  };
+  if (need_u) side(0, a.b, bt, d.N, d.R);
+  if (a.dx) side(1, a.a, at, d.R, d.K);
+  const long prep = pr.plan_blocks + (long)d.G * (pr.tiles[0] + pr.tiles[1]);
+  if (prep > 0) {
+    hipLaunchKernelGGL((lora_prep_kernel<XT>), dim3((uint32_t)prep), dim3(256), 0, st, pr);
     MOE_OKAY(hipGetLastError());
-    // u and dx: the forward's launches with B^T and A^T in the place of A and B
-    // (u is the same with and without dx)
+  }
+  if (grads && !pr.plan_blocks)
+    MOE_OKAY(launch_dispatch_plan(reinterpret_cast<const uint32_t*>(a.adapter), d.T, 1, d.G,
+                                  reinterpret_cast<uint32_t*>(ws + l.counts), offsets, perm,
+                                  reinterpret_cast<uint32_t*>(ws + l.inv),
+                                  reinterpret_cast<uint32_t*>(ws + l.used), ws + l.scratch,
+                                  l.scratch_bytes, st));
+  // u and dx: the forward's launches with B^T and A^T in the place of A and B (u
+  // is the same with and without dx); s: the forward's first half
+  const ExpandArgs es{a.x, a.a, a.b, a.scale, a.adapter, nullptr, nullptr, s, nullptr,
+                      d.T, d.K, d.N, d.R, d.G, 0};
+  bool s_done = !a.db;
+  if (need_u) {
     const LoraDims back{d.dt, d.T, d.N, d.K, d.R, d.G};
     const int S = lora_fused(back) ? 0 : lora_shares(d.T, d.G, d.N, d.dt);
+    const ExpandArgs eu{a.dy, bt, at, a.scale, a.adapter, a.dx_in, a.dx, a.da ? u : nullptr, part_u,
+                        d.T, d.N, d.K, d.R, d.G, S};
     if (S) {
       const ShrinkArgs sh{a.dy, bt, a.adapter, part_u, d.T, d.N, d.R, d.G};
       MOE_OKAY(shrink_typed<XT>(sh, S, st));
+      MOE_OKAY(expand_typed<XT>(eu, st));
+    } else {
+      MOE_OKAY(expand_typed<XT>(eu, st, s_done ? nullptr : &es));
+      s_done = true;
     }
-    const FusedArgs ex{a.dy, bt, at, a.scale, a.adapter, a.dx_in, a.dx, a.da ? u : nullptr, part_u,
-                       d.T, d.N, d.K, d.R, d.G, S};
-    MOE_OKAY(expand_typed<XT>(ex, st));
   }
-  if (!a.da && !a.db) return hipSuccess;
-  if (a.db) {
-    const FusedArgs ex{a.x, a.a, a.b, a.scale, a.adapter, nullptr, nullptr, s, nullptr,
-                       d.T, d.K, d.N, d.R, d.G, 0};
-    MOE_OKAY(expand_typed<XT>(ex, st));
-  }
-  uint32_t* offsets = reinterpret_cast<uint32_t*>(ws + l.offsets);
-  uint32_t* perm = reinterpret_cast<uint32_t*>(ws + l.perm);
-  MOE_OKAY(launch_dispatch_plan(reinterpret_cast<const uint32_t*>(a.adapter), d.T, 1, d.G,
-                                reinterpret_cast<uint32_t*>(ws + l.counts), offsets, perm,
-                                reinterpret_cast<uint32_t*>(ws + l.inv),
-                                reinterpret_cast<uint32_t*>(ws + l.used), ws + l.scratch,
-                                l.scratch_bytes, st));
+  if (!s_done) MOE_OKAY(expand_typed<XT>(es, st));
+  if (!grads) return hipSuccess;
   OuterArgs o{};
   o.perm = perm;
   o.offsets = offsets;
@@ -885,13 +1016,11 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
 #undef MOE_OU2
   MOE_OKAY(hipGetLastError());
   if (o.shares > 1) {
-    auto add = [&](const float* part, void* out, size_t n) {
-      const int gr = (int)std::min<size_t>((n + 2047) / 2048, 2048);
-      hipLaunchKernelGGL((lora_sum_kernel<XT>), dim3(gr), dim3(256), 0, st, part, (XT*)out, (int64_t)n, o.shares);
-      return hipGetLastError();
-    };
-    if (a.da) MOE_OKAY(add(pa, a.da, na));
-    if (a.db) MOE_OKAY(add(pb, a.db, nb));
+    const SumArgs sm{{pa, pb}, {a.da, a.db}, {a.da ? (int64_t)na : 0, a.db ? (int64_t)nb : 0}, o.shares};
+    const size_t n = sm.n[0] + sm.n[1];
+    hipLaunchKernelGGL((lora_sum_kernel<XT>), dim3((uint32_t)std::min<size_t>((n + 2047) / 2048, 2048)),
+                       dim3(256), 0, st, sm);
+    MOE_OKAY(hipGetLastError());
   }
 #undef MOE_OKAY
   return hipSuccess;
@@ -910,7 +1039,7 @@ hipError_t launch_lora(const LoraDims& d, const void* x, const void* a, const vo
   const int S = lora_fused(d) ? 0 : lora_shares(d.T, d.G, d.K, d.dt);
   float* s = reinterpret_cast<float*>(ws);
   const ShrinkArgs sh{x, a, adapter, s, d.T, d.K, d.R, d.G};
-  const FusedArgs ex{x, a, b, scale, adapter, yin, y, nullptr, s, d.T, d.K, d.N, d.R, d.G, S};
+  const ExpandArgs ex{x, a, b, scale, adapter, yin, y, nullptr, s, d.T, d.K, d.N, d.R, d.G, S};
 #define MOE_LO(XT)                                          \
   {                                                         \
     if (S) {                                                \
