@@ -613,177 +613,223 @@ __global__ __launch_bounds__(256) void lora_prep_kernel(PrepArgs a) {
 
 // ----------------------------------------------------- adapter gradients --
 // dA_g[r][k] = sum_t u[t][r] x[t][k] and dB_g[n][r] = sum_t s[t][r] dy[t][n]
-// over the rows of adapter g, which a dispatch plan lists (perm, offsets);
-// u and s with their scale. fp32 matrix products of 4 rows a step: a lane
-// reads 8 neighbouring columns of one row, each of which is one product's
-// operand, so the wide rows go from memory to the operand registers as they
-// lie. A block takes 128 columns, up to four rank tiles and a share of the
-// adapter's rows, its eight waves parts of that share, which meet in LDS; with
-// more than one share the fp32 partials are added by lora_sum_kernel. Steps of
-// 16 rows are loaded one ahead, the list of rows two ahead.
+// over the rows of adapter g, which the plan lists (perm, offsets); u and s
+// with their scale. fp32 matrix products of 4 rows a step: a lane reads 8
+// neighbouring columns of one row, each of which is one product's operand, so
+// the wide rows go from memory to the operand registers as they lie.
+//
+// A block takes 128 columns, up to four rank tiles and a chunk of one adapter's
+// rows (an adapter of n rows has ceil(n / chunk) equal ones, numbered through
+// over the adapters, so that the work is even however the rows spread); its
+// eight waves share the chunk and meet in LDS. The gradient of an adapter with
+// one chunk is stored at once, the chunks of the others as fp32, which
+// lora_sum_kernel adds in order. Steps are loaded one ahead, the list of rows
+// two ahead.
 struct OuterSide {
   const void* wide;    // [T, cols]: x or dy
   const float* small;  // [T, R]: u or s
-  void* out;           // the gradient, or its fp32 partials [shares, G, ...]
+  void* out;           // [G, R, cols] (rank_major: dA) or [G, cols, R] (dB)
+  float* part;         // [chunks, ...] fp32
   int cols;
-  int rank_major;      // out [R, cols] (dA) or [cols, R] (dB)
+  int rank_major;
 };
 struct OuterArgs {
   OuterSide side[2];
   const uint32_t* perm;
   const uint32_t* offsets;
-  int T, R, G, sides, shares;
+  int R, G, sides;
+  uint32_t chunk;  // rows of a chunk, at most
 };
 constexpr int kOuterWaves = 8, kOuterCols = 128;
 
-template <typename XT, typename OT, int RB>
-__global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs p) {
-  constexpr int XW = sizeof(XT) / 2;  // 16-byte loads of 8 columns
-  __shared__ f32x4_t red[kOuterWaves / 2][RB * 8 * 64];
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = (int)blockIdx.z / p.sides;
-  const OuterSide sd = p.side[(int)blockIdx.z % p.sides];
-  const int share = (int)blockIdx.y % p.shares, r0 = (int)blockIdx.y / p.shares * (RB * 16);
-  const int R = p.R, cols = sd.cols, cb = blockIdx.x * kOuterCols;
-  if (cb >= cols) return;
+// The adapter g whose chunks include number y (or, with of >= 0, adapter
+// `of`), its rows [o0, o1) in the plan, its first chunk and how many it has.
+// Uniform over the wave; g = G where y is past the last chunk.
+struct Chunks {
+  int g;
+  uint32_t o0, o1, first, n;
+};
+__device__ __forceinline__ Chunks find_chunks(const uint32_t* __restrict__ offsets, int G,
+                                              uint32_t chunk, uint32_t y, int of) {
+  const int lane = threadIdx.x & 63;
+  Chunks r{G, 0, 0, 0, 0};
+  uint32_t before = 0;
+  for (int i = 0; i < G; i += 64) {
+    const bool in = i + lane < G;
+    const uint32_t a = in ? offsets[i + lane] : 0u, b = in ? offsets[i + lane + 1] : 0u;
+    const uint32_t n = (b - a + chunk - 1) / chunk, last = wave_scan_u32(n) + before;
+    const int k = of >= 0 ? of - i : __popcll(__ballot(in && last <= y));
+    if (k < min(64, G - i)) {
+      r.g = i + k;
+      r.o0 = (uint32_t)__builtin_amdgcn_readlane((int)a, k);
+      r.o1 = (uint32_t)__builtin_amdgcn_readlane((int)b, k);
+      r.n = (uint32_t)__builtin_amdgcn_readlane((int)n, k);
+      r.first = (uint32_t)__builtin_amdgcn_readlane((int)last, k) - r.n;
+      break;
+    }
+    before = (uint32_t)__builtin_amdgcn_readlane((int)last, 63);
+  }
+  return r;
+}
+
+// One adapter's part of the gradient: D[r = 16 k + 4 q + h][column 8 c + j].
+template <typename OT, int RB>
+__device__ __forceinline__ void outer_store(const f32x4_t (&acc)[RB][8], OT* out, bool rank_major,
+                                            int R, int cols, int r0, int cb, int c, int q) {
   const int col = cb + 8 * c;
-  const uint32_t o0 = p.offsets[g], o1 = p.offsets[g + 1];
-  // this wave's rows: parts of a multiple of 4
-  const uint32_t parts = (uint32_t)p.shares * kOuterWaves;
-  const uint32_t len = ((o1 - o0 + parts - 1) / parts + 3u) & ~3u;
-  const uint32_t b0 = min((uint64_t)o1, o0 + (uint64_t)(share * kOuterWaves + wave) * len), b1 = min(o1, b0 + len);
-  const XT* const wide = (const XT*)sd.wide + col;
-  const float* const small = sd.small + r0 + c;
-  f32x4_t acc[RB][8] = {};
-  u32x4_t wv[4][XW];
-  float sv[4][RB];
-  auto rows_at = [&](uint32_t at) { return p.perm[min(at + c, b1 - 1)]; };  // 16 rows, one per lane of a group
-  auto load = [&](uint32_t at, uint32_t pv) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t t = (uint32_t)__shfl((int)pv, 4 * i + q, kWave);
-      const bool in = at + 4 * i + q < b1;
-#pragma unroll
-      for (int h = 0; h < XW; h++) wv[i][h] = u32x4_t{0u, 0u, 0u, 0u};
-      if (in && col < cols) {
-#pragma unroll
-        for (int h = 0; h < XW; h++)
-          wv[i][h] = *reinterpret_cast<const u32x4_t*>(wide + (size_t)t * cols + h * 4);
-      }
-#pragma unroll
-      for (int j = 0; j < RB; j++) {
-        sv[i][j] = 0.f;
-        if (in && r0 + j * 16 + c < R) sv[i][j] = small[(size_t)t * R + j * 16];
-      }
-    }
-  };
-  if (b0 < b1) {
-    uint32_t pv = rows_at(b0), pn = rows_at(b0 + 16);
-    load(b0, pv);
-    for (uint32_t at = b0; at < b1; at += 16) {
-      u32x4_t w0[4][XW];
-      float s0[4][RB];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-#pragma unroll
-        for (int h = 0; h < XW; h++) w0[i][h] = wv[i][h];
-#pragma unroll
-        for (int j = 0; j < RB; j++) s0[i][j] = sv[i][j];
-      }
-      pv = pn;
-      pn = rows_at(at + 32);
-      load(at + 16, pv);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        float w[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          if constexpr (XW == 2) w[j] = __uint_as_float(w0[i][j >> 2][j & 3]);
-          else w[j] = to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(w0[i][0][j >> 1] >> (16 * (j & 1)))));
-        }
-#pragma unroll
-        for (int k = 0; k < RB; k++) {
-          if (sd.rank_major) {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-              acc[k][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s0[i][k], w[j], acc[k][j], 0, 0, 0);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-              acc[k][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], s0[i][k], acc[k][j], 0, 0, 0);
-          }
-        }
-      }
-    }
-  }
-  // the upper half of the waves hands its sums to the lower, down to one
-#pragma unroll
-  for (int half = kOuterWaves / 2; half >= 1; half >>= 1) {
-    if (wave >= half && wave < 2 * half) {
-#pragma unroll
-      for (int k = 0; k < RB; k++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) red[wave - half][(k * 8 + j) * 64 + lane] = acc[k][j];
-    }
-    lds_barrier();
-    if (wave < half) {
-#pragma unroll
-      for (int k = 0; k < RB; k++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) acc[k][j] += red[wave][(k * 8 + j) * 64 + lane];
-    }
-    lds_barrier();
-  }
-  if (wave != 0) return;
-  OT* out = (OT*)sd.out + ((size_t)share * p.G + g) * R * cols;
+  if (col >= cols) return;
 #pragma unroll
   for (int k = 0; k < RB; k++) {
+    const int r = r0 + k * 16 + 4 * q;
+    if (r >= R) continue;  // R is a multiple of 8: the four ranks go together
+    if (rank_major) {
 #pragma unroll
-    for (int h = 0; h < 4; h++) {
-      if (sd.rank_major) {
-        const int r = r0 + k * 16 + 4 * q + h;
-        if (r < R && col < cols) {
-          float o[8];
+      for (int h = 0; h < 4; h++) {
+        float o[8];
 #pragma unroll
-          for (int j = 0; j < 8; j++) o[j] = acc[k][j][h];
-          Vec8<OT>::store(out + (size_t)r * cols + col, o);
-        }
-      } else {
-        const int r = r0 + k * 16 + c;
+        for (int j = 0; j < 8; j++) o[j] = acc[k][j][h];
+        Vec8<OT>::store(out + (size_t)(r + h) * cols + col, o);
+      }
+    } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const int n = cb + 8 * (4 * q + h) + j;
-          if (r < R && n < cols) out[(size_t)n * R + r] = from_f<OT>(acc[k][j][h]);
+      for (int j = 0; j < 8; j++) {
+        OT* at = out + (size_t)(col + j) * R + r;
+        if constexpr (sizeof(OT) == 4) {
+          *reinterpret_cast<f32x4_t*>(at) = acc[k][j];
+        } else {
+          uint32_t w[2];
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            w[h] = (uint32_t)__builtin_bit_cast(uint16_t, from_f<OT>(acc[k][j][2 * h])) |
+                   ((uint32_t)__builtin_bit_cast(uint16_t, from_f<OT>(acc[k][j][2 * h + 1])) << 16);
+          *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
         }
       }
     }
   }
 }
 
-// out[i] = sum over the shares of their fp32 partials, 8 values a thread, of
-// both gradients one after the other.
-struct SumArgs {
-  const float* part[2];
-  void* out[2];
-  int64_t n[2];
-  int shares;
-};
+template <typename XT, int RB>
+__global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs p) {
+  constexpr int XW = sizeof(XT) / 2;            // 16-byte loads of 8 columns
+  constexpr int U = RB == 4 ? 2 : 4, ST = 4 * U;  // rows of a step
+  __shared__ f32x4_t red[kOuterWaves / 2][RB * 8 * 64];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const OuterSide sd = p.side[blockIdx.z % (uint32_t)p.sides];
+  const int r0 = (int)(blockIdx.z / (uint32_t)p.sides) * (RB * 16);
+  const int R = p.R, cols = sd.cols, cb = blockIdx.x * kOuterCols;
+  if (cb >= cols) return;
+  const int col = cb + 8 * c;
+  const Chunks ck = find_chunks(p.offsets, p.G, p.chunk, blockIdx.y, -1);
+  if (ck.g >= p.G) return;
+  const XT* const wide = (const XT*)sd.wide + col;
+  const float* const small = sd.small + r0 + c;
+  const size_t per = (size_t)R * cols;
+  const uint32_t rows = (ck.o1 - ck.o0 + ck.n - 1) / ck.n;  // of an equal chunk
+  const uint32_t s0 = min(ck.o1, ck.o0 + (blockIdx.y - ck.first) * rows), s1 = min(ck.o1, s0 + rows);
+  {
+    const uint32_t len = ((s1 - s0 + kOuterWaves - 1) / kOuterWaves + 3u) & ~3u;
+    const uint32_t b0 = min(s1, s0 + (uint32_t)wave * len), b1 = min(s1, b0 + len);
+    f32x4_t acc[RB][8] = {};
+    if (b0 < b1) {
+      u32x4_t wv[U][XW];
+      float sv[U][RB];
+      auto rows_at = [&](uint32_t at) { return p.perm[min(at + c, b1 - 1)]; };  // a row per lane of a group
+      auto load = [&](uint32_t at, uint32_t pv) {
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+          const uint32_t t = (uint32_t)__shfl((int)pv, 4 * i + q, kWave);
+          const bool in = at + 4 * i + q < b1;
+#pragma unroll
+          for (int h = 0; h < XW; h++) wv[i][h] = u32x4_t{0u, 0u, 0u, 0u};
+          if (in && col < cols) {
+#pragma unroll
+            for (int h = 0; h < XW; h++)
+              wv[i][h] = *reinterpret_cast<const u32x4_t*>(wide + (size_t)t * cols + h * 4);
+          }
+#pragma unroll
+          for (int j = 0; j < RB; j++) {
+            sv[i][j] = 0.f;
+            if (in && r0 + j * 16 + c < R) sv[i][j] = small[(size_t)t * R + j * 16];
+          }
+        }
+      };
+      uint32_t pv = rows_at(b0), pn = rows_at(b0 + ST);
+      load(b0, pv);
+      for (uint32_t at = b0; at < b1; at += ST) {
+        u32x4_t w0[U][XW];
+        float s[U][RB];
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+#pragma unroll
+          for (int h = 0; h < XW; h++) w0[i][h] = wv[i][h];
+#pragma unroll
+          for (int j = 0; j < RB; j++) s[i][j] = sv[i][j];
+        }
+        pv = pn;
+        pn = rows_at(at + 2 * ST);
+        load(at + ST, pv);
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+          float w[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            if constexpr (XW == 2) w[j] = __uint_as_float(w0[i][j >> 2][j & 3]);
+            else w[j] = to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(w0[i][0][j >> 1] >> (16 * (j & 1)))));
+          }
+#pragma unroll
+          for (int k = 0; k < RB; k++)
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+              acc[k][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[i][k], w[j], acc[k][j], 0, 0, 0);
+        }
+      }
+    }
+    // the upper half of the waves hands its sums to the lower, down to one
+#pragma unroll
+    for (int half = kOuterWaves / 2; half >= 1; half >>= 1) {
+      if (wave >= half && wave < 2 * half) {
+#pragma unroll
+        for (int k = 0; k < RB; k++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) red[wave - half][(k * 8 + j) * 64 + lane] = acc[k][j];
+      }
+      lds_barrier();
+      if (wave < half) {
+#pragma unroll
+        for (int k = 0; k < RB; k++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) acc[k][j] += red[wave][(k * 8 + j) * 64 + lane];
+      }
+      lds_barrier();
+    }
+    if (wave == 0) {
+      if (ck.n == 1) outer_store<XT, RB>(acc, (XT*)sd.out + ck.g * per, sd.rank_major, R, cols, r0, cb, c, q);
+      else outer_store<float, RB>(acc, sd.part + blockIdx.y * per, sd.rank_major, R, cols, r0, cb, c, q);
+    }
+  }
+}
+
+// Adds the chunks of the adapters that have several, and writes zeros for
+// those without rows; the others are there already.
 template <typename XT>
-__global__ __launch_bounds__(256) void lora_sum_kernel(SumArgs p) {
-  const int64_t all = p.n[0] + p.n[1];
-  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; at < all; at += (int64_t)gridDim.x * 2048) {
-    const int w = at >= p.n[0];
-    const int64_t i = at - (w ? p.n[0] : 0), n = p.n[w];
-    float a[8];
-    Vec8<float>::load(p.part[w] + i, a);
-    for (int z = 1; z < p.shares; z++) {
+__global__ __launch_bounds__(256) void lora_sum_kernel(OuterArgs p) {
+  const OuterSide sd = p.side[blockIdx.z];
+  const int g = blockIdx.y;
+  const Chunks ck = find_chunks(p.offsets, p.G, p.chunk, 0, g);
+  if (ck.n == 1) return;
+  const size_t per = (size_t)p.R * sd.cols;
+  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8; i < per; i += (size_t)gridDim.x * 2048) {
+    float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t c = 0; c < ck.n; c++) {
       float b[8];
-      Vec8<float>::load(p.part[w] + (size_t)z * n + i, b);
+      Vec8<float>::load(sd.part + (ck.first + c) * per + i, b);
 #pragma unroll
       for (int j = 0; j < 8; j++) a[j] += b[j];
     }
-    Vec8<XT>::store((XT*)p.out[w] + i, a);
+    Vec8<XT>::store((XT*)sd.out + g * per + i, a);
   }
 }
 
@@ -881,13 +927,19 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 // the wide rows are read once.
 int outer_ranks(int R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
 
-// Shares of an adapter's rows in the outer products: a block per CU, no shares
-// below 64 rows.
-int outer_shares(const LoraDims& d) {
+// Rows of a chunk in the outer products: about two blocks per CU with the
+// adapters' last, smaller chunks, at least 64. The chunks of all adapters are
+// at most outer_chunks.
+uint32_t outer_chunk(const LoraDims& d) {
   const int rt = outer_ranks(d.R) * 16;
-  const long blocks = (long)d.G * ((d.K + kOuterCols - 1) / kOuterCols + (d.N + kOuterCols - 1) / kOuterCols) *
+  const long blocks = (long)((d.K + kOuterCols - 1) / kOuterCols + (d.N + kOuterCols - 1) / kOuterCols) *
                       ((d.R + rt - 1) / rt);
-  return (int)std::max(1L, std::min({256 / blocks, (long)(d.T + 63) / 64, 16L}));
+  const long chunks = std::max(4L, 512 / blocks - d.G / 2);
+  return (uint32_t)std::max(64L, (d.T + chunks - 1) / chunks);
+}
+long outer_chunks(const LoraDims& d) {
+  const long chunk = outer_chunk(d);
+  return std::min<long>(d.T, (d.T + chunk - 1) / chunk + d.G);
 }
 
 struct BackwardLayout {
@@ -914,8 +966,7 @@ BackwardLayout backward_layout(const LoraDims& d) {
   l.used = take((G + 1) * 4);
   l.scratch_bytes = dispatch_scratch_bytes(d.T, 1, d.G);
   l.scratch = take(l.scratch_bytes);
-  const size_t sh = outer_shares(d);
-  l.part = take(sh > 1 ? sh * G * R * (K + N) * 4 : 0);
+  l.part = take((size_t)outer_chunks(d) * R * (K + N) * 4);
   l.total = at;
   return l;
 }
@@ -986,42 +1037,32 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
   OuterArgs o{};
   o.perm = perm;
   o.offsets = offsets;
-  o.T = d.T;
   o.R = d.R;
   o.G = d.G;
-  o.shares = outer_shares(d);
-  const size_t na = (size_t)d.G * d.R * d.K, nb = (size_t)d.G * d.R * d.N;
-  float* pa = reinterpret_cast<float*>(ws + l.part);
-  float* pb = pa + (size_t)o.shares * na;
+  o.chunk = outer_chunk(d);
+  const long chunks = outer_chunks(d);
+  float* const part = reinterpret_cast<float*>(ws + l.part);
   int cols = 0;
   if (a.da) {
-    o.side[o.sides++] = {a.x, u, o.shares > 1 ? (void*)pa : a.da, d.K, 1};
+    o.side[o.sides++] = {a.x, u, a.da, part, d.K, 1};
     cols = std::max(cols, d.K);
   }
   if (a.db) {
-    o.side[o.sides++] = {a.dy, s, o.shares > 1 ? (void*)pb : a.db, d.N, 0};
+    o.side[o.sides++] = {a.dy, s, a.db, part + (size_t)chunks * d.R * d.K, d.N, 0};
     cols = std::max(cols, d.N);
   }
   const int RB = outer_ranks(d.R);
-  const dim3 grid((cols + kOuterCols - 1) / kOuterCols, o.shares * ((d.R + RB * 16 - 1) / (RB * 16)), d.G * o.sides);
-#define MOE_OU2(OT, RB) \
-  hipLaunchKernelGGL((lora_outer_kernel<XT, OT, RB>), grid, dim3(64 * kOuterWaves), 0, st, o)
-#define MOE_OU(RB)                   \
-  if (o.shares > 1) MOE_OU2(float, RB); \
-  else MOE_OU2(XT, RB);
-  if (RB == 1) { MOE_OU(1) }
-  else if (RB == 2) { MOE_OU(2) }
-  else { MOE_OU(4) }
+  const dim3 grid((cols + kOuterCols - 1) / kOuterCols, (uint32_t)chunks, o.sides * ((d.R + RB * 16 - 1) / (RB * 16)));
+#define MOE_OU(RB) hipLaunchKernelGGL((lora_outer_kernel<XT, RB>), grid, dim3(64 * kOuterWaves), 0, st, o)
+  if (RB == 1) MOE_OU(1);
+  else if (RB == 2) MOE_OU(2);
+  else MOE_OU(4);
 #undef MOE_OU
-#undef MOE_OU2
   MOE_OKAY(hipGetLastError());
-  if (o.shares > 1) {
-    const SumArgs sm{{pa, pb}, {a.da, a.db}, {a.da ? (int64_t)na : 0, a.db ? (int64_t)nb : 0}, o.shares};
-    const size_t n = sm.n[0] + sm.n[1];
-    hipLaunchKernelGGL((lora_sum_kernel<XT>), dim3((uint32_t)std::min<size_t>((n + 2047) / 2048, 2048)),
-                       dim3(256), 0, st, sm);
-    MOE_OKAY(hipGetLastError());
-  }
+  const size_t per = (size_t)d.R * cols;
+  hipLaunchKernelGGL((lora_sum_kernel<XT>), dim3((uint32_t)std::min<size_t>((per + 2047) / 2048, 512), d.G, o.sides),
+                     dim3(256), 0, st, o);
+  MOE_OKAY(hipGetLastError());
 #undef MOE_OKAY
   return hipSuccess;
 }
