@@ -15,6 +15,7 @@
 // the kernels are made to read x, y and the adapters once, in whole lines, and
 // to spread few rows over the chip.
 #include <algorithm>
+#include <utility>
 
 #include "moe_common.hpp"
 #include "moe_internal.hpp"
@@ -136,8 +137,7 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs p) {
 // y[t][n] = round(y_in[t][n] + sum_r scale_g s[t][r] b[g][n][r]), with s either
 // computed by the same block (FUSED: eight waves share K for a tile of 16
 // rows, meet in LDS, and then share N, so that a call is one launch) or added
-// up from a shrink launch's shares of K (the columns are then also shared by
-// gridDim.z blocks: few rows with large adapters).
+// up from a shrink launch's shares of K (few rows with large adapters).
 //
 // For 16-bit adapters s enters the product as two 16-bit parts, hi = round(s)
 // and lo = round(s - hi), laid side by side along the product's 32-value
@@ -162,8 +162,9 @@ struct ExpandArgs {
 // run side by side.
 struct ExpandJobs {
   ExpandArgs job[2];
-  int leaders;  // blocks of a tile
-  int run;      // tiles of an XCD, 0 for few
+  int team;    // blocks of a tile
+  int shares;  // of an adapter's columns, at most
+  int run;     // tiles of an XCD, 0 for few
 };
 
 constexpr int kFusedWaves = 8;
@@ -227,6 +228,14 @@ __device__ __forceinline__ void expand_operand(const float* row, int c8, int q, 
   }
 }
 
+template <typename F, int... I>
+__device__ __forceinline__ void static_for(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I + 1>{}), ...);
+}
+template <typename F> __device__ __forceinline__ void static_for_15(F&& f) {
+  static_for(f, std::make_integer_sequence<int, 15>{});
+}
+
 // Orders this wave's LDS accesses of different lanes; loads from global memory
 // stay in flight across it.
 __device__ __forceinline__ void wave_lds_sync() {
@@ -241,32 +250,15 @@ constexpr int expand_waves(size_t es, int rt) { return rt <= (es == 4 ? 2 : 4) ?
 
 template <typename XT, int RT, bool FUSED>
 __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) void lora_expand_kernel(ExpandJobs jobs) {
-  const ExpandArgs& p = jobs.job[FUSED ? blockIdx.y : 0];
-  // Consecutive blocks go to the eight XCDs in turn. Many tiles: each XCD takes a
-  // run of neighbours, whose rows share adapters in its L2, all first leaders
-  // before the second ones. Few: the tiles' first leaders are spread, then the
-  // second ones.
-  const int lead_of = jobs.leaders;
-  int leader, tile;
-  if (jobs.run > 0) {
-    const int i = (int)(blockIdx.x >> 3);
-    leader = i / jobs.run;
-    tile = (int)(blockIdx.x & 7u) * jobs.run + i % jobs.run;
-  } else {
-    const uint32_t tiles = (uint32_t)(p.T + kTile - 1) / kTile;
-    leader = (int)(blockIdx.x / tiles);
-    tile = (int)(blockIdx.x % tiles);
-  }
-  if (tile * (long)kTile >= p.T) return;
   constexpr bool F32 = sizeof(XT) == 4;
   constexpr uint32_t ES = sizeof(XT);
   constexpr int V = 16 / sizeof(XT), LD = RT * 16 + 4, W = kFusedWaves;
-  constexpr int UNIT = 8 * V;                             // a unit of K: 128 bytes of a row
-  constexpr int J = F32 ? (RT == 8 ? 2 : 4) : 4;  // neighbouring columns of a lane
-  constexpr int NC = 16 * J;                              // columns of a group
-  constexpr int C8 = RT * 16 / V;                         // 16-byte chunks of the widest adapter row
-  constexpr int BL = NC * C8 / 64;                        // loads of a column group's b rows
-  constexpr bool EARLY = BL < 4;  // the first group's loads go out before the shrink half
+  constexpr int UNIT = 8 * V;                      // a unit of K: 128 bytes of a row
+  constexpr int J = F32 ? (RT == 8 ? 2 : 4) : 4;   // neighbouring columns of a lane
+  constexpr int NC = 16 * J;                       // columns of a group
+  constexpr int C8 = RT * 16 / V;                  // 16-byte chunks of the widest adapter row
+  constexpr int BL = NC * C8 / 64;                 // loads of a column group's b rows
+  constexpr bool EARLY = BL < 4;                   // the first group's loads go out before the shrink half
   constexpr int AREA = (1 + RT) * 128 > NC * (C8 | 1) ? (1 + RT) * 128 : NC * (C8 | 1);  // 16-byte slots
   static_assert(AREA * 4 >= 2 * kTile * LD, "the sums of a wave and of the block fit an area");
   // a wave's area holds in turn its units, its sums and its column groups; the
@@ -275,6 +267,22 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
   float* const sum = reinterpret_cast<float*>(area[0]) + kTile * LD;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const ExpandArgs& p = jobs.job[FUSED ? blockIdx.y : 0];
+  // Consecutive blocks go to the eight XCDs in turn. Many tiles: each XCD takes a
+  // run of neighbours, whose rows share adapters in its L2, all first blocks of
+  // a tile before the second ones. Few: the tiles' first blocks are spread, then
+  // the second ones.
+  int member, tile;  // one of jobs.team blocks of a tile
+  if (jobs.run > 0) {
+    const int i = (int)(blockIdx.x >> 3);
+    member = i / jobs.run;
+    tile = (int)(blockIdx.x & 7u) * jobs.run + i % jobs.run;
+  } else {
+    const uint32_t tiles = (uint32_t)(p.T + kTile - 1) / kTile;
+    member = (int)(blockIdx.x / tiles);
+    tile = (int)(blockIdx.x % tiles);
+  }
+  if (tile * (long)kTile >= p.T) return;
   const int t0 = tile * kTile, rows = min(kTile, p.T - t0);
   const int ad = tile_adapter(p.adapter, t0, rows, tid & 15, p.G);
   const int K = p.K, N = p.N, R = p.R, c8 = R / V;
@@ -283,28 +291,46 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
                               p.yin ? (uint32_t)rows * (uint32_t)N * ES : 0u);
   const rsrc_t wr = make_rsrc((XT*)p.y + (p.y ? (size_t)t0 * N : 0), p.y ? (uint32_t)rows * (uint32_t)N * ES : 0u);
   u32x4_t* const mem = area[wave];
+  // The team's members take the tile's adapters in turn; where there are fewer
+  // adapters than members, several share the columns of one (each repeating
+  // its sums).
+  uint32_t todo = (1u << rows) - 1u;  // rows with something to do
+  if (p.y == nullptr || p.yin == p.y) todo &= (uint32_t)__ballot(ad >= 0);
+  // the first row of each of their distinct adapters: rows whose id no row
+  // before them has
+  bool again = false;
+  static_for_15([&](auto i) { again |= dpp_i32<0x110 + decltype(i)::value, 0xF>(-2, ad) == ad; });
+  uint32_t heads = (uint32_t)__ballot(!again) & todo;
+  const int D = __builtin_popcount(heads);
+  const int team = jobs.team;
+  int first = member, share = 0, shares = 1;
+  if (D == 0) return;
+  if (D < team) {
+    first = member % D;
+    share = member / D;
+    shares = min(p.y ? jobs.shares : 1, (team - first + D - 1) / D);
+    if (share >= shares) return;
+  }
   // a wave's units of K and groups of columns are neighbours, the waves' shares
   // apart: rows are often a multiple of the 4 KB that the memory channels
   // repeat after, so that all rows of a tile ask one channel for the same k
   const int units = (K + UNIT - 1) / UNIT, uper = (units + W - 1) / W;
   const int u0 = wave * uper, u1 = min(units, u0 + uper);
-  const int cw = FUSED ? wave : (int)blockIdx.z * W + wave, cws = FUSED ? W : (int)gridDim.z * W;
+  const int cw = share * W + wave, cws = shares * W;
   const int groups = (N + NC - 1) / NC, gper = (groups + cws - 1) / cws;
   const int g0 = cw * gper, g1 = min(groups, g0 + gper);
-  uint32_t rem = (1u << rows) - 1u;
-  for (int d = 0; rem; d++) {
-    const int lead = __builtin_ctz(rem);
+  for (int d = 0; heads; d++) {
+    const int lead = __builtin_ctz(heads);
+    heads &= heads - 1u;
+    if (d < first || (d - first) % team != 0) continue;
     const int g = __builtin_amdgcn_readlane(ad, lead);
-    const uint32_t same = (uint32_t)__ballot(ad == g) & rem;
-    rem &= ~same;
-    if (d % lead_of != leader) continue;
+    const uint32_t same = (uint32_t)__ballot(ad == g) & todo;
     // (opaque: else what follows from the lane alone, some hundred addresses,
     // is computed ahead of the loop and spilled)
     int lane = tid & 63;
     asm volatile("" : "+v"(lane));
     const int c = lane & 15, q = lane >> 4;
     if (g < 0) {  // rows without an adapter: y = y_in
-      if (p.y == nullptr || p.yin == p.y) continue;
       for (int n = (cw * 8 + (lane & 7)) * V; n < N; n += 8 * cws * V) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -432,7 +458,7 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
       }
       v *= sc;
       sum[at] = v;
-      if (p.s && (FUSED || blockIdx.z == 0) && r < R && ((same >> t) & 1u)) p.s[(size_t)(t0 + t) * R + r] = v;
+      if (p.s && share == 0 && r < R && ((same >> t) & 1u)) p.s[(size_t)(t0 + t) * R + r] = v;
     }
     lds_barrier();
     if (p.y) {
@@ -838,18 +864,14 @@ namespace {
 
 int tiles_of(int T) { return (T + kTile - 1) / kTile; }
 
-// Blocks that share a tile's distinct adapters: as many as a tile can hold
-// while that leaves one block per CU, and two where the tiles fill the chip, for
-// the tiles in which one request ends and the next begins (a block that finds
-// no adapter left costs its dispatch, about a microsecond of a CU).
-int leaders(int T, int G, bool none) {
-  const int most = std::min(std::min(kTile, T), G + (none ? 1 : 0));
-  return std::min(most, std::max(2, 256 / tiles_of(T)));
+// Blocks of the shrink launch that share a tile's distinct adapters.
+int leaders(int T, int G) {
+  return std::max(1, std::min(std::min(std::min(kTile, T), G), 256 / tiles_of(T)));
 }
 
 template <typename XT>
 hipError_t shrink_typed(const ShrinkArgs& a, int S, hipStream_t st) {
-  const dim3 grid(tiles_of(a.T), leaders(a.T, a.G, false), S);
+  const dim3 grid(tiles_of(a.T), leaders(a.T, a.G), S);
 #define MOE_SH(RT) hipLaunchKernelGGL((lora_shrink_kernel<XT, RT>), grid, dim3(256), 0, st, a)
   if (a.R <= 16) MOE_SH(1);
   else if (a.R <= 32) MOE_SH(2);
@@ -859,7 +881,13 @@ hipError_t shrink_typed(const ShrinkArgs& a, int S, hipStream_t st) {
   return hipGetLastError();
 }
 
-constexpr int kRunTiles = 64;
+// The team of a tile: together about one block per CU, which share its adapters
+// or the columns of one (64 rows of 64 adapters 2048 -> 2048 at rank 16 take
+// 9.2 us with a block per adapter and 7.5 with four), and two where the tiles
+// fill the chip, for the tiles in which one request ends and the next begins:
+// there a member without an adapter returns, since repeating the sums would cost
+// more (4096 rows at rank 64: 30 us instead of 24).
+constexpr int kTeamBlocks = 256, kRunTiles = 64;
 
 // S > 0: the sums come from a shrink launch's S shares at a.part; otherwise
 // `also` (nullable) runs beside a.
@@ -868,18 +896,20 @@ hipError_t expand_typed(const ExpandArgs& a, hipStream_t st, const ExpandArgs* a
   ExpandJobs j{};
   j.job[0] = a;
   if (also) j.job[1] = *also;
-  j.leaders = leaders(a.T, a.G, a.y != nullptr && a.yin != a.y);
   const int tiles = tiles_of(a.T);
+  // at least one group of 64 columns per wave; apart all of those
+  const int most = a.y ? (a.N + 64 * kFusedWaves - 1) / (64 * kFusedWaves) : 1;
+  j.shares = a.S ? most : std::max(1, std::min(most, kTeamBlocks / tiles));
+  const int adapters = std::min(std::min(kTile, a.T), a.G + 1);
+  j.team = std::min(adapters * j.shares, std::max(2, a.S ? kTile * j.shares : kTeamBlocks / tiles));
   j.run = tiles >= kRunTiles ? (tiles + 7) / 8 : 0;
-  const uint32_t blocks = (uint32_t)(j.run ? 8 * j.run : tiles) * (uint32_t)j.leaders;
-  const int shares = a.y ? (a.N + 64 * kFusedWaves - 1) / (64 * kFusedWaves) : 1;
-#define MOE_EX(RT)                                                                                  \
-  if (a.S == 0)                                                                                     \
-    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, true>), dim3(blocks, also ? 2 : 1),              \
-                       dim3(64 * kFusedWaves), 0, st, j);                                           \
-  else                                                                                              \
-    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, false>), dim3(blocks, 1, shares),                \
-                       dim3(64 * kFusedWaves), 0, st, j);
+  const uint32_t blocks = (uint32_t)(j.run ? 8 * j.run : tiles) * (uint32_t)j.team;
+#define MOE_EX(RT)                                                                            \
+  if (a.S == 0)                                                                               \
+    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, true>), dim3(blocks, also ? 2 : 1),        \
+                       dim3(64 * kFusedWaves), 0, st, j);                                     \
+  else                                                                                        \
+    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, false>), dim3(blocks), dim3(64 * kFusedWaves), 0, st, j);
   if (a.R <= 16) { MOE_EX(1) }
   else if (a.R <= 32) { MOE_EX(2) }
   else if (a.R <= 64) { MOE_EX(4) }
