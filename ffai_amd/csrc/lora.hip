@@ -640,11 +640,16 @@ __global__ __launch_bounds__(256) void lora_prep_kernel(PrepArgs a) {
 // ----------------------------------------------------- adapter gradients --
 // dA_g[r][k] = sum_t u[t][r] x[t][k] and dB_g[n][r] = sum_t s[t][r] dy[t][n]
 // over the rows of adapter g, which the plan lists (perm, offsets); u and s
-// with their scale. fp32 matrix products of 4 rows a step: a lane reads 8
-// neighbouring columns of one row, each of which is one product's operand, so
-// the wide rows go from memory to the operand registers as they lie.
+// with their scale. A lane reads 8 neighbouring columns of a row. fp32 rows, and
+// one rank tile of any: each column is an operand of an fp32 product of 4 rows
+// (16x16x4), as it lies. More rank tiles of 16-bit rows: a lane reads 8 rows of
+// its columns and turns them in registers into the 8 columns' operands of one
+// product of 32 rows (16x16x32, eight times the rate), which u and s enter as
+// two 16-bit parts as in expand. 4096 rows of 8 adapters 2048 -> 2048: rank 16
+// 13.3 us with products of 4 rows, 15.0 with those of 32 (whose steps the
+// adapters' chunks fill less); rank 64 39 and 26.5.
 //
-// A block takes 128 columns, up to four rank tiles and a chunk of one adapter's
+// A block takes 128 columns, up to two (fp32: four) rank tiles and a chunk of one adapter's
 // rows (an adapter of n rows has ceil(n / chunk) equal ones, numbered through
 // over the adapters, so that the work is even however the rows spread); its
 // eight waves share the chunk and meet in LDS. The gradient of an adapter with
@@ -737,8 +742,9 @@ __device__ __forceinline__ void outer_store(const f32x4_t (&acc)[RB][8], OT* out
 
 template <typename XT, int RB>
 __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs p) {
-  constexpr int XW = sizeof(XT) / 2;            // 16-byte loads of 8 columns
-  constexpr int U = RB == 4 ? 2 : 4, ST = 4 * U;  // rows of a step
+  constexpr bool FOUR = sizeof(XT) == 4 || RB == 1;  // products of four rows
+  constexpr int XW = sizeof(XT) / 2;                 // 16-byte loads of 8 columns
+  constexpr int U = FOUR ? 2 : 8;                    // rows of a lane and step, 4 U of the wave
   __shared__ f32x4_t red[kOuterWaves / 2][RB * 8 * 64];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -759,14 +765,17 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
     const uint32_t b0 = min(s1, s0 + (uint32_t)wave * len), b1 = min(s1, b0 + len);
     f32x4_t acc[RB][8] = {};
     if (b0 < b1) {
+      // row i of a lane in a step: 4 i + q where every product takes four rows,
+      // 8 q + i where one takes all 32
+      auto row_of = [&](int i) { return FOUR ? 4 * i + q : 8 * q + i; };
       u32x4_t wv[U][XW];
       float sv[U][RB];
-      auto rows_at = [&](uint32_t at) { return p.perm[min(at + c, b1 - 1)]; };  // a row per lane of a group
+      auto rows_at = [&](uint32_t at) { return p.perm[min(at + (lane & 31), b1 - 1)]; };
       auto load = [&](uint32_t at, uint32_t pv) {
 #pragma unroll
         for (int i = 0; i < U; i++) {
-          const uint32_t t = (uint32_t)__shfl((int)pv, 4 * i + q, kWave);
-          const bool in = at + 4 * i + q < b1;
+          const uint32_t t = (uint32_t)__shfl((int)pv, row_of(i), kWave);
+          const bool in = at + row_of(i) < b1;
 #pragma unroll
           for (int h = 0; h < XW; h++) wv[i][h] = u32x4_t{0u, 0u, 0u, 0u};
           if (in && col < cols) {
@@ -781,34 +790,92 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
           }
         }
       };
-      uint32_t pv = rows_at(b0), pn = rows_at(b0 + ST);
+      uint32_t pv = rows_at(b0), pn = rows_at(b0 + 4 * U);
       load(b0, pv);
-      for (uint32_t at = b0; at < b1; at += ST) {
+      for (uint32_t at = b0; at < b1; at += 4 * U) {
         u32x4_t w0[U][XW];
-        float s[U][RB];
 #pragma unroll
-        for (int i = 0; i < U; i++) {
+        for (int i = 0; i < U; i++)
 #pragma unroll
           for (int h = 0; h < XW; h++) w0[i][h] = wv[i][h];
+        if constexpr (FOUR) {
+          float s[U][RB];
 #pragma unroll
-          for (int j = 0; j < RB; j++) s[i][j] = sv[i][j];
-        }
-        pv = pn;
-        pn = rows_at(at + 2 * ST);
-        load(at + ST, pv);
+          for (int i = 0; i < U; i++)
 #pragma unroll
-        for (int i = 0; i < U; i++) {
-          float w[8];
+            for (int j = 0; j < RB; j++) s[i][j] = sv[i][j];
+          pv = pn;
+          pn = rows_at(at + 8 * U);
+          load(at + 4 * U, pv);
 #pragma unroll
-          for (int j = 0; j < 8; j++) {
-            if constexpr (XW == 2) w[j] = __uint_as_float(w0[i][j >> 2][j & 3]);
-            else w[j] = to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(w0[i][0][j >> 1] >> (16 * (j & 1)))));
+          for (int i = 0; i < U; i++) {
+            if (at + 4 * i >= b1) continue;
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              if constexpr (XW == 2) w[j] = __uint_as_float(w0[i][j >> 2][j & 3]);
+              else w[j] = to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(w0[i][0][j >> 1] >> (16 * (j & 1)))));
+            }
+#pragma unroll
+            for (int k = 0; k < RB; k++)
+#pragma unroll
+              for (int j = 0; j < 8; j++)
+                acc[k][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[i][k], w[j], acc[k][j], 0, 0, 0);
+          }
+        } else {
+          // s as two 16-bit parts; f16 scaled by a power of two so that the
+          // step's largest value lies in [2^14, 2^15)
+          u32x4_t hi[RB], lo[RB];
+          float fw = 1.f, back = 1.f;
+          if constexpr (__is_same(XT, f16_t)) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < U; i++)
+#pragma unroll
+              for (int k = 0; k < RB; k++) m = fmaxf(m, fabsf(sv[i][k]));
+            m = wave_max_f32(m);
+            const int eb = (int)((__float_as_uint(m) >> 23) & 255u);
+            const int sh = eb == 255 ? 0 : min(14 - (eb - 127), 100);
+            fw = __builtin_ldexpf(1.f, sh);
+            back = __builtin_ldexpf(1.f, -sh);
           }
 #pragma unroll
-          for (int k = 0; k < RB; k++)
+          for (int k = 0; k < RB; k++) {
+            uint32_t h[8], l[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-              acc[k][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[i][k], w[j], acc[k][j], 0, 0, 0);
+            for (int i = 0; i < 8; i++) {
+              const float f = sv[i][k] * fw, fh = round_to<XT>(f);
+              h[i] = (uint32_t)__builtin_bit_cast(uint16_t, from_f<XT>(f));
+              l[i] = (uint32_t)__builtin_bit_cast(uint16_t, from_f<XT>(__builtin_isfinite(fh) ? f - fh : 0.f));
+            }
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+              hi[k][m] = h[2 * m] | (h[2 * m + 1] << 16);
+              lo[k][m] = l[2 * m] | (l[2 * m + 1] << 16);
+            }
+          }
+          pv = pn;
+          pn = rows_at(at + 8 * U);
+          load(at + 4 * U, pv);
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            // column j of the lane's 8 rows
+            u32x4_t x;
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+              x[m] = __builtin_amdgcn_perm(w0[2 * m + 1][0][j >> 1], w0[2 * m][0][j >> 1],
+                                           j & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int k = 0; k < RB; k++) {
+              if constexpr (__is_same(XT, f16_t)) {
+                const f32x4_t o = mma<XT>(lo[k], x, mma<XT>(hi[k], x, f32x4_t{0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+                for (int h = 0; h < 4; h++) acc[k][j][h] = __builtin_fmaf(o[h], back, acc[k][j][h]);
+              } else {
+                acc[k][j] = mma<XT>(lo[k], x, mma<XT>(hi[k], x, acc[k][j]));
+              }
+            }
+          }
         }
       }
     }
@@ -953,15 +1020,15 @@ constexpr int kPrepRows = 16384;  // rows the prep launch lists; more take a pla
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Rank tiles of a block of the outer products: all of them up to four, so that
-// the wide rows are read once.
-int outer_ranks(int R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
+// Rank tiles of a block of the outer products, so that the wide rows are read
+// once or twice: as many as leave the registers for a step ahead.
+int outer_ranks(const LoraDims& d) { return d.R <= 16 ? 1 : d.R <= 32 || d.dt != DT_F32 ? 2 : 4; }
 
 // Rows of a chunk in the outer products: about two blocks per CU with the
 // adapters' last, smaller chunks, at least 64. The chunks of all adapters are
 // at most outer_chunks.
 uint32_t outer_chunk(const LoraDims& d) {
-  const int rt = outer_ranks(d.R) * 16;
+  const int rt = outer_ranks(d) * 16;
   const long blocks = (long)((d.K + kOuterCols - 1) / kOuterCols + (d.N + kOuterCols - 1) / kOuterCols) *
                       ((d.R + rt - 1) / rt);
   const long chunks = std::max(4L, 512 / blocks - d.G / 2);
@@ -1081,12 +1148,12 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
     o.side[o.sides++] = {a.dy, s, a.db, part + (size_t)chunks * d.R * d.K, d.N, 0};
     cols = std::max(cols, d.N);
   }
-  const int RB = outer_ranks(d.R);
+  const int RB = outer_ranks(d);
   const dim3 grid((cols + kOuterCols - 1) / kOuterCols, (uint32_t)chunks, o.sides * ((d.R + RB * 16 - 1) / (RB * 16)));
 #define MOE_OU(RB) hipLaunchKernelGGL((lora_outer_kernel<XT, RB>), grid, dim3(64 * kOuterWaves), 0, st, o)
   if (RB == 1) MOE_OU(1);
   else if (RB == 2) MOE_OU(2);
-  else MOE_OU(4);
+  else if constexpr (sizeof(XT) == 4) MOE_OU(4);
 #undef MOE_OU
   MOE_OKAY(hipGetLastError());
   const size_t per = (size_t)d.R * cols;
