@@ -1188,8 +1188,8 @@ extern "C" moe_status moe_balance_loss(const void* logits, int32_t dtype, int32_
     return fail(MOE_ERR_INVALID, "balance_loss: NULL pointer");
   MOE_TRY(validate_router_rows("balance_loss", dtype, T, n_experts, k, gating, logit_scale, 1.f));
   const size_t need = balance_ws_bytes(T, n_experts);
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(MOE_ERR_WORKSPACE, "balance_loss: workspace of %zu bytes needed", need);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(MOE_ERR_WORKSPACE, "balance_loss: 16-byte aligned workspace of %zu bytes needed", need);
   MOE_HIP(launch_balance_loss(logits, dtype, T, n_experts, k, gating == MOE_SIGMOID_TOPK,
                               logit_scale == 0.f ? 1.f : logit_scale, topk_idx, mask, counts,
                               prob_sum, losses, workspace, stream),

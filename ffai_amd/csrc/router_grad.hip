@@ -184,12 +184,16 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 }
 
 // Partials of block b: P [E4] fp32 and picks [E4] u32 (E4 = E rounded up to
-// 4, the rest zeros), then z and the counted rows.
+// 4, the rest zeros), then z and the counted rows; then what the second
+// launch's blocks leave for the last of them.
+constexpr int kBalMaxBlocks = 256, kFinalCols = 32, kFinalBlocks = kTopkMaxE / kFinalCols;
 struct BalancePart {
   float* P;
   uint32_t* cnt;
   float* z;
   uint32_t* n;
+  double* dot;       // [kFinalBlocks]
+  uint32_t* ticket;  // blocks that are done
 };
 __host__ __device__ inline BalancePart balance_part(void* ws, int nb, int E4) {
   BalancePart p;
@@ -197,6 +201,8 @@ __host__ __device__ inline BalancePart balance_part(void* ws, int nb, int E4) {
   p.cnt = reinterpret_cast<uint32_t*>(p.P + (size_t)nb * E4);
   p.z = reinterpret_cast<float*>(p.cnt + (size_t)nb * E4);
   p.n = reinterpret_cast<uint32_t*>(p.z + nb);
+  p.dot = reinterpret_cast<double*>(p.n + nb);
+  p.ticket = reinterpret_cast<uint32_t*>(p.dot + kFinalBlocks);
   return p;
 }
 
@@ -343,95 +349,102 @@ __global__ __launch_bounds__(64 * kBalWaves) void balance_rows_kernel(BalanceArg
   if (tid == 0) {
     bp.z[blockIdx.x] = z;
     bp.n[blockIdx.x] = nn;
+    if (blockIdx.x == 0) *bp.ticket = 0u;
   }
 }
 
-// Adds the blocks' partials and forms the losses: one workgroup, four experts
-// a thread (16-byte loads), 2^lgc >= E4 / 4 threads across the experts, the
-// others across the blocks.
-constexpr int kBalMaxBlocks = 256;
-__global__ __launch_bounds__(1024) void balance_final_kernel(void* ws, int nb, int E, int k, int lgc,
+// Adds the blocks' partials: a block per 32 experts (a CU reads about 100
+// bytes a nanosecond, 256 x 256 partials are 512 KB: one block took 6.9 us), four
+// experts a thread (16-byte loads), 128 threads across the partials. The last
+// block to finish, by a ticket that the launch before set to 0, adds the
+// blocks' parts of sum_e c_e P_e in their order and forms the losses.
+__global__ __launch_bounds__(1024) void balance_final_kernel(void* ws, int nb, int E, int k,
                                                              uint32_t* __restrict__ counts,
                                                              float* __restrict__ prob_sum,
                                                              float* __restrict__ losses) {
-  __shared__ float sP[1024][4];
-  __shared__ uint32_t sC[1024][4];
-  __shared__ double sDot[16], sZ[16];
-  __shared__ uint32_t sN[16];
+  __shared__ float sP[16][kFinalCols];
+  __shared__ uint32_t sC[16][kFinalCols];
+  __shared__ double sZ[4];
+  __shared__ uint32_t sN[4];
   const int E4 = (E + 3) & ~3;
   const BalancePart bp = balance_part(ws, nb, E4);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int e0 = (tid & ((1 << lgc) - 1)) * 4, sl = tid >> lgc, ns = 1024 >> lgc;
+  const int c0 = blockIdx.x * kFinalCols, e0 = c0 + (tid & 7) * 4;
   const float zb = tid < nb ? bp.z[tid] : 0.f;
   const uint32_t nbk = tid < nb ? bp.n[tid] : 0u;
-  float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
-  uint4 c = make_uint4(0u, 0u, 0u, 0u);
+  float p[4] = {0.f, 0.f, 0.f, 0.f};
+  uint32_t c[4] = {0u, 0u, 0u, 0u};
   if (e0 < E4) {
-    for (int b0 = sl; b0 < nb; b0 += 8 * ns) {  // 16 loads in flight
-      float4 v[8];
-      uint4 w[8];
+    float4 v[2];
+    uint4 w[2];
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int b = b0 + i * ns;
-        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        w[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (b < nb) {
-          v[i] = *reinterpret_cast<const float4*>(bp.P + (size_t)b * E4 + e0);
-          w[i] = *reinterpret_cast<const uint4*>(bp.cnt + (size_t)b * E4 + e0);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        p.x += v[i].x; p.y += v[i].y; p.z += v[i].z; p.w += v[i].w;
-        c.x += w[i].x; c.y += w[i].y; c.z += w[i].z; c.w += w[i].w;
+    for (int i = 0; i < kBalMaxBlocks / 128; i++) {
+      const int b = (tid >> 3) + i * 128;
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      w[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (b < nb) {
+        v[i] = *reinterpret_cast<const float4*>(bp.P + (size_t)b * E4 + e0);
+        w[i] = *reinterpret_cast<const uint4*>(bp.cnt + (size_t)b * E4 + e0);
       }
     }
+    p[0] = v[0].x + v[1].x; p[1] = v[0].y + v[1].y; p[2] = v[0].z + v[1].z; p[3] = v[0].w + v[1].w;
+    c[0] = w[0].x + w[1].x; c[1] = w[0].y + w[1].y; c[2] = w[0].z + w[1].z; c[3] = w[0].w + w[1].w;
   }
-  *reinterpret_cast<float4*>(sP[tid]) = p;
-  *reinterpret_cast<uint4*>(sC[tid]) = c;
-  __syncthreads();
-  // thread e: expert e over the slices, 8 to 256 of them
-  double dot = 0.0;
-  if (tid < E) {
-    const float* ps = &sP[tid >> 2][tid & 3];
-    const uint32_t* cs = &sC[tid >> 2][tid & 3];
-    double pe = 0.0;
-    uint32_t ce = 0;
-    for (int q = 0; q < ns; q += 8) {
-      float a[8];
+  // the wave's eight threads per four experts, then the waves
 #pragma unroll
-      for (int i = 0; i < 8; i++) a[i] = ps[(size_t)((q + i) << lgc) * 4];
+  for (int j = 0; j < 4; j++) {
+    p[j] += dpp_f32<0x128, 0xF>(0.f, p[j]);  // row_ror:8
+    c[j] += (uint32_t)dpp_i32<0x128, 0xF>(0, (int)c[j]);
+    Halves h = swap16(p[j]);
+    p[j] = h.a + h.b;
+    h = swap32(p[j]);
+    p[j] = h.a + h.b;
+    c[j] += (uint32_t)__shfl_xor((int)c[j], 16, kWave);
+    c[j] += (uint32_t)__shfl_xor((int)c[j], 32, kWave);
+  }
+  if (lane < 8) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) ce += cs[(size_t)((q + i) << lgc) * 4];
-      pe += (double)(((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7])));
+    for (int j = 0; j < 4; j++) {
+      sP[wave][lane * 4 + j] = p[j];
+      sC[wave][lane * 4 + j] = c[j];
     }
-    prob_sum[tid] = (float)pe;
-    counts[tid] = ce;
-    dot = pe * (double)ce;
   }
-  const int waves = (max(E, nb) + 63) / 64;  // those that hold an expert or a block
-  if (wave < waves) {
-    dot = wave_sum_f64(dot);
+  if (wave < 4) {  // up to 256 blocks
     const double z = wave_sum_f64((double)zb);
     const uint32_t n = wave_scan_u32(nbk);
     if (lane == 63) {
-      sDot[wave] = dot;
       sZ[wave] = z;
       sN[wave] = n;
     }
   }
   __syncthreads();
-  if (tid == 0) {
-    double d = 0.0, zz = 0.0;
-    uint32_t nn = 0;
-    for (int w = 0; w < waves; w++) {
-      d += sDot[w];
-      zz += sZ[w];
-      nn += sN[w];
+  if (wave != 0) return;
+  double dot = 0.0;
+  if (lane < kFinalCols && c0 + lane < E) {
+    double pe = 0.0;
+    uint32_t ce = 0;
+#pragma unroll
+    for (int w = 0; w < 16; w += 2) {
+      pe += (double)(sP[w][lane] + sP[w + 1][lane]);
+      ce += sC[w][lane] + sC[w + 1][lane];
     }
-    counts[E] = nn;
-    store_losses(d, zz, nn, E, k, losses);
+    prob_sum[c0 + lane] = (float)pe;
+    counts[c0 + lane] = ce;
+    dot = pe * (double)ce;
   }
+  dot = wave_sum_f64(dot);
+  if (lane != 63) return;
+  if (gridDim.x > 1) {
+    __hip_atomic_store(&bp.dot[blockIdx.x], dot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t done = __hip_atomic_fetch_add(bp.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    if (done + 1 != gridDim.x) return;
+    dot = 0.0;
+    for (uint32_t b = 0; b < gridDim.x; b++)
+      dot += __hip_atomic_load(&bp.dot[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  const uint32_t n = (sN[0] + sN[1]) + (sN[2] + sN[3]);
+  counts[E] = n;
+  store_losses(dot, (sZ[0] + sZ[1]) + (sZ[2] + sZ[3]), n, E, k, losses);
 }
 
 namespace {
@@ -455,7 +468,7 @@ int balance_blocks(int T, int E) {
 
 size_t balance_ws_bytes(int T, int E) {
   const int nb = balance_blocks(T, E);
-  return nb == 1 ? 0 : (size_t)nb * (((E + 3) & ~3) + 1) * 8;
+  return nb == 1 ? 0 : (size_t)nb * (((E + 3) & ~3) + 1) * 8 + kFinalBlocks * 8 + 8;
 }
 
 #define MOE_LG(lg, MACRO) \
@@ -486,12 +499,9 @@ static hipError_t balance_typed(const void* logits, int T, int E, int k, bool si
   break;
   MOE_LG(lg, MOE_BL)
 #undef MOE_BL
-  if (nb > 1) {
-    int lgc = 0;
-    while ((4 << lgc) < E) lgc++;
-    hipLaunchKernelGGL(balance_final_kernel, dim3(1), dim3(1024), 0, st, ws, nb, E, k, lgc, counts,
-                       prob_sum, losses);
-  }
+  if (nb > 1)
+    hipLaunchKernelGGL(balance_final_kernel, dim3((E + kFinalCols - 1) / kFinalCols), dim3(1024), 0, st,
+                       ws, nb, E, k, counts, prob_sum, losses);
   return hipGetLastError();
 }
 

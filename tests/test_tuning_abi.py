@@ -47,6 +47,7 @@ BAD_ROWS = [
     (dict(losses=None), MOE_ERR_INVALID, "NULL"),
     (dict(T=100000), MOE_ERR_WORKSPACE, "workspace"),
     (dict(T=100000, ws=p(6), ws_bytes=16), MOE_ERR_WORKSPACE, "workspace"),
+    (dict(T=100000, ws=C.c_void_p(BIG * 7 + 8), ws_bytes=BIG), MOE_ERR_WORKSPACE, "aligned"),
 ])
 def test_balance_loss_refuses(kw, status, needle):
     assert call("moe_balance_loss", BAL, **kw) == status
