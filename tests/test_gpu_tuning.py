@@ -401,6 +401,9 @@ SHAPES = [
     (17, 200, 264, 16, 40, "each"), (64, 512, 512, 16, 64, "each"), (100, 1032, 72, 40, 7, "each"), (15, 128, 2880, 64, 4, "requests"),
     (130, 2880, 128, 128, 5, "requests"), (333, 96, 328, 8, 1, "one"), (700, 320, 256, 72, 9, "requests"), (33, 64, 64, 16, 4, "none"),
     (1100, 128, 128, 16, 300, "each"), (2100, 64, 64, 8, 3, "requests"),
+    # large adapters met by few rows (their sums come from a launch of their own), one and two tiles, the last group
+    # of columns cut short
+    (1, 2048, 1096, 64, 3, "one"), (20, 1544, 2056, 40, 6, "each"), (31, 512, 1600, 128, 2, "requests"),
 ]
 
 
@@ -506,6 +509,31 @@ def test_lora_backward(dt, T, K, N, R, G, kind):
     assert nx is None and same_bits(na, ga) and same_bits(nb, gb)
     zx = l.backward(x.cuda(), dy.cuda(), ac)[0]
     close(zx, rdx - dx.double(), rmag, "dx of the adapters alone")
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_lora_backward_many_rows(dt):
+    """More rows than the first launch lists itself, spread unevenly over the
+    adapters (one has none, one most of them), ids out of range among them."""
+    T, K, N, R, G = 20011, 64, 40, 24, 70
+    x, A, B, scale, _ = lora_case(T, K, N, R, G, dt, 5)
+    g = gen(9)
+    ad = torch.where(torch.rand(T, generator=g) < 0.6, 3, torch.randint(-1, G + 1, (T,), generator=g)).to(torch.int32)
+    ad[ad == 5] = 6
+    dy = torch.randn(T, N, generator=g).to(dt)
+    gx, ga, gb = tuning.LoRAAdapters(A.cuda(), B.cuda(), scale.cuda()).backward(x.cuda(), dy.cuda(), ad.cuda())
+    sp = split_err(dt)
+    assert (ga[5] == 0).all() and (gb[5] == 0).all()
+    for a in (0, 3, 6, 63, 64, 69):
+        r = (ad == a).nonzero()[:, 0]
+        s, X, D, Aa, Bb = float(scale[a]), x[r].double(), dy[r].double(), A[a].double(), B[a].double()
+        u, s1 = s * D @ Bb, s * X @ Aa.t()
+        um, sm = s * D.abs() @ Bb.abs(), s * X.abs() @ Aa.abs().t()
+        close(gx.cpu()[r], u @ Aa, (um @ Aa.abs()) * ((N + R + 16) * U + sp), f"dx {a}")
+        close(ga[a], u.t() @ X, (um.t() @ X.abs()) * ((N + len(r) + 16) * U + sp), f"da {a}")
+        close(gb[a], D.t() @ s1, (D.abs().t() @ sm) * ((K + len(r) + 16) * U + sp), f"db {a}")
+    none = (ad < 0) | (ad >= G)
+    assert (gx.cpu()[none] == 0).all()
 
 
 def test_lora_backward_matches_differences():
