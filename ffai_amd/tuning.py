@@ -28,59 +28,34 @@ from ._lib import Lora, check
 from .layer import MoERouter, moe_dtype
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_MASK = (torch.bool, torch.uint8)
+_I32, _F32 = (torch.int32,), (torch.float32,)
+
+# The current device, and the handle of a device's current stream, without the
+# objects of torch.cuda around them (0.1 us each instead of 0.3 and 1.8: a call's
+# host work is as long as its kernels where there are few rows).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _check(name: str, t: Optional[torch.Tensor], shape, dtypes, device) -> Optional[int]:
+def _check(name: str, t: Optional[torch.Tensor], shape, dtypes, index: int) -> Optional[int]:
     """The address of a tensor the kernels read or write through a raw pointer
-    (None for None)."""
+    (None for None): of `shape`, one of `dtypes`, on GPU `index` (-1: on the
+    host), contiguous."""
     if t is None:
         return None
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor")
-    if t.shape == shape and t.dtype in dtypes and t.device == device and t.is_contiguous():
+    if t.shape == shape and t.dtype in dtypes and t.get_device() == index and t.is_contiguous():
         return t.data_ptr()
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} dtype {t.dtype} is not {' or '.join(str(d) for d in dtypes)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the others on {'cpu' if index < 0 else f'cuda:{index}'}")
     raise ValueError(f"{name} must be contiguous")
-
-
-class _on:
-    """The device and stream a call runs on: `stream`, or the current stream of
-    the tensors' device, which need not be the current device."""
-    __slots__ = ("_ctx", "_handle")
-
-    def __init__(self, device: torch.device, stream):
-        if device.type != "cuda":
-            raise ValueError(f"tensors must be on a GPU, not on {device}")
-        self._ctx = None
-        if stream is not None:
-            if stream.device != device:
-                raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
-            self._ctx = torch.cuda.stream(stream)
-            self._handle = stream.cuda_stream
-        else:
-            if device.index != torch.cuda.current_device():
-                self._ctx = torch.cuda.device(device)
-            self._handle = _raw_stream(device.index)
-
-    def __enter__(self) -> int:
-        if self._ctx is not None:
-            self._ctx.__enter__()
-        return self._handle
-
-    def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
-
-
-# The current stream's handle of a device, without a Stream object where
-# PyTorch offers it (0.1 us instead of 1.8).
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
-                      lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _rows(name: str, t, dims: int) -> torch.Tensor:
@@ -93,10 +68,29 @@ def _rows(name: str, t, dims: int) -> torch.Tensor:
     return t
 
 
-_MASK = (torch.bool, torch.uint8)
+class _on:
+    """The device and stream a call runs on where they are not the current ones."""
+    __slots__ = ("_ctx",)
+
+    def __init__(self, index: int, stream):
+        self._ctx = torch.cuda.device(index) if stream is None else torch.cuda.stream(stream)
+        self._ctx.__enter__()
+
+    def leave(self):
+        self._ctx.__exit__(None, None, None)
 
 
-_I32, _F32 = (torch.int32,), (torch.float32,)
+def _begin(index: int, stream):
+    """(stream handle, context to leave afterwards or None) of a call on GPU
+    `index`: `stream`, or the current stream of that GPU, which need not be the
+    current one."""
+    if index < 0:
+        raise ValueError("tensors must be on a GPU")
+    if stream is None:
+        return _raw_stream(index), (None if index == _current_device() else _on(index, None))
+    if stream.device.index != index:
+        raise ValueError(f"stream is on {stream.device}, the tensors on cuda:{index}")
+    return stream.cuda_stream, _on(index, stream)
 
 
 class BalanceLoss(NamedTuple):
@@ -113,12 +107,13 @@ def balance_loss(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Tensor
     logits [T, E] and their picks topk_idx [T, k] int32, over the rows where
     mask [T] (bool or uint8) is true."""
     T, E, k = _rows("logits", logits, 2).shape[0], router.nExperts, router.topK
-    dev = logits.device
-    lp = _check("logits", logits, (T, E), _FLOATS, dev)
-    ip = _check("topk_idx", topk_idx, (T, k), _I32, dev)
-    mp = _check("mask", mask, (T,), _MASK, dev)
-    lib = _lib.load()
-    with _on(dev, stream) as st:
+    at, dev = logits.get_device(), logits.device
+    lp = _check("logits", logits, (T, E), _FLOATS, at)
+    ip = _check("topk_idx", topk_idx, (T, k), _I32, at)
+    mp = _check("mask", mask, (T,), _MASK, at)
+    st, ctx = _begin(at, stream)
+    try:
+        lib = _lib.load()
         counts = torch.empty(E + 1, dtype=torch.int32, device=dev)
         prob_sum = torch.empty(E, dtype=torch.float32, device=dev)
         losses = torch.empty(2, dtype=torch.float32, device=dev)
@@ -127,6 +122,9 @@ def balance_loss(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Tensor
         check(lib.moe_balance_loss(lp, moe_dtype(logits.dtype), T, E, k, router.gatingMode,
                                    router.logitScale, ip, mp, counts.data_ptr(), prob_sum.data_ptr(),
                                    losses.data_ptr(), None if ws is None else ws.data_ptr(), need, st))
+    finally:
+        if ctx is not None:
+            ctx.leave()
     return BalanceLoss(counts, prob_sum, losses)
 
 
@@ -139,22 +137,26 @@ def router_backward(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Ten
     the routing weights, and balance_coef * balance + z_coef * z, whose counts
     [E + 1] balance_loss returned (or their sum over a job's ranks)."""
     T, E, k = _rows("logits", logits, 2).shape[0], router.nExperts, router.topK
-    dev = logits.device
-    lp = _check("logits", logits, (T, E), _FLOATS, dev)
-    ip = _check("topk_idx", topk_idx, (T, k), _I32, dev)
-    dp = _check("d_weight", d_weight, (T, k), _F32, dev)
-    cp = _check("counts", counts, (E + 1,), _I32, dev)
-    mp = _check("mask", mask, (T,), _MASK, dev)
-    _check("out", out, (T, E), (logits.dtype,), dev)
-    with _on(dev, stream) as st:
+    at, dt = logits.get_device(), logits.dtype
+    lp = _check("logits", logits, (T, E), _FLOATS, at)
+    ip = _check("topk_idx", topk_idx, (T, k), _I32, at)
+    dp = _check("d_weight", d_weight, (T, k), _F32, at)
+    cp = _check("counts", counts, (E + 1,), _I32, at)
+    mp = _check("mask", mask, (T,), _MASK, at)
+    bp = _check("router.expertBias", router.expertBias, (E,), _F32, at)
+    sp = _check("router.expertScale", router.expertScale, (E,), _F32, at)
+    op = _check("out", out, (T, E), (dt,), at)
+    st, ctx = _begin(at, stream)
+    try:
         if out is None:
             out = torch.empty_like(logits)
+            op = out.data_ptr()
         check(_lib.load().moe_router_backward(
-            lp, moe_dtype(logits.dtype), T, E, k, router.gatingMode, int(bool(router.normTopKProb)),
-            _check("router.expertBias", router.expertBias, (E,), _F32, dev), router.logitScale,
-            router.routedScale, _check("router.expertScale", router.expertScale, (E,), _F32, dev),
-            ip, dp, cp,
-            balance_coef, z_coef, mp, out.data_ptr(), st))
+            lp, moe_dtype(dt), T, E, k, router.gatingMode, int(bool(router.normTopKProb)), bp,
+            router.logitScale, router.routedScale, sp, ip, dp, cp, balance_coef, z_coef, mp, op, st))
+    finally:
+        if ctx is not None:
+            ctx.leave()
     return out
 
 
@@ -164,19 +166,24 @@ def unpermute_backward(d_out: torch.Tensor, Y: torch.Tensor, inv_perm: torch.Ten
     d_out [T, hidden]: (dY, d_weight [T, k] float32). inv_perm (T * k int32)
     comes from the dispatch plan; dY may be Y itself."""
     T, H = _rows("d_out", d_out, 2).shape
-    dev = d_out.device
+    at, dts = d_out.get_device(), (d_out.dtype,)
     k = _rows("topk_weight", topk_weight, 2).shape[1]
-    gp = _check("d_out", d_out, (T, H), _FLOATS, dev)
-    yp = _check("Y", Y, (T * k, H), (d_out.dtype,), dev)
-    wp = _check("topk_weight", topk_weight, (T, k), _F32, dev)
-    ip = _check("inv_perm", inv_perm, (T * k,) if inv_perm.dim() == 1 else (T, k), _I32, dev)
-    _check("dY", dY, (T * k, H), (d_out.dtype,), dev)
-    with _on(dev, stream) as st:
+    gp = _check("d_out", d_out, (T, H), _FLOATS, at)
+    yp = _check("Y", Y, (T * k, H), dts, at)
+    wp = _check("topk_weight", topk_weight, (T, k), _F32, at)
+    ip = _check("inv_perm", inv_perm, (T * k,) if inv_perm.dim() == 1 else (T, k), _I32, at)
+    op = _check("dY", dY, (T * k, H), dts, at)
+    st, ctx = _begin(at, stream)
+    try:
         if dY is None:
             dY = torch.empty_like(Y)
-        dw = torch.empty(T, k, dtype=torch.float32, device=dev)
-        check(_lib.load().moe_unpermute_backward(gp, yp, ip, wp, T, H, k, dY.data_ptr(),
-                                                 dw.data_ptr(), moe_dtype(d_out.dtype), st))
+            op = dY.data_ptr()
+        dw = torch.empty_like(topk_weight)
+        check(_lib.load().moe_unpermute_backward(gp, yp, ip, wp, T, H, k, op, dw.data_ptr(),
+                                                 moe_dtype(d_out.dtype), st))
+    finally:
+        if ctx is not None:
+            ctx.leave()
     return dY, dw
 
 
@@ -185,7 +192,8 @@ class LoRAAdapters:
     """A stack of low-rank adapters of one [N, K] projection: a [G, R, K],
     b [G, N, R], scale [G] float32 (None: 1). Ranks that differ are padded
     with zeros to a multiple of 8, at most 128. The tensors may be updated in
-    place (a slot overwritten, an optimiser's step)."""
+    place (a slot overwritten, an optimiser's step) and moved (their .data set);
+    the latter is checked again by the next call."""
     a: torch.Tensor
     b: torch.Tensor
     scale: Optional[torch.Tensor] = None
@@ -193,36 +201,48 @@ class LoRAAdapters:
     def __post_init__(self):
         G, R, K = _rows("a", self.a, 3).shape
         N = _rows("b", self.b, 3).shape[1]
-        dev = self.a.device
-        desc = Lora(_check("a", self.a, (G, R, K), _FLOATS, dev),
-                    _check("b", self.b, (G, N, R), (self.a.dtype,), dev),
-                    _check("scale", self.scale, (G,), _F32, dev),
+        at = self.a.get_device()
+        desc = Lora(_check("a", self.a, (G, R, K), _FLOATS, at),
+                    _check("b", self.b, (G, N, R), (self.a.dtype,), at),
+                    _check("scale", self.scale, (G,), _F32, at),
                     moe_dtype(self.a.dtype), R, N, K, G)
         check(_lib.load().moe_validate_lora(C.byref(desc)))
         object.__setattr__(self, "_struct", desc)
+        object.__setattr__(self, "_ref", C.byref(desc))
 
-    def _ids(self, adapter, T):
-        return _check("adapter", adapter, (T,), _I32, self.a.device)
+    def _current(self) -> Lora:
+        """The descriptor, of the memory the tensors have now."""
+        l, s = self._struct, self.scale
+        if (self.a.data_ptr() != l.a or self.b.data_ptr() != l.b
+                or (s is not None and s.data_ptr() != l.scale)):
+            self.__post_init__()
+            l = self._struct
+        return l
 
     def apply(self, x: torch.Tensor, adapter: torch.Tensor, y: Optional[torch.Tensor] = None,
               out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """y + scale * b (a x) for x [T, K], row t with adapter[t] (int32; -1:
         none). y [T, N] is the shared projection's output (None: zeros); the
         result goes to out, by default to y itself."""
-        l, dt, dev = self._struct, (self.a.dtype,), self.a.device
+        l, dts, at = self._current(), (self.a.dtype,), self.a.get_device()
         T = _rows("x", x, 2).shape[0]
-        xp = _check("x", x, (T, l.k), dt, dev)
-        ap = self._ids(adapter, T)
-        yp = _check("y", y, (T, l.n), dt, dev)
-        _check("out", out, (T, l.n), dt, dev)
-        lib = _lib.load()
-        with _on(dev, stream) as st:
+        xp = _check("x", x, (T, l.k), dts, at)
+        ap = _check("adapter", adapter, (T,), _I32, at)
+        yp = _check("y", y, (T, l.n), dts, at)
+        op = _check("out", out, (T, l.n), dts, at)
+        st, ctx = _begin(at, stream)
+        try:
+            lib = _lib.load()
             if out is None:
-                out = torch.empty(T, l.n, dtype=x.dtype, device=dev) if y is None else y
-            need = lib.moe_lora_workspace_bytes(C.byref(l), T)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            check(lib.moe_lora_apply(C.byref(l), xp, T, ap, yp, out.data_ptr(),
-                                     None if ws is None else ws.data_ptr(), need, st))
+                out = torch.empty(T, l.n, dtype=x.dtype, device=x.device) if y is None else y
+                op = out.data_ptr()
+            need = lib.moe_lora_workspace_bytes(self._ref, T)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+            check(lib.moe_lora_apply(self._ref, xp, T, ap, yp, op, None if ws is None else ws.data_ptr(),
+                                     need, st))
+        finally:
+            if ctx is not None:
+                ctx.leave()
         return out
 
     def backward(self, x: torch.Tensor, dy: torch.Tensor, adapter: torch.Tensor,
@@ -232,23 +252,27 @@ class LoRAAdapters:
         dx [T, K] is the gradient from the shared projection that the adapters'
         is added to (None: zeros); the sum goes to dx_out, by default to dx
         itself. need_dx=False leaves it out (dx is then None)."""
-        l, dt, dev = self._struct, (self.a.dtype,), self.a.device
+        l, dts, at = self._current(), (self.a.dtype,), self.a.get_device()
         T = _rows("x", x, 2).shape[0]
-        xp = _check("x", x, (T, l.k), dt, dev)
-        yp = _check("dy", dy, (T, l.n), dt, dev)
-        ap = self._ids(adapter, T)
-        dp = _check("dx", dx, (T, l.k), dt, dev)
-        _check("dx_out", dx_out, (T, l.k), dt, dev)
+        xp = _check("x", x, (T, l.k), dts, at)
+        yp = _check("dy", dy, (T, l.n), dts, at)
+        ap = _check("adapter", adapter, (T,), _I32, at)
+        dp = _check("dx", dx, (T, l.k), dts, at)
+        op = _check("dx_out", dx_out, (T, l.k), dts, at)
         if not need_dx and (dx is not None or dx_out is not None):
             raise ValueError("dx or dx_out given with need_dx=False")
-        lib = _lib.load()
-        with _on(dev, stream) as st:
+        st, ctx = _begin(at, stream)
+        try:
+            lib = _lib.load()
             if need_dx and dx_out is None:
-                dx_out = torch.empty(T, l.k, dtype=x.dtype, device=dev) if dx is None else dx
+                dx_out = torch.empty(T, l.k, dtype=x.dtype, device=x.device) if dx is None else dx
+                op = dx_out.data_ptr()
             da, db = torch.empty_like(self.a), torch.empty_like(self.b)
-            need = lib.moe_lora_backward_workspace_bytes(C.byref(l), T)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            check(lib.moe_lora_backward(C.byref(l), xp, yp, T, ap, dp,
-                                        None if dx_out is None else dx_out.data_ptr(),
-                                        da.data_ptr(), db.data_ptr(), ws.data_ptr(), need, st))
+            need = lib.moe_lora_backward_workspace_bytes(self._ref, T)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+            check(lib.moe_lora_backward(self._ref, xp, yp, T, ap, dp, op, da.data_ptr(), db.data_ptr(),
+                                        ws.data_ptr(), need, st))
+        finally:
+            if ctx is not None:
+                ctx.leave()
         return dx_out, da, db

@@ -706,6 +706,25 @@ def test_tuning_chain_in_two_graphs():
     assert all(same_bits(new[k], outs[0][k]) for k in new) and not same_bits(new["da"], want[0]["da"])
 
 
+def test_adapters_updated_and_moved():
+    """A slot overwritten in place and tensors whose memory was exchanged are
+    what the next call reads; memory of another shape or type is refused."""
+    x, A, B, scale, ad = lora_case(6, 64, 64, 8, 2, BF16, 1, "one")
+    a, b, s = A.cuda(), B.cuda(), scale.cuda()
+    l = tuning.LoRAAdapters(a, b, s)
+    xc, ac = x.cuda(), ad.cuda()
+    l.apply(xc, ac)
+    a[1].mul_(2)
+    d, tol = lora_ref(x, a.cpu(), B, scale, ad)
+    close(l.apply(xc, ac), d, tol, "slot overwritten")
+    a.data, b.data, s.data = (A * 3).cuda(), (B * 2).cuda(), (scale + 1).cuda()
+    d, tol = lora_ref(x, A * 3, B * 2, scale + 1, ad)
+    close(l.apply(xc, ac), d, tol, "moved")
+    a.data = A.cuda().half()
+    with pytest.raises(ValueError, match="b dtype"):
+        l.apply(xc, ac)
+
+
 def test_refusals_on_the_gpu_launch_nothing():
     """A refused call leaves its outputs alone and the next one works."""
     x, A, B, scale, ad = lora_case(4, 64, 64, 8, 2, BF16, 1)
