@@ -267,16 +267,21 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
   float* const sum = reinterpret_cast<float*>(area[0]) + kTile * LD;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const ExpandArgs& p = jobs.job[FUSED ? blockIdx.y : 0];
+  // all arguments at once (opaque: else each is loaded where it is first used,
+  // and waited for there)
+  ExpandArgs p = jobs.job[FUSED ? blockIdx.y : 0];
+  int team = jobs.team, most = jobs.shares, run = jobs.run;
+  asm volatile("" : "+s"(p.x), "+s"(p.a), "+s"(p.b), "+s"(p.scale), "+s"(p.adapter), "+s"(p.yin), "+s"(p.y), "+s"(p.s));
+  asm volatile("" : "+s"(p.T), "+s"(p.K), "+s"(p.N), "+s"(p.R), "+s"(p.G), "+s"(team), "+s"(most), "+s"(run));
   // Consecutive blocks go to the eight XCDs in turn. Many tiles: each XCD takes a
   // run of neighbours, whose rows share adapters in its L2, all first blocks of
   // a tile before the second ones. Few: the tiles' first blocks are spread, then
   // the second ones.
   int member, tile;  // one of jobs.team blocks of a tile
-  if (jobs.run > 0) {
+  if (run > 0) {
     const int i = (int)(blockIdx.x >> 3);
-    member = i / jobs.run;
-    tile = (int)(blockIdx.x & 7u) * jobs.run + i % jobs.run;
+    member = i / run;
+    tile = (int)(blockIdx.x & 7u) * run + i % run;
   } else {
     const uint32_t tiles = (uint32_t)(p.T + kTile - 1) / kTile;
     member = (int)(blockIdx.x / tiles);
@@ -302,13 +307,12 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
   static_for_15([&](auto i) { again |= dpp_i32<0x110 + decltype(i)::value, 0xF>(-2, ad) == ad; });
   uint32_t heads = (uint32_t)__ballot(!again) & todo;
   const int D = __builtin_popcount(heads);
-  const int team = jobs.team;
   int first = member, share = 0, shares = 1;
   if (D == 0) return;
   if (D < team) {
     first = member % D;
     share = member / D;
-    shares = min(p.y ? jobs.shares : 1, (team - first + D - 1) / D);
+    shares = min(p.y ? most : 1, (team - first + D - 1) / D);
     if (share >= shares) return;
   }
   // a wave's units of K and groups of columns are neighbours, the waves' shares
@@ -343,6 +347,7 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
     }
     const rsrc_t ar = make_rsrc((const XT*)p.a + (size_t)g * R * K, (uint32_t)R * (uint32_t)K * ES);
     const rsrc_t br = make_rsrc((const XT*)p.b + (size_t)g * N * R, (uint32_t)N * (uint32_t)R * ES);
+    const float sc = p.scale ? p.scale[g] : 1.f;
     // ---- loads of b and y
     const uint32_t pieces = (uint32_t)NC * c8;  // a multiple of 64
     uint32_t yo[4];
@@ -443,7 +448,6 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
       for (int i = 0; i < RT; i++) *reinterpret_cast<f32x4_t*>(red + c * LD + i * 16 + 4 * q) = acc[i];
       lds_barrier();
     }
-    const float sc = p.scale ? p.scale[g] : 1.f;
     for (int e = tid; e < RT * 256; e += 64 * W) {
       const int t = e / (RT * 16), r = e % (RT * 16), at = t * LD + r;
       float v = 0.f;
@@ -748,8 +752,9 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
   __shared__ f32x4_t red[kOuterWaves / 2][RB * 8 * 64];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const OuterSide sd = p.side[blockIdx.z % (uint32_t)p.sides];
-  const int r0 = (int)(blockIdx.z / (uint32_t)p.sides) * (RB * 16);
+  const bool second = p.sides == 2 && (blockIdx.z & 1u);
+  const OuterSide sd = second ? p.side[1] : p.side[0];
+  const int r0 = (int)(p.sides == 2 ? blockIdx.z >> 1 : blockIdx.z) * (RB * 16);
   const int R = p.R, cols = sd.cols, cb = blockIdx.x * kOuterCols;
   if (cb >= cols) return;
   const int col = cb + 8 * c;
