@@ -455,12 +455,13 @@ int lanes_lg(int E) {
   return lg;
 }
 
-// Blocks of a balance pass: one for a few rows (one launch), otherwise up to
-// 256 (one per CU, so that the second launch has few partials to add) of at
-// least a row per wave slot.
+// Blocks of a balance pass: one, which needs no second launch, for up to five
+// rounds of its waves (four rounds take 6.7 us in a graph and 8.7 us called one
+// by one, two launches 8.5 and 12.7; eight rounds 10.4 and 10.0), otherwise up
+// to 256, one per CU, of at least a row per wave slot.
 int balance_blocks(int T, int E) {
   const int rows = kBalWaves * (kWave >> lanes_lg(E));  // a block's rows in flight
-  if (T <= 2 * rows) return 1;
+  if (T <= 5 * rows) return 1;
   return (int)std::min<long>(kBalMaxBlocks, (T + rows - 1) / rows);
 }
 
