@@ -1030,18 +1030,21 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 int outer_ranks(const LoraDims& d) { return d.R <= 16 ? 1 : d.R <= 32 || d.dt != DT_F32 ? 2 : 4; }
 
 // Rows of a chunk in the outer products: about two blocks per CU with the
-// adapters' last, smaller chunks, at least 64. The chunks of all adapters are
-// at most outer_chunks.
-uint32_t outer_chunk(const LoraDims& d) {
+// adapters' last, smaller chunks, at least 64.
+long outer_target(const LoraDims& d) {
   const int rt = outer_ranks(d) * 16;
   const long blocks = (long)((d.K + kOuterCols - 1) / kOuterCols + (d.N + kOuterCols - 1) / kOuterCols) *
                       ((d.R + rt - 1) / rt);
-  const long chunks = std::max(4L, 512 / blocks - d.G / 2);
-  return (uint32_t)std::max(64L, (d.T + chunks - 1) / chunks);
+  return std::max(4L, 512 / blocks - d.G / 2);
 }
+uint32_t outer_chunk(const LoraDims& d) {
+  const long n = outer_target(d);
+  return (uint32_t)std::max(64L, (d.T + n - 1) / n);
+}
+// Chunks of all adapters, at most (no fewer for more rows, so that a workspace
+// sized for many rows serves a call of few).
 long outer_chunks(const LoraDims& d) {
-  const long chunk = outer_chunk(d);
-  return std::min<long>(d.T, (d.T + chunk - 1) / chunk + d.G);
+  return std::min<long>(d.T, std::min(outer_target(d), (long)(d.T + 63) / 64) + d.G);
 }
 
 struct BackwardLayout {

@@ -167,6 +167,12 @@ def test_workspace_sizes():
             g = lora(n_adapters=G, n=4096, k=4096, rank=64)
             sizes = [f(C.byref(g), T) for T in list(range(1, 700)) + [1000, 4096, 40000]]
             assert sizes == sorted(sizes)
+            g = lora(n_adapters=G, n=64, k=64, rank=8)  # its gradients are cut into many chunks
+            sizes = [f(C.byref(g), T) for T in range(1, 40000, 7)]
+            assert sizes == sorted(sizes)
+    for E in (1, 32, 129, 512):
+        sizes = [lib.moe_balance_loss_workspace_bytes(T, E) for T in range(1, 40000, 11)]
+        assert sizes == sorted(sizes)
 
 
 # ------------------------------------------------------------- Python side --
