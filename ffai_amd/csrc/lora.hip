@@ -7,8 +7,7 @@
 //              dA_g = sum_t u_t x_t^T,  dB_g = sum_t dy_t (scale_g A_g x_t)^T
 //
 // A row whose id is not in [0, n_adapters) has no adapter: its y and dx stay
-// as they are, it adds to no gradient. No counterpart in the reference, whose
-// adapters are merged into the weights before loading.
+// as they are, it adds to no gradient. No counterpart in the reference.
 //
 // Everything is small products along K or N against R (8 .. 128) columns: two
 // operations per loaded value and rank, far below the matrix cores' ratio, so
@@ -32,7 +31,7 @@ constexpr uint32_t kOut = 0x7FFFFFF0u;  // past the end of every view: reads 0
 // A lane offset with this in it lies past every view (views hold at most 2^29
 // bytes: 2^20 columns of 128 ranks of 4 bytes), also with another one added.
 constexpr uint32_t kFar = 0x40000000u;
-constexpr int kTile = 16;               // rows per matrix tile
+constexpr int kTile = 16;  // rows per matrix tile
 
 // D += A B^T over 16 x 16 tiles: lane (c, q) = (lane % 16, lane / 16) holds
 // 16 bytes of row c of either operand (8 values of a 16-bit type, k = 8 q ..,
@@ -520,7 +519,7 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
           }
         }
         wave_lds_sync();
-        const uint32_t no = grp < g1 && (grp) * NC + J * c < N ? (uint32_t)(grp) * NC * ES : kFar;
+        const uint32_t no = grp < g1 && grp * NC + J * c < N ? (uint32_t)grp * NC * ES : kFar;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           uint32_t w[J * ES / 4];

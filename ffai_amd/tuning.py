@@ -209,12 +209,13 @@ class LoRAAdapters:
         check(_lib.load().moe_validate_lora(C.byref(desc)))
         object.__setattr__(self, "_struct", desc)
         object.__setattr__(self, "_ref", C.byref(desc))
+        object.__setattr__(self, "_as", (self.a.shape, self.b.shape, self.a.dtype, self.b.dtype))
 
     def _current(self) -> Lora:
         """The descriptor, of the memory the tensors have now."""
-        l, s = self._struct, self.scale
-        if (self.a.data_ptr() != l.a or self.b.data_ptr() != l.b
-                or (s is not None and s.data_ptr() != l.scale)):
+        l, a, b, s = self._struct, self.a, self.b, self.scale
+        if (a.data_ptr() != l.a or b.data_ptr() != l.b or (s is not None and s.data_ptr() != l.scale)
+                or (a.shape, b.shape, a.dtype, b.dtype) != self._as):
             self.__post_init__()
             l = self._struct
         return l

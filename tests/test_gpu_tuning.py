@@ -511,6 +511,31 @@ def test_lora_backward(dt, T, K, N, R, G, kind):
     close(zx, rdx - dx.double(), rmag, "dx of the adapters alone")
 
 
+@pytest.mark.parametrize("K,N,R", [(128, 264, 24), (2048, 2056, 64)])
+def test_lora_backward_parts(K, N, R):
+    """Each gradient asked for by itself through the C ABI has the bits of the
+    call for all, and nothing else is written."""
+    T, G = 29, 3
+    x, A, B, scale, ad = lora_case(T, K, N, R, G, BF16, 4, "each")
+    dy, dxi = torch.randn(T, N, generator=gen(1)).to(BF16), torch.randn(T, K, generator=gen(2)).to(BF16)
+    xc, ac, dyc, dxc, a, b, s = (t.cuda() for t in (x, ad, dy, dxi, A, B, scale))
+    want = tuning.LoRAAdapters(a, b, s).backward(xc, dyc, ac, dx=dxc, dx_out=torch.empty_like(dxc))
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    desc = _lib.Lora(a.data_ptr(), b.data_ptr(), s.data_ptr(), moe_dtype(BF16), R, N, K, G)
+    need = lib.moe_lora_backward_workspace_bytes(C.byref(desc), T)
+    ws = torch.empty(need + 256, dtype=torch.uint8, device="cuda")
+    for ask in [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (1, 0, 1), (0, 1, 1)]:
+        out = [torch.full_like(t, 9.0) for t in want]
+        p = [o.data_ptr() if on else None for o, on in zip(out, ask)]
+        ws.fill_(255)
+        check(lib.moe_lora_backward(C.byref(desc), xc.data_ptr(), dyc.data_ptr(), T, ac.data_ptr(),
+                                    dxc.data_ptr() if ask[0] else None, *p, ws.data_ptr(), need, st))
+        torch.cuda.synchronize()
+        for o, w, on in zip(out, want, ask):
+            assert same_bits(o, w) if on else (o == 9).all(), ask
+        assert (ws[need:] == 255).all()
+
+
 @pytest.mark.parametrize("dt", [BF16, F32])
 def test_lora_backward_many_rows(dt):
     """More rows than the first launch lists itself, spread unevenly over the
@@ -720,6 +745,9 @@ def test_adapters_updated_and_moved():
     a.data, b.data, s.data = (A * 3).cuda(), (B * 2).cuda(), (scale + 1).cuda()
     d, tol = lora_ref(x, A * 3, B * 2, scale + 1, ad)
     close(l.apply(xc, ac), d, tol, "moved")
+    a.data = a.data[:1]  # the same address, fewer adapters
+    with pytest.raises(ValueError, match="b must be"):
+        l.apply(xc, ac)
     a.data = A.cuda().half()
     with pytest.raises(ValueError, match="b dtype"):
         l.apply(xc, ac)
