@@ -1148,8 +1148,17 @@ bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
   return a && b && x < y + nb && y < x + na;
 }
 
+// Rows and blocks of a call whose launches stay below 2^32 threads.
+constexpr int kMaxTuneRows = 1 << 23;
+constexpr long kMaxTuneBlocks = 1 << 23;
+
 LoraDims lora_dims(const moe_lora* l, int T) {
   return LoraDims{l->dtype, T, l->k, l->n, l->rank, l->n_adapters};
+}
+
+// Bytes of a (cols k) or b (cols n).
+size_t lora_bytes(const moe_lora* l, int cols) {
+  return (size_t)l->n_adapters * l->rank * cols * dt_size(l->dtype);
 }
 
 moe_status validate_lora(const moe_lora* l) {
@@ -1233,6 +1242,7 @@ extern "C" moe_status moe_unpermute_backward(const void* d_out, const void* Y,
   if (T <= 0 || hidden <= 0 || k <= 0)
     return fail(MOE_ERR_INVALID, "unpermute_backward: T, hidden and k must be positive");
   if ((long)T * k > 0x7fffffffL) return fail(MOE_ERR_INVALID, "unpermute_backward: T*k too large");
+  if (T > kMaxTuneRows) return fail(MOE_ERR_UNSUPPORTED, "unpermute_backward: T above %d", kMaxTuneRows);
   if (hidden % 8) return fail(MOE_ERR_UNSUPPORTED, "unpermute_backward: hidden must be a multiple of 8");
   if (!dt_ok(dtype)) return fail(MOE_ERR_INVALID, "unpermute_backward: bad dtype");
   if (!aligned16(d_out) || !aligned16(Y) || !aligned16(dY))
@@ -1252,7 +1262,7 @@ extern "C" moe_status moe_validate_lora(const moe_lora* l) {
 }
 
 extern "C" size_t moe_lora_workspace_bytes(const moe_lora* l, int32_t T) {
-  if (T <= 0 || validate_lora(l) != MOE_OK) return 0;
+  if (T <= 0 || T > kMaxTuneRows || validate_lora(l) != MOE_OK) return 0;
   return lora_ws_bytes(lora_dims(l, T));
 }
 
@@ -1262,11 +1272,14 @@ extern "C" moe_status moe_lora_apply(const moe_lora* l, const void* x, int32_t T
   MOE_TRY(validate_lora(l));
   if (!x || !adapter || !y) return fail(MOE_ERR_INVALID, "lora_apply: NULL pointer");
   if (T <= 0) return fail(MOE_ERR_INVALID, "lora_apply: T must be positive");
+  if (T > kMaxTuneRows) return fail(MOE_ERR_UNSUPPORTED, "lora_apply: T above %d", kMaxTuneRows);
   if (!aligned16(x) || !aligned16(y_in) || !aligned16(y))
     return fail(MOE_ERR_INVALID, "lora_apply: rows must be 16-byte aligned");
   const LoraDims d = lora_dims(l, T);
   const size_t xb = (size_t)T * l->k * dt_size(l->dtype), yb = (size_t)T * l->n * dt_size(l->dtype);
   if (overlaps(x, xb, y, yb)) return fail(MOE_ERR_INVALID, "lora_apply: y overlaps x");
+  if (overlaps(l->a, lora_bytes(l, l->k), y, yb) || overlaps(l->b, lora_bytes(l, l->n), y, yb))
+    return fail(MOE_ERR_INVALID, "lora_apply: y overlaps the adapters");
   if (y_in != y && overlaps(y_in, yb, y, yb))
     return fail(MOE_ERR_INVALID, "lora_apply: y overlaps y_in (equal or apart)");
   const size_t need = lora_ws_bytes(d);
@@ -1278,7 +1291,7 @@ extern "C" moe_status moe_lora_apply(const moe_lora* l, const void* x, int32_t T
 }
 
 extern "C" size_t moe_lora_backward_workspace_bytes(const moe_lora* l, int32_t T) {
-  if (T <= 0 || validate_lora(l) != MOE_OK || l->n_adapters > 1024) return 0;
+  if (T <= 0 || T > kMaxTuneRows || validate_lora(l) != MOE_OK || l->n_adapters > 1024) return 0;
   return lora_backward_ws_bytes(lora_dims(l, T));
 }
 
@@ -1291,8 +1304,11 @@ extern "C" moe_status moe_lora_backward(const moe_lora* l, const void* x, const 
   if (!dx && !da && !db) return fail(MOE_ERR_INVALID, "lora_backward: no gradient asked for");
   if (dx_in && !dx) return fail(MOE_ERR_INVALID, "lora_backward: dx_in without dx");
   if (T <= 0) return fail(MOE_ERR_INVALID, "lora_backward: T must be positive");
+  if (T > kMaxTuneRows) return fail(MOE_ERR_UNSUPPORTED, "lora_backward: T above %d", kMaxTuneRows);
   if (l->n_adapters > 1024)
     return fail(MOE_ERR_UNSUPPORTED, "lora_backward: n_adapters above 1024");
+  if (lora_prep_blocks(lora_dims(l, T)) > kMaxTuneBlocks)
+    return fail(MOE_ERR_UNSUPPORTED, "lora_backward: a and b too large");
   for (const void* p : {x, dy, dx_in, (const void*)dx, (const void*)da, (const void*)db})
     if (!aligned16(p)) return fail(MOE_ERR_INVALID, "lora_backward: buffers must be 16-byte aligned");
   const LoraDims d = lora_dims(l, T);
@@ -1300,6 +1316,21 @@ extern "C" moe_status moe_lora_backward(const moe_lora* l, const void* x, const 
   const size_t xb = (size_t)T * l->k * es, yb = (size_t)T * l->n * es;
   if (overlaps(x, xb, dx, xb) || overlaps(dy, yb, dx, xb) || (dx_in != dx && overlaps(dx_in, xb, dx, xb)))
     return fail(MOE_ERR_INVALID, "lora_backward: dx overlaps an input (dx_in: equal or apart)");
+  const size_t ab = lora_bytes(l, l->k), bb = lora_bytes(l, l->n);
+  const struct {
+    const void* p;
+    size_t bytes;
+  } out[3] = {{dx, xb}, {da, ab}, {db, bb}};
+  for (int i = 0; i < 3; i++) {
+    if (overlaps(l->a, ab, out[i].p, out[i].bytes) || overlaps(l->b, bb, out[i].p, out[i].bytes))
+      return fail(MOE_ERR_INVALID, "lora_backward: a gradient overlaps the adapters");
+    if (i && (overlaps(x, xb, out[i].p, out[i].bytes) || overlaps(dy, yb, out[i].p, out[i].bytes) ||
+              overlaps(dx_in, xb, out[i].p, out[i].bytes)))
+      return fail(MOE_ERR_INVALID, "lora_backward: da or db overlaps an input");
+    for (int j = 0; j < i; j++)
+      if (overlaps(out[j].p, out[j].bytes, out[i].p, out[i].bytes))
+        return fail(MOE_ERR_INVALID, "lora_backward: gradients overlap");
+  }
   const size_t need = lora_backward_ws_bytes(d);
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
     return fail(MOE_ERR_WORKSPACE, "lora_backward: 16-byte aligned workspace of %zu bytes needed", need);

@@ -257,7 +257,6 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
   constexpr int NC = 16 * J;                       // columns of a group
   constexpr int C8 = RT * 16 / V;                  // 16-byte chunks of the widest adapter row
   constexpr int BL = NC * C8 / 64;                 // loads of a column group's b rows
-  constexpr bool EARLY = BL < 4;                   // the first group's loads go out before the shrink half
   constexpr int AREA = (1 + RT) * 128 > NC * (C8 | 1) ? (1 + RT) * 128 : NC * (C8 | 1);  // 16-byte slots
   static_assert(AREA * 4 >= 2 * kTile * LD, "the sums of a wave and of the block fit an area");
   // a wave's area holds in turn its units, its sums and its column groups; the
@@ -375,10 +374,6 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
 #pragma unroll
       for (int i = 0; i < BL; i++) bv[i] = bload128(br, 64u * i < pieces ? go + 1024u * i : kFar);
     };
-    auto first_cols = [&] {
-      load_b(g0);
-      load_y(g0, yn);
-    };
     // ---- shrink. Eight lanes load a row's 128 bytes (lane l: piece l % 8 of
     // row l / 8): the load unit takes 64 neighbouring bytes a clock but only 16
     // when neighbouring lanes are in different rows, as the matrix operands
@@ -405,7 +400,6 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
       u32x4_t* const put = mem + pr * 8 + (pj ^ pr);
       const u32x4_t* const get = mem + c * 8;
       load(u0);
-      if (EARLY && p.y) first_cols();
       for (int u = u0; u < u1; u++) {
 #pragma unroll
         for (int h = 0; h < 2; h++) put[h * 64] = xv[h];
@@ -440,7 +434,6 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
       }
     }
     // ---- the waves' sums meet
-    if (!FUSED && EARLY && p.y) first_cols();
     float* const red = reinterpret_cast<float*>(mem);
     if constexpr (FUSED) {
 #pragma unroll
@@ -476,10 +469,9 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
 #pragma unroll
         for (int i = 0; i < 4; i++) bk[i] = __shfl(back, 4 * q + i, kWave);
       }
-      if (!EARLY) {
-        __builtin_amdgcn_sched_barrier(0);
-        first_cols();
-      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_b(g0);
+      load_y(g0, yn);
       uint32_t at[RT];
 #pragma unroll
       for (int i = 0; i < RT; i++) {
@@ -1175,6 +1167,10 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
 
 size_t lora_ws_bytes(const LoraDims& d) {
   return up256(partial_bytes(d));
+}
+long lora_prep_blocks(const LoraDims& d) {
+  const long r = (d.R + 31) / 32;
+  return d.G * (1 + r * ((d.K + 31) / 32) + r * ((d.N + 31) / 32));
 }
 size_t lora_backward_ws_bytes(const LoraDims& d) { return backward_layout(d).total; }
 

@@ -171,7 +171,8 @@ def unpermute_backward(d_out: torch.Tensor, Y: torch.Tensor, inv_perm: torch.Ten
     gp = _check("d_out", d_out, (T, H), _FLOATS, at)
     yp = _check("Y", Y, (T * k, H), dts, at)
     wp = _check("topk_weight", topk_weight, (T, k), _F32, at)
-    ip = _check("inv_perm", inv_perm, (T * k,) if inv_perm.dim() == 1 else (T, k), _I32, at)
+    flat = isinstance(inv_perm, torch.Tensor) and inv_perm.dim() == 1
+    ip = _check("inv_perm", inv_perm, (T * k,) if flat else (T, k), _I32, at)
     op = _check("dY", dY, (T * k, H), dts, at)
     st, ctx = _begin(at, stream)
     try:
@@ -187,7 +188,7 @@ def unpermute_backward(d_out: torch.Tensor, Y: torch.Tensor, inv_perm: torch.Ten
     return dY, dw
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class LoRAAdapters:
     """A stack of low-rank adapters of one [N, K] projection: a [G, R, K],
     b [G, N, R], scale [G] float32 (None: 1). Ranks that differ are padded
@@ -215,7 +216,8 @@ class LoRAAdapters:
         """The descriptor, of the memory the tensors have now."""
         l, a, b, s = self._struct, self.a, self.b, self.scale
         if (a.data_ptr() != l.a or b.data_ptr() != l.b or (s is not None and s.data_ptr() != l.scale)
-                or (a.shape, b.shape, a.dtype, b.dtype) != self._as):
+                or (a.shape, b.shape, a.dtype, b.dtype) != self._as
+                or not (a.is_contiguous() and b.is_contiguous())):
             self.__post_init__()
             l = self._struct
         return l

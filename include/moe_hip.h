@@ -338,7 +338,7 @@ moe_status moe_router_backward(const void* logits, int32_t dtype, int32_t T, int
  *   dY[inv_perm[t*k+s], :] = round(w[t,s]) * d_out[t,:]   (nullable; may be Y)
  *   d_weight[t,s]          = <d_out[t,:], Y[inv_perm[t*k+s], :]>   (f32)
  * Rows of dY that no position names stay as they are; a position >= T * k
- * has a zero d_weight. d_out, Y and dY 16-byte aligned. */
+ * has a zero d_weight. d_out, Y and dY 16-byte aligned; T at most 2^23. */
 moe_status moe_unpermute_backward(const void* d_out, const void* Y, const uint32_t* inv_perm,
                                   const float* topk_weight, int32_t T, int32_t hidden, int32_t k,
                                   void* dY, float* d_weight, int32_t dtype, hipStream_t stream);
@@ -365,8 +365,8 @@ moe_status moe_validate_lora(const moe_lora* l);
  *   y[t,:] = round(y_in[t,:] + scale[g] * b[g] (a[g] x[t,:])),  g = adapter[t]
  * with the inner sums in f32. A row whose id is not in [0, n_adapters) (-1)
  * has no adapter: its y is y_in. y_in [T, n] may be y (then such rows are not
- * touched) or NULL (zeros). x [T, k] and y in l->dtype, 16-byte aligned,
- * apart from each other. The workspace is free to be reused by work that the
+ * touched) or NULL (zeros). x [T, k] and y in l->dtype, 16-byte aligned; y
+ * apart from x and the adapters; T at most 2^23. The workspace is free to be reused by work that the
  * stream runs later. */
 size_t moe_lora_workspace_bytes(const moe_lora* l, int32_t T);
 moe_status moe_lora_apply(const moe_lora* l, const void* x, int32_t T, const int32_t* adapter,
@@ -380,7 +380,8 @@ moe_status moe_lora_apply(const moe_lora* l, const void* x, int32_t T, const int
  *   db[g]   = round(sum_t dy[t,:] (scale[g] a[g] x[t,:])^T) [G, n, rank]
  * over the rows t of adapter g, sums in f32; an adapter without rows gets
  * zeros. dx_in as y_in above (the gradient from the shared projection; may be
- * dx, or NULL). All in l->dtype, 16-byte aligned; n_adapters at most 1024. */
+ * dx, or NULL). All in l->dtype, 16-byte aligned, the gradients apart from
+ * each other and from all other inputs; T at most 2^23, n_adapters at most 1024. */
 size_t moe_lora_backward_workspace_bytes(const moe_lora* l, int32_t T);
 moe_status moe_lora_backward(const moe_lora* l, const void* x, const void* dy, int32_t T,
                              const int32_t* adapter, const void* dx_in, void* dx, void* da,

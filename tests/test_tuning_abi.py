@@ -239,3 +239,64 @@ def test_python_lora_call_refusals():
                         (lambda: l.backward(x, dy, ad), "on a GPU")]:
         with pytest.raises(ValueError, match=needle):
             bad()
+
+
+@pytest.mark.parametrize("T", [(1 << 23) + 1, (1 << 31) - 1])
+def test_rows_past_a_launch_refused(T):
+    lib, l = _lib.load(), lora(n=8, k=8, rank=8)
+    far = BIG << 6  # buffers of so many rows stay apart
+    at = [C.c_void_p(far * (i + 1)) for i in range(8)]
+    assert lib.moe_lora_apply(C.byref(l), at[0], T, at[1], at[2], at[3], None, 0, None) == MOE_ERR_UNSUPPORTED
+    assert "T above" in _lib.last_error()
+    assert lib.moe_lora_backward(C.byref(l), at[0], at[1], T, at[2], at[3], at[4], at[5], at[6], at[7], far,
+                                 None) == MOE_ERR_UNSUPPORTED
+    assert "T above" in _lib.last_error()
+    assert lib.moe_lora_workspace_bytes(C.byref(l), T) == lib.moe_lora_backward_workspace_bytes(C.byref(l), T) == 0
+    assert call("moe_unpermute_backward", UB, T=T, k=1, H=8) == MOE_ERR_UNSUPPORTED
+    assert "T above" in _lib.last_error()
+
+
+def test_lora_backward_refuses_stacks_past_a_launch():
+    l = lora(n=1 << 20, k=1 << 20, rank=128, n_adapters=1024)
+    assert _lib.load().moe_lora_backward(C.byref(l), *BACK.values(), None) == MOE_ERR_UNSUPPORTED
+    assert "too large" in _lib.last_error()
+
+
+A, B = C.c_void_p(BIG * 21), C.c_void_p(BIG * 22 + 64)
+
+
+@pytest.mark.parametrize("kw,needle", [
+    (dict(da=p(0)), "input"), (dict(db=p(1)), "input"), (dict(da=p(3)), "input"), (dict(db=p(4)), "gradients overlap"),
+    (dict(da=p(6)), "gradients overlap"), (dict(da=A), "adapters"), (dict(db=B), "adapters"), (dict(dx=B), "adapters"),
+    (dict(dx=A), "adapters"), (dict(dx=None, dxin=None, db=p(5)), "gradients overlap"),
+])
+def test_lora_backward_refuses_overlaps(kw, needle):
+    l = lora()
+    assert _lib.load().moe_lora_backward(C.byref(l), *{**BACK, **kw}.values(), None) == MOE_ERR_INVALID
+    assert needle in _lib.last_error()
+
+
+@pytest.mark.parametrize("y", [A, B])
+def test_lora_apply_refuses_writing_adapters(y):
+    l = lora()
+    assert _lib.load().moe_lora_apply(C.byref(l), *{**APPLY, "y": y, "yin": None}.values(), None) == MOE_ERR_INVALID
+    assert "overlaps the adapters" in _lib.last_error()
+
+
+def test_python_unpermute_backward_inv_perm():
+    g, Y, w = torch.zeros(3, 8), torch.zeros(6, 8), torch.zeros(3, 2)
+    for bad in ([0] * 6, torch.zeros(7, dtype=torch.int32), torch.zeros(3, 1, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="inv_perm must be"):
+            tuning.unpermute_backward(g, Y, bad, w)
+
+
+def test_python_lora_memory_checked_each_call():
+    """A tensor whose memory is set to rows that lie apart is refused, also where
+    its address, shape and type stay."""
+    wide = torch.zeros(4, 8, 16)
+    l = tuning.LoRAAdapters(wide[:2], torch.zeros(2, 24, 8))
+    x, ad = torch.zeros(3, 16), torch.zeros(3, dtype=torch.int32)
+    l.a.data = wide[::2]
+    with pytest.raises(ValueError, match="a must be contiguous"):
+        l.apply(x, ad)
+    assert l == l and l != tuning.LoRAAdapters(l.b, torch.zeros(2, 16, 24))
