@@ -1148,9 +1148,8 @@ bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
   return a && b && x < y + nb && y < x + na;
 }
 
-// Rows and blocks of a call whose launches stay below 2^32 threads.
+// Rows of a call whose launches stay below 2^32 threads.
 constexpr int kMaxTuneRows = 1 << 23;
-constexpr long kMaxTuneBlocks = 1 << 23;
 
 LoraDims lora_dims(const moe_lora* l, int T) {
   return LoraDims{l->dtype, T, l->k, l->n, l->rank, l->n_adapters};
@@ -1307,8 +1306,6 @@ extern "C" moe_status moe_lora_backward(const moe_lora* l, const void* x, const 
   if (T > kMaxTuneRows) return fail(MOE_ERR_UNSUPPORTED, "lora_backward: T above %d", kMaxTuneRows);
   if (l->n_adapters > 1024)
     return fail(MOE_ERR_UNSUPPORTED, "lora_backward: n_adapters above 1024");
-  if (lora_prep_blocks(lora_dims(l, T)) > kMaxTuneBlocks)
-    return fail(MOE_ERR_UNSUPPORTED, "lora_backward: a and b too large");
   for (const void* p : {x, dy, dx_in, (const void*)dx, (const void*)da, (const void*)db})
     if (!aligned16(p)) return fail(MOE_ERR_INVALID, "lora_backward: buffers must be 16-byte aligned");
   const LoraDims d = lora_dims(l, T);

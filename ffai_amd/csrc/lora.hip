@@ -157,10 +157,13 @@ struct ExpandArgs {
   int T, K, N, R, G, S;
 };
 
-// FUSED: blockIdx.y picks one of up to two calls over the same rows, which then
-// run side by side.
+// The backward's form (TURNED) has up to three rows of blocks, which run side by
+// side: the list of every adapter's rows (offsets not null), u and dx, and s.
 struct ExpandJobs {
   ExpandArgs job[2];
+  uint32_t* offsets;  // nullable [G + 1]
+  uint32_t* perm;     // [T]
+  int turned;         // jobs from the first one whose a and b lie turned
   int team;    // blocks of a tile
   int shares;  // of an adapter's columns, at most
   int run;     // tiles of an XCD, 0 for few
@@ -243,11 +246,82 @@ __device__ __forceinline__ void wave_lds_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Value e of each of a lane's N pieces, one after the other.
+template <typename XT, int N>
+__device__ __forceinline__ void turn(const u32x4_t (&v)[N], int e, uint32_t (&w)[N * sizeof(XT) / 4]) {
+#pragma unroll
+  for (int i = 0; i < N * (int)sizeof(XT) / 4; i++) {
+    if constexpr (sizeof(XT) == 4) w[i] = v[i][e];
+    else w[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+  }
+}
+
+// The rows of adapter g by a block of W waves: offsets[g] (and the last one),
+// and perm from there in ascending order, the layout of moe_dispatch_plan. A
+// thread counts ids below and equal to g in a run of 16-byte groups of rows; its
+// rows follow those of the threads before it. meet: 2 W values in LDS, free
+// for the next call.
+template <int W>
+__device__ __forceinline__ void list_rows(const int32_t* __restrict__ adapter, int T, int G, int g,
+                                          uint32_t* __restrict__ offsets, uint32_t* __restrict__ perm,
+                                          uint32_t* meet) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int groups = (T + 3) / 4, per = (groups + 64 * W - 1) / (64 * W);
+  const int q0 = min(groups, tid * per), q1 = min(groups, q0 + per);
+  const bool vec = (reinterpret_cast<uintptr_t>(adapter) & 15) == 0;
+  auto ids = [&](int q, int32_t (&v)[4]) {
+    if (vec && q * 4 + 4 <= T) {
+      const int4 w = *reinterpret_cast<const int4*>(adapter + q * 4);
+      v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = q * 4 + j < T ? adapter[q * 4 + j] : -1;
+    }
+  };
+  uint32_t lt = 0, eq = 0;
+  for (int q = q0; q < q1; q++) {
+    int32_t v[4];
+    ids(q, v);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      lt += v[j] >= 0 && v[j] < g;
+      eq += v[j] == g;
+    }
+  }
+  const uint32_t clt = wave_scan_u32(lt), ceq = wave_scan_u32(eq);
+  if (lane == 63) {
+    meet[wave] = clt;
+    meet[W + wave] = ceq;
+  }
+  __syncthreads();
+  uint32_t base = 0, before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < W; w++) {
+    base += meet[w];
+    all += meet[W + w];
+    before += w < wave ? meet[W + w] : 0u;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    offsets[g] = base;
+    if (g == G - 1) offsets[G] = base + all;
+  }
+  if (eq == 0) return;
+  uint32_t at = base + before + ceq - eq;
+  for (int q = q0; q < q1; q++) {
+    int32_t v[4];
+    ids(q, v);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (v[j] == g) perm[at++] = (uint32_t)(q * 4 + j);
+  }
+}
+
 // Waves per SIMD: two blocks on a CU where LDS has room for them, so that a few
 // blocks more than CUs (requests that end inside a tile) cost no second round.
 constexpr int expand_waves(size_t es, int rt) { return rt <= (es == 4 ? 2 : 4) ? 4 : 2; }
 
-template <typename XT, int RT, bool FUSED>
+template <typename XT, int RT, bool FUSED, bool TURNED>
 __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) void lora_expand_kernel(ExpandJobs jobs) {
   constexpr bool F32 = sizeof(XT) == 4;
   constexpr uint32_t ES = sizeof(XT);
@@ -267,7 +341,19 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // all arguments at once (opaque: else each is loaded where it is first used,
   // and waited for there)
-  ExpandArgs p = jobs.job[FUSED ? blockIdx.y : 0];
+  bool turned = false;  // the job's a is [G, K, R], its b [G, R, N]
+  int job = 0;
+  if constexpr (TURNED) {
+    job = (int)blockIdx.y - (jobs.offsets != nullptr);
+    if (job < 0) {
+      for (int g = blockIdx.x; g < jobs.job[0].G; g += gridDim.x)
+        list_rows<W>(jobs.job[0].adapter, jobs.job[0].T, jobs.job[0].G, g, jobs.offsets, jobs.perm,
+                     reinterpret_cast<uint32_t*>(area[0]));
+      return;
+    }
+    turned = job < jobs.turned;
+  }
+  ExpandArgs p = jobs.job[job];
   int team = jobs.team, most = jobs.shares, run = jobs.run;
   asm volatile("" : "+s"(p.x), "+s"(p.a), "+s"(p.b), "+s"(p.scale), "+s"(p.adapter), "+s"(p.yin), "+s"(p.y), "+s"(p.s));
   asm volatile("" : "+s"(p.T), "+s"(p.K), "+s"(p.N), "+s"(p.R), "+s"(p.G), "+s"(team), "+s"(most), "+s"(run));
@@ -369,7 +455,18 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
         }
       }
     };
+    // turned: a lane takes BL neighbouring ranks of V columns
+    constexpr int PC = NC / V;
     auto load_b = [&](int grp) {
+      if constexpr (TURNED) {
+        int l = lane;
+        asm volatile("" : "+v"(l));  // (opaque: as above)
+        const int bj = l % PC, br0 = l / PC * BL;
+        const uint32_t go = grp < g1 ? (uint32_t)grp * NC * ES + (uint32_t)br0 * N * ES + 16u * bj : kFar;
+#pragma unroll
+        for (int i = 0; i < BL; i++) bv[i] = bload128(br, br0 + i < R ? go + (uint32_t)i * N * ES : kFar);
+        return;
+      }
       const uint32_t go = grp < g1 ? (uint32_t)grp * NC * R * ES + 16u * lane : kFar;
 #pragma unroll
       for (int i = 0; i < BL; i++) bv[i] = bload128(br, 64u * i < pieces ? go + 1024u * i : kFar);
@@ -382,20 +479,28 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
     f32x4_t acc[RT] = {};
     if constexpr (FUSED) {
       const int pr = lane >> 3, pj = lane & 7;
-      uint32_t xo[2], ao[2 * RT];
+      // turned: rows of a are k's of R ranks. A lane takes NR neighbouring k's of V
+      // ranks and turns them in registers into the same order.
+      constexpr int NR = 2 * RT, NP = 64 * NR / UNIT;
+      const int tc = lane % NP, tn = lane / NP * NR;
+      const uint32_t astep = TURNED && turned ? (uint32_t)UNIT * R * ES : 128u;
+      const uint32_t arow = TURNED && turned ? (uint32_t)R * ES : 8u * K * ES;  // between a lane's rows of a
+      const uint32_t ao = !(TURNED && turned) ? (uint32_t)pr * K * ES + 16u * pj
+                          : tc < c8           ? (uint32_t)tn * R * ES + 16u * tc
+                                              : kFar;
+      uint32_t xo[2];
 #pragma unroll
       for (int h = 0; h < 2; h++)
         xo[h] = ((same >> (h * 8 + pr)) & 1u ? (uint32_t)(h * 8 + pr) * K * ES : kFar) + 16u * pj;
-#pragma unroll
-      for (int i = 0; i < 2 * RT; i++)
-        ao[i] = (i * 8 + pr < R ? (uint32_t)(i * 8 + pr) * K * ES : kFar) + 16u * pj;
       u32x4_t xv[2], av[2 * RT];
       auto load = [&](int u) {
         const uint32_t ko = u < u1 && u * UNIT + pj * V < K ? (uint32_t)u * 128u : kFar;
+        const uint32_t ka = !(TURNED && turned) ? ko : u < u1 ? (uint32_t)u * astep : kFar;
 #pragma unroll
         for (int h = 0; h < 2; h++) xv[h] = bload128(xr, xo[h] + ko);
 #pragma unroll
-        for (int i = 0; i < 2 * RT; i++) av[i] = bload128(ar, ao[i] + ko);
+        for (int i = 0; i < 2 * RT; i++)
+          av[i] = bload128(ar, ao + ka + ((TURNED && turned) || i * 8 < R ? i * arow : kFar));
       };
       u32x4_t* const put = mem + pr * 8 + (pj ^ pr);
       const u32x4_t* const get = mem + c * 8;
@@ -403,8 +508,28 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
       for (int u = u0; u < u1; u++) {
 #pragma unroll
         for (int h = 0; h < 2; h++) put[h * 64] = xv[h];
+        if (TURNED && turned) {
+          char* const to = reinterpret_cast<char*>(mem + 128 + tc * V * 8) + tn * ES % 16;
 #pragma unroll
-        for (int i = 0; i < 2 * RT; i++) put[128 + i * 64] = av[i];
+          for (int e = 0; e < V; e++) {
+            uint32_t w[NR * ES / 4];
+            turn<XT, NR>(av, e, w);
+            const int rx = ((tc * V + e) ^ (tc * V >> 3)) & 7;
+            if constexpr (NR * ES >= 16) {
+#pragma unroll
+              for (int z = 0; z < (int)(NR * ES / 16); z++)
+                *reinterpret_cast<u32x4_t*>(to + 16 * (8 * e + ((tn / V + z) ^ rx))) =
+                    u32x4_t{w[4 * z], w[4 * z + 1], w[4 * z + 2], w[4 * z + 3]};
+            } else {
+#pragma unroll
+              for (int z = 0; z < (int)(NR * ES / 4); z++)
+                *reinterpret_cast<uint32_t*>(to + 16 * (8 * e + ((tn / V) ^ rx)) + 4 * z) = w[z];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2 * RT; i++) mem[128 + i * 64 + pr * 8 + (pj ^ pr ^ (TURNED ? i & 7 : 0))] = av[i];
+        }
         wave_lds_sync();
         load(u + 1);
 #pragma unroll
@@ -412,14 +537,14 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
           const int at = (4 * h + q) ^ (c & 7);
           const u32x4_t xf = get[at];
 #pragma unroll
-          for (int i = 0; i < RT; i++) acc[i] = mma<XT>(get[128 + i * 128 + at], xf, acc[i]);
+          for (int i = 0; i < RT; i++) acc[i] = mma<XT>(get[128 + i * 128 + (TURNED ? at ^ (c >> 3) ^ (2 * i & 7) : at)], xf, acc[i]);
           if (RT == 8) __builtin_amdgcn_sched_barrier(0);
         }
         wave_lds_sync();
       }
     }
     uint32_t slot[BL];
-    {
+    if constexpr (!TURNED) {
       int n = lane / c8, cc = lane % c8;
       const int dn = 64 / c8, dc = 64 % c8;
 #pragma unroll
@@ -479,9 +604,30 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
         at[i] = (uint32_t)c * (c8 | 1) + min(cc, c8 - 1);
       }
       for (int grp = g0; grp < g1; grp++) {
+        if constexpr (TURNED) {
+          int l = lane;
+          asm volatile("" : "+v"(l));
+          const int bj = l % PC, br0 = l / PC * BL, bto = bj * (V / J) * (c8 | 1) * 16 + br0 * ES;
 #pragma unroll
-        for (int i = 0; i < BL; i++)
-          if (64u * i < pieces) mem[slot[i]] = bv[i];
+          for (int e = 0; e < V; e++) {
+            uint32_t w[BL * ES / 4];
+            turn<XT, BL>(bv, e, w);
+            char* const to = reinterpret_cast<char*>(mem + ((e % J) * 16 + e / J) * (c8 | 1)) + bto;
+            if constexpr (BL * ES >= 16) {
+#pragma unroll
+              for (int z = 0; z < (int)(BL * ES / 16); z++)
+                if (br0 + z * V < R)
+                  *reinterpret_cast<u32x4_t*>(to + 16 * z) = u32x4_t{w[4 * z], w[4 * z + 1], w[4 * z + 2], w[4 * z + 3]};
+            } else if (br0 < R) {
+#pragma unroll
+              for (int z = 0; z < (int)(BL * ES / 4); z++) *reinterpret_cast<uint32_t*>(to + 4 * z) = w[z];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < BL; i++)
+            if (64u * i < pieces) mem[slot[i]] = bv[i];
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -535,101 +681,6 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
     }
     lds_barrier();  // before the areas' and the sums' next adapter
   }
-}
-
-// ------------------------------------------------------------------ prep --
-// What the backward's launches start from, in one: blocks below plan_blocks
-// list the rows of one adapter each (offsets, and perm in ascending order: the
-// layout of moe_dispatch_plan), the others transpose [G, P, Q] -> [G, Q, P] of
-// one or two stacks by tiles of 32 x 32 through LDS, since the backward's
-// products run along the other axis of A and B.
-struct PrepArgs {
-  const int32_t* adapter;
-  uint32_t* offsets;
-  uint32_t* perm;
-  int T, G, plan_blocks;
-  const void* in[2];
-  void* out[2];
-  int P[2], Q[2], tiles[2];  // tiles of one matrix of either stack
-};
-
-template <typename E>
-__global__ __launch_bounds__(256) void lora_prep_kernel(PrepArgs a) {
-  __shared__ E tile[32][33];
-  __shared__ uint32_t wlt[4], weq[4];
-  const int tid = threadIdx.x;
-  if ((int)blockIdx.x < a.plan_blocks) {
-    // a thread counts ids below and equal to g in a run of 16-byte groups of
-    // rows; its rows follow those of the threads before it
-    const int g = blockIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int groups = (a.T + 3) / 4, per = (groups + 255) / 256;
-    const int q0 = min(groups, tid * per), q1 = min(groups, q0 + per);
-    const bool vec = (reinterpret_cast<uintptr_t>(a.adapter) & 15) == 0;
-    auto ids = [&](int q, int32_t (&v)[4]) {
-      if (vec && q * 4 + 4 <= a.T) {
-        const int4 w = *reinterpret_cast<const int4*>(a.adapter + q * 4);
-        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = q * 4 + j < a.T ? a.adapter[q * 4 + j] : -1;
-      }
-    };
-    uint32_t lt = 0, eq = 0;
-    for (int q = q0; q < q1; q++) {
-      int32_t v[4];
-      ids(q, v);
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        lt += v[j] >= 0 && v[j] < g;
-        eq += v[j] == g;
-      }
-    }
-    const uint32_t clt = wave_scan_u32(lt), ceq = wave_scan_u32(eq);
-    if (lane == 63) {
-      wlt[wave] = clt;
-      weq[wave] = ceq;
-    }
-    __syncthreads();
-    uint32_t base = 0, before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-      base += wlt[w];
-      all += weq[w];
-      before += w < wave ? weq[w] : 0u;
-    }
-    if (tid == 0) {
-      a.offsets[g] = base;
-      if (g == a.G - 1) a.offsets[a.G] = base + all;
-    }
-    if (eq == 0) return;
-    uint32_t at = base + before + ceq - eq;
-    for (int q = q0; q < q1; q++) {
-      int32_t v[4];
-      ids(q, v);
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (v[j] == g) a.perm[at++] = (uint32_t)(q * 4 + j);
-    }
-    return;
-  }
-  int at = (int)blockIdx.x - a.plan_blocks;
-  const int w = at >= a.tiles[0] * a.G;
-  if (w) at -= a.tiles[0] * a.G;
-  const int g = at / a.tiles[w];
-  at %= a.tiles[w];
-  const int P = a.P[w], Q = a.Q[w], qt = (Q + 31) / 32;
-  const size_t base = (size_t)g * P * Q;
-  const E* __restrict__ in = (const E*)a.in[w] + base;
-  E* __restrict__ out = (E*)a.out[w] + base;
-  const int x = tid & 31, y = tid >> 5;
-  const int p0 = at / qt * 32, q0 = at % qt * 32;
-#pragma unroll
-  for (int i = 0; i < 32; i += 8)
-    if (p0 + y + i < P && q0 + x < Q) tile[y + i][x] = in[(size_t)(p0 + y + i) * Q + q0 + x];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 32; i += 8)
-    if (q0 + y + i < Q && p0 + x < P) out[(size_t)(q0 + y + i) * P + p0 + x] = tile[x][y + i];
 }
 
 // ----------------------------------------------------- adapter gradients --
@@ -953,13 +1004,12 @@ hipError_t shrink_typed(const ShrinkArgs& a, int S, hipStream_t st) {
 // more (4096 rows at rank 64: 30 us instead of 24).
 constexpr int kTeamBlocks = 256, kRunTiles = 64;
 
-// S > 0: the sums come from a shrink launch's S shares at a.part; otherwise
-// `also` (nullable) runs beside a.
+// S > 0: the sums come from a shrink launch's S shares at a.part.
 template <typename XT>
-hipError_t expand_typed(const ExpandArgs& a, hipStream_t st, const ExpandArgs* also = nullptr) {
+hipError_t expand_typed(const ExpandArgs& a, hipStream_t st, const ExpandJobs* backward = nullptr, int rows = 1) {
   ExpandJobs j{};
+  if (backward) j = *backward;
   j.job[0] = a;
-  if (also) j.job[1] = *also;
   const int tiles = tiles_of(a.T);
   // at least one group of 64 columns per wave; apart all of those
   const int most = a.y ? (a.N + 64 * kFusedWaves - 1) / (64 * kFusedWaves) : 1;
@@ -968,17 +1018,18 @@ hipError_t expand_typed(const ExpandArgs& a, hipStream_t st, const ExpandArgs* a
   j.team = std::min(adapters * j.shares, std::max(2, a.S ? kTile * j.shares : kTeamBlocks / tiles));
   j.run = tiles >= kRunTiles ? (tiles + 7) / 8 : 0;
   const uint32_t blocks = (uint32_t)(j.run ? 8 * j.run : tiles) * (uint32_t)j.team;
-#define MOE_EX(RT)                                                                            \
-  if (a.S == 0)                                                                               \
-    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, true>), dim3(blocks, also ? 2 : 1),        \
-                       dim3(64 * kFusedWaves), 0, st, j);                                     \
-  else                                                                                        \
-    hipLaunchKernelGGL((lora_expand_kernel<XT, RT, false>), dim3(blocks), dim3(64 * kFusedWaves), 0, st, j);
+#define MOE_EX2(RT, FUSED, TURNED)                                                                   \
+  hipLaunchKernelGGL((lora_expand_kernel<XT, RT, FUSED, TURNED>), dim3(blocks, rows), dim3(64 * kFusedWaves), 0, st, j)
+#define MOE_EX(RT)                       \
+  if (backward) MOE_EX2(RT, true, true); \
+  else if (a.S) MOE_EX2(RT, false, false); \
+  else MOE_EX2(RT, true, false);
   if (a.R <= 16) { MOE_EX(1) }
   else if (a.R <= 32) { MOE_EX(2) }
   else if (a.R <= 64) { MOE_EX(4) }
   else { MOE_EX(8) }
 #undef MOE_EX
+#undef MOE_EX2
   return hipGetLastError();
 }
 
@@ -1013,7 +1064,7 @@ size_t partial_bytes(const LoraDims& d) {
   return std::min((size_t)d.T * 16, (size_t)512 * kTile / std::min(kTile, d.G)) * d.R * 4;
 }
 
-constexpr int kPrepRows = 16384;  // rows the prep launch lists; more take a plan of their own
+constexpr int kListRows = 16384;  // rows the backward's first launch lists; more take a plan of their own
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -1040,7 +1091,7 @@ long outer_chunks(const LoraDims& d) {
 }
 
 struct BackwardLayout {
-  size_t s, u, part_u, at, bt, counts, offsets, perm, inv, used, scratch, scratch_bytes, part, total;
+  size_t s, u, counts, offsets, perm, inv, used, scratch, scratch_bytes, part, total;
 };
 BackwardLayout backward_layout(const LoraDims& d) {
   BackwardLayout l{};
@@ -1050,12 +1101,9 @@ BackwardLayout backward_layout(const LoraDims& d) {
     at += up256(bytes);
     return o;
   };
-  const size_t es = d.dt == DT_F32 ? 4 : 2, T = d.T, R = d.R, G = d.G, K = d.K, N = d.N;
+  const size_t T = d.T, R = d.R, G = d.G, K = d.K, N = d.N;
   l.s = take(T * R * 4);
   l.u = take(T * R * 4);
-  l.part_u = take(partial_bytes(d));
-  l.at = take(G * K * R * es);
-  l.bt = take(G * N * R * es);
   l.counts = take(G * 4);
   l.offsets = take((G + 1) * 4);
   l.perm = take(T * 4);
@@ -1074,62 +1122,32 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
   char* ws = reinterpret_cast<char*>(a.ws);
   float* s = reinterpret_cast<float*>(ws + l.s);
   float* u = reinterpret_cast<float*>(ws + l.u);
-  float* part_u = reinterpret_cast<float*>(ws + l.part_u);
-  XT* at = reinterpret_cast<XT*>(ws + l.at);
-  XT* bt = reinterpret_cast<XT*>(ws + l.bt);
   uint32_t* offsets = reinterpret_cast<uint32_t*>(ws + l.offsets);
   uint32_t* perm = reinterpret_cast<uint32_t*>(ws + l.perm);
   hipError_t e;
 #define MOE_OKAY(expr) \
   if ((e = (expr)) != hipSuccess) return e
-  const bool grads = a.da || a.db, need_u = a.dx || a.da;
-  PrepArgs pr{};
-  pr.adapter = a.adapter;
-  pr.offsets = offsets;
-  pr.perm = perm;
-  pr.T = d.T;
-  pr.G = d.G;
-  pr.plan_blocks = grads && d.T <= kPrepRows ? d.G : 0;
-  auto side = [&](int w, const void* in, void* out, int P, int Q) {
-    pr.in[w] = in;
-    pr.out[w] = out;
-    pr.P[w] = P;
-    pr.Q[w] = Q;
-    pr.tiles[w] = ((P + 31) / 32) * ((Q + 31) / 32);
-  };
-  if (need_u) side(0, a.b, bt, d.N, d.R);
-  if (a.dx) side(1, a.a, at, d.R, d.K);
-  const long prep = pr.plan_blocks + (long)d.G * (pr.tiles[0] + pr.tiles[1]);
-  if (prep > 0) {
-    hipLaunchKernelGGL((lora_prep_kernel<XT>), dim3((uint32_t)prep), dim3(256), 0, st, pr);
-    MOE_OKAY(hipGetLastError());
-  }
-  if (grads && !pr.plan_blocks)
+  const bool grads = a.da || a.db, need_u = a.dx || a.da, list = grads && d.T <= kListRows;
+  if (grads && !list)
     MOE_OKAY(launch_dispatch_plan(reinterpret_cast<const uint32_t*>(a.adapter), d.T, 1, d.G,
                                   reinterpret_cast<uint32_t*>(ws + l.counts), offsets, perm,
                                   reinterpret_cast<uint32_t*>(ws + l.inv),
                                   reinterpret_cast<uint32_t*>(ws + l.used), ws + l.scratch,
                                   l.scratch_bytes, st));
-  // u and dx: the forward's launches with B^T and A^T in the place of A and B (u
-  // is the same with and without dx); s: the forward's first half
+  // u and dx: the forward's kernel with B^T and A^T in the place of A and B (u is
+  // the same with and without dx); s: its first half
+  const ExpandArgs eu{a.dy, a.b, a.a, a.scale, a.adapter, a.dx_in, a.dx, a.da ? u : nullptr, nullptr,
+                      d.T, d.N, d.K, d.R, d.G, 0};
   const ExpandArgs es{a.x, a.a, a.b, a.scale, a.adapter, nullptr, nullptr, s, nullptr,
                       d.T, d.K, d.N, d.R, d.G, 0};
-  bool s_done = !a.db;
-  if (need_u) {
-    const LoraDims back{d.dt, d.T, d.N, d.K, d.R, d.G};
-    const int S = lora_fused(back) ? 0 : lora_shares(d.T, d.G, d.N, d.dt);
-    const ExpandArgs eu{a.dy, bt, at, a.scale, a.adapter, a.dx_in, a.dx, a.da ? u : nullptr, part_u,
-                        d.T, d.N, d.K, d.R, d.G, S};
-    if (S) {
-      const ShrinkArgs sh{a.dy, bt, a.adapter, part_u, d.T, d.N, d.R, d.G};
-      MOE_OKAY(shrink_typed<XT>(sh, S, st));
-      MOE_OKAY(expand_typed<XT>(eu, st));
-    } else {
-      MOE_OKAY(expand_typed<XT>(eu, st, s_done ? nullptr : &es));
-      s_done = true;
-    }
+  ExpandJobs jobs{};
+  jobs.job[1] = es;  // where both are asked for
+  jobs.turned = need_u;
+  if (list) {
+    jobs.offsets = offsets;
+    jobs.perm = perm;
   }
-  if (!s_done) MOE_OKAY(expand_typed<XT>(es, st));
+  MOE_OKAY(expand_typed<XT>(need_u ? eu : es, st, &jobs, (int)list + (int)need_u + (a.db != nullptr)));
   if (!grads) return hipSuccess;
   OuterArgs o{};
   o.perm = perm;
@@ -1168,10 +1186,6 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
 
 size_t lora_ws_bytes(const LoraDims& d) {
   return up256(partial_bytes(d));
-}
-long lora_prep_blocks(const LoraDims& d) {
-  const long r = (d.R + 31) / 32;
-  return d.G * (1 + r * ((d.K + 31) / 32) + r * ((d.N + 31) / 32));
 }
 size_t lora_backward_ws_bytes(const LoraDims& d) { return backward_layout(d).total; }
 

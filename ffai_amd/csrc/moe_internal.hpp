@@ -322,7 +322,6 @@ struct LoraBackward {
 };
 size_t lora_ws_bytes(const LoraDims& d);
 size_t lora_backward_ws_bytes(const LoraDims& d);
-long lora_prep_blocks(const LoraDims& d);  // of the backward's first launch, at most
 hipError_t launch_lora(const LoraDims& d, const void* x, const void* a, const void* b,
                        const float* scale, const int32_t* adapter, const void* yin, void* y,
                        void* ws, hipStream_t st);

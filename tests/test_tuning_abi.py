@@ -256,12 +256,6 @@ def test_rows_past_a_launch_refused(T):
     assert "T above" in _lib.last_error()
 
 
-def test_lora_backward_refuses_stacks_past_a_launch():
-    l = lora(n=1 << 20, k=1 << 20, rank=128, n_adapters=1024)
-    assert _lib.load().moe_lora_backward(C.byref(l), *BACK.values(), None) == MOE_ERR_UNSUPPORTED
-    assert "too large" in _lib.last_error()
-
-
 A, B = C.c_void_p(BIG * 21), C.c_void_p(BIG * 22 + 64)
 
 
