@@ -695,13 +695,15 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) voi
 // 13.3 us with products of 4 rows, 15.0 with those of 32 (whose steps the
 // adapters' chunks fill less); rank 64 39 and 26.5.
 //
-// A block takes 128 columns, up to two (fp32: four) rank tiles and a chunk of one adapter's
-// rows (an adapter of n rows has ceil(n / chunk) equal ones, numbered through
-// over the adapters, so that the work is even however the rows spread); its
-// eight waves share the chunk and meet in LDS. The gradient of an adapter with
-// one chunk is stored at once, the chunks of the others as fp32, which
-// lora_sum_kernel adds in order. Steps are loaded one ahead, the list of rows
-// two ahead.
+// A block takes 128 columns (or several times that, see outer_span), up to two
+// (fp32: four) rank tiles and a chunk of one adapter's rows (an adapter of n rows
+// has ceil(n / chunk) equal ones, numbered through over the adapters, so that the
+// work is even however the rows spread). Its eight waves share the chunk and
+// meet in LDS; where it has fewer rows than their steps they share columns too.
+// The gradient of an adapter with one chunk is stored at once, the chunks of the
+// others as fp32, which lora_sum_kernel adds in order. Steps are loaded one
+// ahead, the list of rows two ahead. SPAN: the form for several column blocks,
+// whose loop takes the plain one's 11.8 us to 13.0.
 struct OuterSide {
   const void* wide;    // [T, cols]: x or dy
   const float* small;  // [T, R]: u or s
@@ -716,6 +718,7 @@ struct OuterArgs {
   const uint32_t* offsets;
   int R, G, sides;
   uint32_t chunk;  // rows of a chunk, at most
+  int span;        // column blocks of a block: 1, 2, 4 or 8
 };
 constexpr int kOuterWaves = 8, kOuterCols = 128;
 
@@ -786,30 +789,35 @@ __device__ __forceinline__ void outer_store(const f32x4_t (&acc)[RB][8], OT* out
   }
 }
 
-template <typename XT, int RB>
+template <typename XT, int RB, bool SPAN>
 __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs p) {
   constexpr bool FOUR = sizeof(XT) == 4 || RB == 1;  // products of four rows
   constexpr int XW = sizeof(XT) / 2;                 // 16-byte loads of 8 columns
   constexpr int U = FOUR ? 2 : 8;                    // rows of a lane and step, 4 U of the wave
   __shared__ f32x4_t red[kOuterWaves / 2][RB * 8 * 64];
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool second = p.sides == 2 && (blockIdx.z & 1u);
   const OuterSide sd = second ? p.side[1] : p.side[0];
   const int r0 = (int)(p.sides == 2 ? blockIdx.z >> 1 : blockIdx.z) * (RB * 16);
-  const int R = p.R, cols = sd.cols, cb = blockIdx.x * kOuterCols;
-  if (cb >= cols) return;
-  const int col = cb + 8 * c;
+  const int R = p.R, cols = sd.cols;
+  const int span = SPAN ? p.span : 1;
+  if ((int)blockIdx.x * span * kOuterCols >= cols) return;
   const Chunks ck = find_chunks(p.offsets, p.G, p.chunk, blockIdx.y, -1);
   if (ck.g >= p.G) return;
-  const XT* const wide = (const XT*)sd.wide + col;
-  const float* const small = sd.small + r0 + c;
-  const size_t per = (size_t)R * cols;
   const uint32_t rows = (ck.o1 - ck.o0 + ck.n - 1) / ck.n;  // of an equal chunk
   const uint32_t s0 = min(ck.o1, ck.o0 + (blockIdx.y - ck.first) * rows), s1 = min(ck.o1, s0 + rows);
-  {
-    const uint32_t len = ((s1 - s0 + kOuterWaves - 1) / kOuterWaves + 3u) & ~3u;
-    const uint32_t b0 = min(s1, s0 + (uint32_t)wave * len), b1 = min(s1, b0 + len);
+  const int few = rows <= 4 * U ? 8 : rows <= 8 * U ? 4 : rows <= 16 * U ? 2 : 1;
+  const int across = min(few, span);  // waves across columns, the others across rows
+  const size_t per = (size_t)R * cols;
+  for (int it = 0; it < span; it += across) {
+    int lane = tid & 63;
+    if constexpr (SPAN) asm volatile("" : "+v"(lane));  // (opaque: else its addresses are kept over the loop)
+    const int c = lane & 15, q = lane >> 4;
+    const float* const small = sd.small + r0 + c;
+    const int cb = ((int)blockIdx.x * span + it + (wave & (across - 1))) * kOuterCols, col = cb + 8 * c;
+    const XT* const wide = (const XT*)sd.wide + col;
+    const uint32_t parts = kOuterWaves / across, len = ((s1 - s0 + parts - 1) / parts + 3u) & ~3u;
+    const uint32_t b0 = min(s1, s0 + (uint32_t)(wave / across) * len), b1 = min(s1, b0 + len);
     f32x4_t acc[RB][8] = {};
     if (b0 < b1) {
       // row i of a lane in a step: 4 i + q where every product takes four rows,
@@ -929,6 +937,7 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
     // the upper half of the waves hands its sums to the lower, down to one
 #pragma unroll
     for (int half = kOuterWaves / 2; half >= 1; half >>= 1) {
+      if (half < across) break;
       if (wave >= half && wave < 2 * half) {
 #pragma unroll
         for (int k = 0; k < RB; k++)
@@ -944,7 +953,7 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
       }
       lds_barrier();
     }
-    if (wave == 0) {
+    if (wave < across) {
       if (ck.n == 1) outer_store<XT, RB>(acc, (XT*)sd.out + ck.g * per, sd.rank_major, R, cols, r0, cb, c, q);
       else outer_store<float, RB>(acc, sd.part + blockIdx.y * per, sd.rank_major, R, cols, r0, cb, c, q);
     }
@@ -1078,7 +1087,8 @@ long outer_target(const LoraDims& d) {
   const int rt = outer_ranks(d) * 16;
   const long blocks = (long)((d.K + kOuterCols - 1) / kOuterCols + (d.N + kOuterCols - 1) / kOuterCols) *
                       ((d.R + rt - 1) / rt);
-  return std::max(4L, 512 / blocks - d.G / 2);
+  const long n = 512 / blocks;
+  return std::max({4L, n / 2, n - d.G / 2});
 }
 uint32_t outer_chunk(const LoraDims& d) {
   const long n = outer_target(d);
@@ -1088,6 +1098,19 @@ uint32_t outer_chunk(const LoraDims& d) {
 // sized for many rows serves a call of few).
 long outer_chunks(const LoraDims& d) {
   return std::min<long>(d.T, std::min(outer_target(d), (long)(d.T + 63) / 64) + d.G);
+}
+
+// Column blocks of a block: more than one where adapters have few rows on
+// average, so that its waves have a step of rows each and the chip is not busy
+// with blocks of one working wave (2048 rows of 64 adapters 4096 -> 4096 at rank 64
+// 38 us instead of 186, 64 rows of 64 adapters 6.3 instead of 11; a single adapter
+// that has all the rows 12.9 and 12.8), as long as 512 blocks remain (512 rows of
+// one of 64 adapters 13.2 us, with 256 blocks 22.4).
+int outer_span(const LoraDims& d, long blocks) {
+  const int step = d.dt == DT_F32 || d.R <= 16 ? 8 : 32, rows = (d.T + d.G - 1) / d.G;
+  int span = rows <= step ? 8 : rows <= 2 * step ? 4 : rows <= 4 * step ? 2 : 1;
+  while (span > 1 && blocks / span < 512) span /= 2;
+  return span;
 }
 
 struct BackwardLayout {
@@ -1167,11 +1190,15 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
     cols = std::max(cols, d.N);
   }
   const int RB = outer_ranks(d);
-  const dim3 grid((cols + kOuterCols - 1) / kOuterCols, (uint32_t)chunks, o.sides * ((d.R + RB * 16 - 1) / (RB * 16)));
-#define MOE_OU(RB) hipLaunchKernelGGL((lora_outer_kernel<XT, RB>), grid, dim3(64 * kOuterWaves), 0, st, o)
-  if (RB == 1) MOE_OU(1);
-  else if (RB == 2) MOE_OU(2);
-  else if constexpr (sizeof(XT) == 4) MOE_OU(4);
+  const int cblocks = (cols + kOuterCols - 1) / kOuterCols, ranks = o.sides * ((d.R + RB * 16 - 1) / (RB * 16));
+  o.span = outer_span(d, cblocks * chunks * ranks);
+  const dim3 grid((cblocks + o.span - 1) / o.span, (uint32_t)chunks, ranks);
+#define MOE_OU(RB)                                                                             \
+  if (o.span > 1) hipLaunchKernelGGL((lora_outer_kernel<XT, RB, true>), grid, dim3(64 * kOuterWaves), 0, st, o); \
+  else hipLaunchKernelGGL((lora_outer_kernel<XT, RB, false>), grid, dim3(64 * kOuterWaves), 0, st, o);
+  if (RB == 1) { MOE_OU(1) }
+  else if (RB == 2) { MOE_OU(2) }
+  else if constexpr (sizeof(XT) == 4) { MOE_OU(4) }
 #undef MOE_OU
   MOE_OKAY(hipGetLastError());
   const size_t per = (size_t)d.R * cols;

@@ -561,6 +561,39 @@ def test_lora_backward_many_rows(dt):
     assert (gx.cpu()[none] == 0).all()
 
 
+@pytest.mark.parametrize("dt,T,K,N,R,G", [
+    (BF16, 900, 2056, 136, 16, 120), (F16, 300, 1096, 520, 8, 200), (F32, 900, 136, 2056, 40, 120),
+    (F32, 500, 1160, 264, 24, 250), (BF16, 700, 2824, 264, 40, 40), (F16, 1500, 520, 1928, 72, 50)])
+def test_lora_backward_many_adapters(dt, T, K, N, R, G):
+    """Few rows an adapter (blocks of the outer products take several column
+    blocks) but for one that has half of all, and a few of about a dozen."""
+    x, A, B, scale, _ = lora_case(T, K, N, R, G, dt, T + R)
+    g = gen(T)
+    ad = torch.randint(-1, G, (T,), generator=g)
+    ad[torch.rand(T, generator=g) < 0.5] = 7
+    ad[:60] = torch.arange(60) // 13 + 20
+    ad[ad == 11] = 12
+    ad = ad[torch.randperm(T, generator=g)].to(torch.int32)
+    dy = torch.randn(T, N, generator=g).to(dt)
+    l = tuning.LoRAAdapters(A.cuda(), B.cuda(), scale.cuda())
+    gx, ga, gb = (t.cpu() for t in l.backward(x.cuda(), dy.cuda(), ad.cuda()))
+    sp = split_err(dt)
+    for a in range(G):
+        r = (ad == a).nonzero()[:, 0]
+        if len(r) == 0:
+            assert (ga[a] == 0).all() and (gb[a] == 0).all()
+            continue
+        s, X, D, Aa, Bb = float(scale[a]), x[r].double(), dy[r].double(), A[a].double(), B[a].double()
+        u, s1 = s * D @ Bb, s * X @ Aa.t()
+        um, sm = s * D.abs() @ Bb.abs(), s * X.abs() @ Aa.abs().t()
+        close(gx[r], u @ Aa, (um @ Aa.abs()) * ((N + R + 16) * U + sp), f"dx {a}")
+        close(ga[a], u.t() @ X, (um.t() @ X.abs()) * ((N + len(r) + 16) * U + sp), f"da {a}")
+        close(gb[a], D.t() @ s1, (D.abs().t() @ sm) * ((K + len(r) + 16) * U + sp), f"db {a}")
+    assert (gx[ad < 0] == 0).all()
+    for first, again in zip((gx, ga, gb), l.backward(x.cuda(), dy.cuda(), ad.cuda())):
+        assert same_bits(first, again.cpu())
+
+
 def test_lora_backward_matches_differences():
     """Gradients against central differences of the float64 forward."""
     T, K, N, R, G = 12, 16, 24, 8, 3
