@@ -326,15 +326,18 @@ __device__ __forceinline__ void list_rows(const int32_t* __restrict__ adapter, i
 
 // Waves per SIMD: two blocks on a CU where LDS has room for them, so that a few
 // blocks more than CUs (requests that end inside a tile) cost no second round.
-constexpr int expand_waves(size_t es, int rt) { return rt <= (es == 4 ? 2 : 4) ? 4 : 2; }
+constexpr int expand_waves(int rt) { return rt <= 4 ? 4 : 2; }
 
 template <typename XT, int RT, bool FUSED, bool TURNED>
-__global__ __launch_bounds__(64 * kFusedWaves, expand_waves(sizeof(XT), RT)) void lora_expand_kernel(ExpandJobs jobs) {
+__global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expand_kernel(ExpandJobs jobs) {
   constexpr bool F32 = sizeof(XT) == 4;
   constexpr uint32_t ES = sizeof(XT);
   constexpr int V = 16 / sizeof(XT), LD = RT * 16 + 4, W = kFusedWaves;
   constexpr int UNIT = 8 * V;                      // a unit of K: 128 bytes of a row
-  constexpr int J = F32 ? (RT == 8 ? 2 : 4) : 4;   // neighbouring columns of a lane
+  // neighbouring columns of a lane: as many as leave LDS for two blocks up to
+  // rank 64 (fp32 at rank 40, 7454 rows backward: 25 us with two columns, 31 with four;
+  // 4096 rows at rank 64, whose tiles are as many as CUs, 54 and 50)
+  constexpr int J = F32 && RT >= 4 ? 2 : 4;
   constexpr int NC = 16 * J;                       // columns of a group
   constexpr int C8 = RT * 16 / V;                  // 16-byte chunks of the widest adapter row
   constexpr int BL = NC * C8 / 64;                 // loads of a column group's b rows
@@ -968,24 +971,59 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
 }
 
 // Adds the chunks of the adapters that have several, and writes zeros for
-// those without rows; the others are there already.
+// those without rows; the others are there already. A lane adds 8 neighbouring
+// values. Up to eight chunks one wave adds them all; more are shared by the
+// block's waves, whose sums meet in LDS (7454 rows of one adapter 264 -> 96 at
+// rank 40, 117 chunks: 5.8 us,
+// by one wave 14).
+constexpr int kSumWaves = 4;
 template <typename XT>
-__global__ __launch_bounds__(256) void lora_sum_kernel(OuterArgs p) {
+__global__ __launch_bounds__(64 * kSumWaves) void lora_sum_kernel(OuterArgs p) {
+  __shared__ float meet[kSumWaves - 1][8][64];
   const OuterSide sd = p.side[blockIdx.z];
-  const int g = blockIdx.y;
+  const int g = blockIdx.y, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Chunks ck = find_chunks(p.offsets, p.G, p.chunk, 0, g);
   if (ck.n == 1) return;
   const size_t per = (size_t)p.R * sd.cols;
-  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8; i < per; i += (size_t)gridDim.x * 2048) {
-    float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto add = [&](size_t i, uint32_t c0, uint32_t c1, float (&a)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) a[j] = 0.f;
+    if (i >= per) return;
 #pragma unroll 4
-    for (uint32_t c = 0; c < ck.n; c++) {
+    for (uint32_t c = c0; c < c1; c++) {
       float b[8];
       Vec8<float>::load(sd.part + (ck.first + c) * per + i, b);
 #pragma unroll
       for (int j = 0; j < 8; j++) a[j] += b[j];
     }
-    Vec8<XT>::store((XT*)sd.out + g * per + i, a);
+  };
+  float a[8];
+  if (ck.n <= 8) {
+    for (size_t i = ((size_t)blockIdx.x * 64 * kSumWaves + threadIdx.x) * 8; i < per;
+         i += (size_t)gridDim.x * 512 * kSumWaves) {
+      add(i, 0, ck.n, a);
+      Vec8<XT>::store((XT*)sd.out + g * per + i, a);
+    }
+    return;
+  }
+  const uint32_t share = (ck.n + kSumWaves - 1) / kSumWaves;
+  for (size_t b = (size_t)blockIdx.x * 512; b < per; b += (size_t)gridDim.x * 512) {
+    const size_t i = b + lane * 8;
+    add(i, min(ck.n, wave * share), min(ck.n, (wave + 1) * share), a);
+    if (wave) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) meet[wave - 1][j][lane] = a[j];
+    }
+    lds_barrier();
+    if (wave == 0 && i < per) {
+#pragma unroll
+      for (int w = 0; w < kSumWaves - 1; w++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) a[j] += meet[w][j][lane];
+      Vec8<XT>::store((XT*)sd.out + g * per + i, a);
+    }
+    lds_barrier();
   }
 }
 
@@ -1209,8 +1247,8 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
 #undef MOE_OU
   MOE_OKAY(hipGetLastError());
   const size_t per = (size_t)d.R * cols;
-  hipLaunchKernelGGL((lora_sum_kernel<XT>), dim3((uint32_t)std::min<size_t>((per + 2047) / 2048, 512), d.G, o.sides),
-                     dim3(256), 0, st, o);
+  hipLaunchKernelGGL((lora_sum_kernel<XT>), dim3((uint32_t)std::min<size_t>((per + 511) / 512, 512), d.G, o.sides),
+                     dim3(64 * kSumWaves), 0, st, o);
   MOE_OKAY(hipGetLastError());
 #undef MOE_OKAY
   return hipSuccess;
