@@ -143,7 +143,10 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs p) {
 // inner axis (against the same b values), which keeps 16 (f16: 22) bits of
 // it: for rank 16 one instruction holds both. f16 rows are first scaled by a
 // power of two to a maximum in [2^14, 2^15), so that neither part over- or
-// underflows, and the sum back afterwards.
+// underflows, and the sum back afterwards. Infinities do not survive that: lo x
+// inf has a sign of its own, and 0 x inf (a lo of 0, a chunk of the product that
+// is not used) is NaN. So a group of columns with a sum that is not finite is
+// computed again from the fp32 sums, by products of 4 ranks (16x16x4).
 struct ExpandArgs {
   const void* x;           // [T, K]
   const void* a;           // [G, R, K]
@@ -343,6 +346,10 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
   constexpr int BL = NC * C8 / 64;                 // loads of a column group's b rows
   constexpr int AREA = (1 + RT) * 128 > NC * (C8 | 1) ? (1 + RT) * 128 : NC * (C8 | 1);  // 16-byte slots
   static_assert(AREA * 4 >= 2 * kTile * LD, "the sums of a wave and of the block fit an area");
+  // 16-bit types: behind the column groups two rows of the block's sums stay,
+  // rows 2 w and 2 w + 1 in area w
+  constexpr int KEPT = AREA - 64;
+  static_assert(F32 || (KEPT >= NC * (C8 | 1) && 64 * 4 >= 2 * RT * 16 && kTile == 2 * W), "room for the kept sums");
   // a wave's area holds in turn its units, its sums and its column groups; the
   // first one's second half the block's sums
   __shared__ u32x4_t area[W][AREA];
@@ -589,6 +596,7 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
       }
       v *= sc;
       sum[at] = v;
+      if constexpr (!F32) reinterpret_cast<float*>(area[t >> 1] + KEPT)[(t & 1) * RT * 16 + r] = v;
       if (p.s && share == 0 && r < R && ((same >> t) & 1u)) p.s[(size_t)(t0 + t) * R + r] = v;
     }
     lds_barrier();
@@ -611,8 +619,11 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
 #pragma unroll
       for (int i = 0; i < RT; i++) {
         const int ci = 4 * i + q, cc = F32 || ci < c8 ? ci : ci - c8;
-        at[i] = (uint32_t)c * (c8 | 1) + min(cc, c8 - 1);
+        at[i] = (uint32_t)c * (c8 | 1) + min(cc, F32 ? c8 : c8 - 1);
       }
+      // fp32: chunks past the rank meet the columns' spare slots (c8 is even), which
+      // hold zeros, since 0 x inf is not 0
+      if (F32 && c8 < C8 && lane < NC) mem[lane * (c8 | 1) + c8] = u32x4_t{0u, 0u, 0u, 0u};
       for (int grp = g0; grp < g1; grp++) {
         if constexpr (TURNED) {
           int l = lane;
@@ -666,6 +677,31 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
             if (BL >= 16) __builtin_amdgcn_sched_barrier(0);
           }
         }
+        bool again = false;  // the same in all lanes
+        if constexpr (!F32) {
+          float nan[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) nan[i] = __builtin_fmaf(o[j][i], 0.f, nan[i]);
+          const float any = (nan[0] + nan[1]) + (nan[2] + nan[3]);
+          again = __builtin_expect(__any(any != any), 0);
+          if (again) {
+            int l = tid & 63;
+            asm volatile("" : "+v"(l));  // (opaque: as above)
+            const int row = l & 15, k = l >> 4;
+            const float* const kept = reinterpret_cast<const float*>(area[row >> 1] + KEPT) + (row & 1) * RT * 16 + k;
+            const XT* const bcol = reinterpret_cast<const XT*>(mem + row * (c8 | 1)) + k;
+#pragma unroll
+            for (int j = 0; j < J; j++) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int r = 0; r < R; r += 4) {
+#pragma unroll
+              for (int j = 0; j < J; j++)
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(kept[r], to_f<XT>(bcol[j * 16 * (c8 | 1) * V + r]), o[j], 0, 0, 0);
+            }
+          }
+        }
         wave_lds_sync();
         const uint32_t no = grp < g1 && grp * NC + J * c < N ? (uint32_t)grp * NC * ES : kFar;
 #pragma unroll
@@ -678,8 +714,9 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
 #pragma unroll
             for (int j = 0; j < J / 2; j++) {
               const uint32_t y2 = yv[i][j];
-              const float lo = __builtin_fmaf(o[2 * j][i], bk[i], to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(y2 & 0xFFFFu))));
-              const float hi = __builtin_fmaf(o[2 * j + 1][i], bk[i], to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(y2 >> 16))));
+              const float m = again ? 1.f : bk[i];
+              const float lo = __builtin_fmaf(o[2 * j][i], m, to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(y2 & 0xFFFFu))));
+              const float hi = __builtin_fmaf(o[2 * j + 1][i], m, to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(y2 >> 16))));
               w[j] = (uint32_t)__builtin_bit_cast(uint16_t, from_f<XT>(lo)) |
                      ((uint32_t)__builtin_bit_cast(uint16_t, from_f<XT>(hi)) << 16);
             }
@@ -701,7 +738,8 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
 // (16x16x4), as it lies. More rank tiles of 16-bit rows: a lane reads 8 rows of
 // its columns and turns them in registers into the 8 columns' operands of one
 // product of 32 rows (16x16x32, eight times the rate), which u and s enter as
-// two 16-bit parts as in expand. 4096 rows of 8 adapters 2048 -> 2048: rank 16
+// two 16-bit parts as in expand; a wave with a sum that is not finite adds its rows
+// again in fp32 products of 4, as there. 4096 rows of 8 adapters 2048 -> 2048: rank 16
 // 13.3 us with products of 4 rows, 15.0 with those of 32 (whose steps the
 // adapters' chunks fill less); rank 64 39 and 26.5.
 //
@@ -939,6 +977,37 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
               } else {
                 acc[k][j] = mma<XT>(lo[k], x, mma<XT>(hi[k], x, acc[k][j]));
               }
+            }
+          }
+        }
+      }
+      if constexpr (!FOUR) {
+        float nan[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < RB; k++)
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int h = 0; h < 4; h++) nan[h] = __builtin_fmaf(acc[k][j][h], 0.f, nan[h]);
+        const float any = (nan[0] + nan[1]) + (nan[2] + nan[3]);
+        if (__builtin_expect(__any(any != any), 0)) {
+#pragma unroll
+          for (int k = 0; k < RB; k++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) acc[k][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+          for (uint32_t at = b0; at < b1; at += 4) {
+            const bool in = at + q < b1;
+            const uint32_t t = p.perm[min(at + q, b1 - 1)];
+            u32x4_t x{0u, 0u, 0u, 0u};
+            if (in && col < cols) x = *reinterpret_cast<const u32x4_t*>(wide + (size_t)t * cols);
+#pragma unroll
+            for (int k = 0; k < RB; k++) {
+              const float s = in && r0 + k * 16 + c < R ? small[(size_t)t * R + k * 16] : 0.f;
+#pragma unroll
+              for (int j = 0; j < 8; j++)
+                acc[k][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                    s, to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(x[j >> 1] >> (16 * (j & 1))))), acc[k][j], 0, 0, 0);
             }
           }
         }

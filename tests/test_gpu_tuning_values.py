@@ -1,0 +1,146 @@
+"""Tuning and adapter entry points on the GPU at values of the far ends: infinities, inner sums outside a 16-bit type's
+range, saturated sigmoids, rows of a type's lowest value. References and bounds in float64, as in test_gpu_tuning.py: a
+result rounded to type t is off by eps(t)/2 of its value, a sum of n fp32 products by (n + c) 2^-24 of the sum of their
+magnitudes, a factor kept as two 16-bit parts by 2^-17 of itself."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from ffai_amd import _lib, tuning  # noqa: E402
+from ffai_amd.layer import MoEGatingMode, MoERouter  # noqa: E402
+
+U = 2.0 ** -24
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+SOFT, PICK, SIGM = MoEGatingMode.softmaxThenTopK, MoEGatingMode.topKThenSoftmax, MoEGatingMode.sigmoidTopK
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    _lib.load()
+    yield
+    torch.cuda.synchronize()
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def cuda(t):
+    return None if t is None else t.cuda()
+
+
+def close(got, ref, tol, what):
+    """|got - ref| <= half a step of got's type + tol where ref is finite; the same NaN and infinities elsewhere."""
+    half = torch.finfo(got.dtype).eps / 2
+    low = torch.finfo(got.dtype).smallest_normal * half
+    got, ref, tol = got.double().cpu(), ref.double().cpu(), torch.as_tensor(tol, dtype=torch.float64)
+    fin = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)), (
+        f"{what}: {int((torch.isnan(got) & ~torch.isnan(ref)).sum())} NaN too many, "
+        f"{int((~torch.isnan(got) & torch.isnan(ref)).sum())} too few")
+    inf = torch.isinf(ref)
+    assert torch.equal(got[inf], ref[inf]), f"{what}: infinities"
+    bound = half * (ref.abs() + tol) + tol + low + torch.finfo(torch.float32).tiny
+    bad = ((got - ref).abs() > bound) & fin
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} off, worst "
+                           f"{((got - ref).abs() / bound)[fin].max():.3g} of the bound")
+
+
+# ------------------------------------------------------------- infinities --
+
+def products(a, b):
+    """Rows of a against rows of b in float64, every product and sum as IEEE has it."""
+    return (a[:, None, :] * b[None, :, :]).sum(-1)
+
+
+def adapter_case(T, K, N, R, G, dt, seed):
+    """Signed inputs whose inner sums are far from zero (1 to 2 of one sign or the other): their signs are not in doubt."""
+    g = gen(seed)
+    x = (torch.rand(T, K, generator=g) + 0.5).to(dt)
+    sign = torch.where(torch.rand(G, R, generator=g) < 0.5, -1.0, 1.0)
+    A = (sign[:, :, None] * (torch.rand(G, R, K, generator=g) + 0.5) * 1.5 / K).to(dt)
+    B = ((torch.rand(G, N, R, generator=g) + 0.1) * torch.where(torch.rand(G, N, 1, generator=g) < 0.5, -0.1, 0.1)).to(dt)
+    dy = (torch.rand(T, N, generator=g) + 0.5).to(dt)
+    return x, A, B, torch.rand(G, generator=g) + 0.5, torch.randint(-1, G, (T,), generator=g).to(torch.int32), dy
+
+
+def adapter_ref(x, A, B, scale, ad, dy):
+    """y, dx, dA, dB of the adapters in float64, with bounds on finite values' fp32 errors."""
+    T, K, N, R = x.shape[0], x.shape[1], B.shape[1], A.shape[1]
+    sp = 0.0 if x.dtype == F32 else 2.0 ** -17
+    z = lambda *s: torch.zeros(*s, dtype=torch.float64)  # noqa: E731
+    y, dx, dA, dB = z(T, N), z(T, K), z(*A.shape), z(*B.shape)
+    ty, tx, tA, tB = z(T, N), z(T, K), z(*A.shape), z(*B.shape)
+    for a in range(A.shape[0]):
+        r = (ad == a).nonzero()[:, 0]
+        if not len(r):
+            continue
+        s, X, D, Aa, Bb = float(scale[a]), x[r].double(), dy[r].double(), A[a].double(), B[a].double()
+        si, u = s * products(X, Aa), s * products(D, Bb.t())
+        sm, um = s * products(X.abs(), Aa.abs()), s * products(D.abs(), Bb.abs().t())
+        y[r], ty[r] = products(si, Bb), products(sm, Bb.abs()) * ((K + R + 16) * U + sp)
+        dx[r], tx[r] = products(u, Aa.t()), products(um, Aa.abs().t()) * ((N + R + 16) * U + sp)
+        dA[a], tA[a] = products(u.t(), X.t()), products(um.t(), X.abs().t()) * ((N + len(r) + 16) * U + sp)
+        dB[a], tB[a] = products(D.t(), si.t()), products(D.abs().t(), sm.t()) * ((K + len(r) + 16) * U + sp)
+    return (y, dx, dA, dB), (ty, tx, tA, tB)
+
+
+# ranks that fill a product's inner axis and ranks that do not; one and several steps; few rows that large adapters meet
+# in two launches; one adapter met by all rows
+ADAPTERS = [(40, 72, 136, 8, 2), (33, 64, 200, 16, 3), (70, 136, 72, 24, 2), (50, 64, 64, 32, 1), (150, 72, 264, 40, 2),
+            (64, 64, 136, 64, 2), (90, 72, 72, 72, 1), (35, 64, 136, 128, 2), (3, 1032, 1096, 64, 2)]
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("T,K,N,R,G", ADAPTERS)
+@pytest.mark.parametrize("where", ["a", "b", "x", "dy", "xb", "none"])
+def test_adapters_carry_infinities(dt, T, K, N, R, G, where):
+    """An infinity in a factor is an infinity (or NaN where it meets a zero or its opposite) in the sums that have it, and
+    leaves all others as they are."""
+    x, A, B, scale, ad, dy = adapter_case(T, K, N, R, G, dt, T + R)
+    ad[0], ad[-1] = 0, G - 1
+    if where == "a":
+        A[0, R - 1, 3], A[G - 1, 0, K - 1] = INF, -INF
+    if where in ("b", "xb"):
+        B[0, 5, R - 1], B[0, N - 1, 0], B[G - 1, 7, R // 2] = INF, -INF, INF
+        B[0, 9, 1], B[0, 9, 2] = INF, 0.0
+    if where in ("x", "xb"):
+        x[0, 2], x[-1, K - 1] = INF, -INF
+    if where == "dy":
+        dy[0, 4], dy[-1, N - 1] = INF, -INF
+    l = tuning.LoRAAdapters(A.cuda(), B.cuda(), scale.cuda())
+    (y, dx, dA, dB), (ty, tx, tA, tB) = adapter_ref(x, A, B, scale, ad, dy)
+    if where != "none":
+        assert torch.isinf(torch.cat([t.flatten() for t in (y, dx, dA, dB)])).any()
+    close(l.apply(x.cuda(), ad.cuda()), y, ty, "y")
+    gx, ga, gb = l.backward(x.cuda(), dy.cuda(), ad.cuda())
+    close(gx, dx, tx, "dx")
+    close(ga, dA, tA, "da")
+    close(gb, dB, tB, "db")
+
+
+@pytest.mark.parametrize("T,R", [(40, 16), (40, 24), (100, 64), (100, 128)])
+def test_f16_sums_beside_an_infinite_one(T, R):
+    """f16 inner sums outside f16's range keep their bits in a row, and in steps of a gradient, that hold an infinite one."""
+    K, N, G = 64, 72, 1
+    x, A, B, scale, ad, dy = adapter_case(T, K, N, R, G, F16, R)
+    ad.fill_(0)
+    A, B, dy = A * 0 + 1000, B * 0 + 2.0 ** -10, dy * 2.0 ** -11
+    A[0, 1:R:2] = 2.0 ** -9  # small sums beside the large ones
+    A[0, R - 1, 3] = INF
+    x = x * 4
+    B[0, :, R - 1] = 0  # (the infinite sum times zero: y is NaN, the gradients of the other ranks are not)
+    l = tuning.LoRAAdapters(A.cuda(), B.cuda(), scale.cuda())
+    (_, dx, dA, dB), (_, tx, tA, tB) = adapter_ref(x, A, B, scale, ad, dy)
+    assert float((x[0].float() @ A[0, 0].float()) * scale[0]) > 65504 and torch.isfinite(dB[0, :, :R - 1]).all()
+    assert dB[0, :, :R - 1].max() < 65504
+    y = l.apply(x.cuda(), ad.cuda())
+    assert torch.isnan(y).all()
+    gx, ga, gb = l.backward(x.cuda(), dy.cuda(), ad.cuda())
+    close(gx, dx, tx, "dx")
+    close(ga, dA, tA, "da")
+    close(gb, dB, tB, "db")
