@@ -210,14 +210,16 @@ class LoRAAdapters:
         check(_lib.load().moe_validate_lora(C.byref(desc)))
         object.__setattr__(self, "_struct", desc)
         object.__setattr__(self, "_ref", C.byref(desc))
-        object.__setattr__(self, "_as", (self.a.shape, self.b.shape, self.a.dtype, self.b.dtype))
+        s = self.scale
+        object.__setattr__(self, "_as", (self.a.shape, self.b.shape, self.a.dtype, self.b.dtype,
+                                         None if s is None else (s.shape, s.dtype)))
 
     def _current(self) -> Lora:
         """The descriptor, of the memory the tensors have now."""
         l, a, b, s = self._struct, self.a, self.b, self.scale
         if (a.data_ptr() != l.a or b.data_ptr() != l.b or (s is not None and s.data_ptr() != l.scale)
-                or (a.shape, b.shape, a.dtype, b.dtype) != self._as
-                or not (a.is_contiguous() and b.is_contiguous())):
+                or (a.shape, b.shape, a.dtype, b.dtype, None if s is None else (s.shape, s.dtype)) != self._as
+                or not (a.is_contiguous() and b.is_contiguous() and (s is None or s.is_contiguous()))):
             self.__post_init__()
             l = self._struct
         return l
