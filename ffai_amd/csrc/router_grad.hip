@@ -142,15 +142,27 @@ __device__ __forceinline__ RowStat row_softmax(const float (&s)[kCols], float (&
   return r;
 }
 
-// 1 / (1 + exp(-s)); the exponent's rounding is put back as a first-order
-// factor (2^d = 1 + d ln 2) where the power is finite, since here it does not
-// cancel.
-__device__ __forceinline__ float sigmoid_acc(float s) {
+// exp(-s); the exponent's rounding is put back as a first-order factor (2^d = 1 +
+// d ln 2) where the power is finite, since here it does not cancel.
+__device__ __forceinline__ float exp_neg_acc(float s) {
   const float t = -s * kLog2e;
-  float e = __builtin_amdgcn_exp2f(t);
+  const float e = __builtin_amdgcn_exp2f(t);
   const float d = __builtin_fmaf(-s, kLog2e, -t);
-  e = __builtin_fabsf(t) < 126.f ? __builtin_fmaf(e, d * 0.69314718f, e) : e;
-  return 1.0f / (1.0f + e);
+  return __builtin_fabsf(t) < 126.f ? __builtin_fmaf(e, d * 0.69314718f, e) : e;
+}
+
+// 1 / (1 + exp(-s)).
+__device__ __forceinline__ float sigmoid_acc(float s) { return 1.0f / (1.0f + exp_neg_acc(s)); }
+
+// The sigmoid v and its complement 1 - v = exp(-s) v, which a subtraction from v
+// near 1 would round away (at s = 12 to 1 %, from 17 on to 0); 1, which the minimum
+// also makes of inf x 0, where the power is past fp32. A NaN is left to v.
+struct Sigmoid {
+  float v, rest;
+};
+__device__ __forceinline__ Sigmoid sigmoid_pair(float s) {
+  const float e = exp_neg_acc(s), v = 1.0f / (1.0f + e);
+  return {v, fminf(e * v, 1.0f)};
 }
 
 }  // namespace
@@ -617,23 +629,25 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
     float d[kCols];
     const float zl = zc * st.lse;
     if (a.sigmoid) {
-      float q[kCols], sg[kCols], S = 0.f;
+      float q[kCols], rest[kCols], S = 0.f;
 #pragma unroll
       for (int j = 0; j < kCols; j++) {
-        sg[j] = sigmoid_acc(s[j]);
-        S += sg[j];
+        const Sigmoid sg = sigmoid_pair(s[j]);
+        q[j] = sg.v;
+        rest[j] = sg.rest;
+        S += sg.v;
       }
       S = row_sum<LG>(S);
       const float inv = S == 0.f ? 0.f : 1.0f / S;
       float c = 0.f;
 #pragma unroll
       for (int j = 0; j < kCols; j++) {
-        q[j] = sg[j] * inv;
+        q[j] *= inv;
         c = __builtin_fmaf(q[j], f[j], c);
       }
       c = row_sum<LG>(c);
 #pragma unroll
-      for (int j = 0; j < kCols; j++) d[j] = q[j] * (1.0f - sg[j]) * (f[j] - c) + zl * p[j];
+      for (int j = 0; j < kCols; j++) d[j] = q[j] * rest[j] * (f[j] - c) + zl * p[j];
     } else {
       float c = 0.f;
 #pragma unroll
@@ -676,8 +690,9 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
           pv[i] = 0.f;
           if ((NP == 1 || i * LPR < k)) {
             if (a.mode == kSigmoid) {
-              v[i] = sigmoid_acc(v[i]);
-              pv[i] = v[i] * (1.0f - v[i]);
+              const Sigmoid sg = sigmoid_pair(v[i]);
+              v[i] = sg.v;
+              pv[i] = sg.v * sg.rest;
             } else {
               v[i] = exp_off(v[i], st.ml) * st.inv;
               pv[i] = v[i];

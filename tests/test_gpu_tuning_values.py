@@ -144,3 +144,50 @@ def test_f16_sums_beside_an_infinite_one(T, R):
     close(gx, dx, tx, "dx")
     close(ga, dA, tA, "da")
     close(gb, dB, tB, "db")
+
+
+# ---------------------------------------------------------------- routers --
+
+def case(T, E, k, seed, lo, hi):
+    g = gen(seed)
+    logits = torch.rand(T, E, generator=g) * (hi - lo) + lo
+    idx = torch.rand(T, E, generator=g).topk(k).indices.to(torch.int32)
+    counts = torch.cat([torch.bincount(idx.flatten().long(), minlength=E), torch.tensor([T])]).to(torch.int32)
+    return logits, idx, counts
+
+
+@pytest.mark.parametrize("lo,hi,deep", [(10.0, 20.0, None), (15.0, 80.0, None), (-80.0, -10.0, None), (-2.0, 2.0, None),
+                                        (-2.0, 2.0, -200.0), (-2.0, 2.0, -INF)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_saturated_sigmoids_keep_their_slope(lo, hi, deep, norm):
+    """v (1 - v) is not rounded away where v is near 1: the gradients are right relative to the slope, not only to 1."""
+    T, E, k = 50, 24, 5
+    lg, idx, counts = case(T, E, k, 3, lo, hi)
+    if deep is not None:  # every third expert: its slope is 0 in fp32
+        lg[:, ::3] = deep
+    dw = torch.randn(T, k, generator=gen(4))
+    s, at = lg.double(), idx.long()
+    v, slope = torch.sigmoid(s), torch.sigmoid(s) * torch.sigmoid(-s)
+    # the slope: the exponential (2 ulp of the hardware's power and its correction), a sum, a reciprocal and two products
+    c = 12 * U
+    # the weights' gradient: g, or (g - sum g w / S) / S, times the slope of the pick
+    g, w = dw.double(), v.gather(1, at)
+    mag = g.abs()
+    if norm:
+        S = w.sum(1, keepdim=True) + 1e-20
+        Gn = (g * w).sum(1, keepdim=True) / S
+        mag = (g.abs() + (g.abs() * w).sum(1, keepdim=True) / S) / S
+        g = (g - Gn) / S
+    want = torch.zeros(T, E, dtype=torch.float64).scatter_add(1, at, g * slope.gather(1, at))
+    tol = torch.zeros(T, E, dtype=torch.float64).scatter_add(1, at, mag * slope.gather(1, at)) * (c + (2 * k + 16) * U)
+    r = MoERouter(E, k, SIGM, norm)
+    got = tuning.router_backward(r, lg.cuda(), idx.cuda(), dw.cuda())
+    close(got, want, tol, "weights")
+    # the balance loss: q (1 - v) (f - sum f q), q = v / sum v
+    f = 0.5 * E * counts[:-1].double() / (k * T * T)
+    q = v / v.sum(1, keepdim=True)
+    mean = (f * q).sum(1, keepdim=True)
+    want = q * torch.sigmoid(-s) * (f - mean)
+    tol = q * torch.sigmoid(-s) * (f + mean) * (c + (2 * E + 16) * U)
+    got = tuning.router_backward(r, lg.cuda(), idx.cuda(), counts=counts.cuda(), balance_coef=0.5)
+    close(got, want, tol, "balance")
