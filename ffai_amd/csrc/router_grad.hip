@@ -625,7 +625,9 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
     const RowStat st = row_softmax<LG>(s, p);
 #pragma unroll
     for (int j = 0; j < kCols; j++) p[j] *= st.inv;
-    // the losses: d_j and the row sum it is centred by
+    // the losses: d_j and the row sum it is centred by. What is not asked for is
+    // left out, not multiplied by 0: an infinite logit makes p NaN, but not the
+    // sigmoids, nor the weights of picks beside it
     float d[kCols];
     const float zl = zc * st.lse;
     if (a.sigmoid) {
@@ -647,7 +649,11 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
       }
       c = row_sum<LG>(c);
 #pragma unroll
-      for (int j = 0; j < kCols; j++) d[j] = q[j] * rest[j] * (f[j] - c) + zl * p[j];
+      for (int j = 0; j < kCols; j++) d[j] = q[j] * rest[j] * (f[j] - c);
+      if (a.z != 0.f) {
+#pragma unroll
+        for (int j = 0; j < kCols; j++) d[j] = __builtin_fmaf(zl, p[j], d[j]);
+      }
     } else {
       float c = 0.f;
 #pragma unroll
@@ -655,6 +661,10 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
       c = row_sum<LG>(c);
 #pragma unroll
       for (int j = 0; j < kCols; j++) d[j] = p[j] * (f[j] - c + zl);
+    }
+    if (!a.counts) {
+#pragma unroll
+      for (int j = 0; j < kCols; j++) d[j] = 0.f;
     }
     if (a.dw) {
       // zero image

@@ -157,7 +157,7 @@ def case(T, E, k, seed, lo, hi):
 
 
 @pytest.mark.parametrize("lo,hi,deep", [(10.0, 20.0, None), (15.0, 80.0, None), (-80.0, -10.0, None), (-2.0, 2.0, None),
-                                        (-2.0, 2.0, -200.0), (-2.0, 2.0, -INF)])
+                                        (-2.0, 2.0, -200.0), (-2.0, 2.0, -INF), (-2.0, 2.0, INF)])
 @pytest.mark.parametrize("norm", [False, True])
 def test_saturated_sigmoids_keep_their_slope(lo, hi, deep, norm):
     """v (1 - v) is not rounded away where v is near 1: the gradients are right relative to the slope, not only to 1."""
@@ -191,3 +191,26 @@ def test_saturated_sigmoids_keep_their_slope(lo, hi, deep, norm):
     tol = q * torch.sigmoid(-s) * (f + mean) * (c + (2 * E + 16) * U)
     got = tuning.router_backward(r, lg.cuda(), idx.cuda(), counts=counts.cuda(), balance_coef=0.5)
     close(got, want, tol, "balance")
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("gating,norm", [(PICK, True), (SOFT, True), (SIGM, False), (SIGM, True)])
+def test_weights_gradient_beside_infinite_logits(dt, gating, norm):
+    """Where the weights are functions of the picks alone, what the other experts hold is not in their gradient."""
+    T, E, k = 21, 40, 4
+    lg, idx, _ = case(T, E, k, 5, -2.0, 2.0)
+    lg, at = lg.to(dt), idx.long()
+    dw = torch.randn(T, k, generator=gen(6))
+    l = lg.double().gather(1, at).requires_grad_(True)
+    w = torch.softmax(l, 1) if gating != SIGM else torch.sigmoid(l)
+    scale = 1.0
+    if gating == SIGM and norm:
+        scale = 1.0 / w.detach().sum(1, keepdim=True)
+        w = w / w.sum(1, keepdim=True)
+    g = torch.autograd.grad((w * dw.double()).sum(), l)[0]
+    want = torch.zeros(T, E, dtype=torch.float64).scatter(1, at, g)
+    other = torch.ones(T, E, dtype=torch.bool).scatter(1, at, False)
+    far = torch.tensor([INF, NAN, -INF])[torch.randint(0, 3, (T, E), generator=gen(7))].to(dt)
+    lg = torch.where(other & (torch.rand(T, E, generator=gen(8)) < 0.2), far, lg)
+    tol = (2 * dw.double().abs().sum(1, keepdim=True) * scale * (k + 24) * U).expand(T, E)
+    close(tuning.router_backward(MoERouter(E, k, gating, norm), lg.cuda(), idx.cuda(), dw.cuda()), want, tol, "d logits")
