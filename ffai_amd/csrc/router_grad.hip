@@ -107,19 +107,21 @@ template <int LG> __device__ __forceinline__ float row_max(float v) {
 
 constexpr float kLog2e = 1.44269504088896341f;
 
-// exp(s - m) as 2^(s log2(e) - m log2(e)) with one rounding of the exponent's
-// sum: the rounding of m log2(e), ml here, is common to a row and cancels in its
-// ratios, and the sum's own, 2^-25 of its size, weighs little where the power
-// is large. -inf gives 0 (m finite), NaN stays.
-__device__ __forceinline__ float exp_off(float s, float ml) {
-  return __builtin_amdgcn_exp2f(__builtin_fmaf(s, kLog2e, -ml));
+// exp(s - m), m the row's maximum, as 2^((s - m) log2(e)): the difference first, so
+// that a row far from zero, down to one of the type's lowest value, is as good as
+// any (m log2(e) taken off by an fma is one instruction less, at the same time, but
+// rounds by up to 2^-24 of itself, a power of its own from |m| of about 2^26 on, and
+// overflows). The two roundings, 2^-24 of the exponent each, weigh little where
+// the power is large. -inf gives 0 (m finite), NaN stays.
+__device__ __forceinline__ float exp_off(float s, float m) {
+  return __builtin_amdgcn_exp2f((s - m) * kLog2e);
 }
 
 // Row statistics of 2^LG lanes: e_j = exp(s_j - m), 1 / sum e and lse. A row
 // of -inf only has e = 0, inv = 0 and lse = 0 (no probability, no loss);
 // NaN or +inf in a row makes all of it NaN.
 struct RowStat {
-  float ml, inv, lse;  // ml: m log2(e)
+  float m, inv, lse;
 };
 template <int LG>
 __device__ __forceinline__ RowStat row_softmax(const float (&s)[kCols], float (&e)[kCols]) {
@@ -129,13 +131,12 @@ __device__ __forceinline__ RowStat row_softmax(const float (&s)[kCols], float (&
   m = row_max<LG>(m);
   if (m == -__builtin_huge_valf()) m = 0.f;
   RowStat r;
-  r.ml = m * kLog2e;
+  r.m = m;
+#pragma unroll
+  for (int j = 0; j < kCols; j++) e[j] = exp_off(s[j], m);
   float z = 0.f;
 #pragma unroll
-  for (int j = 0; j < kCols; j++) {
-    e[j] = exp_off(s[j], r.ml);
-    z += e[j];
-  }
+  for (int j = 0; j < kCols; j++) z += e[j];
   z = row_sum<LG>(z);
   r.inv = z == 0.f ? 0.f : 1.0f / z;
   r.lse = z == 0.f ? 0.f : m + logf(z);
@@ -678,7 +679,7 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
       float S = 0.f, G = 0.f;  // sum of the weights before renormalising, sum g v
       if (a.mode == kPickSoftmax) {
         mx = row_max<LG>(mx);
-        mx = mx == NEG ? 0.f : mx * kLog2e;
+        mx = mx == NEG ? 0.f : mx;
 #pragma unroll
         for (int i = 0; i < NP; i++)
           if ((NP == 1 || i * LPR < k)) {
@@ -704,7 +705,7 @@ __global__ __launch_bounds__(256) void router_backward_kernel(RouterGradArgs a) 
               v[i] = sg.v;
               pv[i] = sg.v * sg.rest;
             } else {
-              v[i] = exp_off(v[i], st.ml) * st.inv;
+              v[i] = exp_off(v[i], st.m) * st.inv;
               pv[i] = v[i];
               if (a.ebias && pe[i] != 0xFFFFFFFFu) v[i] += a.ebias[pe[i]];
             }

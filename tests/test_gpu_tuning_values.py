@@ -214,3 +214,50 @@ def test_weights_gradient_beside_infinite_logits(dt, gating, norm):
     lg = torch.where(other & (torch.rand(T, E, generator=gen(8)) < 0.2), far, lg)
     tol = (2 * dw.double().abs().sum(1, keepdim=True) * scale * (k + 24) * U).expand(T, E)
     close(tuning.router_backward(MoERouter(E, k, gating, norm), lg.cuda(), idx.cuda(), dw.cuda()), want, tol, "d logits")
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("gating,norm,bias", [(SOFT, True, False), (SOFT, False, False), (SOFT, True, True), (PICK, True, False)])
+def test_rows_of_far_values(dt, gating, norm, bias):
+    """Rows that a mask filled with the type's lowest value, wholly or but for a few, and rows far from zero: softmax only
+    depends on the distance to the row's maximum."""
+    T, E, k = 12, 20, 3
+    lg, idx, counts = case(T, E, k, 7, -1.0, 1.0)
+    low, high = torch.finfo(dt).min, torch.finfo(dt).max
+    lg[0] = low
+    lg[1], lg[1, 4], lg[1, 11] = low, 0.5, -0.25
+    lg[2], lg[2, 3] = low, high
+    lg[3] = high
+    for t, far in ((4, 1e5), (5, 3e9), (6, -3e10), (7, 1e20), (8, 2.0 ** 22)):
+        lg[t] = lg[t] * 4 + far
+    lg[9] = torch.where(torch.arange(E) % 2 == 0, 2.0 ** 21, 2.0 ** 21 + 1)
+    lg = lg.clamp(low, high).to(dt)
+    eb = torch.full((E,), 0.125) if bias else None
+    r = MoERouter(E, k, gating, norm, cuda(eb))
+    s, at = lg.double(), idx.long()
+    p = torch.softmax(s, 1)
+    c = (E + 16) * U
+    b = tuning.balance_loss(r, lg.cuda(), idx.cuda())
+    close(b.prob_sum, p.sum(0), p.sum(0) * (c + (T + 8) * U), "P")
+    bal = E * (counts[:-1].double() / (k * T) * p.sum(0) / T).sum()
+    lse = torch.logsumexp(s, 1)
+    z = lse.square().sum() / T  # past fp32's range with the largest values of bf16 and fp32
+    z = torch.where(z > torch.finfo(F32).max, INF, z)
+    close(b.losses, torch.stack([bal, z]), torch.stack([bal * (c + (T + 8) * U), z * (c + (T + 8) * U)]).nan_to_num(0, 0), "losses")
+    dw = torch.randn(T, k, generator=gen(2))
+    l = lg.double().requires_grad_(True)
+    q, g = torch.softmax(l, 1), dw.double()
+    if gating == PICK or (norm and eb is None):
+        w = torch.softmax(l.gather(1, at), 1)
+        scale = 1.0
+    else:
+        w = q.gather(1, at) + (0.0 if eb is None else 0.125)
+        scale = torch.ones(T, 1)
+        if norm:
+            scale = 2.0 / w.detach().sum(1, keepdim=True)
+            w = w / w.sum(1, keepdim=True)
+    loss = (w * g).sum() + 0.5 * E * (counts[:-1].double() / (k * T) * q.sum(0) / T).sum()
+    want = torch.autograd.grad(loss, l)[0]
+    tol = ((2 * g.abs().sum(1, keepdim=True) * scale + E * counts[:-1].max() / (k * T * T)) * (E + k + 24) * U).expand(T, E)
+    got = tuning.router_backward(r, lg.cuda(), idx.cuda(), dw.cuda(), counts.cuda(), 0.5)
+    close(got, want, tol, "d logits")
