@@ -305,9 +305,12 @@ moe_status moe_add_rmsnorm(const void* a, const void* b, const void* weight, flo
  *   losses[0]      balance: E * sum_e counts[e] / (k N) * P_e / N (1 when even)
  *   losses[1]      z: sum_t logsumexp(s_t)^2 / N
  * Both losses are 0 when N is 0. A row of -inf only counts as a row with no
- * probability and no z; NaN or +inf in a counted row makes the probabilities
- * and losses NaN. n_experts at most 512, k at most 64 and n_experts, T * k
- * below 2^31. The workspace may be NULL where its size is 0. */
+ * probability and no z (with MOE_SIGMOID_TOPK so does one whose sigmoids are all 0
+ * in f32, below -88, for its probability). NaN in a counted row makes the
+ * probabilities and losses NaN; +inf does too, except that a sigmoid of it is 1:
+ * with MOE_SIGMOID_TOPK it makes z NaN and nothing else. n_experts at most 512,
+ * k at most 64 and n_experts, T * k below 2^31. The workspace may be NULL where
+ * its size is 0. */
 size_t moe_balance_loss_workspace_bytes(int32_t T, int32_t n_experts);
 moe_status moe_balance_loss(const void* logits, int32_t dtype, int32_t T, int32_t n_experts,
                             int32_t k, int32_t gating, float logit_scale,
@@ -325,7 +328,9 @@ moe_status moe_balance_loss(const void* logits, int32_t dtype, int32_t T, int32_
  * are 0, and are constants, like expert_bias and expert_scale. Every element
  * of d_logits [T, n_experts] (dtype) is written, rows whose mask byte is 0
  * with zeros whatever they hold; it may not overlap logits. An id that a row
- * holds twice adds twice, an id >= n_experts adds nothing. */
+ * holds twice adds twice, an id >= n_experts adds nothing. A logit of NaN or +inf
+ * reaches what depends on it, in its own row: not the weights' gradient where the
+ * weights are functions of the picks alone and it is not picked. */
 moe_status moe_router_backward(const void* logits, int32_t dtype, int32_t T, int32_t n_experts,
                                int32_t k, int32_t gating, int32_t norm_topk_prob,
                                const float* expert_bias, float logit_scale, float routed_scale,

@@ -261,3 +261,23 @@ def test_rows_of_far_values(dt, gating, norm, bias):
     tol = ((2 * g.abs().sum(1, keepdim=True) * scale + E * counts[:-1].max() / (k * T * T)) * (E + k + 24) * U).expand(T, E)
     got = tuning.router_backward(r, lg.cuda(), idx.cuda(), dw.cuda(), counts.cuda(), 0.5)
     close(got, want, tol, "d logits")
+
+
+@pytest.mark.parametrize("T", [30, 4000])
+def test_sigmoid_router_with_infinite_logits(T):
+    """sigmoid(inf) is 1 and sigmoid(-inf) 0: the probabilities and the balance loss stay finite, and z does not."""
+    E, k = 16, 3
+    lg, idx, counts = case(T, E, k, 9, -2.0, 2.0)
+    lg[2, 5], lg[3, 1], lg[4, :8], lg[5] = INF, -INF, INF, -INF
+    r = MoERouter(E, k, SIGM)
+    b = tuning.balance_loss(r, lg.cuda(), idx.cuda())
+    v = torch.sigmoid(lg.double())
+    P = torch.where(v.sum(1, keepdim=True) > 0, v / v.sum(1, keepdim=True), 0.0).sum(0)  # row 5: no probability
+    c = (E + 16 + T + 8) * U
+    close(b.prob_sum, P, P * c, "P")
+    bal = E * (counts[:-1].double() / (k * T) * P / T).sum()
+    close(b.losses[:1], bal[None], bal * c, "balance")
+    assert torch.isnan(b.losses[1])
+    lg[7, 2] = NAN
+    b = tuning.balance_loss(r, lg.cuda(), idx.cuda())
+    assert torch.isnan(b.losses).all() and torch.isnan(b.prob_sum).all()
