@@ -756,7 +756,7 @@ struct OuterSide {
   const void* wide;    // [T, cols]: x or dy
   const float* small;  // [T, R]: u or s
   void* out;           // [G, R, cols] (rank_major: dA) or [G, cols, R] (dB)
-  float* part;         // [chunks, ...] fp32
+  float* part;         // [chunks of adapters with several, ...] fp32
   int cols;
   int rank_major;
 };
@@ -771,30 +771,34 @@ struct OuterArgs {
 constexpr int kOuterWaves = 8, kOuterCols = 128;
 
 // The adapter g whose chunks include number y (or, with of >= 0, adapter
-// `of`), its rows [o0, o1) in the plan, its first chunk and how many it has.
-// Uniform over the wave; g = G where y is past the last chunk.
+// `of`), its rows [o0, o1) in the plan, its first chunk and how many it has, and
+// the place of that first one among the chunks of adapters with several: only those
+// have partial gradients. Uniform over the wave; g = G where y is past the last chunk.
 struct Chunks {
   int g;
-  uint32_t o0, o1, first, n;
+  uint32_t o0, o1, first, n, part;
 };
 __device__ __forceinline__ Chunks find_chunks(const uint32_t* __restrict__ offsets, int G,
                                               uint32_t chunk, uint32_t y, int of) {
   const int lane = threadIdx.x & 63;
-  Chunks r{G, 0, 0, 0, 0};
-  uint32_t before = 0;
+  Chunks r{G, 0, 0, 0, 0, 0};
+  uint32_t before = 0, alone = 0;  // chunks of the adapters before, and those that are their adapter's only one
   for (int i = 0; i < G; i += 64) {
     const bool in = i + lane < G;
     const uint32_t a = in ? offsets[i + lane] : 0u, b = in ? offsets[i + lane + 1] : 0u;
     const uint32_t n = (b - a + chunk - 1) / chunk, last = wave_scan_u32(n) + before;
     const int k = of >= 0 ? of - i : __popcll(__ballot(in && last <= y));
+    const uint64_t one = __ballot(n == 1);
     if (k < min(64, G - i)) {
       r.g = i + k;
       r.o0 = (uint32_t)__builtin_amdgcn_readlane((int)a, k);
       r.o1 = (uint32_t)__builtin_amdgcn_readlane((int)b, k);
       r.n = (uint32_t)__builtin_amdgcn_readlane((int)n, k);
       r.first = (uint32_t)__builtin_amdgcn_readlane((int)last, k) - r.n;
+      r.part = r.first - alone - (uint32_t)__popcll(one & ((1ull << k) - 1ull));
       break;
     }
+    alone += (uint32_t)__popcll(one);
     before = (uint32_t)__builtin_amdgcn_readlane((int)last, 63);
   }
   return r;
@@ -1034,7 +1038,7 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
     }
     if (wave < across) {
       if (ck.n == 1) outer_store<XT, RB>(acc, (XT*)sd.out + ck.g * per, sd.rank_major, R, cols, r0, cb, c, q);
-      else outer_store<float, RB>(acc, sd.part + blockIdx.y * per, sd.rank_major, R, cols, r0, cb, c, q);
+      else outer_store<float, RB>(acc, sd.part + (ck.part + blockIdx.y - ck.first) * per, sd.rank_major, R, cols, r0, cb, c, q);
     }
   }
 }
@@ -1062,7 +1066,7 @@ __global__ __launch_bounds__(64 * kSumWaves) void lora_sum_kernel(OuterArgs p) {
 #pragma unroll 4
     for (uint32_t c = c0; c < c1; c++) {
       float b[8];
-      Vec8<float>::load(sd.part + (ck.first + c) * per + i, b);
+      Vec8<float>::load(sd.part + (ck.part + c) * per + i, b);
 #pragma unroll
       for (int j = 0; j < 8; j++) a[j] += b[j];
     }
@@ -1208,10 +1212,18 @@ uint32_t outer_chunk(const LoraDims& d) {
   const long n = outer_target(d);
   return (uint32_t)std::max(64L, (d.T + n - 1) / n);
 }
-// Chunks of all adapters, at most (no fewer for more rows, so that a workspace
-// sized for many rows serves a call of few).
+// Chunks of all adapters, at most.
 long outer_chunks(const LoraDims& d) {
   return std::min<long>(d.T, std::min(outer_target(d), (long)(d.T + 63) / 64) + d.G);
+}
+
+// Chunks of the adapters that have several, at most, whose gradients are kept in
+// parts: T rows hold at most T / chunk whole ones, and such an adapter at most one
+// more. A chunk has T / target rows and 64 at least. (512 rows of 512 adapters 4096
+// -> 4096 at rank 64: 8 parts, 17 MB; 516 chunks, 1.1 GB.)
+long outer_parts(const LoraDims& d) {
+  const long whole = d.T > 64 ? std::min<long>(outer_target(d), d.T / 64) : 0;
+  return whole + std::min<long>(d.G, whole);
 }
 
 // Column blocks of a block: more than one where adapters have few rows on
@@ -1248,7 +1260,7 @@ BackwardLayout backward_layout(const LoraDims& d) {
   l.used = take((G + 1) * 4);
   l.scratch_bytes = dispatch_scratch_bytes(d.T, 1, d.G);
   l.scratch = take(l.scratch_bytes);
-  l.part = take((size_t)outer_chunks(d) * R * (K + N) * 4);
+  l.part = take((size_t)outer_parts(d) * R * (K + N) * 4);
   l.total = at;
   return l;
 }
@@ -1300,7 +1312,7 @@ hipError_t backward_typed(const LoraDims& d, const LoraBackward& a, hipStream_t 
     cols = std::max(cols, d.K);
   }
   if (a.db) {
-    o.side[o.sides++] = {a.dy, s, a.db, part + (size_t)chunks * d.R * d.K, d.N, 0};
+    o.side[o.sides++] = {a.dy, s, a.db, part + (size_t)outer_parts(d) * d.R * d.K, d.N, 0};
     cols = std::max(cols, d.N);
   }
   const int RB = outer_ranks(d);

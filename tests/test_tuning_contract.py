@@ -1,10 +1,13 @@
 """What the tuning entry points promise about the tensors they are given and the memory they ask for, checked on the host
 before any launch."""
+import ctypes as C
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from ffai_amd import tuning  # noqa: E402
+from ffai_amd import _lib, tuning  # noqa: E402
+from ffai_amd._lib import MOE_BF16, MOE_F32, Lora  # noqa: E402
 
 
 # -------------------------------------------------------- adapters' memory --
@@ -40,3 +43,26 @@ def test_scale_of_the_same_kind_is_taken():
     with pytest.raises(ValueError, match="on a GPU"):  # past the adapters' own checks
         l.apply(x, ad)
     assert l._current().scale == wide.data_ptr() + 16
+
+
+# -------------------------------------------------------------- workspaces --
+
+def backward_bytes(T, G, K, N, R, dt=MOE_BF16):
+    l = Lora(1 << 45, 1 << 46, None, dt, R, N, K, G)
+    return _lib.load().moe_lora_backward_workspace_bytes(C.byref(l), T)
+
+
+@pytest.mark.parametrize("T,G,K,N,R", [
+    (512, 512, 4096, 4096, 64), (64, 64, 4096, 4096, 64), (2048, 512, 4096, 4096, 64), (4096, 1024, 8192, 8192, 128),
+    (1, 1024, 2048, 768, 16), (4096, 8, 2048, 2048, 16), (333, 1, 1024, 384, 8), (40000, 1024, 2048, 768, 16),
+])
+@pytest.mark.parametrize("dt", [MOE_BF16, MOE_F32])
+def test_backward_workspace_follows_the_rows(T, G, K, N, R, dt):
+    """Partial gradients are kept for chunks of at least 64 rows, and for one shorter chunk of each adapter that has such
+    a one: no memory for adapters that have few rows or none."""
+    part = 4 * R * (K + N)
+    rows = T * (8 * R + 8) + 4 * 1024 * (T // 1024 + 1) + 12 * (G + 1)  # inner sums, the plan's lists and its chunks
+    assert backward_bytes(T, G, K, N, R, dt) <= 2 * (T // 64) * part + rows + 10 * 256
+    # and it is what more rows need, at most
+    sizes = [backward_bytes(t, G, K, N, R, dt) for t in [*range(1, 300), 511, 512, 513, 1000, T + 300, T + 301, 2 * T + 300]]
+    assert sizes[:-3] == sorted(sizes[:-3]) and sizes[-3:] == sorted(sizes[-3:])
