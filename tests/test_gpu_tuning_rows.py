@@ -91,3 +91,30 @@ def test_gradients_of_chunks_in_a_workspace_of_its_size(dt, rows, K, N, R):
     check_gradients(out, x, A, B, scale, ad, dy, range(G))
     for a, b in zip(out, tuning.LoRAAdapters(Ac, Bc, sc).backward(xc, dc, ac)):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("T,G,spread", [
+    (16384, 1, "some"), (16385, 1, "some"), (20011, 1, "some"), (20011, 2, "even"), (17001, 300, "even"), (33001, 70, "most"),
+    (33001, 1024, "even"), (20011, 5, "none"), (40000, 3, "last"),
+])
+def test_gradients_of_more_rows_than_a_launch_lists(dt, T, G, spread):
+    """The plans of many rows: a block per adapter, and chunks of rows with their own counts where there are few
+    adapters, or many, or more rows still. Ids out of range among them."""
+    K, N, R = 24, 40, 16
+    x, A, B, scale, dy = inputs(T, K, N, R, G, dt, T + G)
+    g = gen(G)
+    ad = torch.randint(-1, G + 1, (T,), generator=g)
+    if spread == "most":
+        ad = torch.where(torch.rand(T, generator=g) < 0.6, 3, ad)
+    elif spread == "none":
+        ad = torch.where(torch.rand(T, generator=g) < 0.5, -1, 1 << 30)
+    elif spread == "last":
+        ad = torch.where(torch.arange(T) < T - 7, -5, G - 1)
+    ad = ad.to(torch.int32)
+    l = tuning.LoRAAdapters(A.cuda(), B.cuda(), scale.cuda())
+    dev = x.cuda(), dy.cuda(), ad.cuda()
+    got = l.backward(*dev)
+    check_gradients(got, x, A, B, scale, ad, dy, range(G) if G <= 5 else [0, 1, 3, 62, 63, 64, 65, G - 2, G - 1])
+    for a, b in zip(got, l.backward(*dev)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
