@@ -8,12 +8,17 @@ many adapters at once, over PyTorch device buffers through the C ABI.
     adapters            y = LoRAAdapters(a, b, scale).apply(x, adapter, y)
                         dx, da, db = adapters.backward(x, dy, adapter, dx=dx)
 
-Gradients are plain results, not recorded by autograd. Every function takes
-contiguous tensors of one device, checks them before any launch, and runs on
-`stream` (default: that device's current stream), on which its results and its
-workspace are allocated: a result used on another stream has to be waited for
-there, and all calls can be captured into a graph. PyTorch only provides
-memory and streams; every computation is a libmoehip.so kernel.
+Gradients are plain results, not recorded by autograd. While autograd records,
+balance_loss and apply refuse tensors that require a gradient, and every function
+refuses to write into one: call them under torch.no_grad() or in a
+torch.autograd.Function. A tensor of the caller's that a call writes counts as
+changed in place, so that autograd notices where it had saved it.
+
+Every function takes contiguous tensors of one device, checks them before any
+launch, and runs on `stream` (default: that device's current stream), on which
+its results and its workspace are allocated: a result used on another stream has
+to be waited for there, and all calls can be captured into a graph. PyTorch only
+provides memory and streams; every computation is a libmoehip.so kernel.
 """
 from __future__ import annotations
 
@@ -37,6 +42,16 @@ _I32, _F32 = (torch.int32,), (torch.float32,)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                       lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+_grad_enabled = torch.is_grad_enabled
+# (without the public call's look at its argument: 0.15 us)
+_changed = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
+
+
+def _refuse_grad(name: str):
+    raise ValueError(f"{name} requires a gradient, which this call does not record: call it under torch.no_grad() or in a "
+                     "torch.autograd.Function")
 
 
 def _check(name: str, t: Optional[torch.Tensor], shape, dtypes, index: int) -> Optional[int]:
@@ -111,6 +126,8 @@ def balance_loss(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Tensor
     lp = _check("logits", logits, (T, E), _FLOATS, at)
     ip = _check("topk_idx", topk_idx, (T, k), _I32, at)
     mp = _check("mask", mask, (T,), _MASK, at)
+    if logits.requires_grad and _grad_enabled():
+        _refuse_grad("logits")
     st, ctx = _begin(at, stream)
     try:
         lib = _lib.load()
@@ -146,14 +163,19 @@ def router_backward(router: MoERouter, logits: torch.Tensor, topk_idx: torch.Ten
     bp = _check("router.expertBias", router.expertBias, (E,), _F32, at)
     sp = _check("router.expertScale", router.expertScale, (E,), _F32, at)
     op = _check("out", out, (T, E), (dt,), at)
+    if out is not None and out.requires_grad and _grad_enabled():
+        _refuse_grad("out")
     st, ctx = _begin(at, stream)
     try:
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty_like(logits)
             op = out.data_ptr()
         check(_lib.load().moe_router_backward(
             lp, moe_dtype(dt), T, E, k, router.gatingMode, int(bool(router.normTopKProb)), bp,
             router.logitScale, router.routedScale, sp, ip, dp, cp, balance_coef, z_coef, mp, op, st))
+        if given:
+            _changed((out,))
     finally:
         if ctx is not None:
             ctx.leave()
@@ -174,14 +196,19 @@ def unpermute_backward(d_out: torch.Tensor, Y: torch.Tensor, inv_perm: torch.Ten
     flat = isinstance(inv_perm, torch.Tensor) and inv_perm.dim() == 1
     ip = _check("inv_perm", inv_perm, (T * k,) if flat else (T, k), _I32, at)
     op = _check("dY", dY, (T * k, H), dts, at)
+    if dY is not None and dY.requires_grad and _grad_enabled():
+        _refuse_grad("dY")
     st, ctx = _begin(at, stream)
     try:
-        if dY is None:
+        given = dY is not None
+        if not given:
             dY = torch.empty_like(Y)
             op = dY.data_ptr()
         dw = torch.empty_like(topk_weight)
         check(_lib.load().moe_unpermute_backward(gp, yp, ip, wp, T, H, k, op, dw.data_ptr(),
                                                  moe_dtype(d_out.dtype), st))
+        if given:
+            _changed((dY,))
     finally:
         if ctx is not None:
             ctx.leave()
@@ -194,7 +221,8 @@ class LoRAAdapters:
     b [G, N, R], scale [G] float32 (None: 1). Ranks that differ are padded
     with zeros to a multiple of 8, at most 128. The tensors may be updated in
     place (a slot overwritten, an optimiser's step) and moved (their .data set);
-    the latter is checked again by the next call."""
+    the latter, also where only shape, type or spacing change, is checked again by
+    the next call."""
     a: torch.Tensor
     b: torch.Tensor
     scale: Optional[torch.Tensor] = None
@@ -208,43 +236,55 @@ class LoRAAdapters:
                     _check("scale", self.scale, (G,), _F32, at),
                     moe_dtype(self.a.dtype), R, N, K, G)
         check(_lib.load().moe_validate_lora(C.byref(desc)))
+        # (workspaces grow with the rows: none for the most is none for all)
+        object.__setattr__(self, "_no_workspace", _lib.load().moe_lora_workspace_bytes(C.byref(desc), 1 << 23) == 0)
         object.__setattr__(self, "_struct", desc)
         object.__setattr__(self, "_ref", C.byref(desc))
-        s = self.scale
-        object.__setattr__(self, "_as", (self.a.shape, self.b.shape, self.a.dtype, self.b.dtype,
-                                         None if s is None else (s.shape, s.dtype)))
+        object.__setattr__(self, "_dims", (N, K))
+        a, b, s = self.a, self.b, self.scale
+        object.__setattr__(self, "_as", (a.data_ptr(), b.data_ptr(), a.shape, b.shape, a.dtype, b.dtype))
+        object.__setattr__(self, "_scale_as", None if s is None else (s.data_ptr(), s.shape, s.dtype))
 
     def _current(self) -> Lora:
         """The descriptor, of the memory the tensors have now."""
-        l, a, b, s = self._struct, self.a, self.b, self.scale
-        if (a.data_ptr() != l.a or b.data_ptr() != l.b or (s is not None and s.data_ptr() != l.scale)
-                or (a.shape, b.shape, a.dtype, b.dtype, None if s is None else (s.shape, s.dtype)) != self._as
-                or not (a.is_contiguous() and b.is_contiguous() and (s is None or s.is_contiguous()))):
+        a, b, s = self.a, self.b, self.scale
+        if ((a.data_ptr(), b.data_ptr(), a.shape, b.shape, a.dtype, b.dtype) != self._as
+                or not (a.is_contiguous() and b.is_contiguous())
+                or (s is not None and ((s.data_ptr(), s.shape, s.dtype) != self._scale_as or not s.is_contiguous()))):
             self.__post_init__()
-            l = self._struct
-        return l
+        return self._struct
 
     def apply(self, x: torch.Tensor, adapter: torch.Tensor, y: Optional[torch.Tensor] = None,
               out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """y + scale * b (a x) for x [T, K], row t with adapter[t] (int32; -1:
         none). y [T, N] is the shared projection's output (None: zeros); the
         result goes to out, by default to y itself."""
-        l, dts, at = self._current(), (self.a.dtype,), self.a.get_device()
+        self._current()
+        a, b, s, (N, K) = self.a, self.b, self.scale, self._dims
+        dts, at = (a.dtype,), a.get_device()
         T = _rows("x", x, 2).shape[0]
-        xp = _check("x", x, (T, l.k), dts, at)
+        xp = _check("x", x, (T, K), dts, at)
         ap = _check("adapter", adapter, (T,), _I32, at)
-        yp = _check("y", y, (T, l.n), dts, at)
-        op = _check("out", out, (T, l.n), dts, at)
+        yp = _check("y", y, (T, N), dts, at)
+        op = _check("out", out, (T, N), dts, at)
+        if _grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad
+                                or (y is not None and y.requires_grad) or (out is not None and out.requires_grad)
+                                or (s is not None and s.requires_grad)):
+            _refuse_grad(next(n for n, t in (("x", x), ("a", a), ("b", b), ("y", y), ("out", out), ("scale", s))
+                              if t is not None and t.requires_grad))
         st, ctx = _begin(at, stream)
         try:
             lib = _lib.load()
+            given = out is not None or y is not None
             if out is None:
-                out = torch.empty(T, l.n, dtype=x.dtype, device=x.device) if y is None else y
+                out = torch.empty(T, N, dtype=x.dtype, device=x.device) if y is None else y
                 op = out.data_ptr()
-            need = lib.moe_lora_workspace_bytes(self._ref, T)
+            need = 0 if self._no_workspace else lib.moe_lora_workspace_bytes(self._ref, T)
             ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
             check(lib.moe_lora_apply(self._ref, xp, T, ap, yp, op, None if ws is None else ws.data_ptr(),
                                      need, st))
+            if given:
+                _changed((out,))
         finally:
             if ctx is not None:
                 ctx.leave()
@@ -257,26 +297,34 @@ class LoRAAdapters:
         dx [T, K] is the gradient from the shared projection that the adapters'
         is added to (None: zeros); the sum goes to dx_out, by default to dx
         itself. need_dx=False leaves it out (dx is then None)."""
-        l, dts, at = self._current(), (self.a.dtype,), self.a.get_device()
+        self._current()
+        (N, K), dts, at = self._dims, (self.a.dtype,), self.a.get_device()
         T = _rows("x", x, 2).shape[0]
-        xp = _check("x", x, (T, l.k), dts, at)
-        yp = _check("dy", dy, (T, l.n), dts, at)
+        xp = _check("x", x, (T, K), dts, at)
+        yp = _check("dy", dy, (T, N), dts, at)
         ap = _check("adapter", adapter, (T,), _I32, at)
-        dp = _check("dx", dx, (T, l.k), dts, at)
-        op = _check("dx_out", dx_out, (T, l.k), dts, at)
+        dp = _check("dx", dx, (T, K), dts, at)
+        op = _check("dx_out", dx_out, (T, K), dts, at)
         if not need_dx and (dx is not None or dx_out is not None):
             raise ValueError("dx or dx_out given with need_dx=False")
+        into = dx if dx_out is None else dx_out
+        if into is not None and into.requires_grad and _grad_enabled():
+            _refuse_grad("dx" if dx_out is None else "dx_out")
         st, ctx = _begin(at, stream)
         try:
             lib = _lib.load()
-            if need_dx and dx_out is None:
-                dx_out = torch.empty(T, l.k, dtype=x.dtype, device=x.device) if dx is None else dx
+            dx_out = into
+            if need_dx and into is None:
+                dx_out = torch.empty(T, K, dtype=x.dtype, device=x.device)
+            if need_dx:
                 op = dx_out.data_ptr()
             da, db = torch.empty_like(self.a), torch.empty_like(self.b)
             need = lib.moe_lora_backward_workspace_bytes(self._ref, T)
             ws = torch.empty(need, dtype=torch.uint8, device=x.device)
             check(lib.moe_lora_backward(self._ref, xp, yp, T, ap, dp, op, da.data_ptr(), db.data_ptr(),
                                         ws.data_ptr(), need, st))
+            if into is not None:
+                _changed((into,))
         finally:
             if ctx is not None:
                 ctx.leave()

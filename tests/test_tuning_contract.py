@@ -8,6 +8,7 @@ torch = pytest.importorskip("torch")
 
 from ffai_amd import _lib, tuning  # noqa: E402
 from ffai_amd._lib import MOE_BF16, MOE_F32, Lora  # noqa: E402
+from ffai_amd.layer import MoERouter  # noqa: E402
 
 
 # -------------------------------------------------------- adapters' memory --
@@ -66,3 +67,54 @@ def test_backward_workspace_follows_the_rows(T, G, K, N, R, dt):
     # and it is what more rows need, at most
     sizes = [backward_bytes(t, G, K, N, R, dt) for t in [*range(1, 300), 511, 512, 513, 1000, T + 300, T + 301, 2 * T + 300]]
     assert sizes[:-3] == sorted(sizes[:-3]) and sizes[-3:] == sorted(sizes[-3:])
+
+
+# ---------------------------------------------------------------- autograd --
+
+def leaf(*shape):
+    return torch.zeros(*shape).requires_grad_(True)
+
+
+def refused_calls():
+    """(call, the tensor it names) with a tensor that requires a gradient where autograd would have to record the call, or
+    to know of a write."""
+    r = MoERouter(8, 2)
+    x, ad, y, dy = torch.zeros(3, 16), torch.zeros(3, dtype=torch.int32), torch.zeros(3, 24), torch.zeros(3, 24)
+    lg, idx = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int32)
+    a, b = torch.zeros(2, 8, 16), torch.zeros(2, 24, 8)
+    l = tuning.LoRAAdapters(a, b, torch.ones(2))
+    g, Y, inv, w = torch.zeros(3, 8), torch.zeros(6, 8), torch.zeros(6, dtype=torch.int32), torch.zeros(3, 2)
+    return [
+        (lambda: tuning.balance_loss(r, leaf(4, 8), idx), "logits"),
+        (lambda: tuning.router_backward(r, lg, idx, out=leaf(4, 8)), "out"),
+        (lambda: tuning.unpermute_backward(g, Y, inv, w, dY=leaf(6, 8)), "dY"),
+        (lambda: l.apply(leaf(3, 16), ad, y), "x"),
+        (lambda: l.apply(x, ad, leaf(3, 24)), "y"),
+        (lambda: l.apply(x, ad, y, out=leaf(3, 24)), "out"),
+        (lambda: tuning.LoRAAdapters(leaf(2, 8, 16), b).apply(x, ad, y), "a"),
+        (lambda: tuning.LoRAAdapters(a, leaf(2, 24, 8)).apply(x, ad, y), "b"),
+        (lambda: tuning.LoRAAdapters(a, b, leaf(2)).apply(x, ad, y), "scale"),
+        (lambda: l.backward(x, dy, ad, dx=leaf(3, 16)), "dx"),
+        (lambda: l.backward(x, dy, ad, dx=x, dx_out=leaf(3, 16)), "dx_out"),
+    ]
+
+
+@pytest.mark.parametrize("i", range(11))
+def test_tensors_that_require_a_gradient_are_refused_while_autograd_records(i):
+    call, name = refused_calls()[i]
+    with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+        call()
+    for quiet in (torch.no_grad(), torch.inference_mode()):
+        with quiet, pytest.raises(ValueError, match="on a GPU"):  # past that check
+            call()
+
+
+def test_gradient_calls_read_tensors_that_require_one():
+    """What gradients are computed from may require one itself: the results are plain."""
+    r, idx = MoERouter(8, 2), torch.zeros(4, 2, dtype=torch.int32)
+    l = tuning.LoRAAdapters(leaf(2, 8, 16), leaf(2, 24, 8))
+    ad, inv = torch.zeros(3, dtype=torch.int32), torch.zeros(6, dtype=torch.int32)
+    for call in (lambda: tuning.router_backward(r, leaf(4, 8), idx, leaf(4, 2)), lambda: l.backward(leaf(3, 16), leaf(3, 24), ad),
+                 lambda: tuning.unpermute_backward(leaf(3, 8), leaf(6, 8), inv, leaf(3, 2))):
+        with pytest.raises(ValueError, match="on a GPU"):
+            call()
