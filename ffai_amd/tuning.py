@@ -257,7 +257,8 @@ class LoRAAdapters:
     def apply(self, x: torch.Tensor, adapter: torch.Tensor, y: Optional[torch.Tensor] = None,
               out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """y + scale * b (a x) for x [T, K], row t with adapter[t] (int32; -1:
-        none). y [T, N] is the shared projection's output (None: zeros); the
+        none), sums in float32; in a 16-bit type the inner ones enter the second
+        product as two parts, 16 (bfloat16) or 22 bits. y [T, N] is the shared projection's output (None: zeros); the
         result goes to out, by default to y itself."""
         self._current()
         a, b, s, (N, K) = self.a, self.b, self.scale, self._dims

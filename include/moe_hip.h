@@ -368,11 +368,14 @@ moe_status moe_validate_lora(const moe_lora* l);
 /* The adapters of many requests beside their shared projection (whose output
  * rows, from moe_router_logits or moe_expert_matmul, are y_in):
  *   y[t,:] = round(y_in[t,:] + scale[g] * b[g] (a[g] x[t,:])),  g = adapter[t]
- * with the inner sums in f32. A row whose id is not in [0, n_adapters) (-1)
+ * with both products' sums in f32. The inner sums s = scale[g] a[g] x[t,:] meet b as
+ * they are where dtype is f32; else as two parts of the type, which hold them to
+ * 2^-17 of themselves (bf16), or to 2^-23 and 2^-39 of the row's largest (f16).
+ * Infinities and NaN in x, a, b and scale give what the formula gives. A row whose id is not in [0, n_adapters) (-1)
  * has no adapter: its y is y_in. y_in [T, n] may be y (then such rows are not
  * touched) or NULL (zeros). x [T, k] and y in l->dtype, 16-byte aligned; y
- * apart from x and the adapters; T at most 2^23. The workspace is free to be reused by work that the
- * stream runs later. */
+ * apart from x and the adapters; T at most 2^23. The workspace is free to be
+ * reused by work that the stream runs later. */
 size_t moe_lora_workspace_bytes(const moe_lora* l, int32_t T);
 moe_status moe_lora_apply(const moe_lora* l, const void* x, int32_t T, const int32_t* adapter,
                           const void* y_in, void* y, void* workspace, size_t workspace_bytes,
@@ -384,7 +387,9 @@ moe_status moe_lora_apply(const moe_lora* l, const void* x, int32_t T, const int
  *   da[g]   = round(sum_t u_t x[t,:]^T)                     [G, rank, k]
  *   db[g]   = round(sum_t dy[t,:] (scale[g] a[g] x[t,:])^T) [G, n, rank]
  * over the rows t of adapter g, sums in f32; an adapter without rows gets
- * zeros. dx_in as y_in above (the gradient from the shared projection; may be
+ * zeros. u and scale[g] a[g] x[t,:] enter dx as the inner sums enter y above, and so
+ * do they da and db in a 16-bit type at ranks above 16 (f16: 2^-39 of the largest of
+ * 32 rows' sums); at lower ranks, and in f32, they enter those as f32. dx_in as y_in above (the gradient from the shared projection; may be
  * dx, or NULL). All in l->dtype, 16-byte aligned, the gradients apart from
  * each other and from all other inputs; T at most 2^23, n_adapters at most 1024. */
 size_t moe_lora_backward_workspace_bytes(const moe_lora* l, int32_t T);

@@ -146,6 +146,34 @@ def test_f16_sums_beside_an_infinite_one(T, R):
     close(gb, dB, tB, "db")
 
 
+@pytest.mark.parametrize("R", [16, 24, 64])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_inner_sums_of_many_sizes(dt, R):
+    """Sums from the largest to 2^-20 of it, weighed so that each matters: as two 16-bit parts they keep 2^-17 (bf16), or
+    2^-23 of themselves and 2^-39 of the largest (f16)."""
+    T, K, N = 40, 64, 72
+    g = gen(R)
+    x = torch.randn(T, K, generator=g).to(dt)
+    size = 2.0 ** -(torch.arange(R) % 21).float()
+    A = (torch.randn(1, R, K, generator=g) * 64 * size[:, None]).to(dt)
+    B = (torch.randn(1, N, R, generator=g) * 2.0 ** -14 / size).to(dt)
+    dy = (torch.randn(T, N, generator=g) * 2.0 ** -8).to(dt)
+    ad = torch.zeros(T, dtype=torch.int32)
+    X, D, Aa, Bb = x.double(), dy.double(), A[0].double(), B[0].double()
+    s, sm, u, um = X @ Aa.t(), X.abs() @ Aa.abs().t(), D @ Bb, D.abs() @ Bb.abs()
+
+    def parts(v, over):  # what two parts may leave out
+        return v.abs() * 2.0 ** -17 if dt == BF16 else v.abs() * 2.0 ** -23 + 2.0 ** -39 * v.abs().amax(over, keepdim=True)
+
+    l = tuning.LoRAAdapters(A.cuda(), B.cuda())
+    close(l.apply(x.cuda(), ad.cuda()), s @ Bb.t(), parts(s, 1) @ Bb.abs().t() + (sm @ Bb.abs().t()) * (K + R + 16) * U, "y")
+    gx, ga, gb = l.backward(x.cuda(), dy.cuda(), ad.cuda())
+    close(gx, u @ Aa, parts(u, 1) @ Aa.abs() + (um @ Aa.abs()) * (N + R + 16) * U, "dx")
+    whole = R > 16  # else the gradients take the sums as they are
+    close(ga[0], u.t() @ X, whole * parts(u, (0, 1)).t() @ X.abs() + (um.t() @ X.abs()) * (N + T + 16) * U, "da")
+    close(gb[0], D.t() @ s, whole * D.abs().t() @ parts(s, (0, 1)) + (D.abs().t() @ sm) * (K + T + 16) * U, "db")
+
+
 # ---------------------------------------------------------------- routers --
 
 def case(T, E, k, seed, lo, hi):
