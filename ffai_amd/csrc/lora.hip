@@ -338,8 +338,8 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
   constexpr int V = 16 / sizeof(XT), LD = RT * 16 + 4, W = kFusedWaves;
   constexpr int UNIT = 8 * V;                      // a unit of K: 128 bytes of a row
   // neighbouring columns of a lane: as many as leave LDS for two blocks up to
-  // rank 64 (fp32 at rank 40, 7454 rows backward: 25 us with two columns, 31 with four;
-  // 4096 rows at rank 64, whose tiles are as many as CUs, 54 and 50)
+  // rank 64 (fp32, 7454 rows 264 -> 96 backward at rank 40: 26.2 us with two columns,
+  // 31.8 with four; 4096 rows 2048 -> 2048 at rank 64 54.6 and 64.6)
   constexpr int J = F32 && RT >= 4 ? 2 : 4;
   constexpr int NC = 16 * J;                       // columns of a group
   constexpr int C8 = RT * 16 / V;                  // 16-byte chunks of the widest adapter row
@@ -741,7 +741,7 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
 // two 16-bit parts as in expand; a wave with a sum that is not finite adds its rows
 // again in fp32 products of 4, as there. 4096 rows of 8 adapters 2048 -> 2048: rank 16
 // 13.3 us with products of 4 rows, 15.0 with those of 32 (whose steps the
-// adapters' chunks fill less); rank 64 39 and 26.5.
+// adapters' chunks fill less); rank 64 42.8 and 27.6.
 //
 // A block takes 128 columns (or several times that, see outer_span), up to two
 // (fp32: four) rank tiles and a chunk of one adapter's rows (an adapter of n rows
@@ -749,7 +749,7 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
 // work is even however the rows spread). Its eight waves share the chunk and
 // meet in LDS; where it has fewer rows than their steps they share columns too.
 // The gradient of an adapter with one chunk is stored at once, the chunks of the
-// others as fp32, which lora_sum_kernel adds in order. Steps are loaded one
+// others as fp32, which lora_sum_kernel adds. Steps are loaded one
 // ahead, the list of rows two ahead. SPAN: the form for several column blocks,
 // whose loop takes the plain one's 11.8 us to 13.0.
 struct OuterSide {
@@ -1045,8 +1045,8 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
 
 // Adds the chunks of the adapters that have several, and writes zeros for
 // those without rows; the others are there already. A lane adds 8 neighbouring
-// values. Up to eight chunks one wave adds them all; more are shared by the
-// block's waves, whose sums meet in LDS (7454 rows of one adapter 264 -> 96 at
+// values. Up to eight chunks one wave adds them all in order; more are shared by
+// the block's waves, a run of them each, whose sums meet in LDS in the waves' order (7454 rows of one adapter 264 -> 96 at
 // rank 40, 117 chunks: 5.8 us,
 // by one wave 14).
 constexpr int kSumWaves = 4;
@@ -1173,10 +1173,10 @@ size_t adapter_bytes(const LoraDims& d) {
   return (size_t)d.R * (d.K + d.N) * (d.dt == DT_F32 ? 4 : 2);
 }
 
-// One launch, unless few blocks would each read a large adapter alone: one
-// row of 2048 -> 2048 takes 6.9 us fused and 6.7 + a launch apart at rank 16, 21.8
-// and 15.2 at rank 128 (of 4096 -> 4096: 34 and 17), 64 rows of 64 adapters of 4096
-// -> 4096 at rank 64 25 and 26.
+// One launch, unless few blocks would each read a large adapter alone. Kernel
+// times in one launch and in two: one row of 2048 -> 2048 at rank 16 5.7 us and 2.9 +
+// 4.2, at rank 128 17.5 and 5.1 + 11.1 (of 4096 -> 4096 23.0 and 5.1 + 13.2); 64 rows of
+// 64 adapters of 4096 -> 4096 at rank 64 19.9 and 9.9 + 13.2.
 constexpr size_t kFusedBytes = 256u << 10;
 constexpr int kSplitBlocks = 32;
 bool lora_fused(const LoraDims& d) {
@@ -1229,9 +1229,9 @@ long outer_parts(const LoraDims& d) {
 // Column blocks of a block: more than one where adapters have few rows on
 // average, so that its waves have a step of rows each and the chip is not busy
 // with blocks of one working wave (2048 rows of 64 adapters 4096 -> 4096 at rank 64
-// 38 us instead of 186, 64 rows of 64 adapters 6.3 instead of 11; a single adapter
-// that has all the rows 12.9 and 12.8), as long as 512 blocks remain (512 rows of
-// one of 64 adapters 13.2 us, with 256 blocks 22.4).
+// 52 us instead of 195, 64 rows of 64 adapters 23 instead of 110; where one of
+// the 64 has all 2048 rows 61 and 36), as long as 512 blocks remain (512 rows of one
+// of 64 adapters 2048 -> 2048 at rank 16 13.3 us, with 256 blocks 22.6).
 int outer_span(const LoraDims& d, long blocks) {
   const int step = d.dt == DT_F32 || d.R <= 16 ? 8 : 32, rows = (d.T + d.G - 1) / d.G;
   int span = rows <= step ? 8 : rows <= 2 * step ? 4 : rows <= 4 * step ? 2 : 1;

@@ -186,7 +186,9 @@ def unpermute_backward(d_out: torch.Tensor, Y: torch.Tensor, inv_perm: torch.Ten
                        topk_weight: torch.Tensor, dY: Optional[torch.Tensor] = None, stream=None):
     """Gradient of the weighted combine of expert rows Y [T * k, hidden] for
     d_out [T, hidden]: (dY, d_weight [T, k] float32). inv_perm (T * k int32)
-    comes from the dispatch plan; dY may be Y itself."""
+    comes from the dispatch plan, each position once; a position past T * k has a
+    zero d_weight, and rows that no position names are not written (give dY to
+    have them defined). dY may be Y itself."""
     T, H = _rows("d_out", d_out, 2).shape
     at, dts = d_out.get_device(), (d_out.dtype,)
     k = _rows("topk_weight", topk_weight, 2).shape[1]

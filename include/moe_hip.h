@@ -342,8 +342,9 @@ moe_status moe_router_backward(const void* logits, int32_t dtype, int32_t T, int
 /* Gradient of moe_unpermute:
  *   dY[inv_perm[t*k+s], :] = round(w[t,s]) * d_out[t,:]   (nullable; may be Y)
  *   d_weight[t,s]          = <d_out[t,:], Y[inv_perm[t*k+s], :]>   (f32)
- * Rows of dY that no position names stay as they are; a position >= T * k
- * has a zero d_weight. d_out, Y and dY 16-byte aligned; T at most 2^23. */
+ * Rows of dY that no position names stay as they are; a position >= T * k has a
+ * zero d_weight; no other is named twice. d_out, Y and dY 16-byte aligned; T at
+ * most 2^23. */
 moe_status moe_unpermute_backward(const void* d_out, const void* Y, const uint32_t* inv_perm,
                                   const float* topk_weight, int32_t T, int32_t hidden, int32_t k,
                                   void* dY, float* d_weight, int32_t dtype, hipStream_t stream);
