@@ -181,11 +181,11 @@ struct ExpandJobs {
 
 constexpr int kFusedWaves = 8;
 
-// scale * s of tile row c (c8 chunks of 16 bytes' worth of values in LDS) as
-// the matrix operand of expand (see there), a step at a time; back: what the
-// products have to be multiplied by.
+// scale * s of tile row c (c8 chunks of 16 bytes' worth of values in LDS, four
+// floats i at row[i ^ turn]) as the matrix operand of expand (see there), a step at
+// a time; back: what the products have to be multiplied by.
 template <typename XT, int RT>
-__device__ __forceinline__ void expand_operand(const float* row, int c8, int q, bool mine,
+__device__ __forceinline__ void expand_operand(const float4* row, int turn, int c8, int q, bool mine,
                                                u32x4_t (&sv)[RT], float& back) {
   constexpr bool F32 = sizeof(XT) == 4;
   constexpr int V = 16 / sizeof(XT);
@@ -194,7 +194,7 @@ __device__ __forceinline__ void expand_operand(const float* row, int c8, int q, 
     const bool in = mine && cc < c8;
 #pragma unroll
     for (int j = 0; j < V; j += 4) {
-      const float4 f = *reinterpret_cast<const float4*>(row + min(cc, c8 - 1) * V + j);
+      const float4 f = row[((min(cc, c8 - 1) * V + j) >> 2) ^ turn];
       v[j] = in ? f.x : 0.f; v[j + 1] = in ? f.y : 0.f;
       v[j + 2] = in ? f.z : 0.f; v[j + 3] = in ? f.w : 0.f;
     }
@@ -346,14 +346,18 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
   constexpr int BL = NC * C8 / 64;                 // loads of a column group's b rows
   constexpr int AREA = (1 + RT) * 128 > NC * (C8 | 1) ? (1 + RT) * 128 : NC * (C8 | 1);  // 16-byte slots
   static_assert(AREA * 4 >= 2 * kTile * LD, "the sums of a wave and of the block fit an area");
-  // 16-bit types: behind the column groups two rows of the block's sums stay,
-  // rows 2 w and 2 w + 1 in area w
   constexpr int KEPT = AREA - 64;
   static_assert(F32 || (KEPT >= NC * (C8 | 1) && 64 * 4 >= 2 * RT * 16 && kTile == 2 * W), "room for the kept sums");
-  // a wave's area holds in turn its units, its sums and its column groups; the
-  // first one's second half the block's sums
+  // a wave's area holds in turn its units, its sums and its column groups. The
+  // block's sums: fp32 in the first one's second half, until its column groups
+  // overwrite them; 16-bit types behind the column groups, where they stay, rows 2 w
+  // and 2 w + 1 in area w, in an order that puts a chunk's 16 rows on different banks
   __shared__ u32x4_t area[W][AREA];
-  float* const sum = reinterpret_cast<float*>(area[0]) + kTile * LD;
+  auto sums_of = [&](int t) {
+    return F32 ? reinterpret_cast<float*>(area[0]) + kTile * LD + t * LD
+               : reinterpret_cast<float*>(area[t >> 1] + KEPT) + (t & 1) * RT * 16;
+  };
+  auto sums_turn = [](int t) { return F32 ? 0 : RT <= 2 ? (t >> 1) & (4 * RT - 1) : t; };
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // all arguments at once (opaque: else each is loaded where it is first used,
@@ -595,8 +599,7 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
         for (int z = 0; z < p.S; z++) v += ps[(size_t)z * p.T * R];
       }
       v *= sc;
-      sum[at] = v;
-      if constexpr (!F32) reinterpret_cast<float*>(area[t >> 1] + KEPT)[(t & 1) * RT * 16 + r] = v;
+      sums_of(t)[r ^ (sums_turn(t) << 2)] = v;
       if (p.s && share == 0 && r < R && ((same >> t) & 1u)) p.s[(size_t)(t0 + t) * R + r] = v;
     }
     lds_barrier();
@@ -606,8 +609,8 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
       // neighbouring bytes of y
       u32x4_t sv[RT];
       float back, bk[4] = {1.f, 1.f, 1.f, 1.f};
-      expand_operand<XT, RT>(sum + c * LD, c8, q, (same >> c) & 1u, sv, back);
-      lds_barrier();  // the first wave's column groups overwrite the sums
+      expand_operand<XT, RT>(reinterpret_cast<const float4*>(sums_of(c)), sums_turn(c), c8, q, (same >> c) & 1u, sv, back);
+      if constexpr (F32) lds_barrier();  // the first wave's column groups overwrite the sums
       if constexpr (__is_same(XT, f16_t)) {
 #pragma unroll
         for (int i = 0; i < 4; i++) bk[i] = __shfl(back, 4 * q + i, kWave);
@@ -679,18 +682,17 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
         }
         bool again = false;  // the same in all lanes
         if constexpr (!F32) {
-          float nan[4] = {0.f, 0.f, 0.f, 0.f};
+          float top = 0.f;
 #pragma unroll
           for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) nan[i] = __builtin_fmaf(o[j][i], 0.f, nan[i]);
-          const float any = (nan[0] + nan[1]) + (nan[2] + nan[3]);
-          again = __builtin_expect(__any(any != any), 0);
+            for (int i = 0; i < 4; i++) top = __builtin_elementwise_maximum(top, __builtin_fabsf(o[j][i]));  // NaN stays
+          again = __builtin_expect(__any(!(top < __builtin_huge_valf())), 0);
           if (again) {
             int l = tid & 63;
             asm volatile("" : "+v"(l));  // (opaque: as above)
-            const int row = l & 15, k = l >> 4;
-            const float* const kept = reinterpret_cast<const float*>(area[row >> 1] + KEPT) + (row & 1) * RT * 16 + k;
+            const int row = l & 15, k = l >> 4, turn = sums_turn(row) << 2;
+            const float* const sum = sums_of(row) + k;
             const XT* const bcol = reinterpret_cast<const XT*>(mem + row * (c8 | 1)) + k;
 #pragma unroll
             for (int j = 0; j < J; j++) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -698,7 +700,7 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
             for (int r = 0; r < R; r += 4) {
 #pragma unroll
               for (int j = 0; j < J; j++)
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(kept[r], to_f<XT>(bcol[j * 16 * (c8 | 1) * V + r]), o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(sum[r ^ turn], to_f<XT>(bcol[j * 16 * (c8 | 1) * V + r]), o[j], 0, 0, 0);
             }
           }
         }
