@@ -339,7 +339,7 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
   constexpr int UNIT = 8 * V;                      // a unit of K: 128 bytes of a row
   // neighbouring columns of a lane: as many as leave LDS for two blocks up to
   // rank 64 (fp32, 7454 rows 264 -> 96 backward at rank 40: 26.2 us with two columns,
-  // 31.8 with four; 4096 rows 2048 -> 2048 at rank 64 54.6 and 64.6)
+  // 31.8 with four; 4096 rows 2048 -> 2048 at rank 64 54.8 and 64.6)
   constexpr int J = F32 && RT >= 4 ? 2 : 4;
   constexpr int NC = 16 * J;                       // columns of a group
   constexpr int C8 = RT * 16 / V;                  // 16-byte chunks of the widest adapter row
@@ -1177,8 +1177,8 @@ size_t adapter_bytes(const LoraDims& d) {
 
 // One launch, unless few blocks would each read a large adapter alone. Kernel
 // times in one launch and in two: one row of 2048 -> 2048 at rank 16 5.7 us and 2.9 +
-// 4.2, at rank 128 17.5 and 5.1 + 11.1 (of 4096 -> 4096 23.0 and 5.1 + 13.2); 64 rows of
-// 64 adapters of 4096 -> 4096 at rank 64 19.9 and 9.9 + 13.2.
+// 4.2, at rank 128 17.5 and 5.0 + 10.1 (of 4096 -> 4096 23.0 and 5.0 + 13.6); 64 rows of
+// 64 adapters of 4096 -> 4096 at rank 64 19.4 and 9.9 + 13.2.
 constexpr size_t kFusedBytes = 256u << 10;
 constexpr int kSplitBlocks = 32;
 bool lora_fused(const LoraDims& d) {
