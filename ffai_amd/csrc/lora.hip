@@ -680,15 +680,15 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
             if (BL >= 16) __builtin_amdgcn_sched_barrier(0);
           }
         }
-        bool again = false;  // the same in all lanes
+        bool redo = false;  // the same in all lanes
         if constexpr (!F32) {
           float top = 0.f;
 #pragma unroll
           for (int j = 0; j < J; j++)
 #pragma unroll
             for (int i = 0; i < 4; i++) top = __builtin_elementwise_maximum(top, __builtin_fabsf(o[j][i]));  // NaN stays
-          again = __builtin_expect(__any(!(top < __builtin_huge_valf())), 0);
-          if (again) {
+          redo = __builtin_expect(__any(!(top < __builtin_huge_valf())), 0);
+          if (redo) {
             int l = tid & 63;
             asm volatile("" : "+v"(l));  // (opaque: as above)
             const int row = l & 15, k = l >> 4, turn = sums_turn(row) << 2;
@@ -716,7 +716,7 @@ __global__ __launch_bounds__(64 * kFusedWaves, expand_waves(RT)) void lora_expan
 #pragma unroll
             for (int j = 0; j < J / 2; j++) {
               const uint32_t y2 = yv[i][j];
-              const float m = again ? 1.f : bk[i];
+              const float m = redo ? 1.f : bk[i];
               const float lo = __builtin_fmaf(o[2 * j][i], m, to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(y2 & 0xFFFFu))));
               const float hi = __builtin_fmaf(o[2 * j + 1][i], m, to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(y2 >> 16))));
               w[j] = (uint32_t)__builtin_bit_cast(uint16_t, from_f<XT>(lo)) |
@@ -1048,9 +1048,8 @@ __global__ __launch_bounds__(64 * kOuterWaves) void lora_outer_kernel(OuterArgs 
 // Adds the chunks of the adapters that have several, and writes zeros for
 // those without rows; the others are there already. A lane adds 8 neighbouring
 // values. Up to eight chunks one wave adds them all in order; more are shared by
-// the block's waves, a run of them each, whose sums meet in LDS in the waves' order (7454 rows of one adapter 264 -> 96 at
-// rank 40, 117 chunks: 5.8 us,
-// by one wave 14).
+// the block's waves, a run of them each, whose sums meet in LDS in the waves' order
+// (7454 rows of one adapter 264 -> 96 at rank 40, 117 chunks: 5.8 us, by one wave 14).
 constexpr int kSumWaves = 4;
 template <typename XT>
 __global__ __launch_bounds__(64 * kSumWaves) void lora_sum_kernel(OuterArgs p) {
