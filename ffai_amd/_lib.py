@@ -37,6 +37,9 @@ EXPORTS = [
     "moe_balance_loss_workspace_bytes", "moe_balance_loss", "moe_router_backward",
     "moe_unpermute_backward", "moe_validate_lora", "moe_lora_workspace_bytes", "moe_lora_apply",
     "moe_lora_backward_workspace_bytes", "moe_lora_backward",
+    "moe_expert_matmul_backward", "moe_activation_save", "moe_checkpoint_restore",
+    "moe_activation_backward", "moe_permute_backward",
+    "moe_add_rmsnorm_backward_workspace_bytes", "moe_add_rmsnorm_backward",
     "moe_st_open", "moe_st_close", "moe_st_count", "moe_st_name", "moe_st_info", "moe_st_read_host",
     "moe_st_upload", "moe_st_is_quantized", "moe_st_stacked_bytes", "moe_st_load_stacked",
     "moe_st_load_stacked_many", "moe_st_mxfp4_bytes", "moe_st_load_mxfp4",
@@ -161,6 +164,17 @@ def load():
     lib.moe_lora_backward_workspace_bytes.argtypes = [C.POINTER(Lora), i32]
     lib.moe_lora_backward_workspace_bytes.restype = sz
     lib.moe_lora_backward.argtypes = [C.POINTER(Lora), vp, vp, i32, vp, vp, vp, vp, vp, vp, sz, st]
+    lib.moe_expert_matmul_backward.argtypes = [C.POINTER(QProj), vp, C.POINTER(QProj), vp, i32, vp, i32,
+                                               i32, vp, vp, vp, st]
+    lib.moe_activation_save.argtypes = [vp, vp, i32, i32, i32, i32, C.c_float, C.c_float, vp, vp, vp, vp,
+                                        st]
+    lib.moe_checkpoint_restore.argtypes = [vp, vp, C.c_int64, vp, i32, st]
+    lib.moe_activation_backward.argtypes = [vp, vp, vp, i32, i32, i32, i32, C.c_float, C.c_float, vp, vp,
+                                            vp, vp, vp, vp, vp, st]
+    lib.moe_permute_backward.argtypes = [vp, vp, i32, i32, i32, vp, vp, i32, st]
+    lib.moe_add_rmsnorm_backward_workspace_bytes.argtypes = [i32, i32]
+    lib.moe_add_rmsnorm_backward_workspace_bytes.restype = sz
+    lib.moe_add_rmsnorm_backward.argtypes = [vp, vp, vp, vp, C.c_float, i32, i32, i32, vp, vp, vp, sz, st]
     lib.moe_st_open.argtypes = [C.c_char_p, C.POINTER(vp)]
     lib.moe_st_close.argtypes = [vp]
     lib.moe_st_close.restype = None
@@ -189,7 +203,9 @@ def load():
                  "moe_layer_create", "moe_layer_decode",
                  "moe_layer_decode_many", "moe_balance_loss", "moe_router_backward",
                  "moe_unpermute_backward", "moe_validate_lora", "moe_lora_apply",
-                 "moe_lora_backward", "moe_st_open", "moe_st_info", "moe_st_read_host",
+                 "moe_lora_backward", "moe_expert_matmul_backward", "moe_activation_save",
+                 "moe_checkpoint_restore", "moe_activation_backward", "moe_permute_backward",
+                 "moe_add_rmsnorm_backward", "moe_st_open", "moe_st_info", "moe_st_read_host",
                  "moe_st_upload", "moe_st_stacked_bytes", "moe_st_load_stacked",
                  "moe_st_load_stacked_many", "moe_st_mxfp4_bytes", "moe_st_load_mxfp4"]:
         getattr(lib, name).restype = C.c_int

@@ -138,6 +138,25 @@ hipError_t launch_gemv(int bits, int xdt, int sbdt, bool gateup, int tokmax, con
   return hipErrorInvalidValue;
 }
 
+hipError_t launch_expert_grad_b2(int, int, const ExpertGradArgs&, hipStream_t);
+hipError_t launch_expert_grad_b3(int, int, const ExpertGradArgs&, hipStream_t);
+hipError_t launch_expert_grad_b4(int, int, const ExpertGradArgs&, hipStream_t);
+hipError_t launch_expert_grad_b5(int, int, const ExpertGradArgs&, hipStream_t);
+hipError_t launch_expert_grad_b6(int, int, const ExpertGradArgs&, hipStream_t);
+hipError_t launch_expert_grad_b8(int, int, const ExpertGradArgs&, hipStream_t);
+
+hipError_t launch_expert_grad(int bits, int xdt, int sbdt, const ExpertGradArgs& a, hipStream_t st) {
+  switch (bits) {
+    case 2: return launch_expert_grad_b2(xdt, sbdt, a, st);
+    case 3: return launch_expert_grad_b3(xdt, sbdt, a, st);
+    case 4: return launch_expert_grad_b4(xdt, sbdt, a, st);
+    case 5: return launch_expert_grad_b5(xdt, sbdt, a, st);
+    case 6: return launch_expert_grad_b6(xdt, sbdt, a, st);
+    case 8: return launch_expert_grad_b8(xdt, sbdt, a, st);
+  }
+  return hipErrorInvalidValue;
+}
+
 static hipError_t launch_dec1(int bits, int xdt, int sbdt, bool down, int rm, int ur,
                               const void* args, int grid, size_t smem, hipStream_t st,
                               KEvents ev) {
@@ -1333,6 +1352,222 @@ extern "C" moe_status moe_lora_backward(const moe_lora* l, const void* x, const 
     return fail(MOE_ERR_WORKSPACE, "lora_backward: 16-byte aligned workspace of %zu bytes needed", need);
   const LoraBackward a{x, dy, l->a, l->b, l->scale, adapter, dx_in, dx, da, db, workspace};
   MOE_HIP(launch_lora_backward(d, a, stream), "adapter backward launch");
+  return ok();
+}
+
+// ---------------------------------------------------------------------------
+// gradients through the quantised experts
+// ---------------------------------------------------------------------------
+extern "C" moe_status moe_expert_matmul_backward(const moe_qproj* p, const void* dy, const moe_qproj* p2,
+                                                 const void* dy2, int32_t dtype, const uint32_t* perm,
+                                                 int32_t top_k, int32_t M, const uint32_t* offsets,
+                                                 const void* dx_in, void* dx, hipStream_t stream) {
+  MOE_TRY(validate_qproj_named(p, "expert_matmul_backward"));
+  if (!dy || !offsets || !dx) return fail(MOE_ERR_INVALID, "expert_matmul_backward: NULL pointer");
+  if (!p2 != !dy2) return fail(MOE_ERR_INVALID, "expert_matmul_backward: p2 and dy2 come together");
+  if (M <= 0) return fail(MOE_ERR_INVALID, "expert_matmul_backward: M must be positive");
+  if (perm && top_k <= 0) return fail(MOE_ERR_INVALID, "expert_matmul_backward: top_k must be positive");
+  if (!dt_ok(dtype) || !pair_ok(dtype, p->sb_dtype))
+    return fail(MOE_ERR_UNSUPPORTED, "expert_matmul_backward: gradient/scale dtype pair not built");
+  if (p2) {
+    MOE_TRY(validate_qproj_named(p2, "expert_matmul_backward: p2"));
+    if (p2->n != p->n || p2->k != p->k || p2->n_experts != p->n_experts || p2->bits != p->bits ||
+        p2->group_size != p->group_size || p2->sb_dtype != p->sb_dtype)
+      return fail(MOE_ERR_INVALID, "expert_matmul_backward: p2 must have p's shape and formats");
+  }
+  if (p->n_experts > 1024) return fail(MOE_ERR_UNSUPPORTED, "expert_matmul_backward: n_experts above 1024");
+  if (M > kMaxTuneRows) return fail(MOE_ERR_UNSUPPORTED, "expert_matmul_backward: M above %d", kMaxTuneRows);
+  if (p->n % 8)
+    return fail(MOE_ERR_UNSUPPORTED, "expert_matmul_backward: n=%d must be a multiple of 8", p->n);
+  if (p->n > 1 << 20 || p->k > 1 << 20 || (int64_t)p->n * p->k > (int64_t)1 << 31)
+    return fail(MOE_ERR_UNSUPPORTED, "expert_matmul_backward: n (%d) and k (%d) at most 2^20, n * k at most 2^31",
+                p->n, p->k);
+  for (const void* b : {dy, dy2, dx_in, (const void*)dx})
+    if (!aligned16(b)) return fail(MOE_ERR_INVALID, "expert_matmul_backward: rows must be 16-byte aligned");
+  const size_t es = dt_size(dtype), out = (size_t)M * p->k * es;
+  const size_t in = (size_t)(perm ? (M - 1) / top_k + 1 : M) * p->n * es;
+  if (overlaps(dy, in, dx, out) || overlaps(dy2, in, dx, out) || (dx_in != dx && overlaps(dx_in, out, dx, out)))
+    return fail(MOE_ERR_INVALID, "expert_matmul_backward: dx overlaps an input (dx_in: equal or apart)");
+  const size_t words = (size_t)p->n_experts * p->n * p->k / 32 * p->bits * 4;
+  const size_t groups = (size_t)p->n_experts * p->n * (p->k / p->group_size) * dt_size(p->sb_dtype);
+  for (const moe_qproj* q : {p, p2})
+    if (q && (overlaps(q->weight, words, dx, out) || overlaps(q->scales, groups, dx, out) ||
+              overlaps(q->biases, groups, dx, out)))
+      return fail(MOE_ERR_INVALID, "expert_matmul_backward: dx overlaps the experts");
+  if (overlaps(perm, (size_t)M * 4, dx, out) || overlaps(offsets, (size_t)(p->n_experts + 1) * 4, dx, out))
+    return fail(MOE_ERR_INVALID, "expert_matmul_backward: dx overlaps the plan");
+  ExpertGradArgs a{};
+  a.p0 = GemvProj{p->weight, p->scales, p->biases, nullptr};
+  if (p2) a.p1 = GemvProj{p2->weight, p2->scales, p2->biases, nullptr};
+  a.dy = dy;
+  a.dy2 = dy2;
+  a.perm = perm;
+  a.topk = top_k;
+  a.offsets = offsets;
+  a.dx_in = dx_in;
+  a.dx = dx;
+  a.M = M;
+  a.N = p->n;
+  a.K = p->k;
+  a.E = p->n_experts;
+  a.gsh = group_shift(p->group_size);
+  MOE_HIP(launch_expert_grad(p->bits, dtype, p->sb_dtype, a, stream), "expert gradient launch");
+  return ok();
+}
+
+namespace {
+
+// The arguments that the kept activation's two calls share.
+moe_status validate_kept(const char* name, const int8_t* codes, const uint8_t* scales, int M, int n,
+                         int dtype, int activation) {
+  if (!codes || !scales) return fail(MOE_ERR_INVALID, "%s: NULL pointer", name);
+  if (M <= 0 || n <= 0) return fail(MOE_ERR_INVALID, "%s: M and n must be positive", name);
+  if (M > kMaxTuneRows) return fail(MOE_ERR_UNSUPPORTED, "%s: M above %d", name, kMaxTuneRows);
+  if (n % 32) return fail(MOE_ERR_UNSUPPORTED, "%s: n=%d must be a multiple of 32", name, n);
+  if (n > 1 << 20) return fail(MOE_ERR_UNSUPPORTED, "%s: n above 2^20", name);
+  if (!dt_ok(dtype)) return fail(MOE_ERR_INVALID, "%s: bad dtype", name);
+  if (!act_ok(activation)) return fail(MOE_ERR_INVALID, "%s: bad kind", name);
+  if (!aligned16(codes)) return fail(MOE_ERR_INVALID, "%s: codes must be 16-byte aligned", name);
+  return MOE_OK;
+}
+
+}  // namespace
+
+extern "C" moe_status moe_activation_save(const void* gate, const void* up, int32_t M, int32_t n,
+                                          int32_t dtype, int32_t activation, float alpha, float limit,
+                                          const uint32_t* n_rows, void* out, int8_t* codes,
+                                          uint8_t* scales, hipStream_t stream) {
+  MOE_TRY(validate_kept("activation_save", codes, scales, M, n, dtype, activation));
+  const bool gated = activation != MOE_ACT_RELU2;
+  if (!up || (gated && !gate)) return fail(MOE_ERR_INVALID, "activation_save: NULL pointer");
+  if (!gated) gate = nullptr;
+  if (!aligned16(gate) || !aligned16(up) || !aligned16(out))
+    return fail(MOE_ERR_INVALID, "activation_save: rows must be 16-byte aligned");
+  const size_t el = (size_t)M * n, rows = el * dt_size(dtype), kept = (gated ? 2 : 1) * el;
+  const struct {
+    const void* p;
+    size_t bytes;
+  } b[5] = {{gate, rows}, {up, rows}, {out, rows}, {codes, kept}, {scales, kept / 32}};
+  for (int i = 2; i < 5; i++)
+    for (int j = 0; j < i; j++)  // (the value may take its own inputs' place)
+      if (overlaps(b[i].p, b[i].bytes, b[j].p, b[j].bytes) && !(i == 2 && b[i].p == b[j].p))
+        return fail(MOE_ERR_INVALID, "activation_save: buffers overlap (out: gate, up or apart)");
+  MOE_HIP(launch_activation_save(gate, up, M, n, dtype, activation, alpha, limit, n_rows, out, codes,
+                                 scales, stream),
+          "activation save launch");
+  return ok();
+}
+
+extern "C" moe_status moe_checkpoint_restore(const int8_t* codes, const uint8_t* scales, int64_t numel,
+                                             void* out, int32_t dtype, hipStream_t stream) {
+  if (!codes || !scales || !out) return fail(MOE_ERR_INVALID, "checkpoint_restore: NULL pointer");
+  if (numel <= 0) return fail(MOE_ERR_INVALID, "checkpoint_restore: numel must be positive");
+  if (numel % 32) return fail(MOE_ERR_UNSUPPORTED, "checkpoint_restore: numel must be a multiple of 32");
+  if (numel > (int64_t)1 << 44) return fail(MOE_ERR_UNSUPPORTED, "checkpoint_restore: numel above 2^44");
+  if (!dt_ok(dtype)) return fail(MOE_ERR_INVALID, "checkpoint_restore: bad dtype");
+  if (!aligned16(codes) || !aligned16(out))
+    return fail(MOE_ERR_INVALID, "checkpoint_restore: codes and out must be 16-byte aligned");
+  const size_t bytes = (size_t)numel * dt_size(dtype);
+  if (overlaps(codes, (size_t)numel, out, bytes) || overlaps(scales, (size_t)numel / 32, out, bytes))
+    return fail(MOE_ERR_INVALID, "checkpoint_restore: out overlaps an input");
+  MOE_HIP(launch_restore(codes, scales, numel, out, dtype, stream), "checkpoint restore launch");
+  return ok();
+}
+
+extern "C" moe_status moe_activation_backward(const int8_t* codes, const uint8_t* scales, const void* dh,
+                                              int32_t M, int32_t n, int32_t dtype, int32_t activation,
+                                              float alpha, float limit, const float* topk_weight,
+                                              const uint32_t* perm, const uint32_t* n_rows, void* d_gate,
+                                              void* d_up, float* d_weight, void* h, hipStream_t stream) {
+  MOE_TRY(validate_kept("activation_backward", codes, scales, M, n, dtype, activation));
+  const bool gated = activation != MOE_ACT_RELU2;
+  if (!dh || !d_up || (gated && !d_gate)) return fail(MOE_ERR_INVALID, "activation_backward: NULL pointer");
+  if (!gated && d_gate) return fail(MOE_ERR_INVALID, "activation_backward: no gate with squared ReLU");
+  for (const void* b : {dh, (const void*)d_gate, (const void*)d_up, (const void*)h})
+    if (!aligned16(b)) return fail(MOE_ERR_INVALID, "activation_backward: rows must be 16-byte aligned");
+  const size_t el = (size_t)M * n, rows = el * dt_size(dtype), kept = (gated ? 2 : 1) * el;
+  const struct {
+    const void* p;
+    size_t bytes;
+  } in[4] = {{codes, kept}, {scales, kept / 32}, {topk_weight, (size_t)M * 4}, {perm, (size_t)M * 4}},
+    out[4] = {{d_gate, rows}, {d_up, rows}, {h, rows}, {d_weight, (size_t)M * 4}};
+  for (int i = 0; i < 4; i++) {
+    for (const auto& b : in)
+      if (overlaps(out[i].p, out[i].bytes, b.p, b.bytes))
+        return fail(MOE_ERR_INVALID, "activation_backward: a result overlaps an input");
+    if (overlaps(out[i].p, out[i].bytes, dh, rows) && !(i < 2 && out[i].p == dh))
+      return fail(MOE_ERR_INVALID, "activation_backward: a result overlaps dh (d_gate or d_up: equal or apart)");
+    for (int j = 0; j < i; j++)
+      if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
+        return fail(MOE_ERR_INVALID, "activation_backward: results overlap");
+  }
+  MOE_HIP(launch_activation_backward(codes, scales, dh, M, n, dtype, activation, alpha, limit, topk_weight,
+                                     perm, n_rows, d_gate, d_up, d_weight, h, stream),
+          "activation backward launch");
+  return ok();
+}
+
+extern "C" moe_status moe_permute_backward(const void* dX, const uint32_t* inv_perm, int32_t T,
+                                           int32_t hidden, int32_t k, const void* dx_in, void* dx,
+                                           int32_t dtype, hipStream_t stream) {
+  if (!dX || !inv_perm || !dx) return fail(MOE_ERR_INVALID, "permute_backward: NULL pointer");
+  if (T <= 0 || hidden <= 0 || k <= 0)
+    return fail(MOE_ERR_INVALID, "permute_backward: T, hidden and k must be positive");
+  if ((long)T * k > 0x7fffffffL) return fail(MOE_ERR_INVALID, "permute_backward: T*k too large");
+  if (T > kMaxTuneRows) return fail(MOE_ERR_UNSUPPORTED, "permute_backward: T above %d", kMaxTuneRows);
+  if (hidden % 8) return fail(MOE_ERR_UNSUPPORTED, "permute_backward: hidden must be a multiple of 8");
+  if (hidden > 1 << 20) return fail(MOE_ERR_UNSUPPORTED, "permute_backward: hidden above 2^20");
+  if (!dt_ok(dtype)) return fail(MOE_ERR_INVALID, "permute_backward: bad dtype");
+  if (!aligned16(dX) || !aligned16(dx_in) || !aligned16(dx))
+    return fail(MOE_ERR_INVALID, "permute_backward: rows must be 16-byte aligned");
+  const size_t row = (size_t)hidden * dt_size(dtype), out = row * T;
+  if (overlaps(dX, out * k, dx, out) || overlaps(inv_perm, (size_t)T * k * 4, dx, out) ||
+      (dx_in != dx && overlaps(dx_in, out, dx, out)))
+    return fail(MOE_ERR_INVALID, "permute_backward: dx overlaps an input (dx_in: equal or apart)");
+  MOE_HIP(launch_permute_backward(dX, inv_perm, T, hidden, k, dx_in, dx, dtype, stream),
+          "permute backward launch");
+  return ok();
+}
+
+extern "C" size_t moe_add_rmsnorm_backward_workspace_bytes(int32_t n_rows, int32_t row_size) {
+  if (n_rows <= 0 || n_rows > kMaxTuneRows || row_size <= 0 || row_size % 8 || row_size > kMaxHidden) return 0;
+  return norm_backward_ws_bytes(n_rows, row_size);
+}
+
+extern "C" moe_status moe_add_rmsnorm_backward(const void* residual, const void* weight,
+                                               const void* d_normed, const void* d_residual, float eps,
+                                               int32_t n_rows, int32_t row_size, int32_t dtype,
+                                               void* d_in, float* d_weight, void* workspace,
+                                               size_t workspace_bytes, hipStream_t stream) {
+  if (!residual || !weight || !d_normed || !d_in || !d_weight)
+    return fail(MOE_ERR_INVALID, "add_rmsnorm_backward: NULL pointer");
+  if (n_rows <= 0 || row_size <= 0)
+    return fail(MOE_ERR_INVALID, "add_rmsnorm_backward: n_rows and row_size must be positive");
+  if (n_rows > kMaxTuneRows) return fail(MOE_ERR_UNSUPPORTED, "add_rmsnorm_backward: n_rows above %d", kMaxTuneRows);
+  if (!dt_ok(dtype)) return fail(MOE_ERR_INVALID, "add_rmsnorm_backward: bad dtype");
+  if (row_size % 8 || row_size > kMaxHidden)
+    return fail(MOE_ERR_UNSUPPORTED,
+                "add_rmsnorm_backward: row size %d must be a multiple of 8 and at most %d", row_size, kMaxHidden);
+  if (!(eps >= 0.f) || !std::isfinite(eps))
+    return fail(MOE_ERR_INVALID, "add_rmsnorm_backward: eps must be finite and non-negative");
+  for (const void* b : {residual, weight, d_normed, d_residual, (const void*)d_in, (const void*)d_weight})
+    if (!aligned16(b)) return fail(MOE_ERR_INVALID, "add_rmsnorm_backward: buffers must be 16-byte aligned");
+  const size_t wb = (size_t)row_size * dt_size(dtype), rows = wb * n_rows, dwb = (size_t)row_size * 4;
+  if (overlaps(residual, rows, d_in, rows) || overlaps(weight, wb, d_in, rows) ||
+      (d_normed != d_in && overlaps(d_normed, rows, d_in, rows)) ||
+      (d_residual != d_in && overlaps(d_residual, rows, d_in, rows)))
+    return fail(MOE_ERR_INVALID,
+                "add_rmsnorm_backward: d_in overlaps an input (d_normed, d_residual: equal or apart)");
+  if (overlaps(residual, rows, d_weight, dwb) || overlaps(weight, wb, d_weight, dwb) ||
+      overlaps(d_normed, rows, d_weight, dwb) || overlaps(d_residual, rows, d_weight, dwb) ||
+      overlaps(d_in, rows, d_weight, dwb))
+    return fail(MOE_ERR_INVALID, "add_rmsnorm_backward: d_weight overlaps another buffer");
+  const size_t need = norm_backward_ws_bytes(n_rows, row_size);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(MOE_ERR_WORKSPACE, "add_rmsnorm_backward: 16-byte aligned workspace of %zu bytes needed", need);
+  MOE_HIP(launch_norm_backward(residual, weight, d_normed, d_residual, eps, n_rows, row_size, dtype, d_in,
+                               d_weight, workspace, stream),
+          "add + RMSNorm backward launch");
   return ok();
 }
 

@@ -327,4 +327,42 @@ hipError_t launch_lora(const LoraDims& d, const void* x, const void* a, const vo
                        void* ws, hipStream_t st);
 hipError_t launch_lora_backward(const LoraDims& d, const LoraBackward& a, hipStream_t st);
 
+// ------------------------------------------ gradients through the experts --
+// Gradient of the grouped dequantising product with respect to its rows
+// (expert_grad.hip); p1 and dy2 (nullable): a second projection of the same
+// shape and formats whose gradient is added.
+struct ExpertGradArgs {
+  GemvProj p0, p1;
+  const void *dy, *dy2;      // [rows, N]
+  const uint32_t* perm;      // nullable: row(p) = perm[p] / topk, else p
+  int topk;
+  const uint32_t* offsets;   // [E + 1]
+  const void* dx_in;         // nullable [M, K], may be dx
+  void* dx;                  // [M, K]
+  int M, N, K, E;
+  int gsh;                   // log2(group size / 32)
+};
+hipError_t launch_expert_grad(int bits, int xdt, int sbdt, const ExpertGradArgs& a, hipStream_t st);
+
+// The gated activation with its inputs in 8 bits (ckpt8.hip): codes [parts,
+// M, n], exponent bytes [parts, M, n / 32], parts (gate, up) or (up); n a
+// multiple of 32. n_rows (nullable): the rows there are, on the device.
+hipError_t launch_activation_save(const void* g, const void* u, int M, int n, int dt, int act,
+                                  float alpha, float limit, const uint32_t* n_rows, void* out,
+                                  int8_t* codes, uint8_t* scales, hipStream_t st);
+hipError_t launch_restore(const int8_t* codes, const uint8_t* scales, int64_t numel, void* out, int dt,
+                          hipStream_t st);
+hipError_t launch_activation_backward(const int8_t* codes, const uint8_t* scales, const void* dh, int M,
+                                      int n, int dt, int act, float alpha, float limit,
+                                      const float* weight, const uint32_t* perm, const uint32_t* n_rows,
+                                      void* dg, void* du, float* dw, void* h, hipStream_t st);
+
+// Rows sorted by expert back to their tokens, and the gradient of
+// launch_add_rmsnorm (layer_grad.hip).
+hipError_t launch_permute_backward(const void* dX, const uint32_t* inv, int T, int H, int k,
+                                   const void* dx_in, void* dx, int dt, hipStream_t st);
+size_t norm_backward_ws_bytes(int T, int H);
+hipError_t launch_norm_backward(const void* r, const void* w, const void* dn, const void* dr, float eps,
+                                int T, int H, int dt, void* din, float* dw, void* ws, hipStream_t st);
+
 }  // namespace moe

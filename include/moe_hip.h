@@ -399,6 +399,91 @@ moe_status moe_lora_backward(const moe_lora* l, const void* x, const void* dy, i
                              void* db, void* workspace, size_t workspace_bytes,
                              hipStream_t stream);
 
+/* ---- gradients through the quantised experts ---------------------------- */
+
+/* A layer's backward pass with its quantised weights as they are: the experts'
+ * products, their activation (whose inputs the forward keeps in 8 bits), the
+ * rows back in token order, and the add and norm before the layer. The
+ * reference only runs forward. Sums are f32; every result is the same from
+ * call to call. For sorted rows h = act(g, u), Y = W_down h and the combine
+ * out[t] = sum_s w[t,s] Y[inv_perm[t*k+s]], with d_out the gradient of out:
+ *   dh     = moe_expert_matmul_backward(down, d_out through perm)
+ *   dg, du, d w = moe_activation_backward(kept g and u, dh, w through perm)
+ *   dX     = moe_expert_matmul_backward(gate, dg, up, du)
+ *   dx     = moe_permute_backward(dX)
+ * so neither g, u, h nor Y has to be kept. */
+
+/* Gradient of moe_expert_matmul with respect to its rows:
+ *   dx[p,:] = round(dx_in[p,:] + dy[row(p),:] W[e(p)] + dy2[row(p),:] W2[e(p)])
+ * with e(p) and row(p) as there (perm nullable), for the sorted positions
+ * below offsets[n_experts], M at most; rows of dx behind them stay as they are.
+ * p2 and dy2 are NULL together; p2 has p's shape, bits, group size and scale
+ * type. dy [M or ceil(M / top_k), n], dx_in (nullable, may be dx) and dx [M, k]
+ * in dtype, 16-byte aligned; n a multiple of 8, n_experts at most 1024, M at
+ * most 2^23. A 16-bit dtype multiplies weights rounded to it (half a step: 2^-8
+ * of the weight for bf16, 2^-11 for f16); f32 rounds them to f32 only. Output
+ * biases have no part in it. Infinities and NaN stay in their rows of dy, and
+ * in weights in their expert. */
+moe_status moe_expert_matmul_backward(const moe_qproj* p, const void* dy, const moe_qproj* p2,
+                                      const void* dy2, int32_t dtype, const uint32_t* perm,
+                                      int32_t top_k, int32_t M, const uint32_t* offsets,
+                                      const void* dx_in, void* dx, hipStream_t stream);
+
+/* moe_activation_apply of rows gate and up [M, n] (out nullable), with both
+ * kept as microscaled int8: codes [2, M, n] and exponent bytes scales
+ * [2, M, n / 32], gate first; with MOE_ACT_RELU2 [1, ...], up only. A block of
+ * 32 columns has the least e in 0..254 with |v| < 127.5 * 2^(e - 133) for all
+ * its values, and codes round(v * 2^(133 - e)) (ties to even): no value is off
+ * by more than half a step, 2^-7.98 of the block's largest at most. A block
+ * with an infinity, a NaN or a magnitude of 2^128 (1 - 2^-8) or more has e = 255
+ * and reads as NaN. n a multiple of 32. n_rows (nullable, on the device): only
+ * the rows below *n_rows are read and written (a plan's offsets + n_experts). */
+moe_status moe_activation_save(const void* gate, const void* up, int32_t M, int32_t n, int32_t dtype,
+                               int32_t activation, float alpha, float limit, const uint32_t* n_rows,
+                               void* out, int8_t* codes, uint8_t* scales, hipStream_t stream);
+
+/* The values kept: out[i] = round(codes[i] * 2^(scales[i / 32] - 133)), NaN
+ * where the exponent byte is 255. numel a multiple of 32. */
+moe_status moe_checkpoint_restore(const int8_t* codes, const uint8_t* scales, int64_t numel, void* out,
+                                  int32_t dtype, hipStream_t stream);
+
+/* Gradients of the activation at the kept g and u, for dh [M, n] the gradient
+ * of h before the routing weight r[p] = round(topk_weight[perm[p]]) (1 where
+ * topk_weight is NULL; perm NULL: p):
+ *   d_gate[p,:] = round(r[p] dh[p,:] dact/dg)   (not with MOE_ACT_RELU2)
+ *   d_up[p,:]   = round(r[p] dh[p,:] dact/du)
+ *   d_weight[perm[p]] = <dh[p,:], act(g, u)[p,:]>   (f32, nullable)
+ *   h[p,:]      = round(act(g, u)[p,:])             (nullable)
+ * A limit's slope is 1 at the limit itself. A perm entry >= M has a weight of 0
+ * and no d_weight; no other is named twice. d_gate or d_up may be dh. A kept NaN
+ * gives NaN in its own row. Layouts, n_rows and n as in moe_activation_save. */
+moe_status moe_activation_backward(const int8_t* codes, const uint8_t* scales, const void* dh, int32_t M,
+                                   int32_t n, int32_t dtype, int32_t activation, float alpha,
+                                   float limit, const float* topk_weight, const uint32_t* perm,
+                                   const uint32_t* n_rows, void* d_gate, void* d_up, float* d_weight,
+                                   void* h, hipStream_t stream);
+
+/* Gradient of taking row perm[p] / k for every sorted position p:
+ *   dx[t,:] = round(dx_in[t,:] + sum_s dX[inv_perm[t*k+s],:])
+ * ranks added in order; a position >= T * k adds nothing. dX [T * k, hidden],
+ * dx_in (nullable, may be dx) and dx [T, hidden], 16-byte aligned; hidden a
+ * multiple of 8, T at most 2^23. */
+moe_status moe_permute_backward(const void* dX, const uint32_t* inv_perm, int32_t T, int32_t hidden,
+                                int32_t k, const void* dx_in, void* dx, int32_t dtype,
+                                hipStream_t stream);
+
+/* Gradient of moe_add_rmsnorm at its residual_out r, for the gradients of
+ * normed_out and (nullable) of r itself, with s = 1 / sqrt(mean(r^2) + eps):
+ *   d_in[t,:] = round(d_residual + s (d_normed w - r s mean(d_normed w r s)))
+ *   d_weight  = sum_t d_normed[t,:] r[t,:] s                    (f32)
+ * d_in is the gradient of both a and b; it may be d_normed or d_residual. Rows
+ * 16-byte aligned, row_size a multiple of 8, at most 8192; n_rows at most 2^23. */
+size_t moe_add_rmsnorm_backward_workspace_bytes(int32_t n_rows, int32_t row_size);
+moe_status moe_add_rmsnorm_backward(const void* residual, const void* weight, const void* d_normed,
+                                    const void* d_residual, float eps, int32_t n_rows,
+                                    int32_t row_size, int32_t dtype, void* d_in, float* d_weight,
+                                    void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* ---- whole layer ------------------------------------------------------- */
 
 /* Workspace for moe_layer_forward at up to max_tokens rows. */
