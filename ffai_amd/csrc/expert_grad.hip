@@ -9,8 +9,7 @@
 // only runs forward (Ops.swift:4553-5201).
 #include <algorithm>
 
-#include "moe_common.hpp"
-#include "moe_internal.hpp"
+#include "gemm_units.hpp"
 
 #ifndef MOE_BITS
 #define MOE_BITS 4
@@ -131,14 +130,378 @@ static hipError_t launch_f32(const ExpertGradArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// ----------------------------------------------------------- 16-bit products --
+// Rows in a 16-bit type take v_mfma_f32_32x32x16 with the weights dequantised
+// in fp32 and rounded once to that type: bf16 gradients keep their range, and
+// a weight is off by at most half a step of the type.
+//
+// The weights' packed axis is the output's, and the matrix operands want
+// neighbours along the sum. The transposition costs nothing: a thread
+// dequantises units of 32 columns of one weight row, with one scale and bias,
+// into LDS as they lie ([sum][column]), and ds_read_tr16_b64 hands each lane
+// its column's four values of the sum.
+//
+// A block of four waves takes a row tile and 256 columns, the waves 2 x 2 with
+// 128 rows x 128 columns each (smaller shapes below): per 64 values of the sum
+// an operand byte in LDS is then read by two waves, where eight waves of half
+// the size would read it by four, and LDS bandwidth is what such a block runs
+// out of first. The weights are the products' first operand, so that a lane
+// ends with four neighbouring columns of a row of dx.
+//
+// Per chunk of 64 values the block holds the tile's gradient rows (copied from
+// memory straight into a ring of three LDS stages, two chunks ahead) and its
+// weights (loaded three chunks ahead into registers, dequantised into two LDS
+// buffers between the matrix steps of the chunk before). One barrier a chunk.
+constexpr int kGK = 64;  // values of the sum per chunk
+
+template <int MI_, int WM_, int WN_, int NJ_>
+struct GradShape {  // 32-row tiles a wave, waves along rows, along columns, 32-column tiles a wave
+  static constexpr int MI = MI_, WM = WM_, WN = WN_, NJ = NJ_;
+  static constexpr int NT = 64 * WM * WN, MR = 32 * MI * WM, NC = 32 * NJ * WN;
+  static constexpr int UN = NC / 32;              // units of a weight row
+  static constexpr int AI = MR * 8 / NT;          // 16-byte copies per thread and chunk
+  static constexpr int BI = kGK * UN / NT;        // units per thread and chunk
+  static constexpr int ABYTES = MR * 128, BBYTES = NC * 128;
+};
+
+struct GradLds {
+  unsigned char *a0, *a1, *a2, *b;
+};
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+template <typename XT>
+__device__ __forceinline__ f32x16_t mma16(u32x4_t a, u32x4_t b, f32x16_t c) {
+  if constexpr (__is_same(XT, bf16_t))
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// 16 bytes of zeros, which copies of values past the end of a row read.
+__device__ const uint32_t kGradZeros[4] = {0u, 0u, 0u, 0u};
+
+// Slot of 16-byte piece c of gradient row r in its 128 bytes of LDS: rows lie
+// two to a turn of the banks, so 16 rows reading one piece meet every bank once.
+__device__ __forceinline__ int grad_swz(int r) { return (r >> 1) & 7; }
+// Byte of piece s (8 columns) of unit u of weight row n: four rows that a
+// transposing read takes together differ in the unit's slot, the rows and units
+// that 16 lanes store together in the piece's.
+template <int UN>
+__device__ __forceinline__ uint32_t wt_off(int n, int u, int s) {
+  const int f = UN == 8 ? ((u >> 2) & 1) | ((n & 1) << 1) : n & 3;
+  return (uint32_t)(n * UN * 64 + ((u ^ (n & 3)) << 6) + ((s ^ f) << 4));
+}
+
+template <typename S, int BITS, typename XT>
+__device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const GradLds L, const GradTile& t, int j0) {
+  constexpr int MI = S::MI, NJ = S::NJ, UN = S::UN, AI = S::AI, BI = S::BI, NT = S::NT;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / S::WN, wn = wave % S::WN, col = lane & 31, h = lane >> 5;
+  const int N = a.N, K = a.K, CU = K >> 5, groups = CU >> a.gsh, row_words = CU * BITS;
+  const int per = (N + kGK - 1) / kGK, nchunks = a.dy2 ? 2 * per : per;
+  const bool sb_bf16 = a.sb_bf16 != 0;
+  auto stage = [&](auto st) -> unsigned char* {
+    constexpr int ST = decltype(st)::value;
+    return ST == 0 ? L.a0 : (ST == 1 ? L.a1 : L.a2);
+  };
+
+  // ---- gradient rows: thread tid copies, for i < AI, the piece that belongs in
+  // slot tid % 8 of LDS row tid / 8 + NT / 8 * i (a wave's 64 lanes write one KB)
+  const int ac = (tid & 7) ^ grad_swz(tid >> 3);
+  uint64_t arow[AI];
+#pragma unroll
+  for (int i = 0; i < AI; i++) {
+    const uint32_t pos = min(t.m0 + (uint32_t)((tid >> 3) + NT / 8 * i), t.pend - 1);
+    const uint32_t row = a.perm ? a.perm[pos] / (uint32_t)a.topk : pos;
+    arow[i] = (uint64_t)row * (uint64_t)N * 2u + (uint64_t)(16 * ac);
+  }
+  // (every row of a thread is a multiple of 16 apart from its first: one slot)
+  static_assert(NT / 8 % 16 == 0, "slots");
+  const uint64_t zeros = reinterpret_cast<uint64_t>(&kGradZeros[0]);
+  auto copy_rows = [&](int chunk, auto st) {
+    const bool second = chunk >= per;
+    const int c0 = (second ? chunk - per : chunk) * kGK;
+    const uint64_t base = reinterpret_cast<uint64_t>(second ? a.dy2 : a.dy) + (uint64_t)(uint32_t)c0 * 2u;
+    uint32_t in = c0 + 8 * ac < N ? 0xFFFFFFFFu : 0u;
+    asm("" : "+v"(in));  // (a select of the address became a branch around each copy)
+#pragma unroll
+    for (int i = 0; i < AI; i++) {
+      const uint64_t from = base + arow[i];
+      const uint32_t lo = ((uint32_t)from & in) | ((uint32_t)zeros & ~in);
+      const uint32_t hi = ((uint32_t)(from >> 32) & in) | ((uint32_t)(zeros >> 32) & ~in);
+      const uint64_t at = (uint64_t)hi << 32 | lo;
+      unsigned char* dst = stage(st) + (NT / 8 * i + 8 * wave) * 128;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)at,
+                                       (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+    }
+  };
+
+  // ---- weights: thread tid dequantises, for i < BI, unit tid % UN of weight row
+  // tid / UN + NT / UN * i of the chunk. Columns past the end repeat the last
+  // unit (never stored), rows past it read as zeros from the views.
+  const int bu = tid % UN, ju = min((j0 >> 5) + bu, CU - 1), bn = tid / UN;
+  static_assert(NT / UN % 4 == 0, "slots");
+  struct Units {
+    uint32_t w[BI][BITS], s[BI], b[BI];
+  };
+  auto load_units = [&](int chunk, Units& u) {
+    const bool second = chunk >= per;
+    const GemvProj& p = second ? a.p1 : a.p0;
+    const size_t rows = (size_t)t.e * (size_t)N;
+    const rsrc_t wv = make_rsrc(p.w + rows * row_words, (uint32_t)N * (uint32_t)row_words * 4u);
+    const rsrc_t sv = make_rsrc(reinterpret_cast<const uint16_t*>(p.s) + rows * groups, (uint32_t)N * (uint32_t)groups * 2u);
+    const rsrc_t bv = make_rsrc(reinterpret_cast<const uint16_t*>(p.b) + rows * groups, (uint32_t)N * (uint32_t)groups * 2u);
+    const int n0 = (second ? chunk - per : chunk) * kGK + bn;
+#pragma unroll
+    for (int i = 0; i < BI; i++) {
+      const uint32_t n = (uint32_t)(n0 + NT / UN * i);
+      const uint32_t g = (n * (uint32_t)groups + (uint32_t)(ju >> a.gsh)) * 2u;
+      u.s[i] = bload16(sv, g);
+      u.b[i] = bload16(bv, g);
+      bload_unit<BITS>(wv, (n * (uint32_t)row_words + (uint32_t)(ju * BITS)) * 4u, u.w[i]);
+    }
+  };
+  auto sb_value = [&](uint32_t raw) -> float {
+    const float f = (float)__builtin_bit_cast(_Float16, (uint16_t)raw);
+    return sb_bf16 ? __uint_as_float(raw << 16) : f;
+  };
+  // values [8 q, 8 q + 8) of each unit, into buffer buf
+  auto store_quarter = [&](const Units& u, const float (&s)[BI], const float (&b)[BI], int q, int buf) {
+#pragma unroll
+    for (int i = 0; i < BI; i++) {
+      h2_t c[4];
+      quarter_codes<BITS>(u.w[i], q, c);
+      u32x4_t v;
+#pragma unroll
+      for (int p = 0; p < 4; p++) {
+        const float lo = __builtin_fmaf((float)c[p][0], s[i], b[i]), hi = __builtin_fmaf((float)c[p][1], s[i], b[i]);
+        typedef XT x2_t __attribute__((ext_vector_type(2)));
+        v[p] = __builtin_bit_cast(uint32_t, x2_t{(XT)lo, (XT)hi});
+      }
+      *reinterpret_cast<u32x4_t*>(L.b + buf * S::BBYTES + wt_off<UN>(bn + NT / UN * i, bu, q)) = v;
+    }
+  };
+  auto unit_sb = [&](const Units& u, float (&s)[BI], float (&b)[BI]) {
+#pragma unroll
+    for (int i = 0; i < BI; i++) {
+      s[i] = sb_value(u.s[i]);
+      b[i] = sb_value(u.b[i]);
+    }
+  };
+
+  f32x16_t acc[MI][NJ];
+#pragma unroll
+  for (int i = 0; i < MI; i++)
+#pragma unroll
+    for (int j = 0; j < NJ; j++) acc[i][j] = f32x16_t{};
+
+  // operands of one 16-value step: gradient rows 32 (MI wm + i) + col, and for
+  // column tile j two transposing reads, of weight rows 16 s + 8 h + 4 q + (lane %
+  // 16) / 4 (q < 2): their low two bits are the lane's, so one offset serves all
+  struct Frags {
+    u32x4_t w[NJ], d[MI];
+  };
+  const uint32_t doff = (uint32_t)(32 * MI * wm + col) * 128u;
+  const int tr = (lane & 15) >> 2;  // row of four of a transposing read
+  uint32_t woff[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; j++)
+    woff[j] = wt_off<UN>(8 * h + tr, NJ * wn + j, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (uint32_t)(lane & 1) * 8u;
+  auto read_frags = [&](auto st, int buf, int s, Frags& f) {
+    const unsigned char* Ab = stage(st);
+    const unsigned char* Bb = L.b + buf * S::BBYTES + s * (16 * UN * 64);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      typedef __attribute__((address_space(3))) s16x4_t lds_t;
+      const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(Bb + woff[j])));
+      const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(Bb + woff[j] + 4 * UN * 64)));
+      f.w[j] = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+    }
+    const uint32_t sw = (uint32_t)(((2 * s + h) ^ grad_swz(col)) << 4);
+#pragma unroll
+    for (int i = 0; i < MI; i++) f.d[i] = *reinterpret_cast<const u32x4_t*>(Ab + doff + 32 * 128 * i + sw);
+  };
+  auto mma_step = [&](const Frags& f) {
+#pragma unroll
+    for (int i = 0; i < MI; i++)
+#pragma unroll
+      for (int j = 0; j < NJ; j++) acc[i][j] = mma16<XT>(f.w[j], f.d[i], acc[i][j]);
+  };
+
+  // vector-memory instructions of a chunk's units per thread
+  constexpr int kUnitSet = BI * (2 + kUnitLoads<BITS>);
+  // Chunk c: rows in stage ST = c % 3, weights in buffer c % 2. Its first
+  // operands are read behind the barrier while the previous chunk's last matrix
+  // step (operands in registers) runs; chunk c + 2's rows go to the stage that
+  // chunk c - 1 left, chunk c + 3's units to the registers that chunk c used,
+  // and chunk c + 1's weights are dequantised between the matrix steps. Loads
+  // past the end repeat the last chunk, in bounds and unused. At the end the
+  // rows of chunk c + 1 have to be there: what was issued after them is chunk
+  // c + 2's units, this step's AI copies and chunk c + 3's units; waiting until
+  // no more than the last two are out covers them whatever the compiler merged.
+  auto chunk_step = [&](auto first, auto st, int c, Units& cu, const Units& nu, Frags& last) {
+    constexpr int ST = decltype(st)::value;
+    const int buf = c & 1;
+    Frags f0, f1;
+    read_frags(st, buf, 0, f0);
+    if constexpr (!decltype(first)::value) mma_step(last);
+    copy_rows(min(c + 2, nchunks - 1), std::integral_constant<int, (ST + 2) % 3>{});
+    __builtin_amdgcn_sched_barrier(0);
+    load_units(min(c + 3, nchunks - 1), cu);
+    __builtin_amdgcn_sched_barrier(0);
+    float s[BI], b[BI];
+    unit_sb(nu, s, b);
+    read_frags(st, buf, 1, f1);
+    mma_step(f0);
+    store_quarter(nu, s, b, 0, buf ^ 1);
+    read_frags(st, buf, 2, f0);
+    mma_step(f1);
+    store_quarter(nu, s, b, 1, buf ^ 1);
+    read_frags(st, buf, 3, last);
+    mma_step(f0);
+    store_quarter(nu, s, b, 2, buf ^ 1);
+    store_quarter(nu, s, b, 3, buf ^ 1);
+    vmcnt_wait<AI + kUnitSet>();
+    lds_barrier_copies_in_flight();
+  };
+
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  using S2 = std::integral_constant<int, 2>;
+  Units u0, u1, u2;
+  load_units(0, u0);
+  load_units(min(1, nchunks - 1), u1);
+  load_units(min(2, nchunks - 1), u2);
+  __builtin_amdgcn_sched_barrier(0);
+  copy_rows(0, S0{});
+  copy_rows(min(1, nchunks - 1), S1{});
+  __builtin_amdgcn_sched_barrier(0);
+  {
+    float s[BI], b[BI];
+    unit_sb(u0, s, b);
+#pragma unroll
+    for (int q = 0; q < 4; q++) store_quarter(u0, s, b, q, 0);
+  }
+  vmcnt_wait<0>();
+  lds_barrier_copies_in_flight();
+  Frags last;
+  chunk_step(std::true_type{}, S0{}, 0, u0, u1, last);
+  int c = 1;
+  for (; c + 3 <= nchunks; c += 3) {
+    chunk_step(std::false_type{}, S1{}, c, u1, u2, last);
+    chunk_step(std::false_type{}, S2{}, c + 1, u2, u0, last);
+    chunk_step(std::false_type{}, S0{}, c + 2, u0, u1, last);
+  }
+  if (c < nchunks) chunk_step(std::false_type{}, S1{}, c, u1, u2, last);
+  if (c + 1 < nchunks) chunk_step(std::false_type{}, S2{}, c + 1, u2, u0, last);
+  mma_step(last);
+  vmcnt_wait<0>();  // the copies past the end
+  __syncthreads();
+
+  // ---- results: lane holds row col of each 32-row tile and columns 8 (r / 4) +
+  // 4 h + r % 4 of each 32-column tile; through LDS, so that a lane stores 16
+  // bytes of a row and its neighbours the bytes beside them
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.dx);
+  const uint16_t* base = reinterpret_cast<const uint16_t*>(a.dx_in);
+  constexpr int LINE = 16 + (NJ < 2 ? 2 : NJ) * 64;  // bytes of a staged row
+  static_assert(S::WM * S::WN * 32 * LINE <= 2 * S::BBYTES, "staging");
+  unsigned char* mine = L.b + wave * (32 * LINE);
+  const int jw = j0 + 32 * NJ * wn;
+  if (!base) {
+#pragma unroll
+    for (int i = 0; i < MI; i++) {
+#pragma unroll
+      for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          typedef XT x4_t __attribute__((ext_vector_type(4)));
+          const x4_t v{(XT)acc[i][j][r], (XT)acc[i][j][r + 1], (XT)acc[i][j][r + 2], (XT)acc[i][j][r + 3]};
+          *reinterpret_cast<u32x2_t*>(mine + col * LINE + j * 64 + r * 4 + h * 8) = __builtin_bit_cast(u32x2_t, v);
+        }
+      constexpr int PIECES = NJ * 4;  // of a row
+#pragma unroll
+      for (int q = 0; q < NJ * 2; q++) {
+        const int at = 64 * q + lane, row = at / PIECES, c8 = at % PIECES;
+        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(mine + row * LINE + c8 * 16);
+        const uint32_t pos = t.m0 + (uint32_t)(32 * (MI * wm + i) + row);
+        if (pos < t.pend && jw + 8 * c8 < K)
+          *reinterpret_cast<u32x4_t*>(out + (size_t)pos * K + jw + 8 * c8) = v;
+      }
+    }
+  } else {  // added to dx_in in fp32: a 32 x 32 tile at a time
+#pragma unroll
+    for (int i = 0; i < MI; i++)
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          typedef float f32x4_t __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<f32x4_t*>(mine + col * 144 + r * 8 + h * 16) =
+              f32x4_t{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
+        }
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+          const int row = 16 * q + (lane >> 2), c8 = lane & 3;
+          float v[8], o[8];
+          Vec8<float>::load(reinterpret_cast<const float*>(mine + row * 144 + c8 * 32), v);
+          const uint32_t pos = t.m0 + (uint32_t)(32 * (MI * wm + i) + row);
+          const int jc = jw + 32 * j + 8 * c8;
+          if (pos < t.pend && jc < K) {
+            const size_t at = (size_t)pos * K + jc;
+            Vec8<XT>::load(reinterpret_cast<const XT*>(base) + at, o);
+#pragma unroll
+            for (int k = 0; k < 8; k++) o[k] += v[k];
+            Vec8<XT>::store(reinterpret_cast<XT*>(out) + at, o);
+          }
+        }
+      }
+  }
+}
+
+typedef GradShape<4, 2, 2, 4> GradTall;    // 256 rows x 256 columns
+typedef GradShape<2, 2, 2, 4> GradHalf;    // 128 rows
+typedef GradShape<2, 1, 4, 2> GradQuarter; // 64 rows
+
+template <int BITS, typename XT>
+__global__ __launch_bounds__(256) void expert_grad_tall_kernel(const ExpertGradArgs a) {
+  __shared__ __align__(16) unsigned char a0[GradTall::ABYTES], a1[GradTall::ABYTES], a2[GradTall::ABYTES];
+  __shared__ __align__(16) unsigned char b[2 * GradTall::BBYTES];
+  // (tile, column block) pairs, column blocks of a tile together, split into
+  // eight contiguous ranges, one per XCD (blocks b, b + 8, ... share an XCD)
+  const uint32_t nb = (uint32_t)((a.K + GradTall::NC - 1) / GradTall::NC);
+  const uint32_t n = grad_tiles(a.offsets, a.E, GradTall::MR) * nb, per = (n + 7u) >> 3, k = blockIdx.x >> 3;
+  const uint32_t wi = (blockIdx.x & 7u) * per + k;
+  if (k >= per || wi >= n) return;
+  GradTile t;
+  if (!grad_tile(a.offsets, a.E, GradTall::MR, wi / nb, &t)) return;
+  const int j0 = (int)(wi % nb) * GradTall::NC;
+  const GradLds L{a0, a1, a2, b};
+  const uint32_t rows = t.pend - t.m0;
+  if (rows > 128) grad_tile_mma<GradTall, BITS, XT>(a, L, t, j0);
+  else if (rows > 64) grad_tile_mma<GradHalf, BITS, XT>(a, L, t, j0);
+  else grad_tile_mma<GradQuarter, BITS, XT>(a, L, t, j0);
+}
+
+template <int BITS, typename XT>
+static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
+  const int64_t tiles = a.M / GradTall::MR + std::min(a.E, a.M), nb = (a.K + GradTall::NC - 1) / GradTall::NC;
+  hipLaunchKernelGGL((expert_grad_tall_kernel<BITS, XT>), dim3((unsigned)((tiles * nb + 7) / 8 * 8)), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
 #define MOE_CAT2(a, b) a##b
 #define MOE_CAT(a, b) MOE_CAT2(a, b)
 
-hipError_t MOE_CAT(launch_expert_grad_b, MOE_BITS)(int xdt, int sbdt, const ExpertGradArgs& a, hipStream_t st) {
-  if (xdt == DT_F32) return launch_f32<MOE_BITS, float, float>(a, st);
-  if (xdt == DT_BF16)
-    return sbdt == DT_BF16 ? launch_f32<MOE_BITS, bf16_t, bf16_t>(a, st) : launch_f32<MOE_BITS, bf16_t, f16_t>(a, st);
-  return sbdt == DT_BF16 ? launch_f32<MOE_BITS, f16_t, bf16_t>(a, st) : launch_f32<MOE_BITS, f16_t, f16_t>(a, st);
+hipError_t MOE_CAT(launch_expert_grad_b, MOE_BITS)(int xdt, int sbdt, const ExpertGradArgs& a0, hipStream_t st) {
+  if (xdt == DT_F32) return launch_f32<MOE_BITS, float, float>(a0, st);
+  ExpertGradArgs a = a0;
+  a.sb_bf16 = sbdt == DT_BF16;
+  return xdt == DT_BF16 ? launch_mma<MOE_BITS, bf16_t>(a, st) : launch_mma<MOE_BITS, f16_t>(a, st);
 }
 
 }  // namespace moe

@@ -341,6 +341,7 @@ struct ExpertGradArgs {
   void* dx;                  // [M, K]
   int M, N, K, E;
   int gsh;                   // log2(group size / 32)
+  int sb_bf16;               // 16-bit rows: scales and biases stored as bf16 (else f16)
 };
 hipError_t launch_expert_grad(int bits, int xdt, int sbdt, const ExpertGradArgs& a, hipStream_t st);
 
