@@ -8,6 +8,7 @@
 // sum runs along W's rows and the packed axis is the output's. The reference
 // only runs forward (Ops.swift:4553-5201).
 #include <algorithm>
+#include <utility>
 
 #include "gemm_units.hpp"
 
@@ -196,6 +197,12 @@ __device__ __forceinline__ uint32_t wt_off(int n, int u, int s) {
   return (uint32_t)(n * UN * 64 + ((u ^ (n & 3)) << 6) + ((s ^ f) << 4));
 }
 
+// f(0), f(1), ... with the numbers as types.
+template <typename F, int... I>
+__device__ __forceinline__ void each(F& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
 template <typename S, int BITS, typename XT>
 __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const GradLds L, const GradTile& t, int j0) {
   constexpr int MI = S::MI, NJ = S::NJ, UN = S::UN, AI = S::AI, BI = S::BI, NT = S::NT;
@@ -333,6 +340,23 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
       for (int j = 0; j < NJ; j++) acc[i][j] = mma16<XT>(f.w[j], f.d[i], acc[i][j]);
   };
 
+  // Order of a chunk's main part: after each matrix instruction its share of the
+  // vector work (kSetup for the scales, kQuarter per quarter of a unit), which
+  // the matrix cores hide; a quarter's store follows when its values are there.
+  constexpr int kSetup = 10 * BI, kQuarter = 22 * BI, kWork = kSetup + 4 * kQuarter, kSteps = 3 * MI * NJ;
+  auto weave = [&](auto seq) {
+    auto one = [&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      constexpr int done = kWork * i / kSteps, next = kWork * (i + 1) / kSteps;
+      constexpr int stored = done < kSetup ? 0 : (done - kSetup) / kQuarter, store = next < kSetup ? 0 : (next - kSetup) / kQuarter;
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if constexpr (i % (MI * NJ) < (MI * NJ + 1) / 2)  // (the next step's operands, early in this one)
+        __builtin_amdgcn_sched_group_barrier(0x100, (2 * NJ + MI + (MI * NJ + 1) / 2 - 1) / ((MI * NJ + 1) / 2), 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, next - done, 0);
+      if constexpr (store > stored) __builtin_amdgcn_sched_group_barrier(0x200, BI * (store - stored), 0);
+    };
+    each(one, seq);
+  };
   // vector-memory instructions of a chunk's units per thread
   constexpr int kUnitSet = BI * (2 + kUnitLoads<BITS>);
   // Chunk c: rows in stage ST = c % 3, weights in buffer c % 2. Its first
@@ -366,6 +390,8 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
     mma_step(f0);
     store_quarter(nu, s, b, 2, buf ^ 1);
     store_quarter(nu, s, b, 3, buf ^ 1);
+    weave(std::make_integer_sequence<int, 3 * MI * NJ>{});
+    __builtin_amdgcn_sched_barrier(0);
     vmcnt_wait<AI + kUnitSet>();
     lds_barrier_copies_in_flight();
   };
@@ -463,12 +489,12 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
   }
 }
 
-typedef GradShape<4, 2, 2, 4> GradTall;    // 256 rows x 256 columns
-typedef GradShape<2, 2, 2, 4> GradHalf;    // 128 rows
-typedef GradShape<2, 1, 4, 2> GradQuarter; // 64 rows
+typedef GradShape<4, 2, 4, 2> GradTall;    // 256 rows x 256 columns
+typedef GradShape<2, 2, 4, 2> GradHalf;    // 128 rows
+typedef GradShape<2, 1, 8, 1> GradQuarter; // 64 rows
 
 template <int BITS, typename XT>
-__global__ __launch_bounds__(256) void expert_grad_tall_kernel(const ExpertGradArgs a) {
+__global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const ExpertGradArgs a) {
   __shared__ __align__(16) unsigned char a0[GradTall::ABYTES], a1[GradTall::ABYTES], a2[GradTall::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradTall::BBYTES];
   // (tile, column block) pairs, column blocks of a tile together, split into
@@ -490,7 +516,7 @@ __global__ __launch_bounds__(256) void expert_grad_tall_kernel(const ExpertGradA
 template <int BITS, typename XT>
 static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
   const int64_t tiles = a.M / GradTall::MR + std::min(a.E, a.M), nb = (a.K + GradTall::NC - 1) / GradTall::NC;
-  hipLaunchKernelGGL((expert_grad_tall_kernel<BITS, XT>), dim3((unsigned)((tiles * nb + 7) / 8 * 8)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((expert_grad_tall_kernel<BITS, XT>), dim3((unsigned)((tiles * nb + 7) / 8 * 8)), dim3(GradTall::NT), 0, st, a);
   return hipGetLastError();
 }
 
