@@ -17,6 +17,9 @@
 #endif
 
 namespace moe {
+#ifndef FEWMEAN
+#define FEWMEAN 32
+#endif
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
@@ -513,8 +516,153 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
   else grad_tile_mma<GradQuarter, BITS, XT>(a, L, t, j0);
 }
 
+// ------------------------------------------------ 16-bit products, few rows --
+// Experts with few rows are bound by their weights' bytes, so what counts is
+// loads in flight. A block takes up to 32 rows and 128 columns; its four waves
+// share the sum (chunks of 32 values in turn) and meet at the end. A wave
+// dequantises into LDS of its own, so the loop has no barrier: LDS serves a
+// wave's stores and reads in order.
+constexpr int kFewK = 32, kFewC = 128, kFewRows = 32;
+constexpr int kFewWave = kFewK * kFewC * 2;  // a wave's weights in LDS
+constexpr int kFewLine = 64 * 4 + 16;        // a staged row of 64 fp32 columns
+
+template <int BITS, typename XT>
+__global__ __launch_bounds__(256, 3) void expert_grad_few_kernel(const ExpertGradArgs a) {
+  constexpr int kLds = 4 * kFewRows * kFewLine > 4 * kFewWave ? 4 * kFewRows * kFewLine : 4 * kFewWave;
+  __shared__ __align__(16) unsigned char lds[kLds];
+  const uint32_t nb = (uint32_t)((a.K + kFewC - 1) / kFewC);
+  const uint32_t n = grad_tiles(a.offsets, a.E, kFewRows) * nb, per = (n + 7u) >> 3, k = blockIdx.x >> 3;
+  const uint32_t wi = (blockIdx.x & 7u) * per + k;
+  if (k >= per || wi >= n) return;
+  GradTile t;
+  if (!grad_tile(a.offsets, a.E, kFewRows, wi / nb, &t)) return;
+  const int j0 = (int)(wi % nb) * kFewC, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
+  const int N = a.N, K = a.K, CU = K >> 5, groups = CU >> a.gsh, row_words = CU * BITS;
+  const int parts = (N + kFewK - 1) / kFewK, nchunks = a.dy2 ? 2 * parts : parts;
+  const bool sb_bf16 = a.sb_bf16 != 0;
+
+  const uint32_t pos = min(t.m0 + (uint32_t)col, t.pend - 1);
+  const size_t arow = (size_t)(a.perm ? a.perm[pos] / (uint32_t)a.topk : pos) * N;
+  // lane: unit lane % 4 of weight rows lane / 4 and 16 + lane / 4 of a chunk
+  const int bu = lane & 3, ju = min((j0 >> 5) + bu, CU - 1), bn = lane >> 2;
+  struct Chunk {
+    uint32_t w[2][BITS], s[2], b[2];
+    u32x4_t d[2];
+  };
+  auto load = [&](int c, Chunk& u) {
+    const bool second = c >= parts;
+    const GemvProj& p = second ? a.p1 : a.p0;
+    const size_t rows = (size_t)t.e * (size_t)N;
+    const rsrc_t wv = make_rsrc(p.w + rows * row_words, (uint32_t)N * (uint32_t)row_words * 4u);
+    const rsrc_t sv = make_rsrc(reinterpret_cast<const uint16_t*>(p.s) + rows * groups, (uint32_t)N * (uint32_t)groups * 2u);
+    const rsrc_t bv = make_rsrc(reinterpret_cast<const uint16_t*>(p.b) + rows * groups, (uint32_t)N * (uint32_t)groups * 2u);
+    const int n0 = (second ? c - parts : c) * kFewK;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const uint32_t n = (uint32_t)(n0 + bn + 16 * i), g = (n * (uint32_t)groups + (uint32_t)(ju >> a.gsh)) * 2u;
+      bload_unit<BITS>(wv, (n * (uint32_t)row_words + (uint32_t)(ju * BITS)) * 4u, u.w[i]);
+      u.s[i] = bload16(sv, g);
+      u.b[i] = bload16(bv, g);
+    }
+    const uint16_t* dy = reinterpret_cast<const uint16_t*>(second ? a.dy2 : a.dy) + arow;
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+      u.d[s] = *reinterpret_cast<const u32x4_t*>(dy + min(n0 + 16 * s + 8 * h, N - 8));
+  };
+  auto sb_value = [&](uint32_t raw) -> float {
+    const float f = (float)__builtin_bit_cast(_Float16, (uint16_t)raw);
+    return sb_bf16 ? __uint_as_float(raw << 16) : f;
+  };
+  unsigned char* mine = lds + wave * kFewWave;
+  const int tr = (lane & 15) >> 2;
+  uint32_t woff[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    woff[j] = wt_off<4>(8 * h + tr, j, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (uint32_t)(lane & 1) * 8u;
+  f32x16_t acc[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) acc[j] = f32x16_t{};
+  auto products = [&](int c, const Chunk& u) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const float s = sb_value(u.s[i]), b = sb_value(u.b[i]);
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        h2_t cd[4];
+        quarter_codes<BITS>(u.w[i], q, cd);
+        u32x4_t v;
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+          const float lo = __builtin_fmaf((float)cd[p][0], s, b), hi = __builtin_fmaf((float)cd[p][1], s, b);
+          typedef XT x2_t __attribute__((ext_vector_type(2)));
+          v[p] = __builtin_bit_cast(uint32_t, x2_t{(XT)lo, (XT)hi});
+        }
+        *reinterpret_cast<u32x4_t*>(mine + wt_off<4>(bn + 16 * i, bu, q)) = v;
+      }
+    }
+    const int n0 = (c >= parts ? c - parts : c) * kFewK;
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      // (values past the end of the row met zero weights; an infinity there must not)
+      const u32x4_t d = n0 + 16 * s + 8 * h < N ? u.d[s] : u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        typedef __attribute__((address_space(3))) s16x4_t lds_t;
+        const unsigned char* at = mine + woff[j] + s * (16 * kFewC * 2);
+        const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)at));
+        const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(at + 4 * kFewC * 2)));
+        acc[j] = mma16<XT>(u32x4_t{lo[0], lo[1], hi[0], hi[1]}, d, acc[j]);
+      }
+    }
+  };
+  Chunk u0, u1;
+  int c = wave;  // chunks wave, wave + 4, ...; loads past the end repeat the last chunk, unused
+  load(min(c, nchunks - 1), u0);
+  load(min(c + 4, nchunks - 1), u1);
+  for (; c < nchunks; c += 8) {
+    products(c, u0);
+    load(min(c + 8, nchunks - 1), u0);
+    if (c + 4 < nchunks) products(c + 4, u1);
+    load(min(c + 12, nchunks - 1), u1);
+  }
+  // ---- the waves' sums, 64 columns at a time: lane holds row col and columns 8 (r /
+  // 4) + 4 h + r % 4 of each 32; thread tid then adds row tid / 8, columns 8 (tid % 8) on
+#pragma unroll
+  for (int half = 0; half < 2; half++) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const f32x16_t& v = acc[2 * half + j];
+        *reinterpret_cast<float4*>(lds + (wave * kFewRows + col) * kFewLine + j * 128 + r * 8 + h * 16) =
+            make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
+      }
+    __syncthreads();
+    const int row = tid >> 3, jc = j0 + 64 * half + 8 * (tid & 7);
+    const uint32_t p = t.m0 + (uint32_t)row;
+    if (p < t.pend && jc < K) {
+      float v[4][8], o[8] = {};
+#pragma unroll
+      for (int w = 0; w < 4; w++)
+        Vec8<float>::load(reinterpret_cast<const float*>(lds + (w * kFewRows + row) * kFewLine + (tid & 7) * 32), v[w]);
+      const size_t at = (size_t)p * K + jc;
+      if (a.dx_in) Vec8<XT>::load(reinterpret_cast<const XT*>(a.dx_in) + at, o);
+#pragma unroll
+      for (int q = 0; q < 8; q++) o[q] += (v[0][q] + v[1][q]) + (v[2][q] + v[3][q]);
+      Vec8<XT>::store(reinterpret_cast<XT*>(a.dx) + at, o);
+    }
+  }
+}
+
 template <int BITS, typename XT>
 static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
+  if ((int64_t)a.M <= (int64_t)FEWMEAN * a.E) {
+    const int64_t tiles = a.M / kFewRows + std::min(a.E, a.M), nb = (a.K + kFewC - 1) / kFewC;
+    hipLaunchKernelGGL((expert_grad_few_kernel<BITS, XT>), dim3((unsigned)((tiles * nb + 7) / 8 * 8)), dim3(256), 0, st, a);
+    return hipGetLastError();
+  }
   const int64_t tiles = a.M / GradTall::MR + std::min(a.E, a.M), nb = (a.K + GradTall::NC - 1) / GradTall::NC;
   hipLaunchKernelGGL((expert_grad_tall_kernel<BITS, XT>), dim3((unsigned)((tiles * nb + 7) / 8 * 8)), dim3(GradTall::NT), 0, st, a);
   return hipGetLastError();
