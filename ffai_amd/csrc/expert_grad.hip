@@ -23,41 +23,65 @@ namespace moe {
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
-// Row tile number `tile` of the plan, tiles of R rows, experts ascending:
-// its expert, first sorted position and end. Every lane of a wave calls it;
-// false past the last tile. total: all tiles of the plan.
+// A block's part of the work: a tile of up to R sorted rows of one expert and a
+// block of columns. Tiles run through the experts in order and a tile's column
+// blocks (nb) lie together; the whole list is split into eight contiguous
+// ranges, one per XCD (blocks b, b + 8, ... share an XCD), whose L2 then keeps a
+// tile's rows and an expert's weights. Every wave finds it from the offsets by
+// itself: one round of loads, then sums across the lanes. (Two dependent loads per
+// 64 experts, first for the number of tiles and then for the tile, took 5 us of
+// every block's 18 with 256 experts.)
 struct GradTile {
-  uint32_t e, m0, pend;
+  uint32_t e, m0, pend;  // expert, first sorted position, end
+  int block;             // of columns
 };
-__device__ __forceinline__ uint32_t grad_tiles(const uint32_t* offsets, int E, uint32_t R) {
+constexpr int kGradMaxE = 1024;
+__device__ __forceinline__ bool grad_tile(const uint32_t* __restrict__ offsets, int E, uint32_t R, uint32_t nb, GradTile* t) {
+  constexpr int P = kGradMaxE / 64;
   const int lane = threadIdx.x & 63;
-  uint32_t sum = 0;
-  for (int e0 = 0; e0 < E; e0 += 64) {
-    const int e = e0 + lane;
-    if (e < E) sum += (offsets[e + 1] - offsets[e] + R - 1) / R;
-  }
-  return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(sum), 63);
-}
-__device__ __forceinline__ bool grad_tile(const uint32_t* offsets, int E, uint32_t R, uint32_t tile, GradTile* t) {
-  const int lane = threadIdx.x & 63;
-  uint32_t before = 0;
-  for (int e0 = 0; e0 < E; e0 += 64) {
-    const int e = e0 + lane;
-    const uint32_t lo = e < E ? offsets[e] : 0u, hi = e < E ? offsets[e + 1] : 0u;
-    const uint32_t own = (hi - lo + R - 1) / R, upto = before + wave_scan_u32(own);
-    const uint64_t past = __ballot(upto > tile);
-    if (past) {
-      const int at = __ffsll((unsigned long long)past) - 1;
-      const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)(upto - own), at);
-      const uint32_t l = (uint32_t)__builtin_amdgcn_readlane((int)lo, at);
-      t->e = (uint32_t)(e0 + at);
-      t->m0 = l + (tile - first) * R;
-      t->pend = min((uint32_t)__builtin_amdgcn_readlane((int)hi, at), t->m0 + R);
-      return true;
+  uint32_t lo[P], hi[P];
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    lo[i] = hi[i] = 0;
+    if (i * 64 < E) {
+      lo[i] = offsets[min(i * 64 + lane, E)];
+      hi[i] = offsets[min(i * 64 + lane + 1, E)];
     }
-    before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
   }
-  return false;
+  uint32_t upto[P], total = 0;  // tiles up to and with an expert's
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    upto[i] = 0;
+    if (i * 64 < E) {
+      upto[i] = total + wave_scan_u32((hi[i] - lo[i] + R - 1) / R);
+      total = (uint32_t)__builtin_amdgcn_readlane((int)upto[i], 63);
+    }
+  }
+  const uint32_t n = total * nb, per = (n + 7u) >> 3, k = blockIdx.x >> 3, w = (blockIdx.x & 7u) * per + k;
+  if (k >= per || w >= n) return false;
+  const uint32_t tile = w / nb;
+  t->block = (int)(w - tile * nb);
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < P; i++)
+    if (i * 64 < E && !found) {
+      const uint64_t past = __ballot(upto[i] > tile);
+      if (past) {
+        const int at = __ffsll((unsigned long long)past) - 1;
+        const uint32_t l = (uint32_t)__builtin_amdgcn_readlane((int)lo[i], at);
+        const uint32_t h = (uint32_t)__builtin_amdgcn_readlane((int)hi[i], at);
+        const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)upto[i], at) - (h - l + R - 1) / R;
+        t->e = (uint32_t)(i * 64 + at);
+        t->m0 = l + (tile - first) * R;
+        t->pend = min(h, t->m0 + R);
+        found = true;
+      }
+    }
+  return found;
+}
+// Blocks for the most tiles that M rows of E experts can make.
+static unsigned grad_grid(int M, int E, int R, int nb) {
+  return (unsigned)((((int64_t)M / R + std::min(E, M)) * nb + 7) / 8 * 8);
 }
 
 // ------------------------------------------------------------ fp32 products --
@@ -69,10 +93,9 @@ constexpr int kFR = 64, kFC = 64, kFK = 32;
 template <int BITS, typename XT, typename ST>
 __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradArgs a) {
   __shared__ float As[kFR][kFK + 1], Bs[kFK][kFC];
-  const uint32_t nb = (uint32_t)((a.K + kFC - 1) / kFC);
   GradTile t;
-  if (!grad_tile(a.offsets, a.E, kFR, blockIdx.x / nb, &t)) return;
-  const int j0 = (int)(blockIdx.x % nb) * kFC, tid = threadIdx.x;
+  if (!grad_tile(a.offsets, a.E, kFR, (uint32_t)((a.K + kFC - 1) / kFC), &t)) return;
+  const int j0 = t.block * kFC, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int col = lane & 31, half = lane >> 5;
   const int words = a.K / 32 * BITS, groups = a.K / 32 >> a.gsh;
@@ -129,8 +152,8 @@ __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradAr
 
 template <int BITS, typename XT, typename ST>
 static hipError_t launch_f32(const ExpertGradArgs& a, hipStream_t st) {
-  const int64_t tiles = a.M / kFR + std::min(a.E, a.M), nb = (a.K + kFC - 1) / kFC;
-  hipLaunchKernelGGL((expert_grad_f32_kernel<BITS, XT, ST>), dim3((unsigned)(tiles * nb)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((expert_grad_f32_kernel<BITS, XT, ST>), dim3(grad_grid(a.M, a.E, kFR, (a.K + kFC - 1) / kFC)), dim3(256), 0,
+                     st, a);
   return hipGetLastError();
 }
 
@@ -196,9 +219,69 @@ __device__ __forceinline__ int grad_swz(int r) { return (r >> 1) & 7; }
 // that 16 lanes store together in the piece's.
 template <int UN>
 __device__ __forceinline__ uint32_t wt_off(int n, int u, int s) {
-  const int f = UN == 8 ? ((u >> 2) & 1) | ((n & 1) << 1) : n & 3;
+  const int f = (u ^ (u >> 2)) & 3;
   return (uint32_t)(n * UN * 64 + ((u ^ (n & 3)) << 6) + ((s ^ f) << 4));
 }
+
+// Codes 8 q ... 8 q + 7 of a unit, two to a register in the low bits of its
+// halves: code v in pr[code_reg(v)], half code_half(v). As f16 such a half is the
+// subnormal code * 2^-24, exactly, so one mixed fma with the scale * 2^24 gives
+// scale * code + bias in fp32 without a conversion.
+template <int BITS> constexpr int code_reg(int v) { return BITS == 4 ? v & 3 : v >> 1; }
+template <int BITS> constexpr int code_half(int v) { return BITS == 4 ? v >> 2 : v & 1; }
+template <int BITS>
+__device__ __forceinline__ void code_pairs(const uint32_t (&w)[BITS], int q, uint32_t (&pr)[4]) {
+  constexpr uint32_t kPair = ((1u << BITS) - 1u) * 0x10001u;
+  if constexpr (BITS == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) pr[i] = (w[q] >> (4 * i)) & kPair;
+  } else if constexpr (BITS == 8) {
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+      const uint32_t lo = 2 * (p & 1);
+      pr[p] = __builtin_amdgcn_perm(0u, w[2 * q + (p >> 1)], lo | 0x0C00u | ((lo + 1) << 16) | 0x0C000000u);
+    }
+  } else if constexpr (BITS <= 3) {
+    // four codes a, b, c, d of a field y: y | y << (16 - BITS) has a at bit 0, b at 16,
+    // c at 2 BITS and d at 16 + 2 BITS
+#pragma unroll
+    for (int f = 0; f < 2; f++) {
+      const int bit = (2 * q + f) * 4 * BITS, lo = bit >> 5, sh = bit & 31;
+      uint32_t y = sh + 4 * BITS <= 32 ? w[lo] >> sh : __builtin_amdgcn_alignbit(w[lo + 1 < BITS ? lo + 1 : lo], w[lo], (uint32_t)sh);
+      y &= (1u << (4 * BITS)) - 1u;
+      const uint32_t m = y | (y << (16 - BITS));
+      pr[2 * f] = m & kPair;
+      pr[2 * f + 1] = (m >> (2 * BITS)) & kPair;
+    }
+  } else {  // 5 and 6 bits: the 16 bits from a pair's first byte in both halves, each shifted to its code
+    typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+      const int bit = (8 * q + 2 * p) * BITS, byte = bit >> 3, o = bit & 7;
+      const int wi = byte >> 2, bw = byte & 3, wj = wi + 1 < BITS ? wi + 1 : BITS - 1;
+      const uint32_t both = (uint32_t)bw | ((uint32_t)(bw + 1) << 8);
+      const u16x2_t z = __builtin_bit_cast(u16x2_t, __builtin_amdgcn_perm(w[wj], w[wi], both * 0x10001u));
+      const u16x2_t t = z >> u16x2_t{(unsigned short)o, (unsigned short)(o + BITS)};
+      pr[p] = __builtin_bit_cast(uint32_t, t) & kPair;
+    }
+  }
+}
+
+// Columns 8 q ... 8 q + 7 of a unit as weights in XT; s: the scale * 2^24.
+template <int BITS, typename XT>
+__device__ __forceinline__ u32x4_t weights8(const uint32_t (&w)[BITS], int q, float s, float b) {
+  uint32_t pr[4];
+  code_pairs<BITS>(w, q, pr);
+  typedef XT x2_t __attribute__((ext_vector_type(2)));
+  auto weight = [&](int v) {
+    return __builtin_fmaf((float)__builtin_bit_cast(h2_t, pr[code_reg<BITS>(v)])[code_half<BITS>(v)], s, b);
+  };
+  u32x4_t o;
+#pragma unroll
+  for (int p = 0; p < 4; p++) o[p] = __builtin_bit_cast(uint32_t, x2_t{(XT)weight(2 * p), (XT)weight(2 * p + 1)});
+  return o;
+}
+constexpr float kCodeScale = 16777216.0f;  // 2^24
 
 // f(0), f(1), ... with the numbers as types.
 template <typename F, int... I>
@@ -284,22 +367,13 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
   auto store_quarter = [&](const Units& u, const float (&s)[BI], const float (&b)[BI], int q, int buf) {
 #pragma unroll
     for (int i = 0; i < BI; i++) {
-      h2_t c[4];
-      quarter_codes<BITS>(u.w[i], q, c);
-      u32x4_t v;
-#pragma unroll
-      for (int p = 0; p < 4; p++) {
-        const float lo = __builtin_fmaf((float)c[p][0], s[i], b[i]), hi = __builtin_fmaf((float)c[p][1], s[i], b[i]);
-        typedef XT x2_t __attribute__((ext_vector_type(2)));
-        v[p] = __builtin_bit_cast(uint32_t, x2_t{(XT)lo, (XT)hi});
-      }
-      *reinterpret_cast<u32x4_t*>(L.b + buf * S::BBYTES + wt_off<UN>(bn + NT / UN * i, bu, q)) = v;
+      *reinterpret_cast<u32x4_t*>(L.b + buf * S::BBYTES + wt_off<UN>(bn + NT / UN * i, bu, q)) = weights8<BITS, XT>(u.w[i], q, s[i], b[i]);
     }
   };
   auto unit_sb = [&](const Units& u, float (&s)[BI], float (&b)[BI]) {
 #pragma unroll
     for (int i = 0; i < BI; i++) {
-      s[i] = sb_value(u.s[i]);
+      s[i] = sb_value(u.s[i]) * kCodeScale;
       b[i] = sb_value(u.b[i]);
     }
   };
@@ -500,15 +574,9 @@ template <int BITS, typename XT>
 __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const ExpertGradArgs a) {
   __shared__ __align__(16) unsigned char a0[GradTall::ABYTES], a1[GradTall::ABYTES], a2[GradTall::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradTall::BBYTES];
-  // (tile, column block) pairs, column blocks of a tile together, split into
-  // eight contiguous ranges, one per XCD (blocks b, b + 8, ... share an XCD)
-  const uint32_t nb = (uint32_t)((a.K + GradTall::NC - 1) / GradTall::NC);
-  const uint32_t n = grad_tiles(a.offsets, a.E, GradTall::MR) * nb, per = (n + 7u) >> 3, k = blockIdx.x >> 3;
-  const uint32_t wi = (blockIdx.x & 7u) * per + k;
-  if (k >= per || wi >= n) return;
   GradTile t;
-  if (!grad_tile(a.offsets, a.E, GradTall::MR, wi / nb, &t)) return;
-  const int j0 = (int)(wi % nb) * GradTall::NC;
+  if (!grad_tile(a.offsets, a.E, GradTall::MR, (uint32_t)((a.K + GradTall::NC - 1) / GradTall::NC), &t)) return;
+  const int j0 = t.block * GradTall::NC;
   const GradLds L{a0, a1, a2, b};
   const uint32_t rows = t.pend - t.m0;
   if (rows > 128) grad_tile_mma<GradTall, BITS, XT>(a, L, t, j0);
@@ -530,13 +598,9 @@ template <int BITS, typename XT>
 __global__ __launch_bounds__(256, 3) void expert_grad_few_kernel(const ExpertGradArgs a) {
   constexpr int kLds = 4 * kFewRows * kFewLine > 4 * kFewWave ? 4 * kFewRows * kFewLine : 4 * kFewWave;
   __shared__ __align__(16) unsigned char lds[kLds];
-  const uint32_t nb = (uint32_t)((a.K + kFewC - 1) / kFewC);
-  const uint32_t n = grad_tiles(a.offsets, a.E, kFewRows) * nb, per = (n + 7u) >> 3, k = blockIdx.x >> 3;
-  const uint32_t wi = (blockIdx.x & 7u) * per + k;
-  if (k >= per || wi >= n) return;
   GradTile t;
-  if (!grad_tile(a.offsets, a.E, kFewRows, wi / nb, &t)) return;
-  const int j0 = (int)(wi % nb) * kFewC, tid = threadIdx.x, lane = tid & 63;
+  if (!grad_tile(a.offsets, a.E, kFewRows, (uint32_t)((a.K + kFewC - 1) / kFewC), &t)) return;
+  const int j0 = t.block * kFewC, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
   const int N = a.N, K = a.K, CU = K >> 5, groups = CU >> a.gsh, row_words = CU * BITS;
   const int parts = (N + kFewK - 1) / kFewK, nchunks = a.dy2 ? 2 * parts : parts;
@@ -586,20 +650,10 @@ __global__ __launch_bounds__(256, 3) void expert_grad_few_kernel(const ExpertGra
   auto products = [&](int c, const Chunk& u) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const float s = sb_value(u.s[i]), b = sb_value(u.b[i]);
+      const float s = sb_value(u.s[i]) * kCodeScale, b = sb_value(u.b[i]);
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
-        h2_t cd[4];
-        quarter_codes<BITS>(u.w[i], q, cd);
-        u32x4_t v;
-#pragma unroll
-        for (int p = 0; p < 4; p++) {
-          const float lo = __builtin_fmaf((float)cd[p][0], s, b), hi = __builtin_fmaf((float)cd[p][1], s, b);
-          typedef XT x2_t __attribute__((ext_vector_type(2)));
-          v[p] = __builtin_bit_cast(uint32_t, x2_t{(XT)lo, (XT)hi});
-        }
-        *reinterpret_cast<u32x4_t*>(mine + wt_off<4>(bn + 16 * i, bu, q)) = v;
-      }
+      for (int q = 0; q < 4; q++)
+        *reinterpret_cast<u32x4_t*>(mine + wt_off<4>(bn + 16 * i, bu, q)) = weights8<BITS, XT>(u.w[i], q, s, b);
     }
     const int n0 = (c >= parts ? c - parts : c) * kFewK;
 #pragma unroll
@@ -619,13 +673,20 @@ __global__ __launch_bounds__(256, 3) void expert_grad_few_kernel(const ExpertGra
   Chunk u0, u1;
   int c = wave;  // chunks wave, wave + 4, ...; loads past the end repeat the last chunk, unused
   load(min(c, nchunks - 1), u0);
+  __builtin_amdgcn_sched_barrier(0);
   load(min(c + 4, nchunks - 1), u1);
-  for (; c < nchunks; c += 8) {
+  __builtin_amdgcn_sched_barrier(0);
+  for (; c + 4 < nchunks; c += 8) {
     products(c, u0);
+    __builtin_amdgcn_sched_barrier(0);  // (loads sink to their uses otherwise)
     load(min(c + 8, nchunks - 1), u0);
-    if (c + 4 < nchunks) products(c + 4, u1);
+    __builtin_amdgcn_sched_barrier(0);
+    products(c + 4, u1);
+    __builtin_amdgcn_sched_barrier(0);
     load(min(c + 12, nchunks - 1), u1);
+    __builtin_amdgcn_sched_barrier(0);
   }
+  if (c < nchunks) products(c, u0);
   // ---- the waves' sums, 64 columns at a time: lane holds row col and columns 8 (r /
   // 4) + 4 h + r % 4 of each 32; thread tid then adds row tid / 8, columns 8 (tid % 8) on
 #pragma unroll
@@ -659,12 +720,12 @@ __global__ __launch_bounds__(256, 3) void expert_grad_few_kernel(const ExpertGra
 template <int BITS, typename XT>
 static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
   if ((int64_t)a.M <= (int64_t)FEWMEAN * a.E) {
-    const int64_t tiles = a.M / kFewRows + std::min(a.E, a.M), nb = (a.K + kFewC - 1) / kFewC;
-    hipLaunchKernelGGL((expert_grad_few_kernel<BITS, XT>), dim3((unsigned)((tiles * nb + 7) / 8 * 8)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((expert_grad_few_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, kFewRows, (a.K + kFewC - 1) / kFewC)), dim3(256), 0,
+                       st, a);
     return hipGetLastError();
   }
-  const int64_t tiles = a.M / GradTall::MR + std::min(a.E, a.M), nb = (a.K + GradTall::NC - 1) / GradTall::NC;
-  hipLaunchKernelGGL((expert_grad_tall_kernel<BITS, XT>), dim3((unsigned)((tiles * nb + 7) / 8 * 8)), dim3(GradTall::NT), 0, st, a);
+  hipLaunchKernelGGL((expert_grad_tall_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, GradTall::MR, (a.K + GradTall::NC - 1) / GradTall::NC)),
+                     dim3(GradTall::NT), 0, st, a);
   return hipGetLastError();
 }
 
