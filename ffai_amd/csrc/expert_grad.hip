@@ -17,26 +17,34 @@
 #endif
 
 namespace moe {
+#ifndef MIDMEAN
+#define MIDMEAN 128
+#endif
 #ifndef FEWMEAN
-#define FEWMEAN 32
+#define FEWMEAN 20
 #endif
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 // A block's part of the work: a tile of up to R sorted rows of one expert and a
-// block of columns. Tiles run through the experts in order and a tile's column
-// blocks (nb) lie together; the whole list is split into eight contiguous
-// ranges, one per XCD (blocks b, b + 8, ... share an XCD), whose L2 then keeps a
-// tile's rows and an expert's weights. Every wave finds it from the offsets by
-// itself: one round of loads, then sums across the lanes. (Two dependent loads per
-// 64 experts, first for the number of tiles and then for the tile, took 5 us of
-// every block's 18 with 256 experts.)
+// block of columns. Every wave finds it from the offsets by itself: one round of
+// loads, then sums across the lanes.
+//
+// In order (BY_SIZE false) tiles run through the experts, a tile's column blocks
+// (nb) together, the whole list in eight contiguous ranges, one per XCD (blocks b, b
+// + 8, ... share an XCD), whose L2 then keeps a tile's rows and an expert's
+// weights. BY_SIZE, for blocks of many us: whole tiles first, then the experts'
+// remainders of more than R / 2 rows, then the others, so that the last to start
+// are the short ones; tile t and its column blocks belong to XCD t % 8. Experts of
+// unequal popularity, 64 rows on average: 126 us in order, 114 by size; with tiles
+// of 32 rows 110 and 114, since an expert's tiles then share no XCD.
 struct GradTile {
   uint32_t e, m0, pend;  // expert, first sorted position, end
   int block;             // of columns
 };
 constexpr int kGradMaxE = 1024;
-__device__ __forceinline__ bool grad_tile(const uint32_t* __restrict__ offsets, int E, uint32_t R, uint32_t nb, GradTile* t) {
+template <uint32_t R, bool BY_SIZE>
+__device__ __forceinline__ bool grad_tile(const uint32_t* __restrict__ offsets, int E, uint32_t nb, GradTile* t) {
   constexpr int P = kGradMaxE / 64;
   const int lane = threadIdx.x & 63;
   uint32_t lo[P], hi[P];
@@ -48,31 +56,50 @@ __device__ __forceinline__ bool grad_tile(const uint32_t* __restrict__ offsets, 
       hi[i] = offsets[min(i * 64 + lane + 1, E)];
     }
   }
-  uint32_t upto[P], total = 0;  // tiles up to and with an expert's
+  // whole tiles and remainders up to and with an expert's (remainders: long ones
+  // in the low half, short ones in the high half, 1024 at most)
+  uint32_t whole[P], rest[P], wholes = 0, rests = 0;
 #pragma unroll
   for (int i = 0; i < P; i++) {
-    upto[i] = 0;
+    whole[i] = rest[i] = 0;
     if (i * 64 < E) {
-      upto[i] = total + wave_scan_u32((hi[i] - lo[i] + R - 1) / R);
-      total = (uint32_t)__builtin_amdgcn_readlane((int)upto[i], 63);
+      const uint32_t c = hi[i] - lo[i], r = c % R;
+      whole[i] = wholes + wave_scan_u32(BY_SIZE ? c / R : (c + R - 1) / R);
+      wholes = (uint32_t)__builtin_amdgcn_readlane((int)whole[i], 63);
+      if constexpr (BY_SIZE) {
+        rest[i] = rests + wave_scan_u32(r > R / 2 ? 1u : (r ? 0x10000u : 0u));
+        rests = (uint32_t)__builtin_amdgcn_readlane((int)rest[i], 63);
+      }
     }
   }
-  const uint32_t n = total * nb, per = (n + 7u) >> 3, k = blockIdx.x >> 3, w = (blockIdx.x & 7u) * per + k;
-  if (k >= per || w >= n) return false;
-  const uint32_t tile = w / nb;
-  t->block = (int)(w - tile * nb);
+  const uint32_t k = blockIdx.x >> 3, longs = rests & 0xFFFFu;
+  uint32_t tile;
+  if constexpr (BY_SIZE) {
+    tile = (blockIdx.x & 7u) + 8u * (k / nb);
+    t->block = (int)(k % nb);
+    if (tile >= wholes + longs + (rests >> 16)) return false;
+  } else {
+    const uint32_t per = (wholes * nb + 7u) >> 3, w = (blockIdx.x & 7u) * per + k;
+    tile = w / nb;
+    t->block = (int)(w - tile * nb);
+    if (k >= per || tile >= wholes) return false;
+  }
+  const int kind = tile < wholes ? 0 : (tile < wholes + longs ? 1 : 2);
+  tile -= kind == 0 ? 0u : (kind == 1 ? wholes : wholes + longs);
   bool found = false;
 #pragma unroll
   for (int i = 0; i < P; i++)
     if (i * 64 < E && !found) {
-      const uint64_t past = __ballot(upto[i] > tile);
+      const uint32_t upto = kind == 0 ? whole[i] : (kind == 1 ? rest[i] & 0xFFFFu : rest[i] >> 16);
+      const uint64_t past = __ballot(upto > tile);
       if (past) {
         const int at = __ffsll((unsigned long long)past) - 1;
         const uint32_t l = (uint32_t)__builtin_amdgcn_readlane((int)lo[i], at);
         const uint32_t h = (uint32_t)__builtin_amdgcn_readlane((int)hi[i], at);
-        const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)upto[i], at) - (h - l + R - 1) / R;
+        const uint32_t n = BY_SIZE ? (h - l) / R : (h - l + R - 1) / R;
+        const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)upto, at) - n;
         t->e = (uint32_t)(i * 64 + at);
-        t->m0 = l + (tile - first) * R;
+        t->m0 = l + (kind ? n : tile - first) * R;
         t->pend = min(h, t->m0 + R);
         found = true;
       }
@@ -81,7 +108,7 @@ __device__ __forceinline__ bool grad_tile(const uint32_t* __restrict__ offsets, 
 }
 // Blocks for the most tiles that M rows of E experts can make.
 static unsigned grad_grid(int M, int E, int R, int nb) {
-  return (unsigned)((((int64_t)M / R + std::min(E, M)) * nb + 7) / 8 * 8);
+  return (unsigned)(((int64_t)M / R + std::min(E, M) + 7) / 8 * nb * 8);
 }
 
 // ------------------------------------------------------------ fp32 products --
@@ -94,7 +121,7 @@ template <int BITS, typename XT, typename ST>
 __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradArgs a) {
   __shared__ float As[kFR][kFK + 1], Bs[kFK][kFC];
   GradTile t;
-  if (!grad_tile(a.offsets, a.E, kFR, (uint32_t)((a.K + kFC - 1) / kFC), &t)) return;
+  if (!grad_tile<kFR, false>(a.offsets, a.E, (uint32_t)((a.K + kFC - 1) / kFC), &t)) return;
   const int j0 = t.block * kFC, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int col = lane & 31, half = lane >> 5;
@@ -567,6 +594,7 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
 }
 
 typedef GradShape<4, 2, 4, 2> GradTall;    // 256 rows x 256 columns
+typedef GradShape<3, 2, 4, 2> GradMost;    // 192 rows
 typedef GradShape<2, 2, 4, 2> GradHalf;    // 128 rows
 typedef GradShape<2, 1, 8, 1> GradQuarter; // 64 rows
 
@@ -575,11 +603,12 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
   __shared__ __align__(16) unsigned char a0[GradTall::ABYTES], a1[GradTall::ABYTES], a2[GradTall::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradTall::BBYTES];
   GradTile t;
-  if (!grad_tile(a.offsets, a.E, GradTall::MR, (uint32_t)((a.K + GradTall::NC - 1) / GradTall::NC), &t)) return;
+  if (!grad_tile<GradTall::MR, true>(a.offsets, a.E, (uint32_t)((a.K + GradTall::NC - 1) / GradTall::NC), &t)) return;
   const int j0 = t.block * GradTall::NC;
   const GradLds L{a0, a1, a2, b};
   const uint32_t rows = t.pend - t.m0;
-  if (rows > 128) grad_tile_mma<GradTall, BITS, XT>(a, L, t, j0);
+  if (rows > 192) grad_tile_mma<GradTall, BITS, XT>(a, L, t, j0);
+  else if (rows > 128) grad_tile_mma<GradMost, BITS, XT>(a, L, t, j0);
   else if (rows > 64) grad_tile_mma<GradHalf, BITS, XT>(a, L, t, j0);
   else grad_tile_mma<GradQuarter, BITS, XT>(a, L, t, j0);
 }
@@ -599,7 +628,7 @@ __global__ __launch_bounds__(256, 3) void expert_grad_few_kernel(const ExpertGra
   constexpr int kLds = 4 * kFewRows * kFewLine > 4 * kFewWave ? 4 * kFewRows * kFewLine : 4 * kFewWave;
   __shared__ __align__(16) unsigned char lds[kLds];
   GradTile t;
-  if (!grad_tile(a.offsets, a.E, kFewRows, (uint32_t)((a.K + kFewC - 1) / kFewC), &t)) return;
+  if (!grad_tile<kFewRows, false>(a.offsets, a.E, (uint32_t)((a.K + kFewC - 1) / kFewC), &t)) return;
   const int j0 = t.block * kFewC, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
   const int N = a.N, K = a.K, CU = K >> 5, groups = CU >> a.gsh, row_words = CU * BITS;
@@ -717,11 +746,34 @@ __global__ __launch_bounds__(256, 3) void expert_grad_few_kernel(const ExpertGra
   }
 }
 
+typedef GradShape<4, 1, 4, 1> GradMid;  // 128 rows x 128 columns
+typedef GradShape<2, 1, 4, 1> GradMidHalf;
+typedef GradShape<1, 1, 4, 1> GradMidQuarter;
+
+template <int BITS, typename XT>
+__global__ __launch_bounds__(GradMid::NT, 2) void expert_grad_mid_kernel(const ExpertGradArgs a) {
+  __shared__ __align__(16) unsigned char a0[GradMid::ABYTES], a1[GradMid::ABYTES], a2[GradMid::ABYTES];
+  __shared__ __align__(16) unsigned char b[2 * GradMid::BBYTES];
+  GradTile t;
+  if (!grad_tile<GradMid::MR, true>(a.offsets, a.E, (uint32_t)((a.K + GradMid::NC - 1) / GradMid::NC), &t)) return;
+  const int j0 = t.block * GradMid::NC;
+  const GradLds L{a0, a1, a2, b};
+  const uint32_t rows = t.pend - t.m0;
+  if (rows > 64) grad_tile_mma<GradMid, BITS, XT>(a, L, t, j0);
+  else if (rows > 32) grad_tile_mma<GradMidHalf, BITS, XT>(a, L, t, j0);
+  else grad_tile_mma<GradMidQuarter, BITS, XT>(a, L, t, j0);
+}
+
 template <int BITS, typename XT>
 static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
   if ((int64_t)a.M <= (int64_t)FEWMEAN * a.E) {
     hipLaunchKernelGGL((expert_grad_few_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, kFewRows, (a.K + kFewC - 1) / kFewC)), dim3(256), 0,
                        st, a);
+    return hipGetLastError();
+  }
+  if ((int64_t)a.M <= (int64_t)MIDMEAN * a.E) {
+    hipLaunchKernelGGL((expert_grad_mid_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, GradMid::MR, (a.K + GradMid::NC - 1) / GradMid::NC)),
+                       dim3(GradMid::NT), 0, st, a);
     return hipGetLastError();
   }
   hipLaunchKernelGGL((expert_grad_tall_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, GradTall::MR, (a.K + GradTall::NC - 1) / GradTall::NC)),
