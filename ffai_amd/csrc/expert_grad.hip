@@ -17,12 +17,6 @@
 #endif
 
 namespace moe {
-#ifndef MIDMEAN
-#define MIDMEAN 128
-#endif
-#ifndef FEWMEAN
-#define FEWMEAN 20
-#endif
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
@@ -112,75 +106,83 @@ static unsigned grad_grid(int M, int E, int R, int nb) {
 }
 
 // ------------------------------------------------------------ fp32 products --
-// A block takes 64 rows and 64 columns, a wave a 32 x 32 quarter; 32 values of
-// the sum at a time go through LDS in fp32 (the gradient's rows as they are,
-// the weights dequantised, which keeps the packed axis across the lanes).
+// fp32 rows: a block takes 64 rows and 64 columns, a wave a 32 x 32 quarter on
+// v_mfma_f32_32x32x2; 32 values of the sum at a time go through two LDS buffers
+// (the gradient's rows as they are, the weights dequantised, which keeps the
+// packed axis across the lanes), loaded while the chunk before is multiplied.
 constexpr int kFR = 64, kFC = 64, kFK = 32;
 
-template <int BITS, typename XT, typename ST>
+template <int BITS>
 __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradArgs a) {
-  __shared__ float As[kFR][kFK + 1], Bs[kFK][kFC];
+  __shared__ float As[2][kFR][kFK + 1], Bs[2][kFK][kFC];
   GradTile t;
   if (!grad_tile<kFR, false>(a.offsets, a.E, (uint32_t)((a.K + kFC - 1) / kFC), &t)) return;
   const int j0 = t.block * kFC, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int col = lane & 31, half = lane >> 5;
   const int words = a.K / 32 * BITS, groups = a.K / 32 >> a.gsh;
-  f32x16_t acc = {};
-  for (int part = 0; part < (a.dy2 ? 2 : 1); part++) {
-    const GemvProj& p = part ? a.p1 : a.p0;
-    const XT* dy = (const XT*)(part ? a.dy2 : a.dy);
-    const uint32_t* W = p.w + (size_t)t.e * a.N * words;
-    const ST* S = (const ST*)p.s + (size_t)t.e * a.N * groups;
-    const ST* B = (const ST*)p.b + (size_t)t.e * a.N * groups;
-    // thread: a quarter of a gradient row's chunk, eight columns of a weight row
-    const uint32_t pos = min(t.m0 + (uint32_t)(tid >> 2), t.pend - 1);
-    const size_t arow = a.perm ? a.perm[pos] / (uint32_t)a.topk : pos;
-    const int ac = (tid & 3) * 8, bi = tid >> 3, bj = j0 + (tid & 7) * 8;
-    for (int i0 = 0; i0 < a.N; i0 += kFK) {
-      float av[8] = {}, bv[8] = {};
-      if (i0 + ac < a.N) Vec8<XT>::load(dy + arow * a.N + i0 + ac, av);
-      const int i = i0 + bi;
-      if (i < a.N && bj < a.K) {
-        const uint32_t* row = W + (size_t)i * words;
-        const size_t g = (size_t)i * groups + (bj / 32 >> a.gsh);
-        const float s = to_f<ST>(S[g]), b = to_f<ST>(B[g]);
+  const int parts = (a.N + kFK - 1) / kFK, nchunks = a.dy2 ? 2 * parts : parts;
+  // thread: a quarter of a gradient row's chunk, eight columns of a weight row (they
+  // lie in two words, from bit `sh` of the first)
+  const uint32_t pos = min(t.m0 + (uint32_t)(tid >> 2), t.pend - 1);
+  const size_t arow = (size_t)(a.perm ? a.perm[pos] / (uint32_t)a.topk : pos) * a.N;
+  const int ac = (tid & 3) * 8, bi = tid >> 3, bj = min(j0 + (tid & 7) * 8, a.K - 8);
+  const uint32_t bit = (uint32_t)bj * BITS, lo = bit >> 5, sh = bit & 31;
+  struct Part {
+    float d[8], s, b;
+    uint32_t w0, w1;
+  };
+  auto load = [&](int c, Part& u) {
+    const bool second = c >= parts;
+    const GemvProj& p = second ? a.p1 : a.p0;
+    const int i0 = (second ? c - parts : c) * kFK, i = i0 + bi;
 #pragma unroll
-        for (int v = 0; v < 8; v++) {
-          const uint32_t bit = (uint32_t)(bj + v) * BITS, lo = bit >> 5, sh = bit & 31;
-          uint32_t q = row[lo] >> sh;
-          if (sh + BITS > 32) q |= row[lo + 1] << (32 - sh);
-          bv[v] = __builtin_fmaf(s, (float)(q & ((1u << BITS) - 1u)), b);
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int v = 0; v < 8; v++) {
-        As[tid >> 2][ac + v] = av[v];
-        Bs[bi][(tid & 7) * 8 + v] = bv[v];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kFK; k += 2)
-        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(As[32 * wm + col][k + half], Bs[k + half][32 * wn + col], acc, 0, 0, 0);
+    for (int v = 0; v < 8; v++) u.d[v] = 0.0f;
+    if (i0 + ac < a.N) Vec8<float>::load((const float*)(second ? a.dy2 : a.dy) + arow + i0 + ac, u.d);
+    u.s = u.b = 0.0f;
+    u.w0 = u.w1 = 0u;
+    if (i < a.N) {
+      const uint32_t* row = p.w + ((size_t)t.e * a.N + i) * words;
+      const size_t g = ((size_t)t.e * a.N + i) * groups + (bj / 32 >> a.gsh);
+      u.w0 = row[lo];
+      u.w1 = row[min(lo + 1, (uint32_t)words - 1)];
+      u.s = ((const float*)p.s)[g];
+      u.b = ((const float*)p.b)[g];
     }
+  };
+  f32x16_t acc = {};
+  Part u;
+  load(0, u);
+  for (int c = 0; c < nchunks; c++) {
+    const int buf = c & 1;
+    const uint64_t field = ((uint64_t)u.w1 << 32 | u.w0) >> sh;
+    float wv[8];
+#pragma unroll
+    for (int v = 0; v < 8; v++) {
+      As[buf][tid >> 2][ac + v] = u.d[v];
+      wv[v] = __builtin_fmaf(u.s, (float)((uint32_t)(field >> (BITS * v)) & ((1u << BITS) - 1u)), u.b);
+    }
+    Vec8<float>::store(&Bs[buf][bi][(tid & 7) * 8], wv);
+    if (c + 1 < nchunks) load(c + 1, u);
+    lds_barrier();
+#pragma unroll
+    for (int k = 0; k < kFK; k += 2)
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(As[buf][32 * wm + col][k + half], Bs[buf][k + half][32 * wn + col], acc, 0, 0, 0);
   }
   const int j = j0 + 32 * wn + col;
 #pragma unroll
   for (int r = 0; r < 16; r++) {
-    const uint32_t pos = t.m0 + (uint32_t)(32 * wm + 8 * (r >> 2) + 4 * half + (r & 3));
-    if (pos < t.pend && j < a.K) {
-      const size_t at = (size_t)pos * a.K + j;
-      const float base = a.dx_in ? to_f<XT>(((const XT*)a.dx_in)[at]) : 0.0f;
-      ((XT*)a.dx)[at] = from_f<XT>(base + acc[r]);
+    const uint32_t p = t.m0 + (uint32_t)(32 * wm + 8 * (r >> 2) + 4 * half + (r & 3));
+    if (p < t.pend && j < a.K) {
+      const size_t at = (size_t)p * a.K + j;
+      ((float*)a.dx)[at] = (a.dx_in ? ((const float*)a.dx_in)[at] : 0.0f) + acc[r];
     }
   }
 }
 
-template <int BITS, typename XT, typename ST>
+template <int BITS>
 static hipError_t launch_f32(const ExpertGradArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((expert_grad_f32_kernel<BITS, XT, ST>), dim3(grad_grid(a.M, a.E, kFR, (a.K + kFC - 1) / kFC)), dim3(256), 0,
-                     st, a);
+  hipLaunchKernelGGL((expert_grad_f32_kernel<BITS>), dim3(grad_grid(a.M, a.E, kFR, (a.K + kFC - 1) / kFC)), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
@@ -614,34 +616,36 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
 }
 
 // ------------------------------------------------ 16-bit products, few rows --
-// Experts with few rows are bound by their weights' bytes, so what counts is
-// loads in flight. A block takes up to 32 rows and 128 columns; its four waves
-// share the sum (chunks of 32 values in turn) and meet at the end. A wave
-// dequantises into LDS of its own, so the loop has no barrier: LDS serves a
-// wave's stores and reads in order.
-constexpr int kFewK = 32, kFewC = 128, kFewRows = 32;
-constexpr int kFewWave = kFewK * kFewC * 2;  // a wave's weights in LDS
-constexpr int kFewLine = 64 * 4 + 16;        // a staged row of 64 fp32 columns
+// Experts with few rows are bound by how fast their weights arrive. A block takes
+// up to 32 rows and 32 NJ columns; its four waves share the sum (chunks of 128 / NJ
+// values in turn) and meet at the end. A wave dequantises into LDS of its own, so
+// the loop has no barrier: LDS serves a wave's stores and reads in order.
+// Loads cost by the rows they touch rather than by their bytes (a weight row's
+// scale and bias lie in lines of their own), so wide blocks are faster (NJ = 8, two
+// thirds of the rows per byte) where there are enough of them.
+constexpr int kFewRows = 32;
+constexpr int kFewLine = 64 * 4 + 16;  // a staged row of 64 fp32 columns
 
-template <int BITS, typename XT>
-__global__ __launch_bounds__(256, 3) void expert_grad_few_kernel(const ExpertGradArgs a) {
-  constexpr int kLds = 4 * kFewRows * kFewLine > 4 * kFewWave ? 4 * kFewRows * kFewLine : 4 * kFewWave;
+template <int NJ, int BITS, typename XT>
+__global__ __launch_bounds__(256, NJ == 8 ? 2 : 3) void expert_grad_few_kernel(const ExpertGradArgs a) {
+  constexpr int FK = 128 / NJ, FC = 32 * NJ, STEPS = FK / 16, ROWS = 64 / NJ;  // ROWS: weight rows of a unit load
+  constexpr int kWave = FK * FC * 2, kLds = 4 * (kFewRows * kFewLine > kWave ? kFewRows * kFewLine : kWave);
   __shared__ __align__(16) unsigned char lds[kLds];
   GradTile t;
-  if (!grad_tile<kFewRows, false>(a.offsets, a.E, (uint32_t)((a.K + kFewC - 1) / kFewC), &t)) return;
-  const int j0 = t.block * kFewC, tid = threadIdx.x, lane = tid & 63;
+  if (!grad_tile<kFewRows, false>(a.offsets, a.E, (uint32_t)((a.K + FC - 1) / FC), &t)) return;
+  const int j0 = t.block * FC, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
   const int N = a.N, K = a.K, CU = K >> 5, groups = CU >> a.gsh, row_words = CU * BITS;
-  const int parts = (N + kFewK - 1) / kFewK, nchunks = a.dy2 ? 2 * parts : parts;
+  const int parts = (N + FK - 1) / FK, nchunks = a.dy2 ? 2 * parts : parts;
   const bool sb_bf16 = a.sb_bf16 != 0;
 
   const uint32_t pos = min(t.m0 + (uint32_t)col, t.pend - 1);
   const size_t arow = (size_t)(a.perm ? a.perm[pos] / (uint32_t)a.topk : pos) * N;
-  // lane: unit lane % 4 of weight rows lane / 4 and 16 + lane / 4 of a chunk
-  const int bu = lane & 3, ju = min((j0 >> 5) + bu, CU - 1), bn = lane >> 2;
+  // lane: unit lane % NJ of weight rows lane / NJ and ROWS + lane / NJ of a chunk
+  const int bu = lane % NJ, ju = min((j0 >> 5) + bu, CU - 1), bn = lane / NJ;
   struct Chunk {
     uint32_t w[2][BITS], s[2], b[2];
-    u32x4_t d[2];
+    u32x4_t d[STEPS];
   };
   auto load = [&](int c, Chunk& u) {
     const bool second = c >= parts;
@@ -650,87 +654,86 @@ __global__ __launch_bounds__(256, 3) void expert_grad_few_kernel(const ExpertGra
     const rsrc_t wv = make_rsrc(p.w + rows * row_words, (uint32_t)N * (uint32_t)row_words * 4u);
     const rsrc_t sv = make_rsrc(reinterpret_cast<const uint16_t*>(p.s) + rows * groups, (uint32_t)N * (uint32_t)groups * 2u);
     const rsrc_t bv = make_rsrc(reinterpret_cast<const uint16_t*>(p.b) + rows * groups, (uint32_t)N * (uint32_t)groups * 2u);
-    const int n0 = (second ? c - parts : c) * kFewK;
+    const int n0 = (second ? c - parts : c) * FK;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const uint32_t n = (uint32_t)(n0 + bn + 16 * i), g = (n * (uint32_t)groups + (uint32_t)(ju >> a.gsh)) * 2u;
+      const uint32_t n = (uint32_t)(n0 + bn + ROWS * i), g = (n * (uint32_t)groups + (uint32_t)(ju >> a.gsh)) * 2u;
       bload_unit<BITS>(wv, (n * (uint32_t)row_words + (uint32_t)(ju * BITS)) * 4u, u.w[i]);
       u.s[i] = bload16(sv, g);
       u.b[i] = bload16(bv, g);
     }
     const uint16_t* dy = reinterpret_cast<const uint16_t*>(second ? a.dy2 : a.dy) + arow;
 #pragma unroll
-    for (int s = 0; s < 2; s++)
+    for (int s = 0; s < STEPS; s++)
       u.d[s] = *reinterpret_cast<const u32x4_t*>(dy + min(n0 + 16 * s + 8 * h, N - 8));
   };
   auto sb_value = [&](uint32_t raw) -> float {
     const float f = (float)__builtin_bit_cast(_Float16, (uint16_t)raw);
     return sb_bf16 ? __uint_as_float(raw << 16) : f;
   };
-  unsigned char* mine = lds + wave * kFewWave;
+  unsigned char* mine = lds + wave * kWave;
   const int tr = (lane & 15) >> 2;
-  uint32_t woff[4];
+  uint32_t woff[NJ];
 #pragma unroll
-  for (int j = 0; j < 4; j++)
-    woff[j] = wt_off<4>(8 * h + tr, j, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (uint32_t)(lane & 1) * 8u;
-  f32x16_t acc[4];
+  for (int j = 0; j < NJ; j++)
+    woff[j] = wt_off<NJ>(8 * h + tr, j, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (uint32_t)(lane & 1) * 8u;
+  f32x16_t acc[NJ];
 #pragma unroll
-  for (int j = 0; j < 4; j++) acc[j] = f32x16_t{};
+  for (int j = 0; j < NJ; j++) acc[j] = f32x16_t{};
   auto products = [&](int c, const Chunk& u) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       const float s = sb_value(u.s[i]) * kCodeScale, b = sb_value(u.b[i]);
 #pragma unroll
       for (int q = 0; q < 4; q++)
-        *reinterpret_cast<u32x4_t*>(mine + wt_off<4>(bn + 16 * i, bu, q)) = weights8<BITS, XT>(u.w[i], q, s, b);
+        *reinterpret_cast<u32x4_t*>(mine + wt_off<NJ>(bn + ROWS * i, bu, q)) = weights8<BITS, XT>(u.w[i], q, s, b);
     }
-    const int n0 = (c >= parts ? c - parts : c) * kFewK;
+    const int n0 = (c >= parts ? c - parts : c) * FK;
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
+    for (int s = 0; s < STEPS; s++) {
       // (values past the end of the row met zero weights; an infinity there must not)
       const u32x4_t d = n0 + 16 * s + 8 * h < N ? u.d[s] : u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
+      for (int j = 0; j < NJ; j++) {
         typedef __attribute__((address_space(3))) s16x4_t lds_t;
-        const unsigned char* at = mine + woff[j] + s * (16 * kFewC * 2);
+        const unsigned char* at = mine + woff[j] + s * (16 * FC * 2);
         const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)at));
-        const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(at + 4 * kFewC * 2)));
+        const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(at + 4 * FC * 2)));
         acc[j] = mma16<XT>(u32x4_t{lo[0], lo[1], hi[0], hi[1]}, d, acc[j]);
       }
     }
   };
   Chunk u0, u1;
   int c = wave;  // chunks wave, wave + 4, ...; loads past the end repeat the last chunk, unused
-  load(min(c, nchunks - 1), u0);
-  __builtin_amdgcn_sched_barrier(0);
-  load(min(c + 4, nchunks - 1), u1);
-  __builtin_amdgcn_sched_barrier(0);
+  auto ahead = [&](int at, Chunk& u) {
+    __builtin_amdgcn_sched_barrier(0);  // (loads sink to their uses otherwise)
+    load(min(at, nchunks - 1), u);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  ahead(c, u0);
+  ahead(c + 4, u1);
   for (; c + 4 < nchunks; c += 8) {
     products(c, u0);
-    __builtin_amdgcn_sched_barrier(0);  // (loads sink to their uses otherwise)
-    load(min(c + 8, nchunks - 1), u0);
-    __builtin_amdgcn_sched_barrier(0);
+    ahead(c + 8, u0);
     products(c + 4, u1);
-    __builtin_amdgcn_sched_barrier(0);
-    load(min(c + 12, nchunks - 1), u1);
-    __builtin_amdgcn_sched_barrier(0);
+    ahead(c + 12, u1);
   }
   if (c < nchunks) products(c, u0);
   // ---- the waves' sums, 64 columns at a time: lane holds row col and columns 8 (r /
   // 4) + 4 h + r % 4 of each 32; thread tid then adds row tid / 8, columns 8 (tid % 8) on
 #pragma unroll
-  for (int half = 0; half < 2; half++) {
+  for (int part = 0; part < NJ / 2; part++) {
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 2; j++)
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
-        const f32x16_t& v = acc[2 * half + j];
+        const f32x16_t& v = acc[2 * part + j];
         *reinterpret_cast<float4*>(lds + (wave * kFewRows + col) * kFewLine + j * 128 + r * 8 + h * 16) =
             make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
       }
     __syncthreads();
-    const int row = tid >> 3, jc = j0 + 64 * half + 8 * (tid & 7);
+    const int row = tid >> 3, jc = j0 + 64 * part + 8 * (tid & 7);
     const uint32_t p = t.m0 + (uint32_t)row;
     if (p < t.pend && jc < K) {
       float v[4][8], o[8] = {};
@@ -764,20 +767,31 @@ __global__ __launch_bounds__(GradMid::NT, 2) void expert_grad_mid_kernel(const E
   else grad_tile_mma<GradMidQuarter, BITS, XT>(a, L, t, j0);
 }
 
+// Which kernel. Few rows an expert (up to 28 on average, fewer where a weight has
+// more than 4 bits): the few-row kernel, wide where its wide blocks fill the chip
+// twice over. Else the tall kernel, unless its
+// blocks would not fill the chip; then the ordinary one. us per call of gate and up
+// 768 x 2048 at 4 bits, bf16, experts of unequal popularity, few / ordinary / tall:
+// 128 experts of 8 rows 69 / 90 / 101, of 24 97 / 94 / 96, of 64 174 / 122 / 120, of
+// 256 531 / 329 / 248; 8 experts of 256 rows 34 / 23 / 35; one of 4096 63 / 38 / 40.
+// Few rows, narrow / wide: 128 experts of 8 rows 80 / 69, 32 of one row 24 / 26, 8 of
+// one row 14 / 24.
 template <int BITS, typename XT>
 static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
-  if ((int64_t)a.M <= (int64_t)FEWMEAN * a.E) {
-    hipLaunchKernelGGL((expert_grad_few_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, kFewRows, (a.K + kFewC - 1) / kFewC)), dim3(256), 0,
+  const int64_t used = std::min(a.E, a.M);
+  auto columns = [&](int n) { return (a.K + n - 1) / n; };
+  if ((int64_t)a.M <= 28 * (int64_t)a.E && (int64_t)a.M * BITS <= 100 * (int64_t)a.E) {
+    if (used * columns(256) >= 512)
+      hipLaunchKernelGGL((expert_grad_few_kernel<8, BITS, XT>), dim3(grad_grid(a.M, a.E, kFewRows, columns(256))), dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((expert_grad_few_kernel<4, BITS, XT>), dim3(grad_grid(a.M, a.E, kFewRows, columns(128))), dim3(256), 0, st, a);
+  } else if (std::max<int64_t>(used, a.M / GradTall::MR) * columns(GradTall::NC) < 256) {
+    hipLaunchKernelGGL((expert_grad_mid_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, GradMid::MR, columns(GradMid::NC))), dim3(GradMid::NT), 0,
                        st, a);
-    return hipGetLastError();
+  } else {
+    hipLaunchKernelGGL((expert_grad_tall_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, GradTall::MR, columns(GradTall::NC))), dim3(GradTall::NT),
+                       0, st, a);
   }
-  if ((int64_t)a.M <= (int64_t)MIDMEAN * a.E) {
-    hipLaunchKernelGGL((expert_grad_mid_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, GradMid::MR, (a.K + GradMid::NC - 1) / GradMid::NC)),
-                       dim3(GradMid::NT), 0, st, a);
-    return hipGetLastError();
-  }
-  hipLaunchKernelGGL((expert_grad_tall_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, GradTall::MR, (a.K + GradTall::NC - 1) / GradTall::NC)),
-                     dim3(GradTall::NT), 0, st, a);
   return hipGetLastError();
 }
 
@@ -785,7 +799,7 @@ static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
 #define MOE_CAT(a, b) MOE_CAT2(a, b)
 
 hipError_t MOE_CAT(launch_expert_grad_b, MOE_BITS)(int xdt, int sbdt, const ExpertGradArgs& a0, hipStream_t st) {
-  if (xdt == DT_F32) return launch_f32<MOE_BITS, float, float>(a0, st);
+  if (xdt == DT_F32) return launch_f32<MOE_BITS>(a0, st);
   ExpertGradArgs a = a0;
   a.sb_bf16 = sbdt == DT_BF16;
   return xdt == DT_BF16 ? launch_mma<MOE_BITS, bf16_t>(a, st) : launch_mma<MOE_BITS, f16_t>(a, st);

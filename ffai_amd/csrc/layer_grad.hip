@@ -61,8 +61,11 @@ hipError_t launch_permute_backward(const void* dX, const uint32_t* inv, int T, i
 
 // With s = 1 / sqrt(mean(r^2) + eps) and n = r s of a row:
 //   d_in = d_res + s (dn w - n mean(dn w n)),   dw = sum over rows of dn n
-// A block's rows go through its threads one after another; a thread owns
-// the same columns of each and keeps their share of dw in registers.
+// Both row sums come from one pass over the row, which stays in registers: a team
+// of W waves takes a row, each lane up to C pieces of 8 columns, and keeps its
+// columns' share of dw over all its rows. A 16-bit row is loaded while the one
+// before is worked on. The blocks' shares of dw meet in a second launch, in a
+// fixed order; few rows are one block's.
 struct NormBackward {
   const void *r, *w, *dn, *dr;
   void* din;
@@ -70,94 +73,208 @@ struct NormBackward {
   float eps;
   int T, H;
 };
-constexpr int kNormMax = 4;  // chunks of 8 per thread: rows up to 8192 values
 
+// Eight values as they lie in memory.
 template <typename XT>
-__global__ __launch_bounds__(256) void norm_backward_kernel(const NormBackward a) {
-  __shared__ float part[2][4][2];
-  const int H = a.H, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float dw[kNormMax][8] = {};
-  int turn = 0;
-  for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
-    float r[kNormMax][8], g[kNormMax][8];
-    float ss = 0.0f, sg = 0.0f;
+struct Raw8 {
+  uint4 v[sizeof(XT) / 2];
+  __device__ __forceinline__ void load(const XT* p) {
 #pragma unroll
-    for (int c = 0; c < kNormMax; c++) {
-      const int h = (threadIdx.x + c * 256) * 8;
+    for (size_t i = 0; i < sizeof(XT) / 2; i++) v[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      if constexpr (sizeof(XT) == 4)
+        f[j] = __uint_as_float(w[j]);
+      else
+        f[j] = to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(w[j >> 1] >> (16 * (j & 1)))));
+    }
+  }
+};
+
+template <typename XT, int C, int W>
+__global__ __launch_bounds__(256) void norm_backward_kernel(const NormBackward a) {
+  constexpr int TEAMS = 4 / W, COLS = 512 * W;  // columns of a piece across a team
+  constexpr bool AHEAD = sizeof(XT) == 2;
+  __shared__ float part[2][4][2];
+  __shared__ __align__(16) float sums[TEAMS > 1 ? TEAMS : 1][TEAMS > 1 ? C * COLS : 4];
+  const int H = a.H, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, team = wave / W;
+  const int h0 = (threadIdx.x % (64 * W)) * 8;
+  Raw8<XT> w[C], r[C], g[C], d[C];
+#pragma unroll
+  for (int c = 0; c < C; c++)
+    if (h0 + c * COLS < H) w[c].load((const XT*)a.w + h0 + c * COLS);
+  auto load = [&](int64_t t) {
+    if (t >= a.T) return;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      const int h = h0 + c * COLS;
       if (h < H) {
-        float w[8];
-        Vec8<XT>::load((const XT*)a.r + t * H + h, r[c]);
-        Vec8<XT>::load((const XT*)a.dn + t * H + h, g[c]);
-        Vec8<XT>::load((const XT*)a.w + h, w);
+        r[c].load((const XT*)a.r + t * H + h);
+        g[c].load((const XT*)a.dn + t * H + h);
+        if (a.dr) d[c].load((const XT*)a.dr + t * H + h);
+      }
+    }
+  };
+  float dw[C][8] = {};
+  int turn = 0;
+  const int64_t step = (int64_t)gridDim.x * TEAMS;
+  if (AHEAD) load((int64_t)blockIdx.x * TEAMS + team);
+  for (int64_t base = (int64_t)blockIdx.x * TEAMS; base < a.T; base += step, turn ^= 1) {
+    const int64_t t = base + team;
+    if (!AHEAD) load(t);
+    const bool on = t < a.T;
+    float ss = 0.0f, sg = 0.0f;
+    Raw8<XT> rc[C], gc[C], dc[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      if (on && h0 + c * COLS < H) {
+        rc[c] = r[c];
+        gc[c] = g[c];
+        dc[c] = d[c];
+        float rv[8], gv[8], wv[8];
+        rc[c].get(rv);
+        gc[c].get(gv);
+        w[c].get(wv);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          ss = __builtin_fmaf(r[c][j], r[c][j], ss);
-          sg = __builtin_fmaf(g[c][j] * w[j], r[c][j], sg);
+          ss = __builtin_fmaf(rv[j], rv[j], ss);
+          sg = __builtin_fmaf(gv[j] * wv[j], rv[j], sg);
         }
       }
     }
+    if (AHEAD) load(t + step);
     ss = group_sum(ss, 6);
     sg = group_sum(sg, 6);
-    if (lane == 63) {
-      part[turn][wave][0] = ss;
-      part[turn][wave][1] = sg;
+    if constexpr (W == 1) {
+      ss = lane_f32(ss, 63);
+      sg = lane_f32(sg, 63);
+    } else {
+      if (lane == 63) {
+        part[turn][wave][0] = ss;
+        part[turn][wave][1] = sg;
+      }
+      lds_barrier();
+      ss = sg = 0.0f;
+#pragma unroll
+      for (int i = 0; i < W; i++) {
+        ss += part[turn][team * W + i][0];
+        sg += part[turn][team * W + i][1];
+      }
     }
-    __syncthreads();
-    ss = (part[turn][0][0] + part[turn][1][0]) + (part[turn][2][0] + part[turn][3][0]);
-    sg = (part[turn][0][1] + part[turn][1][1]) + (part[turn][2][1] + part[turn][3][1]);
     const float s = 1.0f / sqrtf(ss / (float)H + a.eps);
     const float m = s * sg / (float)H;  // mean(dn w n)
 #pragma unroll
-    for (int c = 0; c < kNormMax; c++) {
-      const int h = (threadIdx.x + c * 256) * 8;
-      if (h < H) {
-        float w[8], d[8] = {};
-        Vec8<XT>::load((const XT*)a.w + h, w);
-        if (a.dr) Vec8<XT>::load((const XT*)a.dr + t * H + h, d);
+    for (int c = 0; c < C; c++) {
+      const int h = h0 + c * COLS;
+      if (on && h < H) {
+        float rv[8], gv[8], wv[8], o[8] = {};
+        rc[c].get(rv);
+        gc[c].get(gv);
+        w[c].get(wv);
+        if (a.dr) dc[c].get(o);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          const float n = r[c][j] * s;
-          d[j] += s * (g[c][j] * w[j] - n * m);
-          dw[c][j] = __builtin_fmaf(g[c][j], n, dw[c][j]);
+          const float n = rv[j] * s;
+          o[j] += s * (gv[j] * wv[j] - n * m);
+          dw[c][j] = __builtin_fmaf(gv[j], n, dw[c][j]);
         }
-        Vec8<XT>::store((XT*)a.din + t * H + h, d);
+        Vec8<XT>::store((XT*)a.din + t * H + h, o);
       }
     }
   }
+  float* out = a.dw + (size_t)blockIdx.x * H;
+  if constexpr (TEAMS == 1) {
 #pragma unroll
-  for (int c = 0; c < kNormMax; c++) {
-    const int h = (threadIdx.x + c * 256) * 8;
-    if (h < H) Vec8<float>::store(a.dw + (size_t)blockIdx.x * H + h, dw[c]);
+    for (int c = 0; c < C; c++)
+      if (h0 + c * COLS < H) Vec8<float>::store(out + h0 + c * COLS, dw[c]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; c++) Vec8<float>::store(&sums[team][h0 + c * COLS], dw[c]);
+    __syncthreads();
+    for (int h = threadIdx.x * 4; h < H; h += 1024) {
+      float4 v = *reinterpret_cast<const float4*>(&sums[0][h]);
+#pragma unroll
+      for (int i = 1; i < TEAMS; i++) {
+        const float4 u = *reinterpret_cast<const float4*>(&sums[i][h]);
+        v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
+      }
+      *reinterpret_cast<float4*>(out + h) = v;
+    }
   }
 }
 
-// Adds the blocks' partial sums in order.
-__global__ __launch_bounds__(256) void norm_weight_kernel(const float* __restrict__ part, int blocks, int H,
-                                                          float* __restrict__ dw) {
-  const int h = blockIdx.x * 256 + threadIdx.x;
-  if (h >= H) return;
+// Adds the blocks' shares: 32 columns a block, 32 runs of blocks in order, then
+// the runs along a tree.
+__global__ __launch_bounds__(1024) void norm_weight_kernel(const float* __restrict__ part, int blocks, int H,
+                                                           float* __restrict__ dw) {
+  __shared__ float sums[32][33];
+  const int col = threadIdx.x & 31, run = threadIdx.x >> 5, h = blockIdx.x * 32 + col;
+  const int per = (blocks + 31) / 32, b0 = run * per, b1 = min(b0 + per, blocks);
   float s = 0.0f;
-  for (int b = 0; b < blocks; b++) s += part[(size_t)b * H + h];
-  dw[h] = s;
+  if (h < H)
+#pragma unroll 8
+    for (int b = b0; b < b1; b++) s += part[(size_t)b * H + h];
+  sums[run][col] = s;
+  __syncthreads();
+  float v = sums[col][run];  // thread (run, col) now holds run col of column run
+#pragma unroll
+  for (int off = 16; off; off >>= 1) v += __shfl_xor(v, off, 32);
+  if (col == 0 && blockIdx.x * 32 + run < H) dw[blockIdx.x * 32 + run] = v;
 }
 
-static int norm_blocks(int T) { return std::min(T, 512); }
+namespace {
+
+// Waves per row: a lane holds up to two pieces (four above 4096 columns), which
+// leaves room for four waves a SIMD. One / two / four waves at 8192 rows of 2048, fp32:
+// 57.2 / 49.2 / 47.5 us, bf16 27.8 / 27.4 / 27.7; at 16384 rows of 512 bf16 15.2 / - / 28.9.
+int norm_waves(int H) { return H <= 1024 ? 1 : (H <= 2048 ? 2 : 4); }
+// Two blocks a CU (four a CU 29.5 us where two take 27.4, one a CU 37 where two take
+// 29). Up to six rows a team one block alone takes less than a second launch: 8 rows
+// of 2048 8.6 us for 13.3, 32 rows 19.9 for 13.1.
+constexpr int kNormBlocks = 512, kNormAlone = 6;
+
+int norm_blocks(int T, int H) {
+  const int teams = 4 / norm_waves(H);
+  return T <= kNormAlone * teams ? 1 : std::min((T + teams - 1) / teams, kNormBlocks);
+}
+
+template <typename XT>
+hipError_t norm_t(const NormBackward& a, int blocks, hipStream_t st) {
+  const int W = norm_waves(a.H), C = (a.H + 512 * W - 1) / (512 * W);
+#define MOE_NB(CC, WW)                                                                       \
+  if (C == CC && W == WW) {                                                                  \
+    hipLaunchKernelGGL((norm_backward_kernel<XT, CC, WW>), dim3(blocks), dim3(256), 0, st, a); \
+    return hipGetLastError();                                                                \
+  }
+  MOE_NB(1, 1)
+  MOE_NB(2, 1)
+  MOE_NB(2, 2)
+  MOE_NB(2, 4)
+  MOE_NB(3, 4)
+  MOE_NB(4, 4)
+#undef MOE_NB
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
 
 size_t norm_backward_ws_bytes(int T, int H) {
-  const int blocks = norm_blocks(T);
+  const int blocks = norm_blocks(T, H);
   return blocks > 1 ? (size_t)blocks * H * 4 : 0;
 }
 
 hipError_t launch_norm_backward(const void* r, const void* w, const void* dn, const void* dr, float eps,
                                 int T, int H, int dt, void* din, float* dw, void* ws, hipStream_t st) {
-  const int blocks = norm_blocks(T);
+  const int blocks = norm_blocks(T, H);
   const NormBackward a{r, w, dn, dr, din, blocks > 1 ? (float*)ws : dw, eps, T, H};
-  if (dt == DT_BF16) hipLaunchKernelGGL((norm_backward_kernel<bf16_t>), dim3(blocks), dim3(256), 0, st, a);
-  else if (dt == DT_F16) hipLaunchKernelGGL((norm_backward_kernel<f16_t>), dim3(blocks), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((norm_backward_kernel<float>), dim3(blocks), dim3(256), 0, st, a);
-  const hipError_t e = hipGetLastError();
+  const hipError_t e = dt == DT_BF16  ? norm_t<bf16_t>(a, blocks, st)
+                       : dt == DT_F16 ? norm_t<f16_t>(a, blocks, st)
+                                      : norm_t<float>(a, blocks, st);
   if (e != hipSuccess || blocks == 1) return e;
-  hipLaunchKernelGGL(norm_weight_kernel, dim3((H + 255) / 256), dim3(256), 0, st, (const float*)ws, blocks, H, dw);
+  hipLaunchKernelGGL(norm_weight_kernel, dim3((H + 31) / 32), dim3(1024), 0, st, (const float*)ws, blocks, H, dw);
   return hipGetLastError();
 }
 
