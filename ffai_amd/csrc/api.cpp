@@ -1411,7 +1411,10 @@ extern "C" moe_status moe_expert_matmul_backward(const moe_qproj* p, const void*
   a.K = p->k;
   a.E = p->n_experts;
   a.gsh = group_shift(p->group_size);
-  MOE_HIP(launch_expert_grad(p->bits, dtype, p->sb_dtype, a, stream), "expert gradient launch");
+  const hipError_t e = launch_expert_grad(p->bits, dtype, p->sb_dtype, a, stream);
+  if (e == hipErrorInvalidConfiguration)
+    return fail(MOE_ERR_UNSUPPORTED, "expert_matmul_backward: M=%d by k=%d is too large for one launch", M, p->k);
+  MOE_HIP(e, "expert gradient launch");
   return ok();
 }
 

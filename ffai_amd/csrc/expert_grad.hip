@@ -100,9 +100,14 @@ __device__ __forceinline__ bool grad_tile(const uint32_t* __restrict__ offsets, 
     }
   return found;
 }
-// Blocks for the most tiles that M rows of E experts can make.
-static unsigned grad_grid(int M, int E, int R, int nb) {
-  return (unsigned)(((int64_t)M / R + std::min(E, M) + 7) / 8 * nb * 8);
+// Launches `kernel` on blocks for the most tiles of R rows that a.M rows of a.E
+// experts can make; hipErrorInvalidConfiguration where a launch cannot hold them
+// (2^32 threads).
+static hipError_t launch_grad(void (*kernel)(const ExpertGradArgs), const ExpertGradArgs& a, int R, int C, int threads, hipStream_t st) {
+  const int64_t nb = (a.K + C - 1) / C, blocks = (a.M / R + std::min(a.E, a.M) + 7) / 8 * nb * 8;
+  if (blocks * threads > 0xFFFFFFFFll) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, st, a);
+  return hipGetLastError();
 }
 
 // ------------------------------------------------------------ fp32 products --
@@ -178,12 +183,6 @@ __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradAr
       ((float*)a.dx)[at] = (a.dx_in ? ((const float*)a.dx_in)[at] : 0.0f) + acc[r];
     }
   }
-}
-
-template <int BITS>
-static hipError_t launch_f32(const ExpertGradArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((expert_grad_f32_kernel<BITS>), dim3(grad_grid(a.M, a.E, kFR, (a.K + kFC - 1) / kFC)), dim3(256), 0, st, a);
-  return hipGetLastError();
 }
 
 // ----------------------------------------------------------- 16-bit products --
@@ -778,28 +777,21 @@ __global__ __launch_bounds__(GradMid::NT, 2) void expert_grad_mid_kernel(const E
 // one row 14 / 24.
 template <int BITS, typename XT>
 static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
-  const int64_t used = std::min(a.E, a.M);
-  auto columns = [&](int n) { return (a.K + n - 1) / n; };
+  const int64_t used = std::min(a.E, a.M), wide = (a.K + 255) / 256;  // blocks of 256 columns
   if ((int64_t)a.M <= 28 * (int64_t)a.E && (int64_t)a.M * BITS <= 100 * (int64_t)a.E) {
-    if (used * columns(256) >= 512)
-      hipLaunchKernelGGL((expert_grad_few_kernel<8, BITS, XT>), dim3(grad_grid(a.M, a.E, kFewRows, columns(256))), dim3(256), 0, st, a);
-    else
-      hipLaunchKernelGGL((expert_grad_few_kernel<4, BITS, XT>), dim3(grad_grid(a.M, a.E, kFewRows, columns(128))), dim3(256), 0, st, a);
-  } else if (std::max<int64_t>(used, a.M / GradTall::MR) * columns(GradTall::NC) < 256) {
-    hipLaunchKernelGGL((expert_grad_mid_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, GradMid::MR, columns(GradMid::NC))), dim3(GradMid::NT), 0,
-                       st, a);
-  } else {
-    hipLaunchKernelGGL((expert_grad_tall_kernel<BITS, XT>), dim3(grad_grid(a.M, a.E, GradTall::MR, columns(GradTall::NC))), dim3(GradTall::NT),
-                       0, st, a);
+    if (used * wide >= 512) return launch_grad(expert_grad_few_kernel<8, BITS, XT>, a, kFewRows, 256, 256, st);
+    return launch_grad(expert_grad_few_kernel<4, BITS, XT>, a, kFewRows, 128, 256, st);
   }
-  return hipGetLastError();
+  if (std::max<int64_t>(used, a.M / GradTall::MR) * wide < 256)
+    return launch_grad(expert_grad_mid_kernel<BITS, XT>, a, GradMid::MR, GradMid::NC, GradMid::NT, st);
+  return launch_grad(expert_grad_tall_kernel<BITS, XT>, a, GradTall::MR, GradTall::NC, GradTall::NT, st);
 }
 
 #define MOE_CAT2(a, b) a##b
 #define MOE_CAT(a, b) MOE_CAT2(a, b)
 
 hipError_t MOE_CAT(launch_expert_grad_b, MOE_BITS)(int xdt, int sbdt, const ExpertGradArgs& a0, hipStream_t st) {
-  if (xdt == DT_F32) return launch_f32<MOE_BITS>(a0, st);
+  if (xdt == DT_F32) return launch_grad(expert_grad_f32_kernel<MOE_BITS>, a0, kFR, kFC, 256, st);
   ExpertGradArgs a = a0;
   a.sb_bf16 = sbdt == DT_BF16;
   return xdt == DT_BF16 ? launch_mma<MOE_BITS, bf16_t>(a, st) : launch_mma<MOE_BITS, f16_t>(a, st);

@@ -15,7 +15,9 @@ namespace moe {
 
 // dx[t] = round(dx_in[t] + sum_s dX[inv[t*k + s]]), eight columns per thread,
 // the chunks of all tokens side by side so that narrow rows fill blocks too.
-// Up to kRankBatch rows in flight; the ranks are added in order.
+// Up to kRankBatch rows in flight; the ranks are added in order. Bound by memory:
+// 4096 tokens of 8 rows of 2048, bf16, take 36 us (4.7 TB/s where a large copy
+// reaches 5.2).
 constexpr int kRankBatch = 8;
 
 template <typename XT>
@@ -23,32 +25,33 @@ __global__ __launch_bounds__(256) void permute_backward_kernel(const XT* __restr
                                                                const uint32_t* __restrict__ inv, int T,
                                                                int H, int k, const XT* dx_in, XT* dx) {
   const uint32_t M = (uint32_t)T * (uint32_t)k, chunks = (uint32_t)H / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t t = i / chunks;
-  if (t >= T) return;
-  const int h = (int)(i - t * chunks) * 8;
-  float acc[8] = {};
-  if (dx_in) Vec8<XT>::load(dx_in + t * H + h, acc);
-  for (int s0 = 0; s0 < k; s0 += kRankBatch) {
-    uint32_t p[kRankBatch];
+  const int64_t all = (int64_t)T * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = all < (int64_t)1 << 32 ? (int64_t)((uint32_t)i / chunks) : i / chunks;
+    const int h = (int)(i - t * chunks) * 8;
+    float acc[8] = {};
+    if (dx_in) Vec8<XT>::load(dx_in + t * H + h, acc);
+    for (int s0 = 0; s0 < k; s0 += kRankBatch) {
+      uint32_t p[kRankBatch];
 #pragma unroll
-    for (int q = 0; q < kRankBatch; q++) p[q] = s0 + q < k ? inv[t * k + s0 + q] : 0xFFFFFFFFu;
-    float v[kRankBatch][8];
+      for (int q = 0; q < kRankBatch; q++) p[q] = s0 + q < k ? inv[t * k + s0 + q] : 0xFFFFFFFFu;
+      float v[kRankBatch][8];
 #pragma unroll
-    for (int q = 0; q < kRankBatch; q++)
-      if (p[q] < M) Vec8<XT>::load(dX + (size_t)p[q] * H + h, v[q]);
+      for (int q = 0; q < kRankBatch; q++)
+        if (p[q] < M) Vec8<XT>::load(dX + (size_t)p[q] * H + h, v[q]);
 #pragma unroll
-    for (int q = 0; q < kRankBatch; q++)
-      if (p[q] < M)
+      for (int q = 0; q < kRankBatch; q++)
+        if (p[q] < M)
 #pragma unroll
-        for (int j = 0; j < 8; j++) acc[j] += v[q][j];
+          for (int j = 0; j < 8; j++) acc[j] += v[q][j];
+    }
+    Vec8<XT>::store(dx + t * H + h, acc);
   }
-  Vec8<XT>::store(dx + t * H + h, acc);
 }
 
 hipError_t launch_permute_backward(const void* dX, const uint32_t* inv, int T, int H, int k,
                                    const void* dx_in, void* dx, int dt, hipStream_t st) {
-  const dim3 grid((unsigned)(((int64_t)T * (H / 8) + 255) / 256));
+  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)T * (H / 8) + 255) / 256, 1 << 22));
 #define MOE_PB(XT)                                                                               \
   hipLaunchKernelGGL((permute_backward_kernel<XT>), grid, dim3(256), 0, st, (const XT*)dX, inv, T, \
                      H, k, (const XT*)dx_in, (XT*)dx)

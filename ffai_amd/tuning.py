@@ -698,7 +698,7 @@ class FrozenExperts:
         router or a shared expert; the sum goes to out, by default to dx itself."""
         T, k = kept.inv_perm.shape
         H, at = self.up.k, d_out.get_device()
-        gp = _check("d_out", _rows("d_out", d_out, 2), (T, H), _FLOATS, at)
+        gp = _check("d_out", _rows("d_out", d_out, 2), (T, H), _FLOATS if kept.Y is None else (kept.Y.dtype,), at)
         st, ctx = _begin(at, stream)
         try:
             dh = expert_matmul_backward(self.down, d_out, kept.offsets, perm=kept.perm, top_k=k)

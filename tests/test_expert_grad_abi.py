@@ -54,6 +54,7 @@ def call(fn, base, **kw):
     (dict(proj2=other(), dy2=p(5, 2)), INV, "aligned"), (dict(proj=proj(weight=p(20, 8))), INV, "aligned"),
     (dict(dx=p(0)), INV, "overlaps"), (dict(dx=p(0, 64 * 128 * 2 - 16)), INV, "overlaps"), (dict(dx_in=p(2, 16)), INV, "overlaps"),
     (dict(proj2=other(), dy2=p(2, 32)), INV, "overlaps"), (dict(dx=p(20, 64)), INV, "experts"), (dict(dx=p(21)), INV, "experts"),
+    (dict(proj=proj(n=8, k=1 << 20, sb_dtype=MOE_F32), dtype=MOE_F32, M=1 << 23, dy=p(0), dx=C.c_void_p(1 << 62)), UNS, "one launch"),
     (dict(proj2=other(), dy2=p(5), dx=p(25)), INV, "experts"), (dict(dx=p(1)), INV, "plan"), (dict(perm=p(2, 64)), INV, "plan"),
 ])
 def test_expert_matmul_backward_refuses(kw, status, needle):

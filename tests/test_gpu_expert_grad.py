@@ -72,6 +72,8 @@ def picks(T, E, k, seed, kind="even"):
         score[:, 0] += 2
         score[:, E // 2:] -= 2
     idx = score.topk(k).indices.to(torch.int32)
+    if kind == "steep":  # from no row to several hundred
+        idx = (torch.rand(T, k, generator=g) ** 3 * E).long().clamp(max=E - 1).to(torch.int32)
     if kind == "some":  # picks of no expert
         idx = torch.where(torch.rand(T, k, generator=g) < 0.2, torch.full_like(idx, -1), idx)
     return idx
@@ -106,6 +108,11 @@ CASES = [
     (64, 8, 2, 128, 320, 2, 32, True, False, False, "some"), (333, 8, 2, 96, 384, 4, 128, False, False, True, "one"),
     (700, 2, 1, 40, 288, 4, 32, True, False, False, "one"), (513, 1, 1, 136, 544, 8, 32, False, True, False, "even"),
     (129, 200, 3, 64, 128, 4, 64, False, False, False, "some"), (300, 4, 2, 520, 640, 3, 128, False, True, True, "even"),
+    # the kernels of many and of few rows: shapes of tiles from 32 to 256 rows, blocks of 128 and 256 columns
+    (4000, 32, 1, 40, 2048, 4, 64, False, True, False, "steep"), (3000, 32, 1, 104, 1952, 3, 32, True, False, True, "steep"),
+    (2600, 64, 1, 72, 1184, 8, 32, False, False, False, "steep"), (1100, 33, 1, 136, 2080, 6, 32, True, False, False, "one"),
+    (300, 300, 2, 40, 512, 4, 64, True, False, False, "steep"), (500, 1024, 2, 72, 224, 5, 32, False, True, True, "steep"),
+    (600, 1024, 1, 8, 32, 2, 32, False, False, False, "one"), (1, 1024, 3, 264, 288, 8, 32, False, True, False, "even"),
     (150, 3, 2, 1032, 96, 6, 32, True, False, False, "even"), (90, 5, 2, 48, 1056, 5, 32, True, True, True, "even"),
 ]
 
