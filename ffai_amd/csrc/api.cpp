@@ -1401,6 +1401,7 @@ extern "C" moe_status moe_expert_matmul_backward(const moe_qproj* p, const void*
   if (p2) a.p1 = GemvProj{p2->weight, p2->scales, p2->biases, nullptr};
   a.dy = dy;
   a.dy2 = dy2;
+  a.rows = perm ? (M - 1) / top_k + 1 : M;
   a.perm = perm;
   a.topk = top_k;
   a.offsets = offsets;

@@ -236,9 +236,6 @@ __device__ __forceinline__ f32x16_t mma16(u32x4_t a, u32x4_t b, f32x16_t c) {
                                                   __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// 16 bytes of zeros, which copies of values past the end of a row read.
-__device__ const uint32_t kGradZeros[4] = {0u, 0u, 0u, 0u};
-
 // Slot of 16-byte piece c of gradient row r in its 128 bytes of LDS: rows lie
 // two to a turn of the banks, so 16 rows reading one piece meet every bank once.
 __device__ __forceinline__ int grad_swz(int r) { return (r >> 1) & 7; }
@@ -317,7 +314,7 @@ __device__ __forceinline__ void each(F& f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, I>{}), ...);
 }
 
-template <typename S, int BITS, typename XT>
+template <typename S, bool FAR, int BITS, typename XT>
 __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const GradLds L, const GradTile& t, int j0) {
   constexpr int MI = S::MI, NJ = S::NJ, UN = S::UN, AI = S::AI, BI = S::BI, NT = S::NT;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -333,29 +330,27 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
 
   // ---- gradient rows: thread tid copies, for i < AI, the piece that belongs in
   // slot tid % 8 of LDS row tid / 8 + NT / 8 * i (a wave's 64 lanes write one KB)
+  // 32-bit offsets from a uniform base (FAR: gathered rows past 4 GB, 64-bit ones).
+  // Behind the end of a row its last piece comes again: it meets zero weights.
   const int ac = (tid & 7) ^ grad_swz(tid >> 3);
-  uint64_t arow[AI];
+  uint32_t row[AI];
+  const uint64_t first = a.perm ? 0 : (uint64_t)t.m0 * (uint64_t)N * 2u;
 #pragma unroll
   for (int i = 0; i < AI; i++) {
     const uint32_t pos = min(t.m0 + (uint32_t)((tid >> 3) + NT / 8 * i), t.pend - 1);
-    const uint32_t row = a.perm ? a.perm[pos] / (uint32_t)a.topk : pos;
-    arow[i] = (uint64_t)row * (uint64_t)N * 2u + (uint64_t)(16 * ac);
+    row[i] = a.perm ? a.perm[pos] / (uint32_t)a.topk : pos - t.m0;
+    if constexpr (!FAR) row[i] *= (uint32_t)N * 2u;
   }
   // (every row of a thread is a multiple of 16 apart from its first: one slot)
   static_assert(NT / 8 % 16 == 0, "slots");
-  const uint64_t zeros = reinterpret_cast<uint64_t>(&kGradZeros[0]);
   auto copy_rows = [&](int chunk, auto st) {
     const bool second = chunk >= per;
-    const int c0 = (second ? chunk - per : chunk) * kGK;
-    const uint64_t base = reinterpret_cast<uint64_t>(second ? a.dy2 : a.dy) + (uint64_t)(uint32_t)c0 * 2u;
-    uint32_t in = c0 + 8 * ac < N ? 0xFFFFFFFFu : 0u;
-    asm("" : "+v"(in));  // (a select of the address became a branch around each copy)
+    const uint32_t c0 = (uint32_t)(second ? chunk - per : chunk) * (kGK * 2);
+    const unsigned char* base = reinterpret_cast<const unsigned char*>(second ? a.dy2 : a.dy) + first;
+    const uint32_t x = min(c0 + (uint32_t)(16 * ac), (uint32_t)N * 2u - 16u);
 #pragma unroll
     for (int i = 0; i < AI; i++) {
-      const uint64_t from = base + arow[i];
-      const uint32_t lo = ((uint32_t)from & in) | ((uint32_t)zeros & ~in);
-      const uint32_t hi = ((uint32_t)(from >> 32) & in) | ((uint32_t)(zeros >> 32) & ~in);
-      const uint64_t at = (uint64_t)hi << 32 | lo;
+      const unsigned char* at = FAR ? base + (uint64_t)row[i] * ((uint64_t)N * 2u) + x : base + (row[i] + x);
       unsigned char* dst = stage(st) + (NT / 8 * i + 8 * wave) * 128;
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)at,
                                        (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
@@ -370,21 +365,28 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
   struct Units {
     uint32_t w[BI][BITS], s[BI], b[BI];
   };
+  const uint32_t row_bytes = (uint32_t)row_words * 4u, group_bytes = (uint32_t)groups * 2u;
+  uint32_t woffs[BI], goffs[BI];
+#pragma unroll
+  for (int i = 0; i < BI; i++) {
+    const uint32_t n = (uint32_t)(bn + NT / UN * i);
+    woffs[i] = n * row_bytes + (uint32_t)(ju * BITS) * 4u;
+    goffs[i] = n * group_bytes + (uint32_t)(ju >> a.gsh) * 2u;
+  }
   auto load_units = [&](int chunk, Units& u) {
     const bool second = chunk >= per;
     const GemvProj& p = second ? a.p1 : a.p0;
-    const size_t rows = (size_t)t.e * (size_t)N;
-    const rsrc_t wv = make_rsrc(p.w + rows * row_words, (uint32_t)N * (uint32_t)row_words * 4u);
-    const rsrc_t sv = make_rsrc(reinterpret_cast<const uint16_t*>(p.s) + rows * groups, (uint32_t)N * (uint32_t)groups * 2u);
-    const rsrc_t bv = make_rsrc(reinterpret_cast<const uint16_t*>(p.b) + rows * groups, (uint32_t)N * (uint32_t)groups * 2u);
-    const int n0 = (second ? chunk - per : chunk) * kGK + bn;
+    const size_t at = (size_t)t.e * (size_t)N;
+    const rsrc_t wv = make_rsrc(reinterpret_cast<const unsigned char*>(p.w) + at * row_bytes, (uint32_t)N * row_bytes);
+    const rsrc_t sv = make_rsrc(reinterpret_cast<const unsigned char*>(p.s) + at * group_bytes, (uint32_t)N * group_bytes);
+    const rsrc_t bv = make_rsrc(reinterpret_cast<const unsigned char*>(p.b) + at * group_bytes, (uint32_t)N * group_bytes);
+    const uint32_t n0 = (uint32_t)((second ? chunk - per : chunk) * kGK);
 #pragma unroll
     for (int i = 0; i < BI; i++) {
-      const uint32_t n = (uint32_t)(n0 + NT / UN * i);
-      const uint32_t g = (n * (uint32_t)groups + (uint32_t)(ju >> a.gsh)) * 2u;
+      const uint32_t g = goffs[i] + n0 * group_bytes;
       u.s[i] = bload16(sv, g);
       u.b[i] = bload16(bv, g);
-      bload_unit<BITS>(wv, (n * (uint32_t)row_words + (uint32_t)(ju * BITS)) * 4u, u.w[i]);
+      bload_unit<BITS>(wv, woffs[i] + n0 * row_bytes, u.w[i]);
     }
   };
   auto sb_value = [&](uint32_t raw) -> float {
@@ -448,7 +450,7 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
   // Order of a chunk's main part: after each matrix instruction its share of the
   // vector work (kSetup for the scales, kQuarter per quarter of a unit), which
   // the matrix cores hide; a quarter's store follows when its values are there.
-  constexpr int kSetup = 10 * BI, kQuarter = 22 * BI, kWork = kSetup + 4 * kQuarter, kSteps = 3 * MI * NJ;
+  constexpr int kSetup = 10 * BI, kQuarter = 26 * BI, kWork = kSetup + 4 * kQuarter, kSteps = 3 * MI * NJ;
   auto weave = [&](auto seq) {
     auto one = [&](auto ic) {
       constexpr int i = decltype(ic)::value;
@@ -599,7 +601,7 @@ typedef GradShape<3, 2, 4, 2> GradMost;    // 192 rows
 typedef GradShape<2, 2, 4, 2> GradHalf;    // 128 rows
 typedef GradShape<2, 1, 8, 1> GradQuarter; // 64 rows
 
-template <int BITS, typename XT>
+template <bool FAR, int BITS, typename XT>
 __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const ExpertGradArgs a) {
   __shared__ __align__(16) unsigned char a0[GradTall::ABYTES], a1[GradTall::ABYTES], a2[GradTall::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradTall::BBYTES];
@@ -608,10 +610,10 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
   const int j0 = t.block * GradTall::NC;
   const GradLds L{a0, a1, a2, b};
   const uint32_t rows = t.pend - t.m0;
-  if (rows > 192) grad_tile_mma<GradTall, BITS, XT>(a, L, t, j0);
-  else if (rows > 128) grad_tile_mma<GradMost, BITS, XT>(a, L, t, j0);
-  else if (rows > 64) grad_tile_mma<GradHalf, BITS, XT>(a, L, t, j0);
-  else grad_tile_mma<GradQuarter, BITS, XT>(a, L, t, j0);
+  if (rows > 192) grad_tile_mma<GradTall, FAR, BITS, XT>(a, L, t, j0);
+  else if (rows > 128) grad_tile_mma<GradMost, FAR, BITS, XT>(a, L, t, j0);
+  else if (rows > 64) grad_tile_mma<GradHalf, FAR, BITS, XT>(a, L, t, j0);
+  else grad_tile_mma<GradQuarter, FAR, BITS, XT>(a, L, t, j0);
 }
 
 // ------------------------------------------------ 16-bit products, few rows --
@@ -752,7 +754,7 @@ typedef GradShape<4, 1, 4, 1> GradMid;  // 128 rows x 128 columns
 typedef GradShape<2, 1, 4, 1> GradMidHalf;
 typedef GradShape<1, 1, 4, 1> GradMidQuarter;
 
-template <int BITS, typename XT>
+template <bool FAR, int BITS, typename XT>
 __global__ __launch_bounds__(GradMid::NT, 2) void expert_grad_mid_kernel(const ExpertGradArgs a) {
   __shared__ __align__(16) unsigned char a0[GradMid::ABYTES], a1[GradMid::ABYTES], a2[GradMid::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradMid::BBYTES];
@@ -761,9 +763,9 @@ __global__ __launch_bounds__(GradMid::NT, 2) void expert_grad_mid_kernel(const E
   const int j0 = t.block * GradMid::NC;
   const GradLds L{a0, a1, a2, b};
   const uint32_t rows = t.pend - t.m0;
-  if (rows > 64) grad_tile_mma<GradMid, BITS, XT>(a, L, t, j0);
-  else if (rows > 32) grad_tile_mma<GradMidHalf, BITS, XT>(a, L, t, j0);
-  else grad_tile_mma<GradMidQuarter, BITS, XT>(a, L, t, j0);
+  if (rows > 64) grad_tile_mma<GradMid, FAR, BITS, XT>(a, L, t, j0);
+  else if (rows > 32) grad_tile_mma<GradMidHalf, FAR, BITS, XT>(a, L, t, j0);
+  else grad_tile_mma<GradMidQuarter, FAR, BITS, XT>(a, L, t, j0);
 }
 
 // Which kernel. Few rows an expert (up to 28 on average, fewer where a weight has
@@ -782,9 +784,12 @@ static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
     if (used * wide >= 512) return launch_grad(expert_grad_few_kernel<8, BITS, XT>, a, kFewRows, 256, 256, st);
     return launch_grad(expert_grad_few_kernel<4, BITS, XT>, a, kFewRows, 128, 256, st);
   }
+  const bool far = a.perm && (int64_t)a.rows * a.N * 2 > 0xFFFFFFFFll;
   if (std::max<int64_t>(used, a.M / GradTall::MR) * wide < 256)
-    return launch_grad(expert_grad_mid_kernel<BITS, XT>, a, GradMid::MR, GradMid::NC, GradMid::NT, st);
-  return launch_grad(expert_grad_tall_kernel<BITS, XT>, a, GradTall::MR, GradTall::NC, GradTall::NT, st);
+    return launch_grad(far ? expert_grad_mid_kernel<true, BITS, XT> : expert_grad_mid_kernel<false, BITS, XT>, a, GradMid::MR,
+                       GradMid::NC, GradMid::NT, st);
+  return launch_grad(far ? expert_grad_tall_kernel<true, BITS, XT> : expert_grad_tall_kernel<false, BITS, XT>, a, GradTall::MR,
+                     GradTall::NC, GradTall::NT, st);
 }
 
 #define MOE_CAT2(a, b) a##b

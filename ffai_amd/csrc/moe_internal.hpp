@@ -334,6 +334,7 @@ hipError_t launch_lora_backward(const LoraDims& d, const LoraBackward& a, hipStr
 struct ExpertGradArgs {
   GemvProj p0, p1;
   const void *dy, *dy2;      // [rows, N]
+  int rows;
   const uint32_t* perm;      // nullable: row(p) = perm[p] / topk, else p
   int topk;
   const uint32_t* offsets;   // [E + 1]
