@@ -248,65 +248,100 @@ __device__ __forceinline__ uint32_t wt_off(int n, int u, int s) {
   return (uint32_t)(n * UN * 64 + ((u ^ (n & 3)) << 6) + ((s ^ f) << 4));
 }
 
-// Codes 8 q ... 8 q + 7 of a unit, two to a register in the low bits of its
-// halves: code v in pr[code_reg(v)], half code_half(v). As f16 such a half is the
-// subnormal code * 2^-24, exactly, so one mixed fma with the scale * 2^24 gives
-// scale * code + bias in fp32 without a conversion.
-template <int BITS> constexpr int code_reg(int v) { return BITS == 4 ? v & 3 : v >> 1; }
-template <int BITS> constexpr int code_half(int v) { return BITS == 4 ? v >> 2 : v & 1; }
+// Codes 8 q ... 8 q + 7 of a unit, two to a register: code v in half half[v] of
+// pr[reg[v]], from bit bit[v] on, and nothing else in that half. As f16 such a half is
+// the subnormal code * 2^(bit - 24), exactly (its ten bits hold bit + BITS), so one
+// mixed fma with the scale * 2^(24 - bit) gives scale * code + bias in fp32 without
+// a shift or a conversion. Codes that would pass bit 10 are shifted down first.
+template <int BITS> struct Codes;
+template <> struct Codes<2> {
+  static constexpr int reg[8] = {0, 1, 2, 3, 0, 1, 2, 3}, half[8] = {0, 0, 0, 0, 1, 1, 1, 1}, bit[8] = {0, 2, 4, 6, 0, 2, 4, 6};
+};
+template <> struct Codes<3> {
+  static constexpr int reg[8] = {0, 1, 2, 3, 0, 1, 2, 3}, half[8] = {0, 0, 0, 0, 1, 1, 1, 1}, bit[8] = {0, 3, 6, 0, 0, 3, 6, 0};
+};
+template <> struct Codes<4> {
+  static constexpr int reg[8] = {0, 1, 2, 3, 0, 1, 2, 3}, half[8] = {0, 0, 0, 0, 1, 1, 1, 1}, bit[8] = {0, 4, 0, 4, 0, 4, 0, 4};
+};
+template <> struct Codes<5> {
+  static constexpr int reg[8] = {0, 0, 1, 3, 1, 2, 3, 2}, half[8] = {0, 1, 0, 0, 1, 0, 1, 1}, bit[8] = {0, 5, 2, 0, 4, 1, 0, 3};
+};
+template <> struct Codes<6> {
+  static constexpr int reg[8] = {0, 3, 0, 1, 1, 3, 2, 2}, half[8] = {0, 0, 1, 0, 1, 1, 0, 1}, bit[8] = {0, 0, 4, 2, 0, 0, 4, 2};
+};
+template <> struct Codes<8> {
+  static constexpr int reg[8] = {0, 0, 1, 1, 2, 2, 3, 3}, half[8] = {0, 1, 0, 1, 0, 1, 0, 1}, bit[8] = {};
+};
 template <int BITS>
 __device__ __forceinline__ void code_pairs(const uint32_t (&w)[BITS], int q, uint32_t (&pr)[4]) {
-  constexpr uint32_t kPair = ((1u << BITS) - 1u) * 0x10001u;
+  constexpr uint32_t kOne = (1u << BITS) - 1u, kPair = kOne * 0x10001u;
   if constexpr (BITS == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) pr[i] = (w[q] >> (4 * i)) & kPair;
+    const uint32_t x = w[q], y = x >> 8;
+    pr[0] = x & kPair;
+    pr[1] = x & (kPair << 4);
+    pr[2] = y & kPair;
+    pr[3] = y & (kPair << 4);
   } else if constexpr (BITS == 8) {
 #pragma unroll
     for (int p = 0; p < 4; p++) {
       const uint32_t lo = 2 * (p & 1);
       pr[p] = __builtin_amdgcn_perm(0u, w[2 * q + (p >> 1)], lo | 0x0C00u | ((lo + 1) << 16) | 0x0C000000u);
     }
-  } else if constexpr (BITS <= 3) {
-    // four codes a, b, c, d of a field y: y | y << (16 - BITS) has a at bit 0, b at 16,
-    // c at 2 BITS and d at 16 + 2 BITS
+  } else if constexpr (BITS == 2) {  // the quarter's two bytes, one to a half
+    const uint32_t lo = 2 * (q & 1);
+    const uint32_t x = __builtin_amdgcn_perm(0u, w[q >> 1], lo | 0x0C00u | ((lo + 1) << 16) | 0x0C000000u);
 #pragma unroll
-    for (int f = 0; f < 2; f++) {
-      const int bit = (2 * q + f) * 4 * BITS, lo = bit >> 5, sh = bit & 31;
-      uint32_t y = sh + 4 * BITS <= 32 ? w[lo] >> sh : __builtin_amdgcn_alignbit(w[lo + 1 < BITS ? lo + 1 : lo], w[lo], (uint32_t)sh);
-      y &= (1u << (4 * BITS)) - 1u;
-      const uint32_t m = y | (y << (16 - BITS));
-      pr[2 * f] = m & kPair;
-      pr[2 * f + 1] = (m >> (2 * BITS)) & kPair;
-    }
-  } else {  // 5 and 6 bits: the 16 bits from a pair's first byte in both halves, each shifted to its code
+    for (int p = 0; p < 4; p++) pr[p] = x & (kPair << (2 * p));
+  } else if constexpr (BITS == 3) {  // four codes (12 bits) to a half
+    const int lo = 24 * q >> 5, sh = 24 * q & 31;
+    const uint32_t f = sh == 8 || sh == 0 ? w[lo] >> sh : __builtin_amdgcn_alignbit(w[lo + 1 < BITS ? lo + 1 : lo], w[lo], (uint32_t)sh);
+    const uint32_t x = (f & 0xFFFFu) | ((f << 4) & 0xFFFF0000u);
+    pr[0] = x & kPair;
+    pr[1] = x & (kPair << 3);
+    pr[2] = x & (kPair << 6);
+    pr[3] = (x >> 9) & kPair;
+  } else {  // 5 and 6 bits: each half takes the two bytes from the one that a code starts in
     typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+    const int at = BITS * q, wi = at >> 2, ob = at & 3;
 #pragma unroll
-    for (int p = 0; p < 4; p++) {
-      const int bit = (8 * q + 2 * p) * BITS, byte = bit >> 3, o = bit & 7;
-      const int wi = byte >> 2, bw = byte & 3, wj = wi + 1 < BITS ? wi + 1 : BITS - 1;
-      const uint32_t both = (uint32_t)bw | ((uint32_t)(bw + 1) << 8);
-      const u16x2_t z = __builtin_bit_cast(u16x2_t, __builtin_amdgcn_perm(w[wj], w[wi], both * 0x10001u));
-      const u16x2_t t = z >> u16x2_t{(unsigned short)o, (unsigned short)(o + BITS)};
-      pr[p] = __builtin_bit_cast(uint32_t, t) & kPair;
+    for (int r = 0; r < 4; r++) {
+      uint32_t sel = 0, mask = 0;
+      int down[2] = {0, 0};
+#pragma unroll
+      for (int v = 0; v < 8; v++)
+        if (Codes<BITS>::reg[v] == r) {
+          const int byte = ob + (BITS * v >> 3), o = BITS * v & 7, h = Codes<BITS>::half[v];
+          const uint32_t two = (uint32_t)byte | (o + BITS > 8 ? (uint32_t)(byte + 1) << 8 : 0x0C00u);
+          sel |= two << (16 * h);
+          mask |= (kOne << Codes<BITS>::bit[v]) << (16 * h);
+          down[h] = o - Codes<BITS>::bit[v];
+        }
+      const uint32_t z = __builtin_amdgcn_perm(w[wi + 1], w[wi], sel);
+      if (down[0] || down[1]) {
+        const u16x2_t t = __builtin_bit_cast(u16x2_t, z) >> u16x2_t{(unsigned short)down[0], (unsigned short)down[1]};
+        pr[r] = __builtin_bit_cast(uint32_t, t) & mask;
+      } else {
+        pr[r] = z & mask;
+      }
     }
   }
 }
 
-// Columns 8 q ... 8 q + 7 of a unit as weights in XT; s: the scale * 2^24.
+// Columns 8 q ... 8 q + 7 of a unit as weights in XT.
 template <int BITS, typename XT>
 __device__ __forceinline__ u32x4_t weights8(const uint32_t (&w)[BITS], int q, float s, float b) {
   uint32_t pr[4];
   code_pairs<BITS>(w, q, pr);
   typedef XT x2_t __attribute__((ext_vector_type(2)));
   auto weight = [&](int v) {
-    return __builtin_fmaf((float)__builtin_bit_cast(h2_t, pr[code_reg<BITS>(v)])[code_half<BITS>(v)], s, b);
+    const float code = (float)__builtin_bit_cast(h2_t, pr[Codes<BITS>::reg[v]])[Codes<BITS>::half[v]];
+    return __builtin_fmaf(code, s * (float)(1 << (24 - Codes<BITS>::bit[v])), b);
   };
   u32x4_t o;
 #pragma unroll
   for (int p = 0; p < 4; p++) o[p] = __builtin_bit_cast(uint32_t, x2_t{(XT)weight(2 * p), (XT)weight(2 * p + 1)});
   return o;
 }
-constexpr float kCodeScale = 16777216.0f;  // 2^24
 
 // f(0), f(1), ... with the numbers as types.
 template <typename F, int... I>
@@ -403,7 +438,7 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
   auto unit_sb = [&](const Units& u, float (&s)[BI], float (&b)[BI]) {
 #pragma unroll
     for (int i = 0; i < BI; i++) {
-      s[i] = sb_value(u.s[i]) * kCodeScale;
+      s[i] = sb_value(u.s[i]);
       b[i] = sb_value(u.b[i]);
     }
   };
@@ -684,7 +719,7 @@ __global__ __launch_bounds__(256, NJ == 8 ? 2 : 3) void expert_grad_few_kernel(c
   auto products = [&](int c, const Chunk& u) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const float s = sb_value(u.s[i]) * kCodeScale, b = sb_value(u.b[i]);
+      const float s = sb_value(u.s[i]), b = sb_value(u.b[i]);
 #pragma unroll
       for (int q = 0; q < 4; q++)
         *reinterpret_cast<u32x4_t*>(mine + wt_off<NJ>(bn + ROWS * i, bu, q)) = weights8<BITS, XT>(u.w[i], q, s, b);
