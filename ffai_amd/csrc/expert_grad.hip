@@ -115,6 +115,10 @@ static hipError_t launch_grad(void (*kernel)(const ExpertGradArgs), const Expert
 // v_mfma_f32_32x32x2; 32 values of the sum at a time go through two LDS buffers
 // (the gradient's rows as they are, the weights dequantised, which keeps the
 // packed axis across the lanes), loaded while the chunk before is multiplied.
+// Bound by the matrix cores where there are blocks enough: 64 rows of each of 128
+// experts, two 768 x 2048 products at 4 bits, 477 us, 108 TFLOP/s (a large fp32
+// product of the library 134). Small layers by the latency of their few chunks:
+// 50 rows of each of 8, 512 x 1024, 18.5 us.
 constexpr int kFR = 64, kFC = 64, kFK = 32;
 
 template <int BITS>
@@ -196,17 +200,26 @@ __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradAr
 // into LDS as they lie ([sum][column]), and ds_read_tr16_b64 hands each lane
 // its column's four values of the sum.
 //
-// A block of four waves takes a row tile and 256 columns, the waves 2 x 2 with
-// 128 rows x 128 columns each (smaller shapes below): per 64 values of the sum
-// an operand byte in LDS is then read by two waves, where eight waves of half
-// the size would read it by four, and LDS bandwidth is what such a block runs
-// out of first. The weights are the products' first operand, so that a lane
-// ends with four neighbouring columns of a row of dx.
+// A block of eight waves takes a row tile and 256 columns, the waves 2 x 4 with
+// 128 rows x 64 columns each (other tiles below): four waves of twice the columns
+// read less from LDS but leave one wave a SIMD, whose vector work then stops the
+// matrix cores (296 us, eight waves 254, before the steps below; two blocks a CU of
+// 256 x 128 300). The weights are the products' first operand, so that a lane ends
+// with four neighbouring columns of a row of dx.
 //
 // Per chunk of 64 values the block holds the tile's gradient rows (copied from
 // memory straight into a ring of three LDS stages, two chunks ahead) and its
 // weights (loaded three chunks ahead into registers, dequantised into two LDS
 // buffers between the matrix steps of the chunk before). One barrier a chunk.
+//
+// 1024 rows of each of 32 experts, 2880 x 2880 at 4 bits, bf16: 486 us, 1118
+// TFLOP/s; 256 of each of 128, two 768 x 2048 products: 199 us, 1034 TFLOP/s (2 and
+// 8 bits 193 and 215; f16 at 4 bits 212). A large bf16 product of the library
+// reaches 1276, a loop of nothing but these matrix instructions on random operands
+// 1543, with four vector instructions to each 1359: the chip lowers its clock (1.6
+// GHz on average here) as both kinds run, so what is left is their number, and a
+// block's start and end, 18% of its cycles at 24 chunks, which no other block hides
+// at one block a CU. Waiting for the first chunk alone at the start: no gain.
 constexpr int kGK = 64;  // values of the sum per chunk
 
 template <int MI_, int WM_, int WN_, int NJ_>
@@ -485,6 +498,8 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
   // Order of a chunk's main part: after each matrix instruction its share of the
   // vector work (kSetup for the scales, kQuarter per quarter of a unit), which
   // the matrix cores hide; a quarter's store follows when its values are there.
+  // (kQuarter: 17 to 20 made 4 bits 4 to 5% slower; 26 took 3 bits from 266 to 253 us
+  // and left the others as they were.)
   constexpr int kSetup = 10 * BI, kQuarter = 26 * BI, kWork = kSetup + 4 * kQuarter, kSteps = 3 * MI * NJ;
   auto weave = [&](auto seq) {
     auto one = [&](auto ic) {
@@ -656,9 +671,16 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
 // up to 32 rows and 32 NJ columns; its four waves share the sum (chunks of 128 / NJ
 // values in turn) and meet at the end. A wave dequantises into LDS of its own, so
 // the loop has no barrier: LDS serves a wave's stores and reads in order.
-// Loads cost by the rows they touch rather than by their bytes (a weight row's
-// scale and bias lie in lines of their own), so wide blocks are faster (NJ = 8, two
-// thirds of the rows per byte) where there are enough of them.
+//
+// 8 rows of each of 128 experts, two 768 x 2048 products at 4 bits, bf16: 64 us, 3.7
+// TB/s of experts and rows; 4 rows of each of 32, 2880 x 2880: 56 us, 2.7 TB/s. Memory
+// moves no byte twice (L2 misses of 161 MB for 149 MB of experts); what costs is the
+// lines that the vector memory path touches, a 16-byte piece per column unit and a
+// line each for a weight row's scale and bias. Without the scales' and biases' loads
+// the second call's kernel takes 41 us for 57, without dequantising or matrix
+// products as long as with them. Wide blocks (NJ = 8) touch two thirds of the lines
+// per byte. A third set of loads in flight, eight waves, loads that bypass the
+// caches, and one load for the scales of two units: nothing gained.
 constexpr int kFewRows = 32;
 constexpr int kFewLine = 64 * 4 + 16;  // a staged row of 64 fp32 columns
 
@@ -804,19 +826,20 @@ __global__ __launch_bounds__(GradMid::NT, 2) void expert_grad_mid_kernel(const E
 }
 
 // Which kernel. Few rows an expert (up to 28 on average, fewer where a weight has
-// more than 4 bits): the few-row kernel, wide where its wide blocks fill the chip
-// twice over. Else the tall kernel, unless its
-// blocks would not fill the chip; then the ordinary one. us per call of gate and up
-// 768 x 2048 at 4 bits, bf16, experts of unequal popularity, few / ordinary / tall:
-// 128 experts of 8 rows 69 / 90 / 101, of 24 97 / 94 / 96, of 64 174 / 122 / 120, of
-// 256 531 / 329 / 248; 8 experts of 256 rows 34 / 23 / 35; one of 4096 63 / 38 / 40.
-// Few rows, narrow / wide: 128 experts of 8 rows 80 / 69, 32 of one row 24 / 26, 8 of
-// one row 14 / 24.
+// more than 4 bits): the few-row kernel, wide where that leaves blocks for most of
+// the chip (320, at two a CU). Else the tall kernel, unless its blocks would not
+// fill the chip; then the ordinary one. us per call of gate and up 768 x 2048 at 4
+// bits, bf16, experts of unequal popularity, few (wide) / ordinary / tall: 128 experts of
+// 16 rows 79 / 85 / 92, of 24 82 / 89 / 94, of 32 94 / 93 / 96, of 64 151 / 117 / 117, of
+// 256 479 / 307 / 243; 8 experts of 256 rows 34 / 23 / 33; one of 4096 61 / 34 / 36.
+// Few rows, narrow / wide, with the wide blocks: 8 experts of 16 rows (64) 14.5 / 23, 32
+// of one row (256) 23.3 / 25.1, 40 of 8 (320) 32.3 / 30.8, 60 of 12, 1408 x 2048 at 3 bits
+// (480) 68 / 60, 20 of 20, 5120 x 5120 (400) 125 / 99.
 template <int BITS, typename XT>
 static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
   const int64_t used = std::min(a.E, a.M), wide = (a.K + 255) / 256;  // blocks of 256 columns
   if ((int64_t)a.M <= 28 * (int64_t)a.E && (int64_t)a.M * BITS <= 100 * (int64_t)a.E) {
-    if (used * wide >= 512) return launch_grad(expert_grad_few_kernel<8, BITS, XT>, a, kFewRows, 256, 256, st);
+    if (used * wide >= 320) return launch_grad(expert_grad_few_kernel<8, BITS, XT>, a, kFewRows, 256, 256, st);
     return launch_grad(expert_grad_few_kernel<4, BITS, XT>, a, kFewRows, 128, 256, st);
   }
   const bool far = a.perm && (int64_t)a.rows * a.N * 2 > 0xFFFFFFFFll;

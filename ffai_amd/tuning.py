@@ -507,9 +507,10 @@ def activation_backward(kept: Checkpoint8, dh: torch.Tensor, activation: int = _
     """Gradients of activation_save at the values kept, for dh [M, n], the
     gradient of h before the routing weights. topk_weight (M float32, any shape)
     are those weights in token order and perm [M] int32 the plan's (None: in
-    order); with them come their gradient too (unless want_weight is False) and
-    h itself if want_h. offsets: as in activation_save; the weights of picks
-    without a row then get a zero gradient."""
+    order; without offsets it names every pick once); with them come their
+    gradient too (unless want_weight is False) and h itself if want_h. offsets: as
+    in activation_save; the weights of picks without a row then get a zero
+    gradient."""
     M, n = _rows("dh", dh, 2).shape
     at, dt = dh.get_device(), dh.dtype
     gated = activation != _lib.MOE_ACT_RELU2
@@ -611,7 +612,8 @@ def add_rmsnorm_backward(residual: torch.Tensor, weight: torch.Tensor, d_normed:
 
 class KeptExperts(NamedTuple):
     """What FrozenExperts.forward keeps for its backward: the plan, the routing
-    weights, the activation's inputs in 8 bits, and the experts' rows where the
+    weights (the tensor itself, not to change before), the activation's inputs in
+    8 bits, and the experts' rows where the
     down projection has an output bias (its part of a routing weight's gradient
     is not in the activation)."""
     perm: torch.Tensor

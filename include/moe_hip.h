@@ -421,9 +421,11 @@ moe_status moe_lora_backward(const moe_lora* l, const void* x, const void* dy, i
  * type. dy [M or ceil(M / top_k), n], dx_in (nullable, may be dx) and dx [M, k]
  * in dtype, 16-byte aligned; n a multiple of 8, n_experts at most 1024, M at
  * most 2^23. A 16-bit dtype multiplies weights rounded to it (half a step: 2^-8
- * of the weight for bf16, 2^-11 for f16); f32 rounds them to f32 only. Output
- * biases have no part in it. Infinities and NaN stay in their rows of dy, and
- * in weights in their expert. */
+ * of the weight for bf16, 2^-11 for f16); f32 rounds them to f32 only, and
+ * scales have to be below 2^104 in magnitude for a 16-bit one. Output biases have
+ * no part in it. Infinities and NaN stay in their rows of dy, and in weights in
+ * their expert; with n not a multiple of 64 an infinity in the last 8 values of a
+ * 16-bit row may give NaN throughout that row of dx. */
 moe_status moe_expert_matmul_backward(const moe_qproj* p, const void* dy, const moe_qproj* p2,
                                       const void* dy2, int32_t dtype, const uint32_t* perm,
                                       int32_t top_k, int32_t M, const uint32_t* offsets,
@@ -455,7 +457,8 @@ moe_status moe_checkpoint_restore(const int8_t* codes, const uint8_t* scales, in
  *   d_weight[perm[p]] = <dh[p,:], act(g, u)[p,:]>   (f32, nullable)
  *   h[p,:]      = round(act(g, u)[p,:])             (nullable)
  * A limit's slope is 1 at the limit itself. A perm entry >= M has a weight of 0
- * and no d_weight; no other is named twice. d_gate or d_up may be dh. A kept NaN
+ * and no d_weight; no other is named twice, and what none names stays as it is in
+ * d_weight. d_gate or d_up may be dh. A kept NaN
  * gives NaN in its own row. Layouts, n_rows and n as in moe_activation_save. */
 moe_status moe_activation_backward(const int8_t* codes, const uint8_t* scales, const void* dh, int32_t M,
                                    int32_t n, int32_t dtype, int32_t activation, float alpha,
