@@ -673,14 +673,14 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
 // the loop has no barrier: LDS serves a wave's stores and reads in order.
 //
 // 8 rows of each of 128 experts, two 768 x 2048 products at 4 bits, bf16: 64 us, 3.7
-// TB/s of experts and rows; 4 rows of each of 32, 2880 x 2880: 56 us, 2.7 TB/s. Memory
-// moves no byte twice (L2 misses of 161 MB for 149 MB of experts); what costs is the
-// lines that the vector memory path touches, a 16-byte piece per column unit and a
-// line each for a weight row's scale and bias. Without the scales' and biases' loads
-// the second call's kernel takes 41 us for 57, without dequantising or matrix
-// products as long as with them. Wide blocks (NJ = 8) touch two thirds of the lines
-// per byte. A third set of loads in flight, eight waves, loads that bypass the
-// caches, and one load for the scales of two units: nothing gained.
+// TB/s of experts and rows; 4 rows of each of 32, 2880 x 2880: 56 us, 2.7 TB/s, where a
+// large copy reaches 5.2. Memory moves no byte twice (the second: L2 misses of 153 MB
+// for 149 MB of experts), and no single part holds it up: without dequantising or
+// without matrix products it takes as long, without the scales' and biases' loads
+// 41 us, without the weights' 36. Three or four sets of loads in flight, eight waves,
+// one load for the scales of two units, column blocks of an expert out of step: no
+// gain. Loads that bypass the caches are slower. Wide blocks (NJ = 8) touch two
+// thirds of the lines per byte.
 constexpr int kFewRows = 32;
 constexpr int kFewLine = 64 * 4 + 16;  // a staged row of 64 fp32 columns
 
