@@ -13,11 +13,38 @@
 
 namespace moe {
 
+// Eight values as they lie in memory.
+template <typename XT>
+struct Raw8 {
+  uint4 v[sizeof(XT) / 2];
+  __device__ __forceinline__ void load(const XT* p) {
+#pragma unroll
+    for (size_t i = 0; i < sizeof(XT) / 2; i++) v[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void stream(const XT* p) {  // keeps no place in the caches
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (size_t i = 0; i < sizeof(XT) / 2; i++) v[i] = __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u4*>(p) + i));
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      if constexpr (sizeof(XT) == 4)
+        f[j] = __uint_as_float(w[j]);
+      else
+        f[j] = to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(w[j >> 1] >> (16 * (j & 1)))));
+    }
+  }
+};
+
 // dx[t] = round(dx_in[t] + sum_s dX[inv[t*k + s]]), eight columns per thread,
 // the chunks of all tokens side by side so that narrow rows fill blocks too.
-// Up to kRankBatch rows in flight; the ranks are added in order. Bound by memory:
-// 4096 tokens of 8 rows of 2048, bf16, added to a gradient take 38 us (4.4 TB/s where
-// a large copy reaches 5.2).
+// Up to kRankBatch rows in flight, as they lie in memory until all are there; the ranks
+// are added in order. Each row is read once, so its loads leave the caches to others.
+// Bound by memory: 4096 tokens of 8 rows of 2048, bf16, added to a gradient take 29 us
+// (5.8 TB/s where a large copy reaches 5.2); with ordinary loads 32, with each row
+// converted where it is loaded 36.
 constexpr int kRankBatch = 8;
 
 template <typename XT>
@@ -35,15 +62,18 @@ __global__ __launch_bounds__(256) void permute_backward_kernel(const XT* __restr
       uint32_t p[kRankBatch];
 #pragma unroll
       for (int q = 0; q < kRankBatch; q++) p[q] = s0 + q < k ? inv[t * k + s0 + q] : 0xFFFFFFFFu;
-      float v[kRankBatch][8];
+      Raw8<XT> v[kRankBatch];
 #pragma unroll
       for (int q = 0; q < kRankBatch; q++)
-        if (p[q] < M) Vec8<XT>::load(dX + (size_t)p[q] * H + h, v[q]);
+        if (p[q] < M) v[q].stream(dX + (size_t)p[q] * H + h);
 #pragma unroll
       for (int q = 0; q < kRankBatch; q++)
-        if (p[q] < M)
+        if (p[q] < M) {
+          float f[8];
+          v[q].get(f);
 #pragma unroll
-          for (int j = 0; j < 8; j++) acc[j] += v[q][j];
+          for (int j = 0; j < 8; j++) acc[j] += f[j];
+        }
     }
     Vec8<XT>::store(dx + t * H + h, acc);
   }
@@ -76,26 +106,6 @@ struct NormBackward {
   float* dw;  // [blocks, H] partial sums, or the result where there is one block
   float eps;
   int T, H;
-};
-
-// Eight values as they lie in memory.
-template <typename XT>
-struct Raw8 {
-  uint4 v[sizeof(XT) / 2];
-  __device__ __forceinline__ void load(const XT* p) {
-#pragma unroll
-    for (size_t i = 0; i < sizeof(XT) / 2; i++) v[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      if constexpr (sizeof(XT) == 4)
-        f[j] = __uint_as_float(w[j]);
-      else
-        f[j] = to_f<XT>(__builtin_bit_cast(XT, (uint16_t)(w[j >> 1] >> (16 * (j & 1)))));
-    }
-  }
 };
 
 template <typename XT, int C, int W>
@@ -231,10 +241,12 @@ __global__ __launch_bounds__(1024) void norm_weight_kernel(const float* __restri
 
 namespace {
 
-// Waves per row: a lane holds up to two pieces (four above 4096 columns), which
-// leaves room for four waves a SIMD. One / two / four waves at 8192 rows of 2048, fp32:
+// Waves per row: a lane holds up to three pieces (four above 6144 columns), two of
+// fp32 with four waves a SIMD. 4096 rows of 2880, bf16: two waves 20.1 us, four (a third
+// of whose lanes have nothing to do) 24.2; of 4096 two waves 25.5, four 26.2, fp32 60.0
+// and 50.4. One / two / four waves at 8192 rows of 2048, fp32:
 // 57.2 / 49.2 / 47.5 us, bf16 27.8 / 27.4 / 27.7; at 16384 rows of 512 bf16 15.2 / - / 28.9.
-int norm_waves(int H) { return H <= 1024 ? 1 : (H <= 2048 ? 2 : 4); }
+int norm_waves(int H) { return H <= 1024 ? 1 : (H <= 3 * 1024 ? 2 : 4); }
 // Two blocks a CU (four a CU 29.5 us where two take 27.4, one a CU 37 where two take
 // 29). Up to six rows a team one block alone takes less than a second launch: 8 rows
 // of 2048 8.6 us for 13.3, 32 rows 19.9 for 13.1.
@@ -256,6 +268,7 @@ hipError_t norm_t(const NormBackward& a, int blocks, hipStream_t st) {
   MOE_NB(1, 1)
   MOE_NB(2, 1)
   MOE_NB(2, 2)
+  MOE_NB(3, 2)
   MOE_NB(2, 4)
   MOE_NB(3, 4)
   MOE_NB(4, 4)

@@ -85,7 +85,7 @@ def test_activation_matches_differences(act):
         assert ((got.d_gate.double() - dh.double() * slope).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("T,H", [(5, 64), (70, 1000), (9, 5000)])
+@pytest.mark.parametrize("T,H", [(5, 64), (70, 1000), (9, 5000), (70, 2504), (3000, 2176)])
 def test_norm_matches_differences(T, H):
     """Along a direction per row and per column, in f32."""
     g, step, eps = gen(H), 2.0 ** -15, 1e-6
