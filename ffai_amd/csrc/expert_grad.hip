@@ -22,7 +22,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 // A block's part of the work: a tile of up to R sorted rows of one expert and a
 // block of columns. Every wave finds it from the offsets by itself: one round of
-// loads, then sums across the lanes.
+// loads, then sums across the lanes. No offset leads past M.
 //
 // In order (BY_SIZE false) tiles run through the experts, a tile's column blocks
 // (nb) together, the whole list in eight contiguous ranges, one per XCD (blocks b, b
@@ -38,16 +38,16 @@ struct GradTile {
 };
 constexpr int kGradMaxE = 1024;
 template <uint32_t R, bool BY_SIZE>
-__device__ __forceinline__ bool grad_tile(const uint32_t* __restrict__ offsets, int E, uint32_t nb, GradTile* t) {
+__device__ __forceinline__ bool grad_tile(const ExpertGradArgs& a, uint32_t nb, GradTile* t) {
   constexpr int P = kGradMaxE / 64;
-  const int lane = threadIdx.x & 63;
+  const int E = a.E, lane = threadIdx.x & 63;
   uint32_t lo[P], hi[P];
 #pragma unroll
   for (int i = 0; i < P; i++) {
     lo[i] = hi[i] = 0;
     if (i * 64 < E) {
-      lo[i] = offsets[min(i * 64 + lane, E)];
-      hi[i] = offsets[min(i * 64 + lane + 1, E)];
+      lo[i] = min(a.offsets[min(i * 64 + lane, E)], (uint32_t)a.M);
+      hi[i] = max(min(a.offsets[min(i * 64 + lane + 1, E)], (uint32_t)a.M), lo[i]);
     }
   }
   // whole tiles and remainders up to and with an expert's (remainders: long ones
@@ -100,6 +100,11 @@ __device__ __forceinline__ bool grad_tile(const uint32_t* __restrict__ offsets, 
     }
   return found;
 }
+// Row of dy that sorted position pos takes.
+__device__ __forceinline__ uint32_t grad_row(const ExpertGradArgs& a, uint32_t pos) {
+  return min(a.perm[pos], (uint32_t)a.M - 1u) / (uint32_t)a.topk;
+}
+
 // Launches `kernel` on blocks for the most tiles of R rows that a.M rows of a.E
 // experts can make; hipErrorInvalidConfiguration where a launch cannot hold them
 // (2^32 threads).
@@ -125,7 +130,7 @@ template <int BITS>
 __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradArgs a) {
   __shared__ float As[2][kFR][kFK + 1], Bs[2][kFK][kFC];
   GradTile t;
-  if (!grad_tile<kFR, false>(a.offsets, a.E, (uint32_t)((a.K + kFC - 1) / kFC), &t)) return;
+  if (!grad_tile<kFR, false>(a, (uint32_t)((a.K + kFC - 1) / kFC), &t)) return;
   const int j0 = t.block * kFC, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int col = lane & 31, half = lane >> 5;
@@ -134,7 +139,7 @@ __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradAr
   // thread: a quarter of a gradient row's chunk, eight columns of a weight row (they
   // lie in two words, from bit `sh` of the first)
   const uint32_t pos = min(t.m0 + (uint32_t)(tid >> 2), t.pend - 1);
-  const size_t arow = (size_t)(a.perm ? a.perm[pos] / (uint32_t)a.topk : pos) * a.N;
+  const size_t arow = (size_t)(a.perm ? grad_row(a, pos) : pos) * a.N;
   const int ac = (tid & 3) * 8, bi = tid >> 3, bj = min(j0 + (tid & 7) * 8, a.K - 8);
   const uint32_t bit = (uint32_t)bj * BITS, lo = bit >> 5, sh = bit & 31;
   struct Part {
@@ -386,7 +391,7 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
 #pragma unroll
   for (int i = 0; i < AI; i++) {
     const uint32_t pos = min(t.m0 + (uint32_t)((tid >> 3) + NT / 8 * i), t.pend - 1);
-    row[i] = a.perm ? a.perm[pos] / (uint32_t)a.topk : pos - t.m0;
+    row[i] = a.perm ? grad_row(a, pos) : pos - t.m0;
     if constexpr (!FAR) row[i] *= (uint32_t)N * 2u;
   }
   // (every row of a thread is a multiple of 16 apart from its first: one slot)
@@ -656,7 +661,7 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
   __shared__ __align__(16) unsigned char a0[GradTall::ABYTES], a1[GradTall::ABYTES], a2[GradTall::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradTall::BBYTES];
   GradTile t;
-  if (!grad_tile<GradTall::MR, true>(a.offsets, a.E, (uint32_t)((a.K + GradTall::NC - 1) / GradTall::NC), &t)) return;
+  if (!grad_tile<GradTall::MR, true>(a, (uint32_t)((a.K + GradTall::NC - 1) / GradTall::NC), &t)) return;
   const int j0 = t.block * GradTall::NC;
   const GradLds L{a0, a1, a2, b};
   const uint32_t rows = t.pend - t.m0;
@@ -690,7 +695,7 @@ __global__ __launch_bounds__(256, NJ == 8 ? 2 : 3) void expert_grad_few_kernel(c
   constexpr int kWave = FK * FC * 2, kLds = 4 * (kFewRows * kFewLine > kWave ? kFewRows * kFewLine : kWave);
   __shared__ __align__(16) unsigned char lds[kLds];
   GradTile t;
-  if (!grad_tile<kFewRows, false>(a.offsets, a.E, (uint32_t)((a.K + FC - 1) / FC), &t)) return;
+  if (!grad_tile<kFewRows, false>(a, (uint32_t)((a.K + FC - 1) / FC), &t)) return;
   const int j0 = t.block * FC, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
   const int N = a.N, K = a.K, CU = K >> 5, groups = CU >> a.gsh, row_words = CU * BITS;
@@ -698,7 +703,7 @@ __global__ __launch_bounds__(256, NJ == 8 ? 2 : 3) void expert_grad_few_kernel(c
   const bool sb_bf16 = a.sb_bf16 != 0;
 
   const uint32_t pos = min(t.m0 + (uint32_t)col, t.pend - 1);
-  const size_t arow = (size_t)(a.perm ? a.perm[pos] / (uint32_t)a.topk : pos) * N;
+  const size_t arow = (size_t)(a.perm ? grad_row(a, pos) : pos) * N;
   // lane: unit lane % NJ of weight rows lane / NJ and ROWS + lane / NJ of a chunk
   const int bu = lane % NJ, ju = min((j0 >> 5) + bu, CU - 1), bn = lane / NJ;
   struct Chunk {
@@ -816,7 +821,7 @@ __global__ __launch_bounds__(GradMid::NT, 2) void expert_grad_mid_kernel(const E
   __shared__ __align__(16) unsigned char a0[GradMid::ABYTES], a1[GradMid::ABYTES], a2[GradMid::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradMid::BBYTES];
   GradTile t;
-  if (!grad_tile<GradMid::MR, true>(a.offsets, a.E, (uint32_t)((a.K + GradMid::NC - 1) / GradMid::NC), &t)) return;
+  if (!grad_tile<GradMid::MR, true>(a, (uint32_t)((a.K + GradMid::NC - 1) / GradMid::NC), &t)) return;
   const int j0 = t.block * GradMid::NC;
   const GradLds L{a0, a1, a2, b};
   const uint32_t rows = t.pend - t.m0;

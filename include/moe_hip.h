@@ -417,6 +417,8 @@ moe_status moe_lora_backward(const moe_lora* l, const void* x, const void* dy, i
  *   dx[p,:] = round(dx_in[p,:] + dy[row(p),:] W[e(p)] + dy2[row(p),:] W2[e(p)])
  * with e(p) and row(p) as there (perm nullable), for the sorted positions
  * below offsets[n_experts], M at most; rows of dx behind them stay as they are.
+ * (No offset or entry of perm leads past the buffers: past M they count as M, as
+ * M - 1.)
  * p2 and dy2 are NULL together; p2 has p's shape, bits, group size and scale
  * type. dy [M or ceil(M / top_k), n], dx_in (nullable, may be dx) and dx [M, k]
  * in dtype, 16-byte aligned; n a multiple of 8, n_experts at most 1024, M at

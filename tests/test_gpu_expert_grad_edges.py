@@ -52,6 +52,26 @@ def test_product_is_the_forwards_adjoint(dt, T, E, k, N, K, bits):
     assert ((here - there).abs() <= mag * (2 * each + (N + K + 64) * U) + 1e-30).all()
 
 
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("E,M,K", [(40, 90, 2048), (4, 700, 544), (70, 9000, 1024)])
+def test_a_plan_past_the_rows(dt, E, M, K):
+    """Offsets past M end there, and perm's entries past M take the last row: nothing is written behind dx."""
+    p, W = stack(E, 64, K, 4, 32, dt, 2)
+    dy = torch.randn(M, 64, generator=gen(2)).to(dt).cuda()
+    good = torch.linspace(0, M, E + 1).round().to(torch.int32)
+    good[-2] = M
+    bad = good.clone()
+    bad[-2:] = torch.tensor([M + 300, 2 ** 31 - 1])
+    perm = torch.randperm(M, generator=gen(3)).to(torch.int32)
+    perm[5] = M - 1
+    wild = perm.clone()
+    wild[5] = -1
+    whole = torch.full((M + 600, K), 7.25, dtype=dt, device="cuda")
+    a = tuning.expert_matmul_backward(p, dy, good.cuda(), perm=perm.cuda())
+    b = tuning.expert_matmul_backward(p, dy, bad.cuda(), perm=wild.cuda(), out=whole[:M])
+    assert same_bits(a, b) and (whole[M:] == 7.25).all()
+
+
 def value(act, g, u):
     """The activation in float64."""
     if act == RELU2:
