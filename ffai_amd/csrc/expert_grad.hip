@@ -38,9 +38,10 @@ struct GradTile {
 };
 constexpr int kGradMaxE = 1024;
 template <uint32_t R, bool BY_SIZE>
-__device__ __forceinline__ bool grad_tile(const ExpertGradArgs& a, uint32_t nb, GradTile* t) {
+__device__ __forceinline__ bool grad_tile(const ExpertGradArgs& a, GradTile* t) {
   constexpr int P = kGradMaxE / 64;
   const int E = a.E, lane = threadIdx.x & 63;
+  const uint32_t nb = (uint32_t)a.nb;
   uint32_t lo[P], hi[P];
 #pragma unroll
   for (int i = 0; i < P; i++) {
@@ -70,12 +71,12 @@ __device__ __forceinline__ bool grad_tile(const ExpertGradArgs& a, uint32_t nb, 
   uint32_t tile;
   if constexpr (BY_SIZE) {
     tile = (blockIdx.x & 7u) + 8u * (k / nb);
-    t->block = (int)(k % nb);
+    t->block = a.first + (int)(k % nb);
     if (tile >= wholes + longs + (rests >> 16)) return false;
   } else {
     const uint32_t per = (wholes * nb + 7u) >> 3, w = (blockIdx.x & 7u) * per + k;
     tile = w / nb;
-    t->block = (int)(w - tile * nb);
+    t->block = a.first + (int)(w - tile * nb);
     if (k >= per || tile >= wholes) return false;
   }
   const int kind = tile < wholes ? 0 : (tile < wholes + longs ? 1 : 2);
@@ -106,13 +107,20 @@ __device__ __forceinline__ uint32_t grad_row(const ExpertGradArgs& a, uint32_t p
 }
 
 // Launches `kernel` on blocks for the most tiles of R rows that a.M rows of a.E
-// experts can make; hipErrorInvalidConfiguration where a launch cannot hold them
-// (2^32 threads).
-static hipError_t launch_grad(void (*kernel)(const ExpertGradArgs), const ExpertGradArgs& a, int R, int C, int threads, hipStream_t st) {
-  const int64_t nb = (a.K + C - 1) / C, blocks = (a.M / R + std::min(a.E, a.M) + 7) / 8 * nb * 8;
-  if (blocks * threads > 0xFFFFFFFFll) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, st, a);
-  return hipGetLastError();
+// experts can make, in two launches (left and right columns) where one cannot hold
+// them (2^32 threads); hipErrorInvalidConfiguration past two.
+static hipError_t launch_grad(void (*kernel)(const ExpertGradArgs), ExpertGradArgs a, int R, int C, int threads, hipStream_t st) {
+  const int64_t tiles = (a.M / R + std::min(a.E, a.M) + 7) / 8 * 8, all = (a.K + C - 1) / C;
+  const int64_t most = 0xFFFFFFFFll / threads / tiles;  // column blocks of a launch
+  if (all > 2 * most) return hipErrorInvalidConfiguration;
+  for (int64_t first = 0; first < all; first += most) {
+    a.first = (int)first;
+    a.nb = (int)std::min(most, all - first);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * a.nb)), dim3(threads), 0, st, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 // ------------------------------------------------------------ fp32 products --
@@ -130,7 +138,7 @@ template <int BITS>
 __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradArgs a) {
   __shared__ float As[2][kFR][kFK + 1], Bs[2][kFK][kFC];
   GradTile t;
-  if (!grad_tile<kFR, false>(a, (uint32_t)((a.K + kFC - 1) / kFC), &t)) return;
+  if (!grad_tile<kFR, false>(a, &t)) return;
   const int j0 = t.block * kFC, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int col = lane & 31, half = lane >> 5;
@@ -195,46 +203,47 @@ __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradAr
 }
 
 // ----------------------------------------------------------- 16-bit products --
-// Rows in a 16-bit type take v_mfma_f32_32x32x16 with the weights dequantised
-// in fp32 and rounded once to that type: bf16 gradients keep their range, and
-// a weight is off by at most half a step of the type.
+// Rows in a 16-bit type take v_mfma_f32_32x32x16. A weight, dequantised in fp32, enters
+// as two values of the rows' type: itself rounded (hi), and what that left, rounded (lo).
+// Together they are within 2^-17 of it in bf16, 2^-23 in f16 (there 2^-25 where that is
+// more, half the type's last bit), so that of 16 bits only the result's own rounding
+// shows; hi alone, for half the matrix instructions, is off by 2^-8 and 2^-11. bf16
+// gradients keep their range. The two are summed apart: a row or a weight that is not
+// finite leaves the lo parts' sum NaN or infinite, and hi's alone is the result.
 //
 // The weights' packed axis is the output's, and the matrix operands want
 // neighbours along the sum. The transposition costs nothing: a thread
-// dequantises units of 32 columns of one weight row, with one scale and bias,
+// dequantises 16 columns of one weight row, with one scale and bias,
 // into LDS as they lie ([sum][column]), and ds_read_tr16_b64 hands each lane
 // its column's four values of the sum.
 //
-// A block of eight waves takes a row tile and 256 columns, the waves 2 x 4 with
-// 128 rows x 64 columns each (other tiles below): four waves of twice the columns
-// read less from LDS but leave one wave a SIMD, whose vector work then stops the
-// matrix cores (296 us, eight waves 254, before the steps below; two blocks a CU of
-// 256 x 128 300). The weights are the products' first operand, so that a lane ends
-// with four neighbouring columns of a row of dx.
+// A block of eight waves takes a row tile and 128 columns, the waves 2 x 4 with
+// 128 rows x 32 columns (hi and lo: 64 columns of LDS) each, other tiles below: four
+// waves of twice the columns read less from LDS but leave one wave a SIMD, whose vector
+// work then stops the matrix cores. The weights are the products' first operand, so
+// that a lane ends with four neighbouring columns of a row of dx.
 //
 // Per chunk of 64 values the block holds the tile's gradient rows (copied from
 // memory straight into a ring of three LDS stages, two chunks ahead) and its
 // weights (loaded three chunks ahead into registers, dequantised into two LDS
 // buffers between the matrix steps of the chunk before). One barrier a chunk.
 //
-// 1024 rows of each of 32 experts, 2880 x 2880 at 4 bits, bf16: 486 us, 1118
-// TFLOP/s; 256 of each of 128, two 768 x 2048 products: 199 us, 1034 TFLOP/s (2 and
-// 8 bits 193 and 215; f16 at 4 bits 212). A large bf16 product of the library
+// 1024 rows of each of 32 experts, 2880 x 2880 at 4 bits, bf16: 1017 us, 535 TFLOP/s of
+// the product, twice that of the matrix cores; 256 of each of 128, two 768 x 2048
+// products: 495 us (8 bits 443; f16 at 4 bits 454). A large bf16 product of the library
 // reaches 1276, a loop of nothing but these matrix instructions on random operands
-// 1543, with four vector instructions to each 1359: the chip lowers its clock (1.6
-// GHz on average here) as both kinds run, so what is left is their number, and a
-// block's start and end, 18% of its cycles at 24 chunks, which no other block hides
-// at one block a CU. Waiting for the first chunk alone at the start: no gain.
+// 1543, with four vector instructions to each 1359: the chip lowers its clock as both
+// kinds run, and a block's start and end are hidden by no other at one block a CU.
 constexpr int kGK = 64;  // values of the sum per chunk
 
-template <int MI_, int WM_, int WN_, int NJ_>
-struct GradShape {  // 32-row tiles a wave, waves along rows, along columns, 32-column tiles a wave
-  static constexpr int MI = MI_, WM = WM_, WN = WN_, NJ = NJ_;
-  static constexpr int NT = 64 * WM * WN, MR = 32 * MI * WM, NC = 32 * NJ * WN;
-  static constexpr int UN = NC / 32;              // units of a weight row
+template <int MI_, int WN_>
+struct GradShape {  // 32-row tiles a wave, waves along columns (32 each); two waves along rows
+  static constexpr int MI = MI_, WM = 2, WN = WN_;
+  static constexpr int NT = 64 * WM * WN, MR = 32 * MI * WM, NC = 32 * WN;
+  static constexpr int UN = 2 * WN;               // units of 32 hi or lo parts in a weight row's LDS
   static constexpr int AI = MR * 8 / NT;          // 16-byte copies per thread and chunk
-  static constexpr int BI = kGK * UN / NT;        // units per thread and chunk
-  static constexpr int ABYTES = MR * 128, BBYTES = NC * 128;
+  static constexpr int ABYTES = MR * 128, BBYTES = kGK * UN * 64;
+  static_assert(kGK * (NC / 16) == NT, "16 columns of a weight row per thread and chunk");
 };
 
 struct GradLds {
@@ -290,8 +299,8 @@ template <> struct Codes<6> {
 template <> struct Codes<8> {
   static constexpr int reg[8] = {0, 0, 1, 1, 2, 2, 3, 3}, half[8] = {0, 1, 0, 1, 0, 1, 0, 1}, bit[8] = {};
 };
-template <int BITS>
-__device__ __forceinline__ void code_pairs(const uint32_t (&w)[BITS], int q, uint32_t (&pr)[4]) {
+template <int BITS, int NW>
+__device__ __forceinline__ void code_pairs(const uint32_t (&w)[NW], int q, uint32_t (&pr)[4]) {
   constexpr uint32_t kOne = (1u << BITS) - 1u, kPair = kOne * 0x10001u;
   if constexpr (BITS == 4) {
     const uint32_t x = w[q], y = x >> 8;
@@ -312,7 +321,7 @@ __device__ __forceinline__ void code_pairs(const uint32_t (&w)[BITS], int q, uin
     for (int p = 0; p < 4; p++) pr[p] = x & (kPair << (2 * p));
   } else if constexpr (BITS == 3) {  // four codes (12 bits) to a half
     const int lo = 24 * q >> 5, sh = 24 * q & 31;
-    const uint32_t f = sh == 8 || sh == 0 ? w[lo] >> sh : __builtin_amdgcn_alignbit(w[lo + 1 < BITS ? lo + 1 : lo], w[lo], (uint32_t)sh);
+    const uint32_t f = sh == 8 || sh == 0 ? w[lo] >> sh : __builtin_amdgcn_alignbit(w[lo + 1 < NW ? lo + 1 : lo], w[lo], (uint32_t)sh);
     const uint32_t x = (f & 0xFFFFu) | ((f << 4) & 0xFFFF0000u);
     pr[0] = x & kPair;
     pr[1] = x & (kPair << 3);
@@ -345,9 +354,9 @@ __device__ __forceinline__ void code_pairs(const uint32_t (&w)[BITS], int q, uin
   }
 }
 
-// Columns 8 q ... 8 q + 7 of a unit as weights in XT.
-template <int BITS, typename XT>
-__device__ __forceinline__ u32x4_t weights8(const uint32_t (&w)[BITS], int q, float s, float b) {
+// Columns 8 q ... 8 q + 7 of a unit as weights: rounded to XT, and what that left.
+template <int BITS, typename XT, int NW>
+__device__ __forceinline__ void weights8(const uint32_t (&w)[NW], int q, float s, float b, u32x4_t& hi, u32x4_t& lo) {
   uint32_t pr[4];
   code_pairs<BITS>(w, q, pr);
   typedef XT x2_t __attribute__((ext_vector_type(2)));
@@ -355,10 +364,48 @@ __device__ __forceinline__ u32x4_t weights8(const uint32_t (&w)[BITS], int q, fl
     const float code = (float)__builtin_bit_cast(h2_t, pr[Codes<BITS>::reg[v]])[Codes<BITS>::half[v]];
     return __builtin_fmaf(code, s * (float)(1 << (24 - Codes<BITS>::bit[v])), b);
   };
-  u32x4_t o;
 #pragma unroll
-  for (int p = 0; p < 4; p++) o[p] = __builtin_bit_cast(uint32_t, x2_t{(XT)weight(2 * p), (XT)weight(2 * p + 1)});
-  return o;
+  for (int p = 0; p < 4; p++) {
+    const float w0 = weight(2 * p), w1 = weight(2 * p + 1);
+    uint32_t pair = __builtin_bit_cast(uint32_t, x2_t{(XT)w0, (XT)w1});
+    asm("" : "+v"(pair));  // (one conversion of both, not another of each)
+    const x2_t h = __builtin_bit_cast(x2_t, pair);
+    hi[p] = pair;
+    lo[p] = __builtin_bit_cast(uint32_t, x2_t{(XT)(w0 - (float)h[0]), (XT)(w1 - (float)h[1])});
+  }
+}
+// The sum of the products with the hi parts and of those with the lo parts.
+__device__ __forceinline__ float joined(float hi, float lo) {
+  return __builtin_fabsf(lo) < __builtin_huge_valf() ? hi + lo : hi;
+}
+
+// The 16 columns of a unit's half, as the first bits of kHalfWords words: loaded
+// from the word that they begin in, `sh` bits (0 or 16) before them.
+template <int BITS>
+constexpr int kHalfWords = (BITS + 1) / 2;
+template <int BITS>
+__device__ __forceinline__ void bload_half(rsrc_t r, uint32_t off, uint32_t (&w)[kHalfWords<BITS>]) {
+  if constexpr (kHalfWords<BITS> == 1) {
+    w[0] = bload32(r, off);
+  } else if constexpr (kHalfWords<BITS> == 2) {
+    const u32x2_t v = bload64(r, off);
+    w[0] = v[0], w[1] = v[1];
+  } else if constexpr (kHalfWords<BITS> == 3) {
+    const u32x3_t v = bload96(r, off);
+    w[0] = v[0], w[1] = v[1], w[2] = v[2];
+  } else {
+    const u32x4_t v = bload128(r, off);
+    w[0] = v[0], w[1] = v[1], w[2] = v[2], w[3] = v[3];
+  }
+}
+template <int BITS>
+__device__ __forceinline__ void shift_half(uint32_t (&w)[kHalfWords<BITS>], uint32_t sh) {
+  if constexpr (BITS & 1) {
+    constexpr int L = kHalfWords<BITS> - 1;
+#pragma unroll
+    for (int i = 0; i < L; i++) w[i] = __builtin_amdgcn_alignbit(w[i + 1], w[i], sh);
+    w[L] >>= sh;
+  }
 }
 
 // f(0), f(1), ... with the numbers as types.
@@ -369,7 +416,7 @@ __device__ __forceinline__ void each(F& f, std::integer_sequence<int, I...>) {
 
 template <typename S, bool FAR, int BITS, typename XT>
 __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const GradLds L, const GradTile& t, int j0) {
-  constexpr int MI = S::MI, NJ = S::NJ, UN = S::UN, AI = S::AI, BI = S::BI, NT = S::NT;
+  constexpr int MI = S::MI, UN = S::UN, AI = S::AI, NT = S::NT, HW = kHalfWords<BITS>;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / S::WN, wn = wave % S::WN, col = lane & 31, h = lane >> 5;
@@ -410,22 +457,17 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
     }
   };
 
-  // ---- weights: thread tid dequantises, for i < BI, unit tid % UN of weight row
-  // tid / UN + NT / UN * i of the chunk. Columns past the end repeat the last
-  // unit (never stored), rows past it read as zeros from the views.
-  const int bu = tid % UN, ju = min((j0 >> 5) + bu, CU - 1), bn = tid / UN;
-  static_assert(NT / UN % 4 == 0, "slots");
+  // ---- weights: thread tid dequantises half tid % 2 of unit tid / 2 % WN of row tid /
+  // UN of the chunk. Columns past the end repeat the last unit (never stored), rows past
+  // it read as zeros from the views.
+  const int bh = tid & 1, bu = (tid >> 1) % S::WN, ju = min((j0 >> 5) + bu, CU - 1), bn = tid / UN;
   struct Units {
-    uint32_t w[BI][BITS], s[BI], b[BI];
+    uint32_t w[HW], s, b;
   };
   const uint32_t row_bytes = (uint32_t)row_words * 4u, group_bytes = (uint32_t)groups * 2u;
-  uint32_t woffs[BI], goffs[BI];
-#pragma unroll
-  for (int i = 0; i < BI; i++) {
-    const uint32_t n = (uint32_t)(bn + NT / UN * i);
-    woffs[i] = n * row_bytes + (uint32_t)(ju * BITS) * 4u;
-    goffs[i] = n * group_bytes + (uint32_t)(ju >> a.gsh) * 2u;
-  }
+  const uint32_t bsh = BITS & 1 ? 16u * bh : 0u;
+  const uint32_t woffs = (uint32_t)bn * row_bytes + (uint32_t)(ju * BITS + bh * (BITS / 2)) * 4u;
+  const uint32_t goffs = (uint32_t)bn * group_bytes + (uint32_t)(ju >> a.gsh) * 2u;
   auto load_units = [&](int chunk, Units& u) {
     const bool second = chunk >= per;
     const GemvProj& p = second ? a.p1 : a.p0;
@@ -434,56 +476,51 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
     const rsrc_t sv = make_rsrc(reinterpret_cast<const unsigned char*>(p.s) + at * group_bytes, (uint32_t)N * group_bytes);
     const rsrc_t bv = make_rsrc(reinterpret_cast<const unsigned char*>(p.b) + at * group_bytes, (uint32_t)N * group_bytes);
     const uint32_t n0 = (uint32_t)((second ? chunk - per : chunk) * kGK);
-#pragma unroll
-    for (int i = 0; i < BI; i++) {
-      const uint32_t g = goffs[i] + n0 * group_bytes;
-      u.s[i] = bload16(sv, g);
-      u.b[i] = bload16(bv, g);
-      bload_unit<BITS>(wv, woffs[i] + n0 * row_bytes, u.w[i]);
-    }
+    u.s = bload16(sv, goffs + n0 * group_bytes);
+    u.b = bload16(bv, goffs + n0 * group_bytes);
+    bload_half<BITS>(wv, woffs + n0 * row_bytes, u.w);
   };
   auto sb_value = [&](uint32_t raw) -> float {
     const float f = (float)__builtin_bit_cast(_Float16, (uint16_t)raw);
     return sb_bf16 ? __uint_as_float(raw << 16) : f;
   };
-  // values [8 q, 8 q + 8) of each unit, into buffer buf
-  auto store_quarter = [&](const Units& u, const float (&s)[BI], const float (&b)[BI], int q, int buf) {
-#pragma unroll
-    for (int i = 0; i < BI; i++) {
-      *reinterpret_cast<u32x4_t*>(L.b + buf * S::BBYTES + wt_off<UN>(bn + NT / UN * i, bu, q)) = weights8<BITS, XT>(u.w[i], q, s[i], b[i]);
-    }
+  // a half's values [8 q, 8 q + 8), hi and lo, into buffer buf
+  auto store_quarter = [&](const uint32_t (&w)[HW], float s, float b, int q, int buf) {
+    u32x4_t hi, lo;
+    weights8<BITS, XT>(w, q, s, b, hi, lo);
+    unsigned char* at = L.b + buf * S::BBYTES;
+    *reinterpret_cast<u32x4_t*>(at + wt_off<UN>(bn, 2 * bu, 2 * bh + q)) = hi;
+    *reinterpret_cast<u32x4_t*>(at + wt_off<UN>(bn, 2 * bu + 1, 2 * bh + q)) = lo;
   };
-  auto unit_sb = [&](const Units& u, float (&s)[BI], float (&b)[BI]) {
+  auto unit_values = [&](const Units& u, uint32_t (&w)[HW], float& s, float& b) {
+    s = sb_value(u.s);
+    b = sb_value(u.b);
 #pragma unroll
-    for (int i = 0; i < BI; i++) {
-      s[i] = sb_value(u.s[i]);
-      b[i] = sb_value(u.b[i]);
-    }
+    for (int i = 0; i < HW; i++) w[i] = u.w[i];
+    shift_half<BITS>(w, bsh);
   };
 
-  f32x16_t acc[MI][NJ];
+  f32x16_t acc[MI][2];  // of the hi parts, of the lo parts
 #pragma unroll
-  for (int i = 0; i < MI; i++)
-#pragma unroll
-    for (int j = 0; j < NJ; j++) acc[i][j] = f32x16_t{};
+  for (int i = 0; i < MI; i++) acc[i][0] = acc[i][1] = f32x16_t{};
 
-  // operands of one 16-value step: gradient rows 32 (MI wm + i) + col, and for
-  // column tile j two transposing reads, of weight rows 16 s + 8 h + 4 q + (lane %
+  // operands of one 16-value step: gradient rows 32 (MI wm + i) + col, and for hi
+  // and lo two transposing reads, of weight rows 16 s + 8 h + 4 q + (lane %
   // 16) / 4 (q < 2): their low two bits are the lane's, so one offset serves all
   struct Frags {
-    u32x4_t w[NJ], d[MI];
+    u32x4_t w[2], d[MI];
   };
   const uint32_t doff = (uint32_t)(32 * MI * wm + col) * 128u;
   const int tr = (lane & 15) >> 2;  // row of four of a transposing read
-  uint32_t woff[NJ];
+  uint32_t woff[2];
 #pragma unroll
-  for (int j = 0; j < NJ; j++)
-    woff[j] = wt_off<UN>(8 * h + tr, NJ * wn + j, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (uint32_t)(lane & 1) * 8u;
+  for (int j = 0; j < 2; j++)
+    woff[j] = wt_off<UN>(8 * h + tr, 2 * wn + j, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (uint32_t)(lane & 1) * 8u;
   auto read_frags = [&](auto st, int buf, int s, Frags& f) {
     const unsigned char* Ab = stage(st);
     const unsigned char* Bb = L.b + buf * S::BBYTES + s * (16 * UN * 64);
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
+    for (int j = 0; j < 2; j++) {
       typedef __attribute__((address_space(3))) s16x4_t lds_t;
       const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(Bb + woff[j])));
       const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(Bb + woff[j] + 4 * UN * 64)));
@@ -497,30 +534,27 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
 #pragma unroll
     for (int i = 0; i < MI; i++)
 #pragma unroll
-      for (int j = 0; j < NJ; j++) acc[i][j] = mma16<XT>(f.w[j], f.d[i], acc[i][j]);
+      for (int j = 0; j < 2; j++) acc[i][j] = mma16<XT>(f.w[j], f.d[i], acc[i][j]);
   };
 
   // Order of a chunk's main part: after each matrix instruction its share of the
   // vector work (kSetup for the scales, kQuarter per quarter of a unit), which
-  // the matrix cores hide; a quarter's store follows when its values are there.
-  // (kQuarter: 17 to 20 made 4 bits 4 to 5% slower; 26 took 3 bits from 266 to 253 us
-  // and left the others as they were.)
-  constexpr int kSetup = 10 * BI, kQuarter = 26 * BI, kWork = kSetup + 4 * kQuarter, kSteps = 3 * MI * NJ;
+  // the matrix cores hide; a quarter's stores follow when its values are there.
+  constexpr int kSetup = 10, kQuarter = 46, kWork = kSetup + 2 * kQuarter, kSteps = 6 * MI;
   auto weave = [&](auto seq) {
     auto one = [&](auto ic) {
       constexpr int i = decltype(ic)::value;
       constexpr int done = kWork * i / kSteps, next = kWork * (i + 1) / kSteps;
       constexpr int stored = done < kSetup ? 0 : (done - kSetup) / kQuarter, store = next < kSetup ? 0 : (next - kSetup) / kQuarter;
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if constexpr (i % (MI * NJ) < (MI * NJ + 1) / 2)  // (the next step's operands, early in this one)
-        __builtin_amdgcn_sched_group_barrier(0x100, (2 * NJ + MI + (MI * NJ + 1) / 2 - 1) / ((MI * NJ + 1) / 2), 0);
+      if constexpr (i % (2 * MI) < MI)  // (the next step's operands, early in this one)
+        __builtin_amdgcn_sched_group_barrier(0x100, (4 + MI + MI - 1) / MI, 0);
       __builtin_amdgcn_sched_group_barrier(0x002, next - done, 0);
-      if constexpr (store > stored) __builtin_amdgcn_sched_group_barrier(0x200, BI * (store - stored), 0);
+      if constexpr (store > stored) __builtin_amdgcn_sched_group_barrier(0x200, 2 * (store - stored), 0);
     };
     each(one, seq);
   };
-  // vector-memory instructions of a chunk's units per thread
-  constexpr int kUnitSet = BI * (2 + kUnitLoads<BITS>);
+  constexpr int kUnitSet = 3;  // vector-memory instructions of a chunk's units per thread
   // Chunk c: rows in stage ST = c % 3, weights in buffer c % 2. Its first
   // operands are read behind the barrier while the previous chunk's last matrix
   // step (operands in registers) runs; chunk c + 2's rows go to the stage that
@@ -540,19 +574,18 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
     __builtin_amdgcn_sched_barrier(0);
     load_units(min(c + 3, nchunks - 1), cu);
     __builtin_amdgcn_sched_barrier(0);
-    float s[BI], b[BI];
-    unit_sb(nu, s, b);
+    uint32_t w[HW];
+    float s, b;
+    unit_values(nu, w, s, b);
     read_frags(st, buf, 1, f1);
     mma_step(f0);
-    store_quarter(nu, s, b, 0, buf ^ 1);
+    store_quarter(w, s, b, 0, buf ^ 1);
     read_frags(st, buf, 2, f0);
     mma_step(f1);
-    store_quarter(nu, s, b, 1, buf ^ 1);
     read_frags(st, buf, 3, last);
     mma_step(f0);
-    store_quarter(nu, s, b, 2, buf ^ 1);
-    store_quarter(nu, s, b, 3, buf ^ 1);
-    weave(std::make_integer_sequence<int, 3 * MI * NJ>{});
+    store_quarter(w, s, b, 1, buf ^ 1);
+    weave(std::make_integer_sequence<int, 6 * MI>{});
     __builtin_amdgcn_sched_barrier(0);
     vmcnt_wait<AI + kUnitSet>();
     lds_barrier_copies_in_flight();
@@ -570,10 +603,11 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
   copy_rows(min(1, nchunks - 1), S1{});
   __builtin_amdgcn_sched_barrier(0);
   {
-    float s[BI], b[BI];
-    unit_sb(u0, s, b);
-#pragma unroll
-    for (int q = 0; q < 4; q++) store_quarter(u0, s, b, q, 0);
+    uint32_t w[HW];
+    float s, b;
+    unit_values(u0, w, s, b);
+    store_quarter(w, s, b, 0, 0);
+    store_quarter(w, s, b, 1, 0);
   }
   vmcnt_wait<0>();
   lds_barrier_copies_in_flight();
@@ -592,76 +626,75 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
   __syncthreads();
 
   // ---- results: lane holds row col of each 32-row tile and columns 8 (r / 4) +
-  // 4 h + r % 4 of each 32-column tile; through LDS, so that a lane stores 16
-  // bytes of a row and its neighbours the bytes beside them
+  // 4 h + r % 4; through LDS, so that a lane stores 16 bytes of a row and its
+  // neighbours the bytes beside them
   uint16_t* out = reinterpret_cast<uint16_t*>(a.dx);
   const uint16_t* base = reinterpret_cast<const uint16_t*>(a.dx_in);
-  constexpr int LINE = 16 + (NJ < 2 ? 2 : NJ) * 64;  // bytes of a staged row
+  constexpr int LINE = 144;  // bytes of a staged row
   static_assert(S::WM * S::WN * 32 * LINE <= 2 * S::BBYTES, "staging");
   unsigned char* mine = L.b + wave * (32 * LINE);
-  const int jw = j0 + 32 * NJ * wn;
+  const int jw = j0 + 32 * wn;
   if (!base) {
 #pragma unroll
     for (int i = 0; i < MI; i++) {
 #pragma unroll
-      for (int j = 0; j < NJ; j++)
+      for (int r = 0; r < 16; r += 4) {
+        typedef XT x4_t __attribute__((ext_vector_type(4)));
+        x4_t v;
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          typedef XT x4_t __attribute__((ext_vector_type(4)));
-          const x4_t v{(XT)acc[i][j][r], (XT)acc[i][j][r + 1], (XT)acc[i][j][r + 2], (XT)acc[i][j][r + 3]};
-          *reinterpret_cast<u32x2_t*>(mine + col * LINE + j * 64 + r * 4 + h * 8) = __builtin_bit_cast(u32x2_t, v);
-        }
-      constexpr int PIECES = NJ * 4;  // of a row
+        for (int k = 0; k < 4; k++) v[k] = (XT)joined(acc[i][0][r + k], acc[i][1][r + k]);
+        *reinterpret_cast<u32x2_t*>(mine + col * LINE + r * 4 + h * 8) = __builtin_bit_cast(u32x2_t, v);
+      }
 #pragma unroll
-      for (int q = 0; q < NJ * 2; q++) {
-        const int at = 64 * q + lane, row = at / PIECES, c8 = at % PIECES;
+      for (int q = 0; q < 2; q++) {
+        const int row = 16 * q + (lane >> 2), c8 = lane & 3;
         const u32x4_t v = *reinterpret_cast<const u32x4_t*>(mine + row * LINE + c8 * 16);
         const uint32_t pos = t.m0 + (uint32_t)(32 * (MI * wm + i) + row);
         if (pos < t.pend && jw + 8 * c8 < K)
           *reinterpret_cast<u32x4_t*>(out + (size_t)pos * K + jw + 8 * c8) = v;
       }
     }
-  } else {  // added to dx_in in fp32: a 32 x 32 tile at a time
+  } else {  // added to dx_in in fp32
 #pragma unroll
-    for (int i = 0; i < MI; i++)
+    for (int i = 0; i < MI; i++) {
 #pragma unroll
-      for (int j = 0; j < NJ; j++) {
+      for (int r = 0; r < 16; r += 4) {
+        typedef float f32x4_t __attribute__((ext_vector_type(4)));
+        f32x4_t v;
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          typedef float f32x4_t __attribute__((ext_vector_type(4)));
-          *reinterpret_cast<f32x4_t*>(mine + col * 144 + r * 8 + h * 16) =
-              f32x4_t{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
-        }
+        for (int k = 0; k < 4; k++) v[k] = joined(acc[i][0][r + k], acc[i][1][r + k]);
+        *reinterpret_cast<f32x4_t*>(mine + col * LINE + r * 8 + h * 16) = v;
+      }
 #pragma unroll
-        for (int q = 0; q < 2; q++) {
-          const int row = 16 * q + (lane >> 2), c8 = lane & 3;
-          float v[8], o[8];
-          Vec8<float>::load(reinterpret_cast<const float*>(mine + row * 144 + c8 * 32), v);
-          const uint32_t pos = t.m0 + (uint32_t)(32 * (MI * wm + i) + row);
-          const int jc = jw + 32 * j + 8 * c8;
-          if (pos < t.pend && jc < K) {
-            const size_t at = (size_t)pos * K + jc;
-            Vec8<XT>::load(reinterpret_cast<const XT*>(base) + at, o);
+      for (int q = 0; q < 2; q++) {
+        const int row = 16 * q + (lane >> 2), c8 = lane & 3;
+        float v[8], o[8];
+        Vec8<float>::load(reinterpret_cast<const float*>(mine + row * LINE + c8 * 32), v);
+        const uint32_t pos = t.m0 + (uint32_t)(32 * (MI * wm + i) + row);
+        const int jc = jw + 8 * c8;
+        if (pos < t.pend && jc < K) {
+          const size_t at = (size_t)pos * K + jc;
+          Vec8<XT>::load(reinterpret_cast<const XT*>(base) + at, o);
 #pragma unroll
-            for (int k = 0; k < 8; k++) o[k] += v[k];
-            Vec8<XT>::store(reinterpret_cast<XT*>(out) + at, o);
-          }
+          for (int k = 0; k < 8; k++) o[k] += v[k];
+          Vec8<XT>::store(reinterpret_cast<XT*>(out) + at, o);
         }
       }
+    }
   }
 }
 
-typedef GradShape<4, 2, 4, 2> GradTall;    // 256 rows x 256 columns
-typedef GradShape<3, 2, 4, 2> GradMost;    // 192 rows
-typedef GradShape<2, 2, 4, 2> GradHalf;    // 128 rows
-typedef GradShape<2, 1, 8, 1> GradQuarter; // 64 rows
+typedef GradShape<4, 4> GradTall;     // 256 rows x 128 columns
+typedef GradShape<3, 4> GradMost;     // 192 rows
+typedef GradShape<2, 4> GradHalf;     // 128 rows
+typedef GradShape<1, 4> GradQuarter;  // 64 rows
 
 template <bool FAR, int BITS, typename XT>
 __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const ExpertGradArgs a) {
   __shared__ __align__(16) unsigned char a0[GradTall::ABYTES], a1[GradTall::ABYTES], a2[GradTall::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradTall::BBYTES];
   GradTile t;
-  if (!grad_tile<GradTall::MR, true>(a, (uint32_t)((a.K + GradTall::NC - 1) / GradTall::NC), &t)) return;
+  if (!grad_tile<GradTall::MR, true>(a, &t)) return;
   const int j0 = t.block * GradTall::NC;
   const GradLds L{a0, a1, a2, b};
   const uint32_t rows = t.pend - t.m0;
@@ -672,42 +705,52 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
 }
 
 // ------------------------------------------------ 16-bit products, few rows --
-// Experts with few rows are bound by how fast their weights arrive. A block takes
-// up to 32 rows and 32 NJ columns; its four waves share the sum (chunks of 128 / NJ
-// values in turn) and meet at the end. A wave dequantises into LDS of its own, so
-// the loop has no barrier: LDS serves a wave's stores and reads in order.
+// Experts with few rows are bound by how fast their weights arrive and are dequantised.
+// A block takes up to 32 rows and 128 WN columns; four waves, WN side by side along the
+// columns, share the sum (chunks of 32 values in turn) and meet at the end. A wave
+// dequantises into LDS of its own, 16 weight rows at a time, so the loop has no barrier:
+// LDS serves a wave's stores and reads in order.
 //
-// 8 rows of each of 128 experts, two 768 x 2048 products at 4 bits, bf16: 64 us, 3.7
-// TB/s of experts and rows; 4 rows of each of 32, 2880 x 2880: 56 us, 2.7 TB/s, where a
-// large copy reaches 5.2. Memory moves no byte twice (the second: L2 misses of 153 MB
-// for 149 MB of experts), and no single part holds it up: without dequantising or
-// without matrix products it takes as long, without the scales' and biases' loads
-// 41 us, without the weights' 36. Three or four sets of loads in flight, eight waves,
-// one load for the scales of two units, column blocks of an expert out of step: no
-// gain. Loads that bypass the caches are slower. Wide blocks (NJ = 8) touch two
-// thirds of the lines per byte.
+// 8 rows of each of 128 experts, two 768 x 2048 products at 4 bits, bf16: 106 us, 2.2
+// TB/s of experts and rows; 6 rows of each of 32, 2880 x 2880: 73 us, 2.1 TB/s, where a
+// large copy reaches 5.2. Of a chunk's 350 vector instructions a wave, a third make the lo
+// parts; with three waves a SIMD for two the second takes 73 us for 87.
+//
+// The hi and lo parts are summed together (128 registers of sums would leave two waves a
+// SIMD): where a sum is not finite, the block sums the hi parts alone again for the
+// elements that were not.
 constexpr int kFewRows = 32;
 constexpr int kFewLine = 64 * 4 + 16;  // a staged row of 64 fp32 columns
 
-template <int NJ, int BITS, typename XT>
-__global__ __launch_bounds__(256, NJ == 8 ? 2 : 3) void expert_grad_few_kernel(const ExpertGradArgs a) {
-  constexpr int FK = 128 / NJ, FC = 32 * NJ, STEPS = FK / 16, ROWS = 64 / NJ;  // ROWS: weight rows of a unit load
-  constexpr int kWave = FK * FC * 2, kLds = 4 * (kFewRows * kFewLine > kWave ? kFewRows * kFewLine : kWave);
-  __shared__ __align__(16) unsigned char lds[kLds];
+// Keeps the compiler from moving a wave's LDS accesses across each other where lanes
+// read what other lanes store. (The hardware serves them in order.)
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
+template <int WN, int BITS, typename XT>
+__global__ __launch_bounds__(256, BITS == 8 ? 2 : 3) void expert_grad_few_kernel(const ExpertGradArgs a) {
+  constexpr int NJ = 4, FK = 32, FC = 128 * WN, STEPS = FK / 16, WK = 4 / WN;
+  constexpr int kPart = 16 * 256;  // hi parts of 16 weight rows; the lo parts behind them
+  constexpr int kWave = kFewRows * kFewLine;
+  static_assert(kWave >= 2 * kPart, "staging");
+  __shared__ __align__(16) unsigned char lds[4 * kWave];
   GradTile t;
-  if (!grad_tile<kFewRows, false>(a, (uint32_t)((a.K + FC - 1) / FC), &t)) return;
+  if (!grad_tile<kFewRows, false>(a, &t)) return;
   const int j0 = t.block * FC, tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, col = lane & 31, h = lane >> 5;
   const int N = a.N, K = a.K, CU = K >> 5, groups = CU >> a.gsh, row_words = CU * BITS;
   const int parts = (N + FK - 1) / FK, nchunks = a.dy2 ? 2 * parts : parts;
   const bool sb_bf16 = a.sb_bf16 != 0;
 
   const uint32_t pos = min(t.m0 + (uint32_t)col, t.pend - 1);
   const size_t arow = (size_t)(a.perm ? grad_row(a, pos) : pos) * N;
-  // lane: unit lane % NJ of weight rows lane / NJ and ROWS + lane / NJ of a chunk
-  const int bu = lane % NJ, ju = min((j0 >> 5) + bu, CU - 1), bn = lane / NJ;
+  // lane: unit lane % 4 of weight rows lane / 4 and 16 + lane / 4 of a chunk
+  const int bu = lane % NJ, ju = min((j0 >> 5) + NJ * wn + bu, CU - 1), bn = lane / NJ;
   struct Chunk {
-    uint32_t w[2][BITS], s[2], b[2];
+    uint32_t w[STEPS][BITS], s[STEPS], b[STEPS];
     u32x4_t d[STEPS];
   };
   auto load = [&](int c, Chunk& u) {
@@ -719,8 +762,8 @@ __global__ __launch_bounds__(256, NJ == 8 ? 2 : 3) void expert_grad_few_kernel(c
     const rsrc_t bv = make_rsrc(reinterpret_cast<const uint16_t*>(p.b) + rows * groups, (uint32_t)N * (uint32_t)groups * 2u);
     const int n0 = (second ? c - parts : c) * FK;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const uint32_t n = (uint32_t)(n0 + bn + ROWS * i), g = (n * (uint32_t)groups + (uint32_t)(ju >> a.gsh)) * 2u;
+    for (int i = 0; i < STEPS; i++) {
+      const uint32_t n = (uint32_t)(n0 + bn + 16 * i), g = (n * (uint32_t)groups + (uint32_t)(ju >> a.gsh)) * 2u;
       bload_unit<BITS>(wv, (n * (uint32_t)row_words + (uint32_t)(ju * BITS)) * 4u, u.w[i]);
       u.s[i] = bload16(sv, g);
       u.b[i] = bload16(bv, g);
@@ -741,114 +784,154 @@ __global__ __launch_bounds__(256, NJ == 8 ? 2 : 3) void expert_grad_few_kernel(c
   for (int j = 0; j < NJ; j++)
     woff[j] = wt_off<NJ>(8 * h + tr, j, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (uint32_t)(lane & 1) * 8u;
   f32x16_t acc[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; j++) acc[j] = f32x16_t{};
-  auto products = [&](int c, const Chunk& u) {
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const float s = sb_value(u.s[i]), b = sb_value(u.b[i]);
-#pragma unroll
-      for (int q = 0; q < 4; q++)
-        *reinterpret_cast<u32x4_t*>(mine + wt_off<NJ>(bn + ROWS * i, bu, q)) = weights8<BITS, XT>(u.w[i], q, s, b);
-    }
+  auto products = [&](auto both, int c, const Chunk& u) {
+    constexpr int PARTS = decltype(both)::value ? 2 : 1;
     const int n0 = (c >= parts ? c - parts : c) * FK;
 #pragma unroll
     for (int s = 0; s < STEPS; s++) {
+      const float sc = sb_value(u.s[s]), bi = sb_value(u.b[s]);
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        u32x4_t hi, lo;
+        weights8<BITS, XT>(u.w[s], q, sc, bi, hi, lo);
+        unsigned char* at = mine + wt_off<NJ>(bn, bu, q);
+        *reinterpret_cast<u32x4_t*>(at) = hi;
+        if constexpr (PARTS == 2) *reinterpret_cast<u32x4_t*>(at + kPart) = lo;
+      }
+      wave_lds_order();
       // (values past the end of the row met zero weights; an infinity there must not)
       const u32x4_t d = n0 + 16 * s + 8 * h < N ? u.d[s] : u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        typedef __attribute__((address_space(3))) s16x4_t lds_t;
-        const unsigned char* at = mine + woff[j] + s * (16 * FC * 2);
-        const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)at));
-        const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(at + 4 * FC * 2)));
-        acc[j] = mma16<XT>(u32x4_t{lo[0], lo[1], hi[0], hi[1]}, d, acc[j]);
+      for (int part = 0; part < PARTS; part++)
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+          typedef __attribute__((address_space(3))) s16x4_t lds_t;
+          const unsigned char* at = mine + part * kPart + woff[j];
+          const u32x2_t x = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)at));
+          const u32x2_t y = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(at + 4 * 256)));
+          acc[j] = mma16<XT>(u32x4_t{x[0], x[1], y[0], y[1]}, d, acc[j]);
+        }
+      wave_lds_order();
+    }
+  };
+  auto sums = [&](auto both) {
+#pragma unroll
+    for (int j = 0; j < NJ; j++) acc[j] = f32x16_t{};
+    Chunk u0, u1;
+    int c = wave / WN;  // chunks c, c + WK, ...; loads past the end repeat the last chunk, unused
+    auto ahead = [&](int at, Chunk& u) {
+      __builtin_amdgcn_sched_barrier(0);  // (loads sink to their uses otherwise)
+      load(min(at, nchunks - 1), u);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    ahead(c, u0);
+    ahead(c + WK, u1);
+    for (; c + WK < nchunks; c += 2 * WK) {
+      products(both, c, u0);
+      ahead(c + 2 * WK, u0);
+      products(both, c + WK, u1);
+      ahead(c + 3 * WK, u1);
+    }
+    if (c < nchunks) products(both, c, u0);
+  };
+  // The waves' sums, 64 columns of each at a time: lane holds row col and columns 8 (r /
+  // 4) + 4 h + r % 4 of each 32; thread tid then adds row tid / 8, columns 8 (tid % 8) on.
+  // Bit q of `left`'s byte (part WN + g): an element that is left, since it is not finite.
+  uint32_t left = 0;
+  auto results = [&](auto both) {
+#pragma unroll
+    for (int part = 0; part < NJ / 2; part++) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const f32x16_t& v = acc[2 * part + j];
+          *reinterpret_cast<float4*>(lds + (wave * kFewRows + col) * kFewLine + j * 128 + r * 8 + h * 16) =
+              make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
+        }
+      __syncthreads();
+      const int row = tid >> 3;
+      const uint32_t p = t.m0 + (uint32_t)row;
+#pragma unroll
+      for (int g = 0; g < WN; g++) {
+        const int jc = j0 + 128 * g + 64 * part + 8 * (tid & 7), byte = 8 * (part * WN + g);
+        if (p < t.pend && jc < K) {
+          float v[WK][8], o[8] = {};
+#pragma unroll
+          for (int w = 0; w < WK; w++)
+            Vec8<float>::load(reinterpret_cast<const float*>(lds + ((w * WN + g) * kFewRows + row) * kFewLine + (tid & 7) * 32), v[w]);
+          const size_t at = (size_t)p * K + jc;
+          if (a.dx_in) Vec8<XT>::load(reinterpret_cast<const XT*>(a.dx_in) + at, o);
+          uint32_t odd = 0;
+#pragma unroll
+          for (int q = 0; q < 8; q++) {
+            float sum = v[0][q] + v[1][q];
+            if constexpr (WK == 4) sum += v[2][q] + v[3][q];
+            if (!(__builtin_fabsf(sum) < __builtin_huge_valf())) odd |= 1u << q;
+            o[q] += sum;
+          }
+          XT* out = reinterpret_cast<XT*>(a.dx) + at;
+          if (decltype(both)::value && !odd) {
+            Vec8<XT>::store(out, o);
+          } else {
+            const uint32_t now = decltype(both)::value ? ~odd : left >> byte;
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+              if (now >> q & 1u) out[q] = (XT)o[q];
+            if constexpr (decltype(both)::value) left |= odd << byte;
+          }
+        }
       }
     }
   };
-  Chunk u0, u1;
-  int c = wave;  // chunks wave, wave + 4, ...; loads past the end repeat the last chunk, unused
-  auto ahead = [&](int at, Chunk& u) {
-    __builtin_amdgcn_sched_barrier(0);  // (loads sink to their uses otherwise)
-    load(min(at, nchunks - 1), u);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  ahead(c, u0);
-  ahead(c + 4, u1);
-  for (; c + 4 < nchunks; c += 8) {
-    products(c, u0);
-    ahead(c + 8, u0);
-    products(c + 4, u1);
-    ahead(c + 12, u1);
-  }
-  if (c < nchunks) products(c, u0);
-  // ---- the waves' sums, 64 columns at a time: lane holds row col and columns 8 (r /
-  // 4) + 4 h + r % 4 of each 32; thread tid then adds row tid / 8, columns 8 (tid % 8) on
-#pragma unroll
-  for (int part = 0; part < NJ / 2; part++) {
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 2; j++)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const f32x16_t& v = acc[2 * part + j];
-        *reinterpret_cast<float4*>(lds + (wave * kFewRows + col) * kFewLine + j * 128 + r * 8 + h * 16) =
-            make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
-      }
-    __syncthreads();
-    const int row = tid >> 3, jc = j0 + 64 * part + 8 * (tid & 7);
-    const uint32_t p = t.m0 + (uint32_t)row;
-    if (p < t.pend && jc < K) {
-      float v[4][8], o[8] = {};
-#pragma unroll
-      for (int w = 0; w < 4; w++)
-        Vec8<float>::load(reinterpret_cast<const float*>(lds + (w * kFewRows + row) * kFewLine + (tid & 7) * 32), v[w]);
-      const size_t at = (size_t)p * K + jc;
-      if (a.dx_in) Vec8<XT>::load(reinterpret_cast<const XT*>(a.dx_in) + at, o);
-#pragma unroll
-      for (int q = 0; q < 8; q++) o[q] += (v[0][q] + v[1][q]) + (v[2][q] + v[3][q]);
-      Vec8<XT>::store(reinterpret_cast<XT*>(a.dx) + at, o);
-    }
-  }
+  sums(std::true_type{});
+  results(std::true_type{});
+  if (!__syncthreads_or(left != 0)) return;
+  sums(std::false_type{});
+  results(std::false_type{});
 }
 
-typedef GradShape<4, 1, 4, 1> GradMid;  // 128 rows x 128 columns
-typedef GradShape<2, 1, 4, 1> GradMidHalf;
-typedef GradShape<1, 1, 4, 1> GradMidQuarter;
+typedef GradShape<2, 2> GradMid;  // 128 rows x 64 columns
+typedef GradShape<1, 2> GradMidHalf;
 
 template <bool FAR, int BITS, typename XT>
 __global__ __launch_bounds__(GradMid::NT, 2) void expert_grad_mid_kernel(const ExpertGradArgs a) {
   __shared__ __align__(16) unsigned char a0[GradMid::ABYTES], a1[GradMid::ABYTES], a2[GradMid::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradMid::BBYTES];
   GradTile t;
-  if (!grad_tile<GradMid::MR, true>(a, (uint32_t)((a.K + GradMid::NC - 1) / GradMid::NC), &t)) return;
+  if (!grad_tile<GradMid::MR, true>(a, &t)) return;
   const int j0 = t.block * GradMid::NC;
   const GradLds L{a0, a1, a2, b};
   const uint32_t rows = t.pend - t.m0;
   if (rows > 64) grad_tile_mma<GradMid, FAR, BITS, XT>(a, L, t, j0);
-  else if (rows > 32) grad_tile_mma<GradMidHalf, FAR, BITS, XT>(a, L, t, j0);
-  else grad_tile_mma<GradMidQuarter, FAR, BITS, XT>(a, L, t, j0);
+  else grad_tile_mma<GradMidHalf, FAR, BITS, XT>(a, L, t, j0);
 }
 
-// Which kernel. Few rows an expert (up to 28 on average, fewer where a weight has
-// more than 4 bits): the few-row kernel, wide where that leaves blocks for most of
-// the chip (320, at two a CU). Else the tall kernel, unless its blocks would not
-// fill the chip; then the ordinary one. us per call of gate and up 768 x 2048 at 4
-// bits, bf16, experts of unequal popularity, few (wide) / ordinary / tall: 128 experts of
-// 16 rows 79 / 85 / 92, of 24 82 / 89 / 94, of 32 94 / 93 / 96, of 64 151 / 117 / 117, of
-// 256 479 / 307 / 243; 8 experts of 256 rows 34 / 23 / 33; one of 4096 61 / 34 / 36.
-// Few rows, narrow / wide, with the wide blocks: 8 experts of 16 rows (64) 14.5 / 23, 32
-// of one row (256) 23.3 / 25.1, 40 of 8 (320) 32.3 / 30.8, 60 of 12, 1408 x 2048 at 3 bits
-// (480) 68 / 60, 20 of 20, 5120 x 5120 (400) 125 / 99.
+// Which kernel. Up to 44 rows an expert on average the few-row kernel, its blocks wide
+// from 20 rows on where that leaves enough for most of the chip (320); else the tall
+// kernel, unless its blocks would not fill the chip (160), then the ordinary one.
+// us per call of gate and up 768 x 2048 at 4 bits, bf16, experts of unequal popularity,
+// few / wide / ordinary / tall: 128 experts of 16 rows 110 / 118 / 180 / 178, of 24 122 /
+// 119 / 185 / 180, of 32 143 / 140 / 192 / 189, of 48 196 / 188 / 204 / 193, of 64 238 /
+// 228 / 218 / 219, of 128 426 / 389 / 340 / 284. Other formats: 32 rows of 2 bits 139 / 132
+// / 186 / 190, 5 bits 166 / 158 / 205 / 202, 6 bits 168 / 157 / 210 / 197, 8 bits 183 / 167
+// / 211 / 203; 48 rows of 2 bits 188 / 178 / 191 / 191, 5 bits 224 / 208 / 213 / 211, 6 bits
+// 224 / 211 / 215 / 204, 8 bits 246 / 223 / 218 / 207; f16, 3 bits, 256 experts 512 x 2048 of
+// 24 rows 192 / 184 / 280 / 298, of 48 322 / 288 / 311 / 314.
+// Few blocks: 32 experts of 32 rows (256 wide ones) 33 / 38, 20 of 20 rows, 5120 x 5120
+// (400) 164 / 160; ordinary and tall, 8 of 256 rows (128 tall ones) 34 / 39, 4 of 512, 2880
+// x 2880 (184) 85 / 70, one of 4096 (256) 67 / 49.
 template <int BITS, typename XT>
 static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
-  const int64_t used = std::min(a.E, a.M), wide = (a.K + 255) / 256;  // blocks of 256 columns
-  if ((int64_t)a.M <= 28 * (int64_t)a.E && (int64_t)a.M * BITS <= 100 * (int64_t)a.E) {
-    if (used * wide >= 320) return launch_grad(expert_grad_few_kernel<8, BITS, XT>, a, kFewRows, 256, 256, st);
-    return launch_grad(expert_grad_few_kernel<4, BITS, XT>, a, kFewRows, 128, 256, st);
+  const int64_t used = std::min(a.E, a.M);
+  if ((int64_t)a.M <= 44 * (int64_t)a.E) {
+    if ((int64_t)a.M >= 20 * (int64_t)a.E && used * ((a.K + 255) / 256) >= 320)
+      return launch_grad(expert_grad_few_kernel<2, BITS, XT>, a, kFewRows, 256, 256, st);
+    return launch_grad(expert_grad_few_kernel<1, BITS, XT>, a, kFewRows, 128, 256, st);
   }
   const bool far = a.perm && (int64_t)a.rows * a.N * 2 > 0xFFFFFFFFll;
-  if (std::max<int64_t>(used, a.M / GradTall::MR) * wide < 256)
+  if (std::max<int64_t>(used, a.M / GradTall::MR) * ((a.K + GradTall::NC - 1) / GradTall::NC) < 160)
     return launch_grad(far ? expert_grad_mid_kernel<true, BITS, XT> : expert_grad_mid_kernel<false, BITS, XT>, a, GradMid::MR,
                        GradMid::NC, GradMid::NT, st);
   return launch_grad(far ? expert_grad_tall_kernel<true, BITS, XT> : expert_grad_tall_kernel<false, BITS, XT>, a, GradTall::MR,

@@ -343,6 +343,7 @@ struct ExpertGradArgs {
   int M, N, K, E;
   int gsh;                   // log2(group size / 32)
   int sb_bf16;               // 16-bit rows: scales and biases stored as bf16 (else f16)
+  int first, nb;             // the launch's blocks of columns
 };
 hipError_t launch_expert_grad(int bits, int xdt, int sbdt, const ExpertGradArgs& a, hipStream_t st);
 

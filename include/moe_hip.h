@@ -422,10 +422,11 @@ moe_status moe_lora_backward(const moe_lora* l, const void* x, const void* dy, i
  * p2 and dy2 are NULL together; p2 has p's shape, bits, group size and scale
  * type. dy [M or ceil(M / top_k), n], dx_in (nullable, may be dx) and dx [M, k]
  * in dtype, 16-byte aligned; n a multiple of 8, n_experts at most 1024, M at
- * most 2^23. A 16-bit dtype multiplies weights rounded to it (half a step: 2^-8
- * of the weight for bf16, 2^-11 for f16); f32 rounds them to f32 only, and
- * scales have to be below 2^104 in magnitude for a 16-bit one. Output biases have
- * no part in it. Infinities and NaN stay in their rows of dy, and in weights in
+ * most 2^23. A 16-bit dtype multiplies each weight as two values of that type,
+ * off by 2^-17 of it at most for bf16, by 2^-23 of it or 2^-25 (the larger) for
+ * f16, where a weight of 65520 or more in magnitude is infinite; f32 rounds
+ * weights to f32. Scales have to be below 2^104 in magnitude for a 16-bit dtype.
+ * Output biases have no part in it. Infinities and NaN stay in their rows of dy, and in weights in
  * their expert; with n not a multiple of 64 an infinity in the last 8 values of a
  * 16-bit row may give NaN throughout that row of dx. */
 moe_status moe_expert_matmul_backward(const moe_qproj* p, const void* dy, const moe_qproj* p2,

@@ -1,0 +1,127 @@
+"""What the gradients through the experts keep of their inputs: weights, sums and slopes to fp32's precision,
+kept values in every type, rows apart from one another."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_gpu_expert_grad import CASES, grad64, picks, plan, stack  # noqa: E402
+from test_gpu_tuning import BF16, F16, F32, U, close, cuda, gen, same_bits  # noqa: E402
+
+from ffai_amd import _lib, tuning  # noqa: E402
+from ffai_amd.layer import StackedExperts  # noqa: E402
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    _lib.load()
+    yield
+    torch.cuda.synchronize()
+
+
+def packed(q, s, b, bits, gs):
+    """A stack of codes q [E, N, K] with scales and biases [E, N, K / gs]."""
+    E, N, K = q.shape
+    stream = ((q[..., None] >> torch.arange(bits)) & 1).reshape(E, N, K * bits // 32, 32)
+    w = (stream.long() << torch.arange(32)).sum(-1)
+    return StackedExperts(torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32).cuda(), s.cuda(), b.cuda(), bits, gs)
+
+
+# rows that take the kernels of few rows (narrow and wide blocks), of 128 and of 256 rows
+ROWS = [(8, 30), (64, 100), (4, 900), (40, 2000)]
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("bits", [2, 3, 4, 5, 6, 8])
+@pytest.mark.parametrize("E,T", ROWS)
+def test_weights_that_differ_in_their_last_bits(dt, bits, E, T):
+    """Weights 1 + q 2^-10 (bf16) or 1 + q 2^-13 (f16), whose bits pass the type's: the difference of two, which the
+    type holds, comes out exactly."""
+    N, K, gs = 104, 2080, 32
+    low = -10 if dt == BF16 else -13
+    g = gen(bits)
+    q = torch.randint(0, 2 ** bits, (E, N, K), generator=g)
+    s, b = torch.full((E, N, K // gs), 2.0 ** low, dtype=dt), torch.ones(E, N, K // gs, dtype=dt)
+    p = packed(q, s, b, bits, gs)
+    _, _, offsets = plan(picks(T, E, 1, 5), E)
+    at = torch.stack([torch.randperm(N, generator=g)[:2] for _ in range(T)])
+    dy = torch.zeros(T, N).scatter_(1, at[:, :1], 1.0).scatter_(1, at[:, 1:], -1.0).to(dt)
+    e = torch.searchsorted(offsets[1:].long(), torch.arange(T), right=True)
+    ref = (q[e, at[:, 0]] - q[e, at[:, 1]]).double() * 2.0 ** low
+    for kw in ({}, dict(proj2=p, dy2=dy.cuda())):
+        got = tuning.expert_matmul_backward(p, dy.cuda(), offsets.cuda(), **kw)
+        assert torch.equal(got.cpu().double(), ref * (2 if kw else 1))
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("T,E,k,N,K,bits,gs,pair,gather,add,kind", CASES)
+def test_products_keep_their_weights(dt, T, E, k, N, K, bits, gs, pair, gather, add, kind):
+    """A weight enters as two values of the type: the second is off by at most half a step of at most half a step, 2^-16
+    (bf16) or 2^-22 (f16, there 2^-25 at least) of the weight. Sums are fp32."""
+    M, g = T * k, gen(T + N)
+    sb = dt if T != 37 else (F16 if dt == BF16 else BF16)
+    stacks = [stack(E, N, K, bits, gs, sb, 7 * i + E) for i in range(2 if pair else 1)]
+    perm, _, offsets = plan(picks(T, E, k, T, kind), E)
+    if not gather:
+        perm = None
+    dys = [(torch.randn(T if gather else M, N, generator=g) * 0.01).to(dt) for _ in stacks]
+    base = (torch.randn(M, K, generator=g) * 0.01).to(dt) if add else torch.zeros(M, K, dtype=dt)
+    ref, mag, only = grad64([w for _, w in stacks], dys, offsets, perm, k, base)
+    kw = dict(perm=cuda(perm), top_k=k, dx=base.cuda() if add else None, out=torch.zeros(M, K, dtype=dt).cuda())
+    if pair:
+        kw.update(proj2=stacks[1][0], dy2=dys[1].cuda())
+    got = tuning.expert_matmul_backward(stacks[0][0], dys[0].cuda(), offsets.cuda(), **kw)
+    used, n = int(offsets[-1]), N * len(stacks)
+    two = torch.finfo(dt).eps ** 2 / 4
+    tol = mag * (two + (2 * n + 8) * U) + only * (2.0 ** -25 if dt == F16 else 0.0) + base.double().abs() * 2 * U
+    close(got[:used], ref[:used], tol[:used], "dx")
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("E,T", ROWS)
+def test_infinities_come_out_as_such(dt, E, T):
+    """An infinite gradient or weight gives infinities of its sign, as the sum has them, not NaN."""
+    N, K, gs = 64, 2080, 32
+    q = torch.randint(1, 16, (E, N, K), generator=gen(1))
+    s, b = torch.full((E, N, K // gs), 2.0 ** -10, dtype=dt), torch.full((E, N, K // gs), 0.75, dtype=dt)
+    p = packed(q, s, b, 4, gs)
+    _, _, offsets = plan(picks(T, E, 1, 5), E)
+    dy = torch.ones(T, N, dtype=dt)
+    plain = tuning.expert_matmul_backward(p, dy.cuda(), offsets.cuda())
+    dy[0, 3], dy[T - 1, 50] = float("inf"), float("-inf")
+    got = tuning.expert_matmul_backward(p, dy.cuda(), offsets.cuda())
+    assert (got[0] == float("inf")).all() and (got[T - 1] == float("-inf")).all()
+    assert same_bits(got[1:T - 1], plain[1:T - 1])
+    last = int((offsets[1:] > offsets[:-1]).nonzero().max())
+    p.biases[last, 9, 1] = float("-inf")
+    got = tuning.expert_matmul_backward(p, torch.ones(T, N, dtype=dt).cuda(), offsets.cuda())
+    a = int(offsets[last])
+    assert (got[a:, 32:64] == float("-inf")).all() and same_bits(got[:a], plain[:a])
+    assert same_bits(got[a:, :32], plain[a:, :32]) and same_bits(got[a:, 64:], plain[a:, 64:])
+
+
+def test_wide_rows_of_many_experts():
+    """Just past the few-row kernel's rows, 1024 experts of 2^20 columns: more column blocks than one launch holds."""
+    if torch.cuda.mem_get_info()[0] < 130 << 30:
+        pytest.skip("needs 130 GB")
+    E, N, K, M = 1024, 8, 1 << 20, 45100
+    w = torch.randint(-2 ** 31, 2 ** 31 - 1, (1, N, K // 16), dtype=torch.int64, generator=gen(1)).to(torch.int32)
+    w = w.cuda().repeat(E, 1, 1)
+    s = torch.full((E, N, K // 128), 2.0 ** -6, dtype=BF16, device="cuda")
+    b = torch.arange(E, device="cuda").to(BF16)[:, None, None].expand(E, N, K // 128).contiguous()
+    p = StackedExperts(w, s, b, 2, 128)
+    offsets = torch.linspace(0, M, E + 1, dtype=torch.float64).round().to(torch.int32)
+    dy = (torch.arange(M * N) % 7 - 3).reshape(M, N).to(BF16)
+    dx = tuning.expert_matmul_backward(p, dy.cuda(), offsets.cuda())
+    q = (w[0, :, :, None] >> (2 * torch.arange(16, device="cuda"))) & 3
+    q = q.reshape(N, K).double()
+    for row in (0, 44, 22550, M - 1):
+        e = int(torch.searchsorted(offsets[1:].long(), torch.tensor(row), right=True))
+        d = dy[row].double().cuda()
+        ref = d @ (q * 2.0 ** -6 + b[e, 0, 0].double())
+        mag = d.abs() @ (q * 2.0 ** -6 + b[e, 0, 0].double())
+        close(dx[row], ref, mag.cpu() * (2.0 ** -16 + 32 * U), f"row {row}")
+    del dx
+    torch.cuda.empty_cache()
