@@ -408,6 +408,14 @@ __device__ __forceinline__ void shift_half(uint32_t (&w)[kHalfWords<BITS>], uint
   }
 }
 
+// Keeps the compiler from moving a wave's LDS accesses across each other where lanes
+// read what other lanes store. (The hardware serves them in order.)
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // f(0), f(1), ... with the numbers as types.
 template <typename F, int... I>
 __device__ __forceinline__ void each(F& f, std::integer_sequence<int, I...>) {
@@ -645,6 +653,7 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
         for (int k = 0; k < 4; k++) v[k] = (XT)joined(acc[i][0][r + k], acc[i][1][r + k]);
         *reinterpret_cast<u32x2_t*>(mine + col * LINE + r * 4 + h * 8) = __builtin_bit_cast(u32x2_t, v);
       }
+      wave_lds_order();
 #pragma unroll
       for (int q = 0; q < 2; q++) {
         const int row = 16 * q + (lane >> 2), c8 = lane & 3;
@@ -653,6 +662,7 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
         if (pos < t.pend && jw + 8 * c8 < K)
           *reinterpret_cast<u32x4_t*>(out + (size_t)pos * K + jw + 8 * c8) = v;
       }
+      wave_lds_order();
     }
   } else {  // added to dx_in in fp32
 #pragma unroll
@@ -665,6 +675,7 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
         for (int k = 0; k < 4; k++) v[k] = joined(acc[i][0][r + k], acc[i][1][r + k]);
         *reinterpret_cast<f32x4_t*>(mine + col * LINE + r * 8 + h * 16) = v;
       }
+      wave_lds_order();
 #pragma unroll
       for (int q = 0; q < 2; q++) {
         const int row = 16 * q + (lane >> 2), c8 = lane & 3;
@@ -680,6 +691,7 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
           Vec8<XT>::store(reinterpret_cast<XT*>(out) + at, o);
         }
       }
+      wave_lds_order();
     }
   }
 }
@@ -721,14 +733,6 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
 // elements that were not.
 constexpr int kFewRows = 32;
 constexpr int kFewLine = 64 * 4 + 16;  // a staged row of 64 fp32 columns
-
-// Keeps the compiler from moving a wave's LDS accesses across each other where lanes
-// read what other lanes store. (The hardware serves them in order.)
-__device__ __forceinline__ void wave_lds_order() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-}
 
 template <int WN, int BITS, typename XT>
 __global__ __launch_bounds__(256, BITS == 8 ? 2 : 3) void expert_grad_few_kernel(const ExpertGradArgs a) {
