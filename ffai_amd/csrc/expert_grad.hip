@@ -439,7 +439,8 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
   // ---- gradient rows: thread tid copies, for i < AI, the piece that belongs in
   // slot tid % 8 of LDS row tid / 8 + NT / 8 * i (a wave's 64 lanes write one KB)
   // 32-bit offsets from a uniform base (FAR: gathered rows past 4 GB, 64-bit ones).
-  // Behind the end of a row its last piece comes again: it meets zero weights.
+  // Behind the end of a row its last piece comes again, and zeros take its place when it
+  // has arrived (end_rows): an infinity there must not meet the zero weights.
   const int ac = (tid & 7) ^ grad_swz(tid >> 3);
   uint32_t row[AI];
   const uint64_t first = a.perm ? 0 : (uint64_t)t.m0 * (uint64_t)N * 2u;
@@ -463,6 +464,13 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)at,
                                        (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
     }
+  };
+  auto end_rows = [&](int chunk, auto st) {
+    const int c0 = (chunk >= per ? chunk - per : chunk) * kGK;
+    if (chunk < nchunks && c0 + kGK > N && c0 + 8 * ac >= N)
+#pragma unroll
+      for (int i = 0; i < AI; i++)
+        *reinterpret_cast<u32x4_t*>(stage(st) + NT / 8 * i * 128 + tid * 16) = u32x4_t{0u, 0u, 0u, 0u};
   };
 
   // ---- weights: thread tid dequantises half tid % 2 of unit tid / 2 % WN of row tid /
@@ -596,6 +604,7 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
     weave(std::make_integer_sequence<int, 6 * MI>{});
     __builtin_amdgcn_sched_barrier(0);
     vmcnt_wait<AI + kUnitSet>();
+    end_rows(c + 1, std::integral_constant<int, (ST + 1) % 3>{});
     lds_barrier_copies_in_flight();
   };
 
@@ -618,6 +627,7 @@ __device__ __forceinline__ void grad_tile_mma(const ExpertGradArgs& a, const Gra
     store_quarter(w, s, b, 1, 0);
   }
   vmcnt_wait<0>();
+  end_rows(0, S0{});
   lds_barrier_copies_in_flight();
   Frags last;
   chunk_step(std::true_type{}, S0{}, 0, u0, u1, last);

@@ -426,9 +426,8 @@ moe_status moe_lora_backward(const moe_lora* l, const void* x, const void* dy, i
  * off by 2^-17 of it at most for bf16, by 2^-23 of it or 2^-25 (the larger) for
  * f16, where a weight of 65520 or more in magnitude is infinite; f32 rounds
  * weights to f32. Scales have to be below 2^104 in magnitude for a 16-bit dtype.
- * Output biases have no part in it. Infinities and NaN stay in their rows of dy, and in weights in
- * their expert; with n not a multiple of 64 an infinity in the last 8 values of a
- * 16-bit row may give NaN throughout that row of dx. */
+ * Output biases have no part in it. Infinities and NaN stay in their rows of dy,
+ * and in weights in their expert. */
 moe_status moe_expert_matmul_backward(const moe_qproj* p, const void* dy, const moe_qproj* p2,
                                       const void* dy2, int32_t dtype, const uint32_t* perm,
                                       int32_t top_k, int32_t M, const uint32_t* offsets,

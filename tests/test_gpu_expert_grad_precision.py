@@ -125,3 +125,23 @@ def test_wide_rows_of_many_experts():
         close(dx[row], ref, mag.cpu() * (2.0 ** -16 + 32 * U), f"row {row}")
     del dx
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("N", [8, 56, 72, 104])
+@pytest.mark.parametrize("E,T", ROWS)
+def test_infinity_in_the_last_values_of_a_row(dt, N, E, T):
+    """Of n values that end inside a chunk: weights of one sign give the infinity, whatever the number of rows."""
+    K = 2080
+    q = torch.randint(0, 16, (E, N, K), generator=gen(N))
+    p = packed(q, torch.full((E, N, K // 32), 2.0 ** -6, dtype=dt), torch.ones(E, N, K // 32, dtype=dt), 4, 32)
+    _, _, offsets = plan(picks(T, E, 1, 5), E)
+    dy = torch.ones(T, N, dtype=dt)
+    plain = tuning.expert_matmul_backward(p, dy.cuda(), offsets.cuda(), proj2=p, dy2=dy.cuda())
+    bad, bad2 = dy.clone(), dy.clone()
+    bad[T // 2, N - 1], bad2[T - 1, N - 8:] = float("inf"), float("-inf")
+    got = tuning.expert_matmul_backward(p, bad.cuda(), offsets.cuda(), proj2=p, dy2=bad2.cuda())
+    assert (got[T // 2] == float("inf")).all() and (got[T - 1] == float("-inf")).all()
+    keep = torch.ones(T, dtype=torch.bool)
+    keep[[T // 2, T - 1]] = False
+    assert same_bits(got[keep.cuda()], plain[keep.cuda()])
