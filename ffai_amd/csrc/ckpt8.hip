@@ -106,6 +106,10 @@ __global__ __launch_bounds__(256) void restore_kernel(const int8_t* __restrict__
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < numel; i += (int64_t)gridDim.x * 2048) {
     float v[8];
     kept_values(*reinterpret_cast<const uint2*>(codes + i), scales[i / kKeepBlock], v);
+    if constexpr (__is_same(XT, f16_t)) {  // (65024 to 65504 are kept as 64 steps of 1024, which f16 has not)
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = __builtin_fabsf(v[j]) == 65536.0f ? __builtin_copysignf(65504.0f, v[j]) : v[j];
+    }
     Vec8<XT>::store(out + i, v);
   }
 }

@@ -447,7 +447,8 @@ moe_status moe_activation_save(const void* gate, const void* up, int32_t M, int3
                                void* out, int8_t* codes, uint8_t* scales, hipStream_t stream);
 
 /* The values kept: out[i] = round(codes[i] * 2^(scales[i / 32] - 133)), NaN
- * where the exponent byte is 255. numel a multiple of 32. */
+ * where the exponent byte is 255; in f16 65504 for 65536, as which the largest
+ * values of f16 rows are kept. numel a multiple of 32. */
 moe_status moe_checkpoint_restore(const int8_t* codes, const uint8_t* scales, int64_t numel, void* out,
                                   int32_t dtype, hipStream_t stream);
 

@@ -145,3 +145,24 @@ def test_infinity_in_the_last_values_of_a_row(dt, N, E, T):
     keep = torch.ones(T, dtype=torch.bool)
     keep[[T // 2, T - 1]] = False
     assert same_bits(got[keep.cuda()], plain[keep.cuda()])
+
+
+# ---------------------------------------------------------------- kept values --
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+def test_the_largest_values_come_back(dt):
+    """Finite values of the type's last steps are restored within half a step of their block's: f16 has no 65536."""
+    top = {F16: [65504.0, 65472.0, 65280.0, 65248.0, 65024.0, 64992.0, 64512.0],
+           BF16: [3.36e38, 3.2e38, 1.7e38], F32: [3.38e38, 3.2e38, 1.7e38]}[dt]
+    v = torch.randn(2 * len(top), 32, generator=gen(2)) * (top[0] / 8)
+    for i, x in enumerate(top):
+        v[2 * i, 5], v[2 * i + 1, 9] = x, -x
+    v = v.to(dt)
+    _, kept = tuning.activation_save(None, v.cuda(), _lib.MOE_ACT_RELU2)
+    back = kept.restore(dt).cpu()[0]
+    step = torch.exp2(kept.scales[0].double().cpu() - 133).repeat_interleave(32, -1)
+    assert back.isfinite().all() and ((back.double() - v.double()).abs() <= step / 2).all()
+    if dt == F16:  # what no f16 row holds is rounded as ever
+        far = torch.tensor([[70000.0] + [0.0] * 31])
+        _, kept = tuning.activation_save(None, far.cuda(), _lib.MOE_ACT_RELU2)
+        assert kept.restore(F16)[0, 0, 0] == float("inf")
