@@ -438,7 +438,8 @@ moe_status moe_expert_matmul_backward(const moe_qproj* p, const void* dy, const 
  * [2, M, n / 32], gate first; with MOE_ACT_RELU2 [1, ...], up only. A block of
  * 32 columns has the least e in 0..254 with |v| < 127.5 * 2^(e - 133) for all
  * its values, and codes round(v * 2^(133 - e)) (ties to even): no value is off
- * by more than half a step, 2^-7.98 of the block's largest at most. A block
+ * by more than half a step, 2^-6.99 of the block's largest at most (the largest
+ * is 63.75 steps or more; with e = 0, below 2^-126, 2^-134 instead). A block
  * with an infinity, a NaN or a magnitude of 2^128 (1 - 2^-8) or more has e = 255
  * and reads as NaN. n a multiple of 32. n_rows (nullable, on the device): only
  * the rows below *n_rows are read and written (a plan's offsets + n_experts). */

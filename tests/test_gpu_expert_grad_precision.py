@@ -166,3 +166,28 @@ def test_the_largest_values_come_back(dt):
         far = torch.tensor([[70000.0] + [0.0] * 31])
         _, kept = tuning.activation_save(None, far.cuda(), _lib.MOE_ACT_RELU2)
         assert kept.restore(F16)[0, 0, 0] == float("inf")
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+def test_how_far_a_kept_value_is_off(dt):
+    """By half a step, and a block's largest is 63.75 steps at least: 2^-6.99 of it. A largest value just above that
+    and a tie come to 2^-7, more than 2^-7.98. Where the exponent ends, half of 2^-133."""
+    most = 0.5 / 63.75
+    g = gen(7)
+    top = 1.0 + torch.rand(512, 1, generator=g) ** 4
+    v = (torch.rand(512, 32, generator=g) * 2 - 1) * top
+    v[:, :1] = top
+    v[0], v[1] = 0.0, 0.0
+    v[0, 0], v[0, 1] = 1.0, 0.5 + 2.0 ** -7  # 32.5 steps of 2^-6
+    v[1, 0], v[1, 1] = 63.75 / 64, 33.5 / 64  # the least that takes this step (in f32, f16)
+    v = (v * torch.exp2(torch.randint(-10, 10, (512, 1), generator=g).float())).to(dt)
+    _, kept = tuning.activation_save(None, v.cuda(), _lib.MOE_ACT_RELU2)
+    off = (kept.restore(F32)[0].double().cpu() - v.double()).abs().amax(1) / v.double().abs().amax(1)
+    assert (off <= most).all() and off[0] == 2.0 ** -7
+    if dt != F16:  # f16 has no value so small
+        v = torch.zeros(3, 32)
+        v[0, 0], v[1, 0], v[1, 1], v[2, 0], v[2, 1] = 2.0 ** -133, 2.0 ** -127, 2.0 ** -133, 1.5 * 2.0 ** -132, 1.5 * 2.0 ** -133
+        v = v.to(dt)
+        _, kept = tuning.activation_save(None, v.cuda(), _lib.MOE_ACT_RELU2)
+        assert (kept.scales == 0).all()
+        assert ((kept.restore(F32)[0].double().cpu() - v.double()).abs() <= 2.0 ** -134).all()
