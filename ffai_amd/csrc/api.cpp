@@ -1569,6 +1569,13 @@ extern "C" moe_status moe_add_rmsnorm_backward(const void* residual, const void*
   const size_t need = norm_backward_ws_bytes(n_rows, row_size);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(MOE_ERR_WORKSPACE, "add_rmsnorm_backward: 16-byte aligned workspace of %zu bytes needed", need);
+  if (need) {
+    for (const void* b : {residual, d_normed, d_residual, (const void*)d_in})
+      if (overlaps(workspace, need, b, rows))
+        return fail(MOE_ERR_INVALID, "add_rmsnorm_backward: the workspace overlaps rows");
+    if (overlaps(workspace, need, weight, wb) || overlaps(workspace, need, d_weight, dwb))
+      return fail(MOE_ERR_INVALID, "add_rmsnorm_backward: the workspace overlaps a weight");
+  }
   MOE_HIP(launch_norm_backward(residual, weight, d_normed, d_residual, eps, n_rows, row_size, dtype, d_in,
                                d_weight, workspace, stream),
           "add + RMSNorm backward launch");
