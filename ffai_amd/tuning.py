@@ -507,10 +507,9 @@ def activation_backward(kept: Checkpoint8, dh: torch.Tensor, activation: int = _
     """Gradients of activation_save at the values kept, for dh [M, n], the
     gradient of h before the routing weights. topk_weight (M float32, any shape)
     are those weights in token order and perm [M] int32 the plan's (None: in
-    order; without offsets it names every pick once); with them come their
+    order; it names no pick twice, and an entry past M none); with them come their
     gradient too (unless want_weight is False) and h itself if want_h. offsets: as
-    in activation_save; the weights of picks without a row then get a zero
-    gradient."""
+    in activation_save. The weights of picks without a row get a zero gradient."""
     M, n = _rows("dh", dh, 2).shape
     at, dt = dh.get_device(), dh.dtype
     gated = activation != _lib.MOE_ACT_RELU2
@@ -531,7 +530,8 @@ def activation_backward(kept: Checkpoint8, dh: torch.Tensor, activation: int = _
         d_up = torch.empty_like(dh)
         dw = None
         if topk_weight is not None and want_weight:
-            dw = torch.empty_like(topk_weight) if offsets is None else torch.zeros_like(topk_weight)
+            # (in order every pick has a row; a plan may leave one out)
+            dw = torch.empty_like(topk_weight) if perm is None and offsets is None else torch.zeros_like(topk_weight)
         h = torch.empty_like(dh) if want_h else None
         check(_lib.load().moe_activation_backward(
             cp, sp, hp, M, n, moe_dtype(dt), activation, alpha, limit, wp, pp, np_,

@@ -191,3 +191,24 @@ def test_how_far_a_kept_value_is_off(dt):
         _, kept = tuning.activation_save(None, v.cuda(), _lib.MOE_ACT_RELU2)
         assert (kept.scales == 0).all()
         assert ((kept.restore(F32)[0].double().cpu() - v.double()).abs() <= 2.0 ** -134).all()
+
+
+# ------------------------------------------------------------- the weights' gradient --
+
+def test_a_pick_that_no_row_names_has_no_gradient():
+    """A perm entry past M, with and without the plan's offsets: the pick it does not name gets zero, not what lay in
+    the memory."""
+    M, n = 4096, 64
+    _, kept = tuning.activation_save(torch.randn(M, n, device="cuda"), torch.randn(M, n, device="cuda"))
+    dh, w = torch.randn(M, n, device="cuda"), torch.rand(M, device="cuda")
+    perm = torch.randperm(M, generator=gen(1)).to(torch.int32)
+    lost = [int(perm[5]), int(perm[4000])]
+    perm[5], perm[4000] = M, -1
+    rest = torch.ones(M, dtype=torch.bool)
+    rest[lost] = False
+    for offsets in (None, torch.tensor([0, 7, M], dtype=torch.int32).cuda()):
+        for _ in range(4):
+            dirt = [torch.full((M,), float("nan"), device="cuda") for _ in range(8)]
+            del dirt
+            dw = tuning.activation_backward(kept, dh, topk_weight=w, perm=perm.cuda(), offsets=offsets).d_weight.cpu()
+            assert (dw[lost] == 0).all() and (dw[rest] != 0).any() and dw.isfinite().all()
