@@ -1456,6 +1456,9 @@ extern "C" moe_status moe_activation_save(const void* gate, const void* up, int3
     for (int j = 0; j < i; j++)  // (the value may take its own inputs' place)
       if (overlaps(b[i].p, b[i].bytes, b[j].p, b[j].bytes) && !(i == 2 && b[i].p == b[j].p))
         return fail(MOE_ERR_INVALID, "activation_save: buffers overlap (out: gate, up or apart)");
+  for (int i = 2; i < 5; i++)
+    if (overlaps(n_rows, 4, b[i].p, b[i].bytes))
+      return fail(MOE_ERR_INVALID, "activation_save: a result overlaps n_rows");
   MOE_HIP(launch_activation_save(gate, up, M, n, dtype, activation, alpha, limit, n_rows, out, codes,
                                  scales, stream),
           "activation save launch");
@@ -1493,7 +1496,7 @@ extern "C" moe_status moe_activation_backward(const int8_t* codes, const uint8_t
   const struct {
     const void* p;
     size_t bytes;
-  } in[4] = {{codes, kept}, {scales, kept / 32}, {topk_weight, (size_t)M * 4}, {perm, (size_t)M * 4}},
+  } in[5] = {{codes, kept}, {scales, kept / 32}, {topk_weight, (size_t)M * 4}, {perm, (size_t)M * 4}, {n_rows, 4}},
     out[4] = {{d_gate, rows}, {d_up, rows}, {h, rows}, {d_weight, (size_t)M * 4}};
   for (int i = 0; i < 4; i++) {
     for (const auto& b : in)
