@@ -127,7 +127,9 @@ static hipError_t launch_grad(void (*kernel)(const ExpertGradArgs), ExpertGradAr
 // fp32 rows: a block takes 64 rows and 64 columns, a wave a 32 x 32 quarter on
 // v_mfma_f32_32x32x2; 32 values of the sum at a time go through two LDS buffers
 // (the gradient's rows as they are, the weights dequantised, which keeps the
-// packed axis across the lanes), loaded while the chunk before is multiplied.
+// packed axis across the lanes), loaded while the chunk before is multiplied. A chunk is
+// summed by itself and then added, so that a sum of n values goes through 32 + n / 32
+// roundings one after another, not n.
 // Bound by the matrix cores where there are blocks enough: 64 rows of each of 128
 // experts, two 768 x 2048 products at 4 bits, 477 us, 108 TFLOP/s (a large fp32
 // product of the library 134). Small layers by the latency of their few chunks:
@@ -187,9 +189,11 @@ __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradAr
     Vec8<float>::store(&Bs[buf][bi][(tid & 7) * 8], wv);
     if (c + 1 < nchunks) load(c + 1, u);
     lds_barrier();
+    f32x16_t part = {};
 #pragma unroll
     for (int k = 0; k < kFK; k += 2)
-      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(As[buf][32 * wm + col][k + half], Bs[buf][k + half][32 * wn + col], acc, 0, 0, 0);
+      part = __builtin_amdgcn_mfma_f32_32x32x2f32(As[buf][32 * wm + col][k + half], Bs[buf][k + half][32 * wn + col], part, 0, 0, 0);
+    acc += part;
   }
   const int j = j0 + 32 * wn + col;
 #pragma unroll

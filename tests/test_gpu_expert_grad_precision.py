@@ -212,3 +212,29 @@ def test_a_pick_that_no_row_names_has_no_gradient():
             del dirt
             dw = tuning.activation_backward(kept, dh, topk_weight=w, perm=perm.cuda(), offsets=offsets).d_weight.cpu()
             assert (dw[lost] == 0).all() and (dw[rest] != 0).any() and dw.isfinite().all()
+
+
+# ------------------------------------------------------------------------- sums --
+
+@pytest.mark.parametrize("T", [3, 130])
+def test_long_sums_in_f32(T):
+    """8192 values of 1 + 2^-15, twice: a sum that takes them one after another loses their last bits from 2^11 on."""
+    N, K = 8192, 64
+    p = packed(torch.zeros(1, N, K, dtype=torch.int64), torch.ones(1, N, 2), torch.full((1, N, 2), 1 + 2.0 ** -15), 4, 32)
+    dy, offsets = torch.ones(T, N, device="cuda"), torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    assert (tuning.expert_matmul_backward(p, dy, offsets) == 8192.25).all()
+    assert (tuning.expert_matmul_backward(p, dy, offsets, proj2=p, dy2=dy) == 16384.5).all()
+
+
+@pytest.mark.parametrize("pair", [False, True])
+def test_sums_in_f32_stay_short(pair):
+    """A chunk's 32 values, the chunks one after another and a few roundings more, of the sum of magnitudes."""
+    T, E, N, K = 90, 3, 4100 - 4, 96
+    stacks = [stack(E, N, K, 6, 32, F32, i) for i in range(1 + pair)]
+    _, _, offsets = plan(picks(T, E, 1, 4), E)
+    dys = [torch.rand(T, N, generator=gen(i)) for i in range(1 + pair)]
+    zero = torch.zeros(T, K)
+    ref, mag, _ = grad64([w for _, w in stacks], dys, offsets, None, 1, zero)
+    kw = dict(proj2=stacks[1][0], dy2=dys[1].cuda()) if pair else {}
+    got = tuning.expert_matmul_backward(stacks[0][0], dys[0].cuda(), offsets.cuda(), **kw)
+    close(got, ref, mag * (32 + len(stacks) * N / 32 + 8) * U, "dx")
