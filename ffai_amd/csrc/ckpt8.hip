@@ -114,6 +114,17 @@ __global__ __launch_bounds__(256) void restore_kernel(const int8_t* __restrict__
   }
 }
 
+// e^x to a few roundings wherever it is normal: 2^h for the product h of x and log2 e as
+// rounded, times 2^l for what that left (one product alone is off by |x| 2^-24 of the
+// result). Past 128 infinity and 0, which the result is in fp32; NaN stays.
+__device__ __forceinline__ float near_exp(float x) {
+  constexpr float kLog2e = 1.44269502f, kRest = 1.92596303e-8f;  // log2 e and what fp32 leaves of it
+  x = x > 128.0f ? 128.0f : (x < -128.0f ? -128.0f : x);
+  const float h = x * kLog2e;
+  const float l = __builtin_fmaf(x, kRest, __builtin_fmaf(x, kLog2e, -h));
+  return __builtin_amdgcn_exp2f(h) * __builtin_fmaf(l, 0.69314718f, 1.0f);
+}
+
 // Value and slopes of the activation at (g, u); NaN in either gives NaN in all
 // that depends on it (apply_act's clamps would drop it).
 template <typename XT, int ACT>
@@ -127,14 +138,14 @@ __device__ __forceinline__ void act_slopes(float g, float u, float alpha, float 
   } else if constexpr (ACT == ACT_GPTOSS) {
     const float gc = g > limit ? limit : g;
     const float uc = u > limit ? limit : (u < -limit ? -limit : u);
-    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-alpha * gc));
+    const float s = __builtin_amdgcn_rcpf(1.0f + near_exp(-alpha * gc));
     const float a = gc * s;
     h = a * (uc + 1.0f);
     hg = g > limit ? 0.0f : (s + alpha * a * (1.0f - s)) * (uc + 1.0f);
     hu = uc == u ? a : uc - uc;  // past the limit 0, a NaN's own
   } else if constexpr (ACT == ACT_GEGLU) {
     const float y = 0.7978845608f * (g + 0.044715f * g * g * g);
-    const float l = __builtin_amdgcn_rcpf(1.0f + __expf(-2.0f * y));
+    const float l = __builtin_amdgcn_rcpf(1.0f + near_exp(-2.0f * y));
     const float t = l * (1.0f - l);  // 0 where g * g may be infinite
     const float d = t > 0.0f ? l + t * g * (1.5957691216f * (1.0f + 0.134145f * g * g)) : l;
     const float a = round_to<XT>(g * l);
@@ -142,7 +153,7 @@ __device__ __forceinline__ void act_slopes(float g, float u, float alpha, float 
     hg = d * u;
     hu = a;
   } else {
-    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+    const float s = __builtin_amdgcn_rcpf(1.0f + near_exp(-g));
     const float a = g * s;
     h = a * u;
     hg = (s + a * (1.0f - s)) * u;

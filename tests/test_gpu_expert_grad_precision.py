@@ -238,3 +238,31 @@ def test_sums_in_f32_stay_short(pair):
     kw = dict(proj2=stacks[1][0], dy2=dys[1].cuda()) if pair else {}
     got = tuning.expert_matmul_backward(stacks[0][0], dys[0].cuda(), offsets.cuda(), **kw)
     close(got, ref, mag * (32 + len(stacks) * N / 32 + 8) * U, "dx")
+
+
+# ----------------------------------------------------------------------- slopes --
+
+@pytest.mark.parametrize("act", [_lib.MOE_ACT_SWIGLU, _lib.MOE_ACT_GPTOSS])
+def test_slopes_far_from_zero(act):
+    """In f32 the logistic of g is off by a dozen roundings wherever it is (an exponential of 2, its two factors, a sum,
+    a reciprocal of 2, three products), and by |alpha g| of them for the rounded product alpha g that it is taken of;
+    not by |g| again for the exponential's own."""
+    g = torch.linspace(-84, 84, 32 * 256).reshape(256, 32)
+    if act == _lib.MOE_ACT_GPTOSS:
+        g = g / 1.75
+    u = torch.rand(256, 32, generator=gen(3)) + 0.5
+    _, kept = tuning.activation_save(g.cuda(), u.cuda(), act, 1.702, 1e4)
+    v = kept.restore(F32).double().cpu()
+    dh = (torch.rand(256, 32, generator=gen(4)) + 0.5)
+    got = tuning.activation_backward(kept, dh.cuda(), act, 1.702, 1e4, want_h=True)
+    alpha = float(torch.tensor(1.702)) if act == _lib.MOE_ACT_GPTOSS else 1.0
+    one = 1.0 if act == _lib.MOE_ACT_GPTOSS else 0.0
+    s = torch.sigmoid(alpha * v[0])
+    a, c = v[0] * s, (16 + (alpha * v[0].abs() if one else 0.0)) * U
+    d, up = dh.double(), v[1] + one
+    close(got.d_up, d * a, (d * a).abs() * c, "d_up")
+    close(got.h, a * up, (a * up).abs() * c, "h")
+    # 1 - s is off by what s is, s (1 - s) by both
+    rest = alpha * a * (1 - s)
+    size = s + (alpha * a).abs() * ((1 - s) + s)
+    close(got.d_gate, d * (s + rest) * up, (d * up).abs() * size * (c + 4 * U), "d_gate")
