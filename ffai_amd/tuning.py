@@ -697,7 +697,9 @@ class FrozenExperts:
                  out: Optional[torch.Tensor] = None, stream=None):
         """(dx [T, hidden], d_weight [T, k] float32) of forward for d_out
         [T, hidden]. dx is a gradient that x's is added to (None: zeros), from the
-        router or a shared expert; the sum goes to out, by default to dx itself."""
+        router or a shared expert; the sum goes to out, by default to dx itself.
+        Gate and up of two formats (bits, group size, scales' type) take a launch
+        each, and the sorted rows' gradient is rounded to their type between the two."""
         T, k = kept.inv_perm.shape
         H, at = self.up.k, d_out.get_device()
         gp = _check("d_out", _rows("d_out", d_out, 2), (T, H), _FLOATS if kept.Y is None else (kept.Y.dtype,), at)

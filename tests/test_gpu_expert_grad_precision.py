@@ -5,7 +5,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_expert_grad import CASES, grad64, picks, plan, stack  # noqa: E402
+from test_gpu_expert_grad import (ALPHA, CASES, GPTOSS, LIMIT, RELU2, SWIGLU, act64, act_tol, grad64, half, picks,  # noqa: E402
+                                  plan, stack)
 from test_gpu_tuning import BF16, F16, F32, U, close, cuda, gen, same_bits  # noqa: E402
 
 from ffai_amd import _lib, tuning  # noqa: E402
@@ -266,3 +267,76 @@ def test_slopes_far_from_zero(act):
     rest = alpha * a * (1 - s)
     size = s + (alpha * a).abs() * ((1 - s) + s)
     close(got.d_gate, d * (s + rest) * up, (d * up).abs() * size * (c + 4 * U), "d_gate")
+
+
+# ------------------------------------------------------------------------ chain --
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("act,two_formats,bias", [(SWIGLU, False, False), (SWIGLU, True, False), (GPTOSS, False, True), (RELU2, False, False)])
+@pytest.mark.parametrize("T", [1, 61, 700])
+def test_experts_in_16_bits(dt, act, two_formats, bias, T):
+    """Forward and backward of the chain against float64: the backward at the values kept, every rounding on the way
+    counted once."""
+    E, k, I, H = 6, 2, 104 - 8, 192
+    up, Wu = stack(E, I, H, 4, 64, dt, 1)
+    gate, Wg = (None, None) if act == RELU2 else stack(E, I, H, 8 if two_formats else 4, 32 if two_formats else 64, dt, 2)
+    down, Wd = stack(E, H, I, 6, 32, dt, 3)
+    bd = torch.zeros(E, H, dtype=dt)
+    if bias:
+        bd = (torch.randn(E, H, generator=gen(4)) * 0.1).to(dt)
+        down.out_bias = bd.cuda()
+    ex = tuning.FrozenExperts(gate, up, down, act, ALPHA, LIMIT)
+    idx, g = picks(T, E, k, 3, "some"), gen(5)
+    perm, inv, offsets = plan(idx, E)
+    x, wt, d = (torch.randn(T, H, generator=g) * 0.5).to(dt), torch.rand(T, k, generator=g), (torch.randn(T, H, generator=g) * 0.1).to(dt)
+    base = (torch.randn(T, H, generator=g) * 0.1).to(dt)
+    y, kept = ex.forward(x.cuda(), idx.cuda(), wt.cuda())
+    dx, dw = ex.backward(d.cuda(), kept, dx=base.cuda())
+    used, hf, two = int(offsets[-1]), half(dt), torch.finfo(dt).eps ** 2 / 4 + (2 * H + 8) * U
+    p = perm[:used].long()
+    row, e = p // k, torch.searchsorted(offsets[1:].long(), torch.arange(used), right=True)
+    tiny = 2.0 ** -25 if dt == F16 else 0.0
+
+    def times(rows, W):  # rows [used, n] by their experts' [n, m]
+        out = torch.zeros(used, W.shape[2], dtype=torch.float64)
+        for i in range(E):
+            out[e == i] = rows[e == i] @ W[i]
+        return out
+
+    # forward: the activation's inputs off by a rounding of theirs, of the weights (f16) and half a step more of the
+    # value, the experts' rows and their sum a rounding each: 8 half steps of the whole
+    xd = x.double()[row]
+    gd, ud = None if Wg is None else times(xd, Wg.transpose(1, 2)), times(xd, Wu.transpose(1, 2))
+    Y = times(act64(act, gd, ud, F32)[0], Wd.transpose(1, 2)) + bd.double()[e]
+    ref = torch.zeros(T, H, dtype=torch.float64).index_add(0, row, wt.double().flatten()[p][:, None] * Y)
+    assert (y.double().cpu() - ref).norm() <= 8 * hf * ref.norm()
+    # backward
+    v = kept.kept.restore(F32).double().cpu()[:, :used]
+    gk, uk = None if act == RELU2 else v[0], v[-1]
+    h, hg, hu = act64(act, gk, uk, F32)
+    th, tg, tu = act_tol(act, gk, uk, F32)
+    r = wt.to(dt).double().flatten()[p][:, None]
+    D = d.double()[row]
+    dh = times(D, Wd)
+    off = dh.abs() * hf + times(D.abs(), Wd.abs()) * two + D.abs().sum(1, keepdim=True) * tiny + tiny
+    dX, oX = torch.zeros(used, H, dtype=torch.float64), torch.zeros(used, H, dtype=torch.float64)
+    for W, slope, ts in ((Wg, hg, tg), (Wu, hu, tu)):
+        if W is None:
+            continue
+        a = r * dh * slope
+        oa = (r * slope).abs() * off + (r * dh).abs() * ts + a.abs() * 3 * U
+        oa = oa + (a.abs() + oa) * hf + tiny
+        dX += times(a, W)
+        oX += times(oa, W.abs()) + times(a.abs(), W.abs()) * two + a.abs().sum(1, keepdim=True) * tiny
+        if W is Wg and two_formats:  # rounded before the second projection's is added
+            oX += (dX.abs() + oX) * hf + tiny
+    oX += (dX.abs() + oX) * hf + tiny
+    rx, ox = base.double().index_add(0, row, dX), (base.double().abs() * 4 * U).index_add(0, row, oX + dX.abs() * 4 * U)
+    close(dx, rx, ox, "dx")
+    rw, ow = torch.zeros(T * k, dtype=torch.float64), torch.zeros(T * k, dtype=torch.float64)
+    if bias:  # from the experts' rows, which the forward rounded
+        Yk = kept.Y[:used].double().cpu()
+        rw[p], ow[p] = (D * Yk).sum(1), (D * Yk).abs().sum(1) * (H + 8) * U
+    else:
+        rw[p], ow[p] = (dh * h).sum(1), (off * h.abs() + dh.abs() * th + (dh * h).abs() * (I + 8) * U).sum(1)
+    close(dw.flatten(), rw, ow, "d_weight")
