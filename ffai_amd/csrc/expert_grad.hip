@@ -24,20 +24,18 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 // block of columns. Every wave finds it from the offsets by itself: one round of
 // loads, then sums across the lanes. No offset leads past M.
 //
-// In order (BY_SIZE false) tiles run through the experts, a tile's column blocks
-// (nb) together, the whole list in eight contiguous ranges, one per XCD (blocks b, b
-// + 8, ... share an XCD), whose L2 then keeps a tile's rows and an expert's
-// weights. BY_SIZE, for blocks of many us: whole tiles first, then the experts'
-// remainders of more than R / 2 rows, then the others, so that the last to start
-// are the short ones; tile t and its column blocks belong to XCD t % 8. Experts of
-// unequal popularity, 64 rows on average: 126 us in order, 114 by size; with tiles
-// of 32 rows 110 and 114, since an expert's tiles then share no XCD.
+// Tiles run through the experts, a tile's column blocks together, the whole list
+// in eight contiguous ranges, one per XCD (blocks b, b + 8, ... share an XCD), whose
+// L2 then keeps a tile's rows and an expert's weights. Whole tiles first and the
+// shortest last, each tile on one XCD, came to the same or more: 128 experts of unequal
+// popularity, 64 rows on average, 232 us for 231, 96 267 for 262, 32 of 128 rows, 2880 x
+// 2880, 208 for 191, 60 of 150 rows, 1408 x 2048, 269 for 278.
 struct GradTile {
   uint32_t e, m0, pend;  // expert, first sorted position, end
   int block;             // of columns
 };
 constexpr int kGradMaxE = 1024;
-template <uint32_t R, bool BY_SIZE>
+template <uint32_t R>
 __device__ __forceinline__ bool grad_tile(const ExpertGradArgs& a, GradTile* t) {
   constexpr int P = kGradMaxE / 64;
   const int E = a.E, lane = threadIdx.x & 63;
@@ -51,50 +49,30 @@ __device__ __forceinline__ bool grad_tile(const ExpertGradArgs& a, GradTile* t) 
       hi[i] = max(min(a.offsets[min(i * 64 + lane + 1, E)], (uint32_t)a.M), lo[i]);
     }
   }
-  // whole tiles and remainders up to and with an expert's (remainders: long ones
-  // in the low half, short ones in the high half, 1024 at most)
-  uint32_t whole[P], rest[P], wholes = 0, rests = 0;
+  uint32_t upto[P], tiles = 0;  // up to and with an expert's
 #pragma unroll
   for (int i = 0; i < P; i++) {
-    whole[i] = rest[i] = 0;
+    upto[i] = 0;
     if (i * 64 < E) {
-      const uint32_t c = hi[i] - lo[i], r = c % R;
-      whole[i] = wholes + wave_scan_u32(BY_SIZE ? c / R : (c + R - 1) / R);
-      wholes = (uint32_t)__builtin_amdgcn_readlane((int)whole[i], 63);
-      if constexpr (BY_SIZE) {
-        rest[i] = rests + wave_scan_u32(r > R / 2 ? 1u : (r ? 0x10000u : 0u));
-        rests = (uint32_t)__builtin_amdgcn_readlane((int)rest[i], 63);
-      }
+      upto[i] = tiles + wave_scan_u32((hi[i] - lo[i] + R - 1) / R);
+      tiles = (uint32_t)__builtin_amdgcn_readlane((int)upto[i], 63);
     }
   }
-  const uint32_t k = blockIdx.x >> 3, longs = rests & 0xFFFFu;
-  uint32_t tile;
-  if constexpr (BY_SIZE) {
-    tile = (blockIdx.x & 7u) + 8u * (k / nb);
-    t->block = a.first + (int)(k % nb);
-    if (tile >= wholes + longs + (rests >> 16)) return false;
-  } else {
-    const uint32_t per = (wholes * nb + 7u) >> 3, w = (blockIdx.x & 7u) * per + k;
-    tile = w / nb;
-    t->block = a.first + (int)(w - tile * nb);
-    if (k >= per || tile >= wholes) return false;
-  }
-  const int kind = tile < wholes ? 0 : (tile < wholes + longs ? 1 : 2);
-  tile -= kind == 0 ? 0u : (kind == 1 ? wholes : wholes + longs);
+  const uint32_t k = blockIdx.x >> 3, per = (tiles * nb + 7u) >> 3, w = (blockIdx.x & 7u) * per + k, tile = w / nb;
+  if (k >= per || tile >= tiles) return false;
+  t->block = a.first + (int)(w - tile * nb);
   bool found = false;
 #pragma unroll
   for (int i = 0; i < P; i++)
     if (i * 64 < E && !found) {
-      const uint32_t upto = kind == 0 ? whole[i] : (kind == 1 ? rest[i] & 0xFFFFu : rest[i] >> 16);
-      const uint64_t past = __ballot(upto > tile);
+      const uint64_t past = __ballot(upto[i] > tile);
       if (past) {
         const int at = __ffsll((unsigned long long)past) - 1;
         const uint32_t l = (uint32_t)__builtin_amdgcn_readlane((int)lo[i], at);
         const uint32_t h = (uint32_t)__builtin_amdgcn_readlane((int)hi[i], at);
-        const uint32_t n = BY_SIZE ? (h - l) / R : (h - l + R - 1) / R;
-        const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)upto, at) - n;
+        const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)upto[i], at) - (h - l + R - 1) / R;
         t->e = (uint32_t)(i * 64 + at);
-        t->m0 = l + (kind ? n : tile - first) * R;
+        t->m0 = l + (tile - first) * R;
         t->pend = min(h, t->m0 + R);
         found = true;
       }
@@ -140,7 +118,7 @@ template <int BITS>
 __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradArgs a) {
   __shared__ float As[2][kFR][kFK + 1], Bs[2][kFK][kFC];
   GradTile t;
-  if (!grad_tile<kFR, false>(a, &t)) return;
+  if (!grad_tile<kFR>(a, &t)) return;
   const int j0 = t.block * kFC, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int col = lane & 31, half = lane >> 5;
@@ -232,9 +210,9 @@ __global__ __launch_bounds__(256) void expert_grad_f32_kernel(const ExpertGradAr
 // weights (loaded three chunks ahead into registers, dequantised into two LDS
 // buffers between the matrix steps of the chunk before). One barrier a chunk.
 //
-// 1024 rows of each of 32 experts, 2880 x 2880 at 4 bits, bf16: 1017 us, 535 TFLOP/s of
+// 1024 rows of each of 32 experts, 2880 x 2880 at 4 bits, bf16: 966 us, 563 TFLOP/s of
 // the product, twice that of the matrix cores; 256 of each of 128, two 768 x 2048
-// products: 495 us (8 bits 443; f16 at 4 bits 454). A large bf16 product of the library
+// products: 465 us (8 bits 421; f16 at 4 bits 445). A large bf16 product of the library
 // reaches 1276, a loop of nothing but these matrix instructions on random operands
 // 1543, with four vector instructions to each 1359: the chip lowers its clock as both
 // kinds run, and a block's start and end are hidden by no other at one block a CU.
@@ -720,7 +698,7 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
   __shared__ __align__(16) unsigned char a0[GradTall::ABYTES], a1[GradTall::ABYTES], a2[GradTall::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradTall::BBYTES];
   GradTile t;
-  if (!grad_tile<GradTall::MR, true>(a, &t)) return;
+  if (!grad_tile<GradTall::MR>(a, &t)) return;
   const int j0 = t.block * GradTall::NC;
   const GradLds L{a0, a1, a2, b};
   const uint32_t rows = t.pend - t.m0;
@@ -737,10 +715,12 @@ __global__ __launch_bounds__(GradTall::NT) void expert_grad_tall_kernel(const Ex
 // dequantises into LDS of its own, 16 weight rows at a time, so the loop has no barrier:
 // LDS serves a wave's stores and reads in order.
 //
-// 8 rows of each of 128 experts, two 768 x 2048 products at 4 bits, bf16: 106 us, 2.2
-// TB/s of experts and rows; 6 rows of each of 32, 2880 x 2880: 73 us, 2.1 TB/s, where a
-// large copy reaches 5.2. Of a chunk's 350 vector instructions a wave, a third make the lo
-// parts; with three waves a SIMD for two the second takes 73 us for 87.
+// 8 rows of each of 128 experts, two 768 x 2048 products at 4 bits, bf16: 100 us, 2.3
+// TB/s of experts and rows; 6 rows of each of 32, 2880 x 2880: 69 us, 2.2 TB/s, where a
+// large copy reaches 5.2. Bound by instructions: the vector units are busy 59% of a SIMD's
+// time and the matrix cores 21%. Of a chunk's 330 vector instructions a wave, a third make
+// the lo parts. Three waves a SIMD for two (8 bits: two, they need 207 registers): 75 us for
+// 87.
 //
 // The hi and lo parts are summed together (128 registers of sums would leave two waves a
 // SIMD): where a sum is not finite, the block sums the hi parts alone again for the
@@ -756,7 +736,7 @@ __global__ __launch_bounds__(256, BITS == 8 ? 2 : 3) void expert_grad_few_kernel
   static_assert(kWave >= 2 * kPart, "staging");
   __shared__ __align__(16) unsigned char lds[4 * kWave];
   GradTile t;
-  if (!grad_tile<kFewRows, false>(a, &t)) return;
+  if (!grad_tile<kFewRows>(a, &t)) return;
   const int j0 = t.block * FC, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, col = lane & 31, h = lane >> 5;
   const int N = a.N, K = a.K, CU = K >> 5, groups = CU >> a.gsh, row_words = CU * BITS;
@@ -918,7 +898,7 @@ __global__ __launch_bounds__(GradMid::NT, 2) void expert_grad_mid_kernel(const E
   __shared__ __align__(16) unsigned char a0[GradMid::ABYTES], a1[GradMid::ABYTES], a2[GradMid::ABYTES];
   __shared__ __align__(16) unsigned char b[2 * GradMid::BBYTES];
   GradTile t;
-  if (!grad_tile<GradMid::MR, true>(a, &t)) return;
+  if (!grad_tile<GradMid::MR>(a, &t)) return;
   const int j0 = t.block * GradMid::NC;
   const GradLds L{a0, a1, a2, b};
   const uint32_t rows = t.pend - t.m0;
