@@ -917,9 +917,10 @@ __global__ __launch_bounds__(GradMid::NT, 2) void expert_grad_mid_kernel(const E
 // / 211 / 203; 48 rows of 2 bits 188 / 178 / 191 / 191, 5 bits 224 / 208 / 213 / 211, 6 bits
 // 224 / 211 / 215 / 204, 8 bits 246 / 223 / 218 / 207; f16, 3 bits, 256 experts 512 x 2048 of
 // 24 rows 192 / 184 / 280 / 298, of 48 322 / 288 / 311 / 314.
-// Few blocks: 32 experts of 32 rows (256 wide ones) 33 / 38, 20 of 20 rows, 5120 x 5120
-// (400) 164 / 160; ordinary and tall, 8 of 256 rows (128 tall ones) 34 / 39, 4 of 512, 2880
-// x 2880 (184) 85 / 70, one of 4096 (256) 67 / 49.
+// Few blocks: few and ordinary, 8 experts of 16 rows 21 / 19, one of one row 20 / 19, 4 of
+// one row, 2880 x 2880, 34 / 41; few and wide, 32 experts of 32 rows (256 wide ones) 33 / 38, 20 of
+// 20 rows, 5120 x 5120 (400) 164 / 160; ordinary and tall, 8 of 256 rows (128 tall ones) 34 /
+// 39, 4 of 512, 2880 x 2880 (184) 85 / 70, one of 4096 (256) 67 / 49.
 template <int BITS, typename XT>
 static hipError_t launch_mma(const ExpertGradArgs& a, hipStream_t st) {
   const int64_t used = std::min(a.E, a.M);
