@@ -30,8 +30,8 @@ def packed(q, s, b, bits, gs):
     return StackedExperts(torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32).cuda(), s.cuda(), b.cuda(), bits, gs)
 
 
-# rows that take the kernels of few rows (narrow and wide blocks), of 128 and of 256 rows
-ROWS = [(8, 30), (64, 100), (4, 900), (40, 2000)]
+# rows that take the kernels of few rows (narrow blocks twice, wide ones), of 128 and of 256 rows
+ROWS = [(8, 30), (64, 100), (64, 1500), (4, 900), (40, 2000)]
 
 
 @pytest.mark.parametrize("dt", [BF16, F16])
@@ -126,6 +126,70 @@ def test_wide_rows_of_many_experts():
         close(dx[row], ref, mag.cpu() * (2.0 ** -16 + 32 * U), f"row {row}")
     del dx
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("bits", [3, 4, 8])
+@pytest.mark.parametrize("E,T", ROWS)
+def test_infinities_added_in_place(dt, bits, E, T):
+    """What is not finite is added to dx once, and what is finite beside it keeps its bits: in dx's own place, apart from
+    it, and in a replayed graph."""
+    N, K = 72, 2080
+    p, _ = stack(E, N, K, bits, 32, dt, 3)
+    _, _, offsets = plan(picks(T, E, 1, 5), E)
+    g = gen(1)
+    dy, base = (torch.randn(T, N, generator=g) * 0.01).to(dt).cuda(), (torch.randn(T, K, generator=g) * 0.01).to(dt).cuda()
+    off = offsets.cuda()
+    plain = tuning.expert_matmul_backward(p, dy, off, dx=base, out=torch.empty_like(base))
+    bad = dy.clone()
+    bad[T // 2, 70], bad[T - 1, 3] = float("inf"), float("nan")
+    last = int((offsets[1:] > offsets[:-1]).nonzero().max())
+    p.scales[last, 9, 2] = float("inf")
+    apart = tuning.expert_matmul_backward(p, bad, off, dx=base, out=torch.empty_like(base))
+    place = base.clone()
+    assert same_bits(tuning.expert_matmul_backward(p, bad, off, dx=place), apart)
+    ok = torch.ones(T, K, dtype=torch.bool)
+    ok[[T // 2, T - 1]] = False
+    ok[int(offsets[last]):, 64:96] = False
+    ok = ok.cuda()
+    assert same_bits(apart[ok], plain[ok]) and not apart[~ok].isfinite().any()
+    held = bad.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        tuning.expert_matmul_backward(p, held, off, dx=base, out=place)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tuning.expert_matmul_backward(p, held, off, dx=base, out=place)
+    clean = tuning.expert_matmul_backward(p, dy, off, dx=base, out=torch.empty_like(base))
+    for rows, want in ((bad, apart), (dy, clean), (bad, apart)):
+        held.copy_(rows)
+        place.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same_bits(place, want)
+
+
+@pytest.mark.parametrize("E,T", ROWS)
+def test_weights_past_f16(E, T):
+    """bf16 scales beside f16 rows: a weight of 65504 is itself, one of 65520 or more infinite, in every kernel."""
+    N, K = 64, 2080
+    s, b = torch.zeros(E, N, K // 32, dtype=BF16), torch.ones(E, N, K // 32, dtype=BF16)
+    s[:, :, 1], b[:, :, 1] = 16.0, 65280.0  # 65280, 65296, ... 65504, 65520
+    b[:, :, 2] = 70144.0
+    q = (torch.arange(K) % 16).expand(E, N, K).contiguous()
+    p = packed(q, s, b, 4, 32)
+    _, _, offsets = plan(picks(T, E, 1, 5), E)
+    dy = torch.zeros(T, N, dtype=F16)
+    dy[:, 7] = 0.5
+    w = 65280.0 + 16.0 * q[0, 0, 32:64].double()
+    # (beside 0.5 the rows are 0, and 0 times an infinite weight is NaN; of 64 values of 2^-7 the sum is w / 2 too)
+    for rows, past in ((dy, float("nan")), (torch.full((T, N), 2.0 ** -7, dtype=F16), float("inf"))):
+        got = tuning.expert_matmul_backward(p, rows.cuda(), offsets.cuda())
+        ref = torch.full((K,), 0.5, dtype=torch.float64)
+        ref[32:64], ref[64:96] = torch.where(w < 65520, w / 2, past), past
+        close(got, ref.expand(T, K), 0.0, "dx")
 
 
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
